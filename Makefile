@@ -36,7 +36,7 @@ ifdef cuda
 	CUDA_LDFLAGS = -L$(CUDA_LIB) -lcudart_static -lrt -ldl
 	CPPFLAGS += -DHAVE_CUDA=1 -I $(CUDA_INC)
 	GPU_OBJ = $(BUILD_DIR)/fluke_sm100.o $(BUILD_DIR)/nn_gpu.o $(BUILD_DIR)/fused_i8.o \
-	          $(BUILD_DIR)/fused_fp8.o $(BUILD_DIR)/lstm_host.o
+	          $(BUILD_DIR)/fused_fp8.o $(BUILD_DIR)/fp4.o $(BUILD_DIR)/lstm_host.o
 	SHARED_LINK = $(NVCC) -shared $(SM100_ARCH)
 	LDFLAGS += $(CUDA_LDFLAGS)
 endif

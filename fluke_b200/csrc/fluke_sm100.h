@@ -112,6 +112,43 @@ typedef struct {
 
 int fluke_sm100_gemm(const fluke_sm100_gemm_t *g, void *stream);
 
+/* ---- microscaled 4-bit floating point ---------------------------------------------------- */
+
+enum fluke_sm100_fp4 {
+    FLUKE_SM100_FP4_MX = 1,   /* blocks of 32 under an e8m0 scale                                  */
+    FLUKE_SM100_FP4_NV = 2    /* blocks of 16 under an e4m3 scale and a power of two per row       */
+};
+#define FLUKE_SM100_FP4_MAX_ROW 16384   /* columns of the kernels that hold a row in registers */
+
+int fluke_sm100_quant_fp4(const void *in, void *codes, void *scale, void *row_scale, int rows, int cols,
+                          int format, int bf16, void *stream);
+int fluke_sm100_dequant_fp4(const void *codes, const void *scale, const void *row_scale, void *out,
+                            int rows, int cols, int format, int bf16, void *stream);
+
+typedef struct {
+    int rows, cols, seqlen;     /* seqlen: rows that share a row of gate; 0 = one row for all     */
+    int bf16;                   /* type of every 16-bit tensor here: 0 f16, 1 bf16                */
+    int out_format;             /* 0: 16 bits, enum fluke_sm100_fp4, 3: no output but the stream  */
+    const void *x, *residual, *w_post, *gate, *w_pre;   /* w_post and gate may be null            */
+    void *residual_out;         /* may be residual                                                */
+    void *out, *scale;
+    float *row_scale;
+    float alpha, eps;
+} fluke_sm100_rmsnorm_block_t;
+int fluke_sm100_rmsnorm_block(const fluke_sm100_rmsnorm_block_t *b, void *stream);
+
+typedef struct {
+    int format;                 /* enum fluke_sm100_fp4                                           */
+    int bf16;                   /* type of out: 0 f16, 1 bf16                                     */
+    int M, N, K;                /* out [M,N]; a [M,K]; b (and b2) [N,K]                           */
+    const void *a, *a_scale;
+    const void *b, *b_scale;
+    const void *b2, *b2_scale;  /* second weight: out = silu(a b^T) * (a b2^T); else null         */
+    const float *a_row, *b_row, *b2_row;    /* NV: f32 [M], [N], [N]                               */
+    void *out;
+} fluke_sm100_gemm_fp4_t;
+int fluke_sm100_gemm_fp4(const fluke_sm100_gemm_fp4_t *g, void *stream);
+
 /* ---- factored LSTM ------------------------------------------------------------------------ */
 
 typedef struct {

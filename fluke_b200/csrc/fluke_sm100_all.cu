@@ -3,6 +3,8 @@
 // tcgen05/TMA helpers, and the library needs no relocatable device code.
 #include "rowwise_sm100.cu"
 #include "gemm_sm100.cu"
+#include "fp4_rows_sm100.cu"
+#include "fp4_gemm_sm100.cu"
 #include "lstm_sm100.cu"
 #include "lstm_persist_sm100.cu"
 #include "lstm_cluster_sm100.cu"

@@ -1,0 +1,552 @@
+// fp4_rows_sm100.cu -- the memory-bound kernels of microscaled 4-bit floating point: quantisation of
+// rows in two formats, reading back, and the norms before and after a block (with its gate and
+// residual scale) whose result may leave quantised.
+//
+// Elements are E2M1 (0, 0.5, 1, 1.5, 2, 3, 4, 6 and sign), two to a byte, the earlier one in the low half;
+// rounding to nearest, ties to the even code, saturating at 6.
+//   MX  blocks of 32 along the row (OCP Microscaling Formats v1.0): scale 2^e, e = floor(log2(amax)) - 2 limited to
+//       -127 .. 127, stored as e + 127; an all-zero block has e = -127. Scaling is exact, so the
+//       only rounding is that of the element.
+//   NV  blocks of 16 under an e4m3 scale s, and a power of two g per row: the least with
+//       amax(row) <= 2688 g = 6 * 448 g (at least 2^-100; 1 for a row of zeros). s = e4m3(bmax / (6 g)),
+//       element = e2m1(x / (s g)), both quotients rounded to f32 first; s = 0 gives zeros.
+//       A power of two keeps s g exact in four bits, so that ties are what they are in real numbers.
+// A block (MX) or row (NV) with an infinity or a NaN has no value: its scale is the NaN code (MX 255; NV
+// 0x7F, and g is NaN) and its elements are zero.
+//
+// Block scales are stored in the order in which a tensor-memory copy wants them: 512-byte tiles of 128 rows
+// x 4 blocks, tile (r / 128, c / 4) with block c of row r at byte (r % 32) * 16 + (r / 32 % 4) * 4 + c % 4. Blocks behind
+// the end of a row up to the next multiple of 4 are written as zero; rows behind the last are left as they were.
+#include <cuda_bf16.h>
+
+namespace fluke_sm100 {
+namespace {
+
+enum Fp4Out { kFp4Plain = 0, kFp4Mx = 1, kFp4Nv = 2, kFp4None = 3 };
+
+__device__ __forceinline__ float2 unpack2(uint32_t v, __half) { return half2_bits_to_float2(v); }
+__device__ __forceinline__ float2 unpack2(uint32_t v, __nv_bfloat16) {
+    return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xFFFF0000u));
+}
+__device__ __forceinline__ uint32_t pack2(float2 f, __half) { return float2_to_half2_bits(f); }
+__device__ __forceinline__ uint32_t pack2(float2 f, __nv_bfloat16) {
+    const __nv_bfloat162 h = __float22bfloat162_rn(f);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+// Eight values as codes, the first in the lowest four bits.
+__device__ __forceinline__ uint32_t e2m1x8(float2 a, float2 b, float2 c, float2 d) {
+    uint32_t w;
+    asm("{\n.reg .b8 p, q, r, s;\n"
+        "cvt.rn.satfinite.e2m1x2.f32 p, %2, %1;\n"
+        "cvt.rn.satfinite.e2m1x2.f32 q, %4, %3;\n"
+        "cvt.rn.satfinite.e2m1x2.f32 r, %6, %5;\n"
+        "cvt.rn.satfinite.e2m1x2.f32 s, %8, %7;\n"
+        "mov.b32 %0, {p, q, r, s};\n}"
+        : "=r"(w) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y), "f"(d.x), "f"(d.y));
+    return w;
+}
+// Eight codes as values.
+__device__ __forceinline__ void e2m1x8_to_float(uint32_t w, float2 (&v)[4]) {
+    uint32_t h[4];
+    asm("{\n.reg .b8 p, q, r, s;\n"
+        "mov.b32 {p, q, r, s}, %4;\n"
+        "cvt.rn.f16x2.e2m1x2 %0, p;\n"
+        "cvt.rn.f16x2.e2m1x2 %1, q;\n"
+        "cvt.rn.f16x2.e2m1x2 %2, r;\n"
+        "cvt.rn.f16x2.e2m1x2 %3, s;\n}"
+        : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3]) : "r"(w));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = half2_bits_to_float2(h[i]);
+}
+
+// The bit pattern of the largest magnitude of 16 values: patterns order like the values, infinities above every
+// number and NaNs above those.
+__device__ __forceinline__ uint32_t max_bits16(const float2 (&v)[8]) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, max(__float_as_uint(v[i].x) & 0x7FFFFFFFu, __float_as_uint(v[i].y) & 0x7FFFFFFFu));
+    return m;
+}
+constexpr uint32_t kInfBits = 0x7F800000u;
+
+// 2^(e - 127) for a stored exponent of 0 .. 254, the smallest of which is not a normal number; 255 gives NaN.
+__device__ __forceinline__ float e8m0_value(uint32_t e) {
+    return __uint_as_float(e == 0 ? 0x00400000u : e == 255 ? 0x7FFFFFFFu : e << 23);
+}
+__device__ __forceinline__ float e4m3_value(uint32_t s) {
+    uint32_t h;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(uint16_t(s)));
+    return half2_bits_to_float2(h).x;
+}
+
+// Byte of the scale of block c of row r; `tiles` of four blocks to a row.
+__device__ __forceinline__ int64_t scale_byte(int64_t r, int c, int tiles) {
+    return ((r >> 7) * tiles + (c >> 2)) * 512 + int((r & 31) * 16 + ((r >> 5) & 3) * 4) + (c & 3);
+}
+// Zeros behind the last block of a row, up to a multiple of four.
+__device__ __forceinline__ void pad_scales(uint8_t *scale, int64_t row, int blocks, int tiles) {
+    for (int c = blocks; c < tiles * 4; ++c) scale[scale_byte(row, c, tiles)] = 0;
+}
+
+// MX: the stored exponent of a block by the bits of its largest magnitude. 255: no value.
+__device__ __forceinline__ uint32_t mx_exponent(uint32_t amax_bits) {
+    if (amax_bits >= kInfBits) return 255;
+    const uint32_t e = amax_bits >> 23;
+    return e > 2 ? e - 2 : 0;
+}
+// MX: 16 codes of a block with that exponent.
+__device__ __forceinline__ uint2 mx_codes(const float2 (&v)[8], uint32_t e) {
+    if (e == 255) return make_uint2(0, 0);
+    const float f = __uint_as_float((254 - e) << 23);  // 2^(127 - e), e <= 253
+    const float2 f2 = make_float2(f, f);
+    float2 q[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) q[i] = mul2(v[i], f2);
+    return make_uint2(e2m1x8(q[0], q[1], q[2], q[3]), e2m1x8(q[4], q[5], q[6], q[7]));
+}
+
+// NV: the power of two of a row by the bits of its largest magnitude; NaN without one.
+__device__ __forceinline__ float nv_row_scale(uint32_t amax_bits) {
+    if (amax_bits == 0) return 1.0f;
+    if (amax_bits >= kInfBits) return __uint_as_float(0x7FFFFFFFu);
+    // amax = f 2^E with 1 <= f < 2 and 2688 = 1.3125 * 2^11
+    const int E = int(amax_bits >> 23) - 127 - 11 + ((amax_bits & 0x7FFFFFu) > 0x280000u ? 1 : 0);
+    return __uint_as_float(uint32_t(max(E, -100) + 127) << 23);
+}
+// NV: 16 codes of a block (its own largest magnitude given) in a row of scale g, and its e4m3 scale.
+__device__ __forceinline__ uint2 nv_codes(const float2 (&v)[8], uint32_t bmax_bits, float g, uint32_t &s8) {
+    if (!(g > 0.f)) {
+        s8 = 0x7F;
+        return make_uint2(0, 0);
+    }
+    const float t = __fdiv_rn(__uint_as_float(bmax_bits), 6.0f * g);
+    uint16_t pair;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(pair) : "f"(0.f), "f"(t));
+    s8 = pair & 0xFFu;
+    if (s8 == 0) return make_uint2(0, 0);
+    const float s = e4m3_value(s8) * g;
+    // v / s, correctly rounded: s has four significant bits, and with the correctly rounded reciprocal one exact residual
+    // is enough for all of them (every one of the 2^23 mantissas tried against all eight divisors). The sign of a
+    // zero is put back.
+    const float r = __frcp_rn(s);
+    const float2 r2 = make_float2(r, r), s2 = make_float2(-s, -s);
+    float2 q[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        q[i] = mul2(v[i], r2);
+        q[i] = fma2(fma2(q[i], s2, v[i]), r2, q[i]);
+        q[i].x = copysignf(q[i].x, v[i].x);
+        q[i].y = copysignf(q[i].y, v[i].y);
+    }
+    return make_uint2(e2m1x8(q[0], q[1], q[2], q[3]), e2m1x8(q[4], q[5], q[6], q[7]));
+}
+
+// A unit: 16 consecutive values of a row, 32 bytes in 16 bits and 8 as codes.
+template <typename T>
+__device__ __forceinline__ void unpack16(const uint32_t (&r)[8], float2 (&v)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = unpack2(r[i], T());
+}
+
+// ---- quantisation, MX -------------------------------------------------------------------------
+// Blocks do not depend on their row: thread = unit, a block is two neighbouring lanes (rows are whole blocks, so
+// a pair never straddles two). Bound by memory: 2 bytes in and 0.53 out per value.
+template <typename T>
+__global__ void __launch_bounds__(256)
+quant_mxfp4_kernel(const T *in, uint8_t *codes, uint8_t *scale, uint32_t units, uint32_t units_per_row, int tiles) {
+    dependency_wait();
+    const uint32_t u = blockIdx.x * 256u + threadIdx.x;
+    const bool live = u < units;
+    uint32_t raw[8] = {};
+    if (live) load32(in + int64_t(u) * 16, raw);
+    float2 v[8];
+    unpack16<T>(raw, v);
+    uint32_t m = max_bits16(v);
+    m = max(m, __shfl_xor_sync(kFull, m, 1));
+    if (!live) return;
+    const uint32_t e = mx_exponent(m);
+    *reinterpret_cast<uint2 *>(codes + int64_t(u) * 8) = mx_codes(v, e);
+    const uint32_t row = u / units_per_row, at = u - row * units_per_row;
+    if ((at & 1u) == 0) scale[scale_byte(row, int(at >> 1), tiles)] = uint8_t(e);
+    if (at == units_per_row - 1) pad_scales(scale, row, int(units_per_row >> 1), tiles);
+}
+
+// ---- reading back -----------------------------------------------------------------------------
+// value = code * 2^e, or (code * s) * g, rounded once. Thread = unit.
+template <typename T, bool MX>
+__global__ void __launch_bounds__(256)
+dequant_fp4_kernel(const uint8_t *codes, const uint8_t *scale, const float *row_scale, T *out, uint32_t units, uint32_t units_per_row,
+                   int tiles) {
+    dependency_wait();
+    const uint32_t u = blockIdx.x * 256u + threadIdx.x;
+    if (u >= units) return;
+    const uint32_t row = u / units_per_row, at = u - row * units_per_row;
+    const uint2 c = *reinterpret_cast<const uint2 *>(codes + int64_t(u) * 8);
+    const uint32_t s8 = scale[scale_byte(row, int(MX ? at >> 1 : at), tiles)];
+    const float s = MX ? e8m0_value(s8) : e4m3_value(s8), g = MX ? 1.f : row_scale[row];
+    const float2 s2 = make_float2(s, s), g2 = make_float2(g, g);
+    float2 lo[4], hi[4];
+    e2m1x8_to_float(c.x, lo);
+    e2m1x8_to_float(c.y, hi);
+    uint32_t r[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 a = mul2(lo[i], s2), b = mul2(hi[i], s2);
+        r[i] = pack2(MX ? a : mul2(a, g2), T());
+        r[i + 4] = pack2(MX ? b : mul2(b, g2), T());
+    }
+    store32(out + int64_t(u) * 16, r);
+}
+
+// ---- rows held in registers -------------------------------------------------------------------
+// A row belongs to one warp (8 rows to a block) or to one whole block of up to 8 warps; lane l of the row's
+// `lanes` holds units l, l + lanes, ... (U of them).
+constexpr int kFp4RowWarps = 8;
+
+template <bool BLOCK_ROW>
+__device__ __forceinline__ uint32_t row_max(uint32_t m, uint32_t *shared) {
+    m = __reduce_max_sync(kFull, m);
+    if constexpr (BLOCK_ROW) {
+        const int warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+        if ((threadIdx.x & 31) == 0) shared[warp] = m;
+        __syncthreads();
+        m = 0;
+        for (int w = 0; w < warps; ++w) m = max(m, shared[w]);
+    }
+    return m;
+}
+template <bool BLOCK_ROW>
+__device__ __forceinline__ double row_sum(double s, double *shared) {
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(kFull, s, d);
+    if constexpr (BLOCK_ROW) {
+        const int warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+        if ((threadIdx.x & 31) == 0) shared[warp] = s;
+        __syncthreads();
+        s = 0;
+        for (int w = 0; w < warps; ++w) s += shared[w];
+    }
+    return s;
+}
+
+// Quantisation, NV.
+template <typename T, int U, bool BLOCK_ROW>
+__global__ void __launch_bounds__(kFp4RowWarps * 32)
+quant_nvfp4_kernel(const T *in, uint8_t *codes, uint8_t *scale, float *row_scale, int rows, int units, int tiles) {
+    __shared__ uint32_t shared[kFp4RowWarps];
+    dependency_wait();
+    const int lanes = BLOCK_ROW ? blockDim.x : 32;
+    const int lane = BLOCK_ROW ? threadIdx.x : threadIdx.x & 31;
+    const int64_t row = BLOCK_ROW ? int64_t(blockIdx.x) : int64_t(blockIdx.x) * kFp4RowWarps + (threadIdx.x >> 5);
+    if (row >= rows) return;
+    uint32_t raw[U][8];
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+        if (lane + j * lanes < units) load32(in + (row * units + lane + j * lanes) * 16, raw[j]);
+        else
+#pragma unroll
+            for (int i = 0; i < 8; ++i) raw[j][i] = 0;
+    }
+    uint32_t bmax[U], amax = 0;
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+        float2 v[8];
+        unpack16<T>(raw[j], v);
+        bmax[j] = max_bits16(v);
+        amax = max(amax, bmax[j]);
+    }
+    const float g = nv_row_scale(row_max<BLOCK_ROW>(amax, shared));
+    if (lane == 0) row_scale[row] = g;
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+        const int at = lane + j * lanes;
+        if (at >= units) break;
+        float2 v[8];
+        unpack16<T>(raw[j], v);
+        uint32_t s8;
+        *reinterpret_cast<uint2 *>(codes + (row * units + at) * 8) = nv_codes(v, bmax[j], g, s8);
+        scale[scale_byte(row, at, tiles)] = uint8_t(s8);
+        if (at == units - 1) pad_scales(scale, row, units, tiles);
+    }
+}
+
+// Norms around a block. Per row, with r(v) = 1 / sqrt(mean(v^2) + eps):
+//     y = round16(alpha * residual + gate * ((x * r(x)) * w_post))          the new residual stream
+//     h = (y * r(y)) * w_pre                                                 the next block's input
+// every product and sum rounded to f32 on its own, in this order. The means are taken in 64 bits and r is
+// rounded once to f32: what is quantised behind them lies next to borders, and like this the result depends on
+// the values alone, not on how a row is spread over lanes. One Newton step from the hardware's reciprocal root leaves a
+// relative error of 1e-13 before that rounding.
+__device__ __forceinline__ float inv_rms(double sum, double inv_n, float eps) {
+    const double a = fma(sum, inv_n, double(eps));
+    if (!(a > 1e-37 && a < 1e38)) return float(1.0 / sqrt(a));  // no f32 holds it: rows of very large or very small bf16 values, NaN
+    const double r = double(rsqrtf(float(a)));
+    return float(fma(r, fma(-0.5 * a * r, r, 0.5), r));
+}
+
+struct RmsnormBlockDev {
+    const void *x, *residual, *w_post, *gate, *w_pre;
+    void *residual_out, *out;
+    uint8_t *scale;
+    float *row_scale;
+    int rows, units, tiles, seqlen;
+    float alpha, eps;
+};
+
+template <typename T, int OUT, int U, bool BLOCK_ROW>
+__global__ void __launch_bounds__(kFp4RowWarps * 32)
+rmsnorm_block_kernel(const RmsnormBlockDev p) {
+    __shared__ double sums[2][kFp4RowWarps];
+    __shared__ uint32_t maxima[kFp4RowWarps];
+    dependency_wait();
+    const int lanes = BLOCK_ROW ? blockDim.x : 32;
+    const int lane = BLOCK_ROW ? threadIdx.x : threadIdx.x & 31;
+    const int64_t row = BLOCK_ROW ? int64_t(blockIdx.x) : int64_t(blockIdx.x) * kFp4RowWarps + (threadIdx.x >> 5);
+    if (row >= p.rows) return;
+    const int units = p.units;
+    const double inv_n = 1.0 / (double(units) * 16.0);
+    uint32_t y[U][8], res[U][8];
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+        const int at = lane + j * lanes;
+        if (at < units) {
+            load32(static_cast<const T *>(p.x) + (row * units + at) * 16, y[j]);
+            load32(static_cast<const T *>(p.residual) + (row * units + at) * 16, res[j]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) y[j][i] = res[j][i] = 0;
+        }
+    }
+    // A unit of a weight vector.
+    auto weight = [&](const void *w, int at, float2 (&v)[8]) {
+        uint32_t raw[8];
+        const uint4 *q = reinterpret_cast<const uint4 *>(static_cast<const T *>(w) + int64_t(at) * 16);
+        const uint4 a = load16_keep(q), b = load16_keep(q + 1);
+        raw[0] = a.x; raw[1] = a.y; raw[2] = a.z; raw[3] = a.w;
+        raw[4] = b.x; raw[5] = b.y; raw[6] = b.z; raw[7] = b.w;
+        unpack16<T>(raw, v);
+    };
+    auto squares = [&](const uint32_t (&raw)[8], double s) {
+        float2 v[8];
+        unpack16<T>(raw, v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            s = fma(double(v[i].x), double(v[i].x), s);
+            s = fma(double(v[i].y), double(v[i].y), s);
+        }
+        return s;
+    };
+
+    float rx = 1.f;
+    if (p.w_post) {
+        double s = 0;
+#pragma unroll
+        for (int j = 0; j < U; ++j) s = squares(y[j], s);
+        rx = inv_rms(row_sum<BLOCK_ROW>(s, sums[0]), inv_n, p.eps);
+    }
+    const int64_t gate_row = p.seqlen > 0 ? (row / p.seqlen) * units * 16 : 0;
+    double s = 0;
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+        const int at = lane + j * lanes;
+        if (at >= units) break;
+        float2 v[8], w[8], r[8];
+        unpack16<T>(y[j], v);
+        unpack16<T>(res[j], r);
+        if (p.w_post) {
+            weight(p.w_post, at, w);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = mul2(mul2(v[i], make_float2(rx, rx)), w[i]);
+        }
+        if (p.gate) {
+            weight(static_cast<const T *>(p.gate) + gate_row, at, w);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = mul2(w[i], v[i]);
+        }
+        const float2 one = make_float2(1.f, 1.f), alpha = make_float2(p.alpha, p.alpha);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[j][i] = pack2(fma2(mul2(alpha, r[i]), one, v[i]), T());
+        store32(static_cast<T *>(p.residual_out) + (row * units + at) * 16, y[j]);
+        if constexpr (OUT != kFp4None) s = squares(y[j], s);
+    }
+    if constexpr (OUT != kFp4None) {
+        const float ry = inv_rms(row_sum<BLOCK_ROW>(s, sums[1]), inv_n, p.eps);
+        auto normed = [&](int j, int at, float2 (&v)[8]) {
+            float2 w[8];
+            unpack16<T>(y[j], v);
+            weight(p.w_pre, at, w);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = mul2(mul2(v[i], make_float2(ry, ry)), w[i]);
+        };
+        uint32_t bmax[U], amax = 0;
+        float g = 1.f;
+        if constexpr (OUT == kFp4Nv) {
+#pragma unroll
+            for (int j = 0; j < U; ++j) {
+                bmax[j] = 0;
+                if (lane + j * lanes < units) {
+                    float2 v[8];
+                    normed(j, lane + j * lanes, v);
+                    bmax[j] = max_bits16(v);
+                }
+                amax = max(amax, bmax[j]);
+            }
+            g = nv_row_scale(row_max<BLOCK_ROW>(amax, maxima));
+            if (lane == 0) p.row_scale[row] = g;
+        }
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+            const int at = lane + j * lanes;
+            const bool in = at < units;
+            float2 v[8];
+            if (in) normed(j, at, v);
+            if constexpr (OUT == kFp4Plain) {
+                if (!in) break;
+                uint32_t r[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) r[i] = pack2(v[i], T());
+                store32(static_cast<T *>(p.out) + (row * units + at) * 16, r);
+            } else {
+                uint8_t *codes = static_cast<uint8_t *>(p.out) + (row * units + at) * 8;
+                if constexpr (OUT == kFp4Mx) {
+                    uint32_t m = in ? max_bits16(v) : 0;
+                    m = max(m, __shfl_xor_sync(kFull, m, 1));
+                    if (!in) continue;
+                    const uint32_t e = mx_exponent(m);
+                    *reinterpret_cast<uint2 *>(codes) = mx_codes(v, e);
+                    if ((at & 1) == 0) p.scale[scale_byte(row, at >> 1, p.tiles)] = uint8_t(e);
+                    if (at == units - 1) pad_scales(p.scale, row, units >> 1, p.tiles);
+                } else {
+                    if (!in) break;
+                    uint32_t s8;
+                    *reinterpret_cast<uint2 *>(codes) = nv_codes(v, bmax[j], g, s8);
+                    p.scale[scale_byte(row, at, p.tiles)] = uint8_t(s8);
+                    if (at == units - 1) pad_scales(p.scale, row, units, p.tiles);
+                }
+            }
+        }
+    }
+}
+
+// How a row of `units` is spread: one warp, or a block of `warps`, and the units of a lane. With few rows a row is spread over as
+// many warps as it has units for.
+struct RowSpread { int per_lane, warps; bool block_row; };
+inline RowSpread row_spread(int rows, int units) {
+    const bool few = rows < 4 * device_sm_count();
+    RowSpread s = {1, 1, false};
+    if (few && units > 32) {
+        s.block_row = true;
+        s.warps = (units + 31) / 32 < kFp4RowWarps ? (units + 31) / 32 : kFp4RowWarps;
+    } else if (units > 128) {
+        s.block_row = true;
+        s.warps = units > 512 ? 8 : units > 256 ? 4 : 2;
+    }
+    while (s.per_lane * s.warps * 32 < units) s.per_lane *= 2;
+    return s;
+}
+
+template <typename T>
+int launch_quant_nvfp4(const void *in, void *codes, void *scale, void *row_scale, int rows, int units, cudaStream_t stream) {
+    const RowSpread s = row_spread(rows, units);
+    const int block = s.block_row ? s.warps * 32 : kFp4RowWarps * 32;
+    const int grid = s.block_row ? rows : (rows + kFp4RowWarps - 1) / kFp4RowWarps;
+    using fn = void (*)(const T *, uint8_t *, uint8_t *, float *, int, int, int);
+    static constexpr fn kernels[2][3] = {{quant_nvfp4_kernel<T, 1, false>, quant_nvfp4_kernel<T, 2, false>, quant_nvfp4_kernel<T, 4, false>},
+                                         {quant_nvfp4_kernel<T, 1, true>, quant_nvfp4_kernel<T, 2, true>, quant_nvfp4_kernel<T, 4, true>}};
+    return launch_dependent(kernels[s.block_row][s.per_lane >> 1], grid, block, 0, stream, static_cast<const T *>(in), static_cast<uint8_t *>(codes),
+                            static_cast<uint8_t *>(scale), static_cast<float *>(row_scale), rows, units, (units + 3) / 4);
+}
+
+template <typename T, int OUT>
+int launch_rmsnorm_block(const RmsnormBlockDev &p, cudaStream_t stream) {
+    const RowSpread s = row_spread(p.rows, p.units);
+    const int block = s.block_row ? s.warps * 32 : kFp4RowWarps * 32;
+    const int grid = s.block_row ? p.rows : (p.rows + kFp4RowWarps - 1) / kFp4RowWarps;
+    using fn = void (*)(RmsnormBlockDev);
+    static constexpr fn kernels[2][3] = {
+        {rmsnorm_block_kernel<T, OUT, 1, false>, rmsnorm_block_kernel<T, OUT, 2, false>, rmsnorm_block_kernel<T, OUT, 4, false>},
+        {rmsnorm_block_kernel<T, OUT, 1, true>, rmsnorm_block_kernel<T, OUT, 2, true>, rmsnorm_block_kernel<T, OUT, 4, true>}};
+    return launch_dependent(kernels[s.block_row][s.per_lane >> 1], grid, block, 0, stream, p);
+}
+template <typename T>
+int launch_rmsnorm_block(const RmsnormBlockDev &p, int out, cudaStream_t stream) {
+    switch (out) {
+        case kFp4Plain: return launch_rmsnorm_block<T, kFp4Plain>(p, stream);
+        case kFp4Mx: return launch_rmsnorm_block<T, kFp4Mx>(p, stream);
+        case kFp4Nv: return launch_rmsnorm_block<T, kFp4Nv>(p, stream);
+        default: return launch_rmsnorm_block<T, kFp4None>(p, stream);
+    }
+}
+
+// Sizes and addresses that every kernel here needs: rows of whole blocks (and of whole 16-byte pieces as codes, which the
+// products ask for), 16-bit tensors on 32 bytes, codes on 16, scales on 16.
+inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+inline bool fp4_shape_ok(int rows, int cols) { return rows >= 0 && cols >= 32 && cols % 32 == 0; }
+inline int fp4_tiles(int cols, int format) { return (cols / (format == FLUKE_SM100_FP4_MX ? 32 : 16) + 3) / 4; }
+
+}  // namespace
+}  // namespace fluke_sm100
+
+using namespace fluke_sm100;
+
+extern "C" int fluke_sm100_quant_fp4(const void *in, void *codes, void *scale, void *row_scale, int rows, int cols, int format, int bf16,
+                                     void *stream) {
+    if (!fp4_shape_ok(rows, cols) || (format == FLUKE_SM100_FP4_NV && cols > FLUKE_SM100_FP4_MAX_ROW)) return (int)cudaErrorInvalidValue;
+    if (rows == 0) return 0;
+    if (!in || !codes || !scale || (format == FLUKE_SM100_FP4_NV && !row_scale)) return (int)cudaErrorInvalidValue;
+    if (!aligned32(in) || !aligned16(codes) || !aligned16(scale)) return (int)cudaErrorMisalignedAddress;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    const int units = cols / 16;
+    if (format == FLUKE_SM100_FP4_NV)
+        return bf16 ? launch_quant_nvfp4<__nv_bfloat16>(in, codes, scale, row_scale, rows, units, s)
+                    : launch_quant_nvfp4<__half>(in, codes, scale, row_scale, rows, units, s);
+    const int64_t total = int64_t(rows) * units;
+    if (format != FLUKE_SM100_FP4_MX || total > INT32_MAX) return (int)cudaErrorInvalidValue;
+    const int grid = int((total + 255) / 256), tiles = fp4_tiles(cols, format);
+    if (bf16)
+        return launch_dependent(quant_mxfp4_kernel<__nv_bfloat16>, grid, 256, 0, s, static_cast<const __nv_bfloat16 *>(in),
+                                static_cast<uint8_t *>(codes), static_cast<uint8_t *>(scale), uint32_t(total), uint32_t(units), tiles);
+    return launch_dependent(quant_mxfp4_kernel<__half>, grid, 256, 0, s, static_cast<const __half *>(in), static_cast<uint8_t *>(codes),
+                            static_cast<uint8_t *>(scale), uint32_t(total), uint32_t(units), tiles);
+}
+
+extern "C" int fluke_sm100_dequant_fp4(const void *codes, const void *scale, const void *row_scale, void *out, int rows, int cols, int format,
+                                       int bf16, void *stream) {
+    if (!fp4_shape_ok(rows, cols) || (format != FLUKE_SM100_FP4_MX && format != FLUKE_SM100_FP4_NV)) return (int)cudaErrorInvalidValue;
+    if (rows == 0) return 0;
+    if (!out || !codes || !scale || (format == FLUKE_SM100_FP4_NV && !row_scale)) return (int)cudaErrorInvalidValue;
+    if (!aligned32(out) || !aligned16(codes) || !aligned16(scale)) return (int)cudaErrorMisalignedAddress;
+    const int64_t total = int64_t(rows) * (cols / 16);
+    if (total > INT32_MAX) return (int)cudaErrorInvalidValue;
+    const bool mx = format == FLUKE_SM100_FP4_MX;
+    auto run = [&](auto *o) {
+        using T = std::remove_pointer_t<decltype(o)>;
+        return launch_dependent(mx ? dequant_fp4_kernel<T, true> : dequant_fp4_kernel<T, false>, int((total + 255) / 256), 256, 0,
+                                static_cast<cudaStream_t>(stream), static_cast<const uint8_t *>(codes), static_cast<const uint8_t *>(scale),
+                                static_cast<const float *>(row_scale), o, uint32_t(total), uint32_t(cols / 16), fp4_tiles(cols, format));
+    };
+    return bf16 ? run(static_cast<__nv_bfloat16 *>(out)) : run(static_cast<__half *>(out));
+}
+
+extern "C" int fluke_sm100_rmsnorm_block(const fluke_sm100_rmsnorm_block_t *b, void *stream) {
+    if (!b || !fp4_shape_ok(b->rows, b->cols) || b->cols > FLUKE_SM100_FP4_MAX_ROW || b->seqlen < 0) return (int)cudaErrorInvalidValue;
+    if (b->out_format < kFp4Plain || b->out_format > kFp4None) return (int)cudaErrorInvalidValue;
+    if (b->rows == 0) return 0;
+    const bool quant = b->out_format == kFp4Mx || b->out_format == kFp4Nv;
+    if (!b->x || !b->residual || !b->residual_out) return (int)cudaErrorInvalidValue;
+    if (b->out_format != kFp4None && (!b->w_pre || !b->out)) return (int)cudaErrorInvalidValue;
+    if ((quant && !b->scale) || (b->out_format == kFp4Nv && !b->row_scale)) return (int)cudaErrorInvalidValue;
+    if (!aligned32(b->x, b->residual, b->residual_out, quant ? nullptr : b->out) || (quant && !(aligned16(b->out) && aligned16(b->scale))) ||
+        !aligned16(b->w_post) || !aligned16(b->gate) || !aligned16(b->w_pre))
+        return (int)cudaErrorMisalignedAddress;
+    RmsnormBlockDev p;
+    p.x = b->x; p.residual = b->residual; p.w_post = b->w_post; p.gate = b->gate; p.w_pre = b->w_pre;
+    p.residual_out = b->residual_out; p.out = b->out;
+    p.scale = static_cast<uint8_t *>(b->scale); p.row_scale = b->row_scale;
+    p.rows = b->rows; p.units = b->cols / 16; p.seqlen = b->gate ? b->seqlen : 0;
+    p.tiles = b->out_format == kFp4Mx ? fp4_tiles(b->cols, FLUKE_SM100_FP4_MX) : fp4_tiles(b->cols, FLUKE_SM100_FP4_NV);
+    p.alpha = b->alpha; p.eps = b->eps;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    return b->bf16 ? launch_rmsnorm_block<__nv_bfloat16>(p, b->out_format, s) : launch_rmsnorm_block<__half>(p, b->out_format, s);
+}

@@ -15,6 +15,9 @@
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAFunctions.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/DynamicTypes.h>
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -30,7 +33,9 @@ namespace {
     X(fluke_silu_mul_gpu) X(fluke_flstm_step_gpu) X(fluke_qkv_rotary_i8_gpu) X(fluke_gated_mlp_i8_gpu) \
     X(fluke_qkv_rotary_fp8_gpu) X(fluke_gated_mlp_fp8_gpu) X(fluke_qkv_rotary_fp8_plain_gpu) \
     X(fluke_gated_mlp_fp8_plain_gpu) X(fluke_gemm_i8_gpu) X(fluke_gemm_fp8_gpu) X(fluke_down_proj_i8_gpu) \
-    X(fluke_down_proj_fp8_gpu) X(fluke_factored_lstm_step_i8_gpu) X(fluke_factored_lstm_step_fp8_gpu) X(fluke_last_error)
+    X(fluke_down_proj_fp8_gpu) X(fluke_factored_lstm_step_i8_gpu) X(fluke_factored_lstm_step_fp8_gpu) X(fluke_last_error) \
+    X(fluke_fp4_scale_bytes) X(fluke_quant_mxfp4_gpu) X(fluke_quant_nvfp4_gpu) X(fluke_dequant_mxfp4_gpu) X(fluke_dequant_nvfp4_gpu) \
+    X(fluke_gemm_mxfp4_gpu) X(fluke_gemm_nvfp4_gpu) X(fluke_gated_mlp_mxfp4_gpu) X(fluke_gated_mlp_nvfp4_gpu) X(fluke_rmsnorm_block_gpu)
 
 struct Entry {
 #define X(name) decltype(&::name) name = nullptr;
@@ -360,6 +365,179 @@ PyObject *lstm_step(Args a) {
     return wrap(out);
 }
 
+// ---- microscaled 4-bit floating point -------------------------------------------------------------
+
+template <typename... A>
+[[noreturn]] void refuse(const char *format, A... a) {
+    PyErr_Format(PyExc_ValueError, format, a...);
+    throw Failed();
+}
+int small(int64_t v, const char *what) {
+    if (v > INT32_MAX) refuse("fluke_b200.ops: %s of %lld", what, (long long)v);
+    return int(v);
+}
+// 0 f16, 1 bf16 (FLUKE_F16, FLUKE_BF16)
+int activation_type(at::ScalarType t) {
+    if (t != at::kHalf && t != at::kBFloat16) refuse("fluke_b200.ops: float16 or bfloat16 is needed, got %s", c10::toString(t));
+    return t == at::kBFloat16;
+}
+at::ScalarType out_type(PyObject *o) {
+    if (!THPDtype_Check(o)) {
+        PyErr_Format(PyExc_TypeError, "fluke_b200.ops: a torch.dtype is needed, got %s", Py_TYPE(o)->tp_name);
+        throw Failed();
+    }
+    const at::ScalarType t = reinterpret_cast<THPDtype *>(o)->scalar_type;
+    activation_type(t);
+    return t;
+}
+// An argument that must have this type, these sizes and `like`'s device.
+void expect(const at::Tensor &t, const char *what, at::ScalarType type, at::IntArrayRef size, const at::Tensor &like) {
+    if (t.scalar_type() != type) refuse("fluke_b200.ops: %s is %s, %s is needed", what, c10::toString(t.scalar_type()), c10::toString(type));
+    if (t.device() != like.device()) refuse("fluke_b200.ops: %s is on another device", what);
+    bool same = t.dim() == int64_t(size.size());
+    for (size_t i = 0; same && i < size.size(); ++i) same = t.size(i) == size[i];
+    if (!same) refuse("fluke_b200.ops: %s has the wrong shape", what);
+}
+// A quantised matrix: codes [rows, cols / 2], block scales, and row scales in nvfp4.
+struct Fp4 {
+    const at::Tensor &codes, &scale;
+    const at::Tensor *row;
+    int rows, cols;
+};
+Fp4 fp4_matrix(PyObject *codes, PyObject *scale, PyObject *row, bool nv, const char *what, const at::Tensor *like) {
+    const at::Tensor &c = required(codes, 2), &s = required(scale);
+    const at::Tensor *r = nv ? &required(row) : nullptr;
+    if (!nv && row != Py_None) refuse("fluke_b200.ops: %s has row scales, a has none", what);
+    const int64_t rows = c.size(0), cols = 2 * c.size(1), block = nv ? 16 : 32;
+    if (!like) like = &c;
+    expect(c, what, at::kByte, c.sizes(), *like);
+    expect(s, "a block scale", at::kByte, {(rows + 127) / 128, (cols / block + 3) / 4, 512}, *like);
+    if (nv) expect(*r, "a row scale", at::kFloat, {rows}, *like);
+    if (cols % 32 != 0 || cols == 0) refuse("fluke_b200.ops: %s has %lld columns, a multiple of 32 is needed", what, (long long)cols);
+    return {c, s, r, small(rows, "rows"), small(cols, "columns")};
+}
+at::Tensor new_scale(const at::Tensor &like, int64_t rows, int64_t cols, bool nv) {
+    return empty_on(like, {(rows + 127) / 128, (cols / (nv ? 16 : 32) + 3) / 4, 512}, at::kByte);
+}
+// The calls run on the tensors' device, whichever is current.
+template <typename F>
+int on_device(const at::Tensor &like, F f) {
+    c10::cuda::OptionalCUDAGuard guard;
+    if (like.device().index() != c10::cuda::current_device()) guard.set_device(like.device());
+    return unlocked(f);
+}
+PyObject *wrap_all(std::initializer_list<const at::Tensor *> list) {
+    Py_ssize_t n = 0;
+    for (auto t : list) n += t != nullptr;
+    PyObject *r = PyTuple_New(n);
+    Py_ssize_t i = 0;
+    for (auto t : list) {
+        if (!r || !t) continue;
+        PyObject *o = wrap(*t);
+        if (!o) {
+            Py_DECREF(r);
+            return nullptr;
+        }
+        PyTuple_SET_ITEM(r, i++, o);
+    }
+    return r;
+}
+
+// x, nv
+PyObject *quant_fp4(Args a) {
+    const at::Tensor &x = required(a[0], 2);
+    const bool nv = truth(a[1]);
+    const int type = activation_type(x.scalar_type()), m = small(x.size(0), "rows"), k = small(x.size(1), "columns");
+    if (k % 32 != 0 || k == 0) refuse("fluke_b200.ops: %d columns, a multiple of 32 is needed", k);
+    at::Tensor codes = empty_on(x, {m, k / 2}, at::kByte), scale = new_scale(x, m, k, nv), row;
+    if (nv) row = empty_on(x, {m}, at::kFloat);
+    check(on_device(x, [&] {
+              return nv ? L.fluke_quant_nvfp4_gpu(ptr(x), ptr(codes), ptr(scale), ptr(row), m, k, type)
+                        : L.fluke_quant_mxfp4_gpu(ptr(x), ptr(codes), ptr(scale), m, k, type);
+          }),
+          nv ? "fluke_quant_nvfp4_gpu" : "fluke_quant_mxfp4_gpu");
+    return wrap_all({&codes, &scale, nv ? &row : nullptr});
+}
+
+// codes, scale, row_scale or None (mxfp4), dtype
+PyObject *dequant_fp4(Args a) {
+    const bool nv = a[2] != Py_None;
+    const Fp4 q = fp4_matrix(a[0], a[1], a[2], nv, "the codes", nullptr);
+    const at::ScalarType dtype = out_type(a[3]);
+    const int type = activation_type(dtype);
+    at::Tensor out = empty_on(q.codes, {q.rows, q.cols}, dtype);
+    check(on_device(q.codes, [&] {
+              return nv ? L.fluke_dequant_nvfp4_gpu(ptr(q.codes), ptr(q.scale), ptr(q.row), ptr(out), q.rows, q.cols, type)
+                        : L.fluke_dequant_mxfp4_gpu(ptr(q.codes), ptr(q.scale), ptr(out), q.rows, q.cols, type);
+          }),
+          nv ? "fluke_dequant_nvfp4_gpu" : "fluke_dequant_mxfp4_gpu");
+    return wrap(out);
+}
+
+// a: codes, scale, row scale or None (mxfp4); b the same; up the same or three times None; dtype
+PyObject *gemm_fp4(Args v) {
+    const bool nv = v[2] != Py_None, gated = v[6] != Py_None;
+    const at::ScalarType dtype = out_type(v[9]);
+    const int type = activation_type(dtype);
+    const Fp4 a = fp4_matrix(v[0], v[1], v[2], nv, "a", nullptr), b = fp4_matrix(v[3], v[4], v[5], nv, gated ? "gate" : "b", &a.codes);
+    const Fp4 u = gated ? fp4_matrix(v[6], v[7], v[8], nv, "up", &a.codes) : b;
+    const int m = a.rows, n = b.rows, k = a.cols;
+    if (b.cols != k || u.cols != k) refuse("fluke_b200.ops: the matrices have %d, %d and %d columns", k, b.cols, u.cols);
+    if (u.rows != n) refuse("fluke_b200.ops: gate has %d rows, up %d", n, u.rows);
+    if (n % 8 != 0 || n == 0) refuse("fluke_b200.ops: a weight of %d rows, a multiple of 8 is needed", n);
+    at::Tensor out = empty_on(a.codes, {m, n}, dtype);
+    check(on_device(a.codes, [&] {
+              if (gated)
+                  return nv ? L.fluke_gated_mlp_nvfp4_gpu(ptr(out), ptr(a.codes), ptr(a.scale), ptr(a.row), ptr(b.codes), ptr(b.scale), ptr(b.row),
+                                                          ptr(u.codes), ptr(u.scale), ptr(u.row), m, n, k, type)
+                            : L.fluke_gated_mlp_mxfp4_gpu(ptr(out), ptr(a.codes), ptr(a.scale), ptr(b.codes), ptr(b.scale), ptr(u.codes),
+                                                          ptr(u.scale), m, n, k, type);
+              return nv ? L.fluke_gemm_nvfp4_gpu(ptr(out), ptr(a.codes), ptr(a.scale), ptr(a.row), ptr(b.codes), ptr(b.scale), ptr(b.row), m, n, k,
+                                                 type)
+                        : L.fluke_gemm_mxfp4_gpu(ptr(out), ptr(a.codes), ptr(a.scale), ptr(b.codes), ptr(b.scale), m, n, k, type);
+          }),
+          gated ? "fluke_gated_mlp_fp4_gpu" : "fluke_gemm_fp4_gpu");
+    return wrap(out);
+}
+
+// x, residual, post_weight, gate, pre_weight, alpha, eps, seqlen, format (0: 16 bits), residual_out or None
+PyObject *rmsnorm_block(Args a) {
+    const at::Tensor &x = required(a[0], 2), &res = required(a[1]);
+    const at::Tensor *post = input(a[2]), *gate = input(a[3]), *pre = input(a[4]);
+    const int format = pre ? integer(a[8]) : 0, m = small(x.size(0), "rows"), k = small(x.size(1), "columns"), seqlen = integer(a[7]);
+    const at::ScalarType type = x.scalar_type();
+    if (k % 32 != 0 || k == 0) refuse("fluke_b200.ops: %d columns, a multiple of 32 is needed", k);
+    if (seqlen < 0) refuse("fluke_b200.ops: a seqlen of %d", seqlen);
+    fluke_rmsnorm_block_t b = {};
+    b.dtype = activation_type(type);
+    expect(res, "residual", type, {m, k}, x);
+    if (post) expect(*post, "post_weight", type, {k}, x);
+    if (pre) expect(*pre, "pre_weight", type, {k}, x);
+    if (gate) {
+        if (seqlen > 0) expect(*gate, "gate", type, {(int64_t(m) + seqlen - 1) / seqlen, k}, x);
+        else if (gate->dim() == 1) expect(*gate, "gate", type, {k}, x);
+        else expect(*gate, "gate", type, {1, k}, x);
+    }
+    at::Tensor stream = output(a[9], x, {m, k}, type), out, scale, row;
+    if (a[9] != Py_None) {
+        required(a[9]);
+        expect(stream, "residual_out", type, {m, k}, x);
+    }
+    if (pre) out = format == 0 ? empty_on(x, {m, k}, type) : empty_on(x, {m, k / 2}, at::kByte);
+    if (format != 0) scale = new_scale(x, m, k, format == FLUKE_FP4_NV);
+    if (format == FLUKE_FP4_NV) row = empty_on(x, {m}, at::kFloat);
+    b.n_tokens = m; b.hidden_dim = k; b.seqlen = gate ? seqlen : 0;
+    b.x = ptr(x); b.residual = ptr(res); b.post_weight = ptr(post); b.gate = ptr(gate); b.pre_weight = ptr(pre);
+    b.alpha = real(a[5]); b.eps = real(a[6]);
+    b.residual_out = ptr(stream);
+    b.out_format = format;
+    if (pre) b.out = ptr(out);
+    if (format != 0) b.scale = ptr(scale);
+    if (format == FLUKE_FP4_NV) b.row_scale = ptr(row);
+    check(on_device(x, [&] { return L.fluke_rmsnorm_block_gpu(&b); }), "fluke_rmsnorm_block_gpu");
+    return wrap_all({&stream, pre ? &out : nullptr, format != 0 ? &scale : nullptr, format == FLUKE_FP4_NV ? &row : nullptr});
+}
+
 // {name: address} of the loaded library's entry points
 PyObject *bind(PyObject *, PyObject *dict) {
     Entry e;
@@ -395,7 +573,7 @@ PyMethodDef methods[] = {
     {"bind", bind, METH_O, nullptr}, {"names", names, METH_NOARGS, nullptr},
     FAST(rmsnorm, 6), FAST(rmsnorm_quant, 7), FAST(quant, 4), FAST(dequant_transpose, 3), FAST(rotary_emb, 11), FAST(rotary_qkv, 4),
     FAST(silu_mul, 1), FAST(flstm_step, 4), FAST(qkv_rotary, 11), FAST(gated_mlp, 10), FAST(gemm_i8, 5), FAST(gemm_fp8, 4),
-    FAST(down_proj, 6), FAST(lstm_step, 6), {nullptr, nullptr, 0, nullptr}};
+    FAST(down_proj, 6), FAST(lstm_step, 6), FAST(quant_fp4, 2), FAST(dequant_fp4, 4), FAST(gemm_fp4, 10), FAST(rmsnorm_block, 10), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

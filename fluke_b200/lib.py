@@ -38,6 +38,14 @@ class fluke_flstm_weights_t(ctypes.Structure):
                 ("w_up_f16", P), ("bias_f32", P), ("reverse", I)]
 
 
+class fluke_rmsnorm_block_t(ctypes.Structure):
+    _fields_ = [("n_tokens", I), ("hidden_dim", I), ("dtype", I), ("seqlen", I),
+                ("x", P), ("residual", P), ("post_weight", P), ("gate", P), ("pre_weight", P),
+                ("alpha", F), ("eps", F), ("residual_out", P), ("out_format", I), ("out", P), ("scale", P), ("row_scale", P)]
+
+
+FP4_MX, FP4_NV = 1, 2
+
 # name -> (restype, argtypes). The first ten are exactly fluke_lib._SIGNATURES of the reference.
 VOID_SIGNATURES = {
     "fluke_rotary_emb_gpu": [P, P, P, I, I, I, I, I, I, I, I],
@@ -97,6 +105,17 @@ SIGNATURES = {
     "fluke_flstm_stream_destroy": (None, [P]),
     "fluke_fp8_prepare_weight": (I, [P, I, I]),
     "fluke_fp8_release_weight": (I, [P]),
+    # microscaled 4-bit floating point
+    "fluke_fp4_scale_bytes": (Z, [I, I, I]),
+    "fluke_quant_mxfp4_gpu": (I, [P, P, P, I, I, I]),
+    "fluke_quant_nvfp4_gpu": (I, [P, P, P, P, I, I, I]),
+    "fluke_dequant_mxfp4_gpu": (I, [P, P, P, I, I, I]),
+    "fluke_dequant_nvfp4_gpu": (I, [P, P, P, P, I, I, I]),
+    "fluke_gemm_mxfp4_gpu": (I, [P] * 5 + [I] * 4),
+    "fluke_gemm_nvfp4_gpu": (I, [P] * 7 + [I] * 4),
+    "fluke_gated_mlp_mxfp4_gpu": (I, [P] * 7 + [I] * 4),
+    "fluke_gated_mlp_nvfp4_gpu": (I, [P] * 10 + [I] * 4),
+    "fluke_rmsnorm_block_gpu": (I, [ctypes.POINTER(fluke_rmsnorm_block_t)]),
     # internal status word (bounded device waits)
     "fluke_sm100_read_status": (I, [ctypes.POINTER(ctypes.c_uint), I]),
     "fluke_sm100_copy_rows_async": (I, [P, ctypes.c_size_t, P, ctypes.c_size_t, ctypes.c_size_t, ctypes.c_size_t, I, P]),

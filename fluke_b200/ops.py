@@ -161,6 +161,62 @@ def fp8_unshuffle(w_preshuffled, n, k):
     return out
 
 
+# ---- microscaled 4-bit floating point (additive) --------------------------------------------
+# A quantised matrix is (codes, scale) in mxfp4 and (codes, scale, row_scale) in nvfp4: uint8 codes
+# [rows, cols / 2], uint8 block scales [ceil(rows / 128), ceil(blocks / 4), 512] in the tiles that fluke.h
+# describes, f32 row scales [rows]. Activations are f16 or bf16. A wrong type, shape, device or
+# alignment raises; the calls run on the tensors' device.
+
+def quant_mxfp4(x):
+    """x [rows, cols] -> (codes, scale): blocks of 32 under a power of two."""
+    return _N.quant_fp4(x, False)
+
+
+def quant_nvfp4(x):
+    """x [rows, cols] -> (codes, scale, row_scale): blocks of 16 under an e4m3 scale, rows under a power of two."""
+    return _N.quant_fp4(x, True)
+
+
+def dequant_mxfp4(codes, scale, dtype=torch.float16):
+    return _N.dequant_fp4(codes, scale, None, dtype)
+
+
+def dequant_nvfp4(codes, scale, row_scale, dtype=torch.float16):
+    return _N.dequant_fp4(codes, scale, row_scale, dtype)
+
+
+def gemm_mxfp4(a, a_scale, b, b_scale, dtype=torch.float16):
+    """[M, N] = a [M, K] @ b [N, K]^T of two quantised matrices."""
+    return _N.gemm_fp4(a, a_scale, None, b, b_scale, None, None, None, None, dtype)
+
+
+def gemm_nvfp4(a, a_scale, a_row, b, b_scale, b_row, dtype=torch.float16):
+    return _N.gemm_fp4(a, a_scale, a_row, b, b_scale, b_row, None, None, None, dtype)
+
+
+def gated_mlp_mxfp4(a, a_scale, gate, gate_scale, up, up_scale, dtype=torch.float16):
+    """[M, N] = silu(a @ gate^T) * (a @ up^T), gate and up [N, K]."""
+    return _N.gemm_fp4(a, a_scale, None, gate, gate_scale, None, up, up_scale, None, dtype)
+
+
+def gated_mlp_nvfp4(a, a_scale, a_row, gate, gate_scale, gate_row, up, up_scale, up_row, dtype=torch.float16):
+    return _N.gemm_fp4(a, a_scale, a_row, gate, gate_scale, gate_row, up, up_scale, up_row, dtype)
+
+
+def rmsnorm_block(x, residual, post_weight, gate, pre_weight, alpha, eps, seqlen=0, quant=None, residual_out=None):
+    """Norms around a block: stream = alpha * residual + gate * norm(x, post_weight), then norm(stream, pre_weight)
+    for the next block, as 16-bit values (quant None) or quantised ("mxfp4", "nvfp4"). gate [cols], or
+    [ceil(rows / seqlen), cols] with seqlen > 0. post_weight, gate and pre_weight may be None. Returns the
+    stream (written to `residual_out`, which may be `residual`, or to a new tensor) followed by the
+    next block's input: (stream, out), (stream, codes, scale[, row_scale]), or (stream,) without pre_weight."""
+    if quant not in _QUANT:
+        raise ValueError(f"quant is None, 'mxfp4' or 'nvfp4', not {quant!r}")
+    return _N.rmsnorm_block(x, residual, post_weight, gate, pre_weight, alpha, eps, seqlen, _QUANT[quant], residual_out)
+
+
+_QUANT = {None: 0, "mxfp4": _lib.FP4_MX, "nvfp4": _lib.FP4_NV}
+
+
 # ---- factored LSTM (additive) ---------------------------------------------------------------
 
 def down_proj_i8(a_i8, w_i8, scale_a, scale_b, out=None):

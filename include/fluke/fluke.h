@@ -520,6 +520,85 @@ void fluke_flstm_stream_destroy(fluke_flstm_stream_t *s);
 #define FLUKE_LSTM_NOALLOC_SCRATCH_BYTES (4u << 20)
 int fluke_factored_lstm_layer_i8_noalloc_gpu(const fluke_flstm_layer_t *layer);
 
+/* ------------------------------------------------------------------------------------
+ * Part 6 -- microscaled 4-bit floating point (no counterpart in the reference): rows quantised in
+ * two formats, read back, multiplied, and the norms around a block. All return 0 or a CUDA error
+ * code (fluke_last_error() tells it in words), check sizes and alignment before they launch, and
+ * take f16 or bf16 activations by `dtype`.
+ *
+ * Elements are E2M1 codes (bit 3 the sign; 0, 0.5, 1, 1.5, 2, 3, 4, 6), two to a byte, the earlier one
+ * in the low half: [rows, cols / 2] bytes. Rounding is to nearest, ties to the even code,
+ * saturating at 6.
+ *   mxfp4  (OCP Microscaling Formats v1.0) blocks of 32 along a row under a power of two:
+ *          value = element * 2^(scale - 127), scale = clamp(floor(log2(amax)) - 2, -127, 127) + 127.
+ *   nvfp4  blocks of 16 under an e4m3 scale s, and a power of two g per row:
+ *          value = (element * s) * g, g = the least power of two with amax(row) <= 2688 g (at
+ *          least 2^-100; 1 for a row of zeros), s = e4m3(amax(block) / (6 g)),
+ *          element = e2m1(x / (s g)).
+ * A block (mxfp4) or row (nvfp4) with an infinity or a NaN reads back as NaN: its scale is 255,
+ * or 0x7F and g = NaN.
+ * `scale` holds the block scales in tiles of 128 rows x 4 blocks, 512 bytes each: tile
+ * (r / 128, c / 4), row-major over ceil(rows / 128) x ceil(blocks / 4), has block c of row r at byte
+ * (r % 32) * 16 + (r / 32 % 4) * 4 + c % 4. The quantisers write zeros for blocks behind the end of a
+ * row up to a multiple of 4 (the products read them) and leave rows behind the last as they were.
+ * cols is a multiple of 32. 16-bit tensors start on 32 bytes (weights of norms on 16), codes, scales, row
+ * scales of weights and outputs of products on 16.
+ * ---------------------------------------------------------------------------------- */
+enum { FLUKE_F16 = 0, FLUKE_BF16 = 1 };
+enum { FLUKE_FP4_MX = 1, FLUKE_FP4_NV = 2 };
+
+/* Bytes of the block scales of a [rows, cols] matrix; 0 for sizes or a format that there is not. */
+size_t fluke_fp4_scale_bytes(int rows, int cols, int format);
+
+/* in [n_tokens, hidden_dim] 16-bit -> codes, scales (and f32 [n_tokens] row scales). nvfp4: hidden_dim <= 16384. */
+int fluke_quant_mxfp4_gpu(const void *in, void *out, void *scale, int n_tokens, int hidden_dim, int dtype);
+int fluke_quant_nvfp4_gpu(const void *in, void *out, void *scale, void *row_scale, int n_tokens, int hidden_dim,
+                          int dtype);
+/* Back to 16 bits, each value rounded once. */
+int fluke_dequant_mxfp4_gpu(const void *in, const void *scale, void *out, int n_tokens, int hidden_dim, int dtype);
+int fluke_dequant_nvfp4_gpu(const void *in, const void *scale, const void *row_scale, void *out, int n_tokens,
+                            int hidden_dim, int dtype);
+
+/* out [M,N] = a [M,K] @ b [N,K]^T, f32 accumulation, rounded once. K % 32 == 0, N % 8 == 0, any M. */
+int fluke_gemm_mxfp4_gpu(void *out, const void *a, const void *a_scale, const void *b, const void *b_scale, int M, int N,
+                         int K, int dtype);
+int fluke_gemm_nvfp4_gpu(void *out, const void *a, const void *a_scale, const void *a_row, const void *b,
+                         const void *b_scale, const void *b_row, int M, int N, int K, int dtype);
+
+/* out [M,N] = silu(a @ gate^T) * (a @ up^T), gate and up [N,K]; sizes as above. */
+int fluke_gated_mlp_mxfp4_gpu(void *out, const void *a, const void *a_scale, const void *gate, const void *gate_scale,
+                              const void *up, const void *up_scale, int M, int N, int K, int dtype);
+int fluke_gated_mlp_nvfp4_gpu(void *out, const void *a, const void *a_scale, const void *a_row, const void *gate,
+                              const void *gate_scale, const void *gate_row, const void *up, const void *up_scale,
+                              const void *up_row, int M, int N, int K, int dtype);
+
+/* What lies between two blocks of a transformer whose blocks are normed on both sides: the block's
+ * output x is normalised, gated and added to the scaled residual stream, and the stream is
+ * normalised for the next block. Per row, with r(v) = 1 / sqrt(mean(v^2) + eps):
+ *     stream = alpha * residual + gate * ((x * r(x)) * post_weight)       rounded to 16 bits
+ *     out    = (stream * r(stream)) * pre_weight                          16 bits, or quantised
+ * in f32, each product and sum rounded on its own in this order; the means are taken in 64 bits, so
+ * that codes do not depend on how a row is spread over threads.
+ * post_weight NULL: x is added as it is. gate NULL: no gate. pre_weight NULL: only the stream is
+ * written (the last block). hidden_dim % 32 == 0 and <= 16384. */
+typedef struct {
+    int n_tokens, hidden_dim;
+    int dtype;                  /* of x, residual, weights, gate, residual_out and a 16-bit out     */
+    int seqlen;                 /* gate is [ceil(n_tokens / seqlen), hidden_dim]; 0: [hidden_dim]   */
+    const void *x;              /* [n_tokens, hidden_dim]                                           */
+    const void *residual;       /* [n_tokens, hidden_dim]                                           */
+    const void *post_weight;    /* [hidden_dim] or NULL                                             */
+    const void *gate;           /* or NULL                                                          */
+    const void *pre_weight;     /* [hidden_dim] or NULL                                             */
+    float alpha, eps;
+    void *residual_out;         /* [n_tokens, hidden_dim]; may be residual itself                   */
+    int out_format;             /* 0: 16 bits, FLUKE_FP4_MX, FLUKE_FP4_NV                           */
+    void *out;                  /* 16-bit values or codes                                           */
+    void *scale;                /* quantised: block scales                                          */
+    void *row_scale;            /* nvfp4: f32 [n_tokens]                                            */
+} fluke_rmsnorm_block_t;
+int fluke_rmsnorm_block_gpu(const fluke_rmsnorm_block_t *block);
+
 #endif /* HAVE_CUDA || HAVE_ROCM */
 
 #ifdef __cplusplus
