@@ -77,7 +77,8 @@ def half_step(want, dtype):
     return np.abs(want) * torch.finfo(t).eps / 2 + (2.0 ** -25 if dtype == "f16" else 0)
 
 
-PRODUCTS = [(1, 64, 64), (1, 8, 32), (5, 136, 96), (127, 128, 256), (128, 128, 512), (129, 256, 288), (300, 1536, 512), (1000, 72, 2048), (77, 264, 4128), (2, 4096, 1024)]
+PRODUCTS = [(1, 64, 64), (1, 8, 32), (5, 136, 96), (127, 128, 256), (128, 128, 512), (129, 256, 288), (300, 1536, 512), (1000, 72, 2048), (77, 264, 4128), (2, 4096, 1024),
+            (2600, 1032, 544), (2561, 1096, 2080), (10300, 200, 96)]
 
 
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
