@@ -60,13 +60,19 @@ __device__ __forceinline__ void e2m1x8_to_float(uint32_t w, float2 (&v)[4]) {
     for (int i = 0; i < 4; ++i) v[i] = half2_bits_to_float2(h[i]);
 }
 
+// max(|a|, |b|, |c|), NaN where one of them is.
+__device__ __forceinline__ float max_abs3(float a, float b, float c) {
+    float m;
+    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(a), "f"(b), "f"(c));
+    return m;
+}
 // The bit pattern of the largest magnitude of 16 values: patterns order like the values, infinities above every
 // number and NaNs above those.
 __device__ __forceinline__ uint32_t max_bits16(const float2 (&v)[8]) {
-    uint32_t m = 0;
+    float m = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m = max(m, max(__float_as_uint(v[i].x) & 0x7FFFFFFFu, __float_as_uint(v[i].y) & 0x7FFFFFFFu));
-    return m;
+    for (int i = 0; i < 8; ++i) m = max_abs3(m, v[i].x, v[i].y);
+    return __float_as_uint(m);
 }
 constexpr uint32_t kInfBits = 0x7F800000u;
 
@@ -120,26 +126,26 @@ __device__ __forceinline__ uint2 nv_codes(const float2 (&v)[8], uint32_t bmax_bi
         s8 = 0x7F;
         return make_uint2(0, 0);
     }
-    const float t = __fdiv_rn(__uint_as_float(bmax_bits), 6.0f * g);
+    // Two quotients, each correctly rounded: with the correctly rounded reciprocal of a divisor of four significant bits one exact
+    // residual is enough (every one of the 2^23 mantissas tried against all eight divisors). First bmax / (6 g), g a power of two.
+    const float b = __uint_as_float(bmax_bits) * __uint_as_float((254u << 23) - __float_as_uint(g));
+    constexpr float kSixth = 1.0f / 6.0f;
+    float t = b * kSixth;
+    t = fmaf(fmaf(-6.0f, t, b), kSixth, t);
     uint16_t pair;
     asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(pair) : "f"(0.f), "f"(t));
     s8 = pair & 0xFFu;
     if (s8 == 0) return make_uint2(0, 0);
-    const float s = e4m3_value(s8) * g;
-    // v / s, correctly rounded: s has four significant bits, and with the correctly rounded reciprocal one exact residual
-    // is enough for all of them (every one of the 2^23 mantissas tried against all eight divisors). The sign of a
-    // zero is put back.
-    const float r = __frcp_rn(s);
-    const float2 r2 = make_float2(r, r), s2 = make_float2(-s, -s);
+    // Then v / s, computed as its negative: like this a zero keeps its sign through the residual, and all signs are turned at once.
+    const float s = e4m3_value(s8) * g, r = -__frcp_rn(s);
+    const float2 r2 = make_float2(r, r), s2 = make_float2(s, s);
     float2 q[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         q[i] = mul2(v[i], r2);
         q[i] = fma2(fma2(q[i], s2, v[i]), r2, q[i]);
-        q[i].x = copysignf(q[i].x, v[i].x);
-        q[i].y = copysignf(q[i].y, v[i].y);
     }
-    return make_uint2(e2m1x8(q[0], q[1], q[2], q[3]), e2m1x8(q[4], q[5], q[6], q[7]));
+    return make_uint2(e2m1x8(q[0], q[1], q[2], q[3]) ^ 0x88888888u, e2m1x8(q[4], q[5], q[6], q[7]) ^ 0x88888888u);
 }
 
 // A unit: 16 consecutive values of a row, 32 bytes in 16 bits and 8 as codes.
@@ -230,44 +236,63 @@ __device__ __forceinline__ double row_sum(double s, double *shared) {
     return s;
 }
 
-// Quantisation, NV.
+// The units of a row that this lane holds; zeros behind the end.
+template <int U>
+__device__ __forceinline__ void load_row(const void *base, int64_t row, int units, int lane, int lanes, uint32_t (&raw)[U][8]) {
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+        if (lane + j * lanes < units) load32(static_cast<const uint8_t *>(base) + (row * units + lane + j * lanes) * 32, raw[j]);
+        else
+#pragma unroll
+            for (int i = 0; i < 8; ++i) raw[j][i] = 0;
+    }
+}
+template <int U>
+__device__ __forceinline__ void copy_row(uint32_t (&to)[U][8], const uint32_t (&from)[U][8]) {
+#pragma unroll
+    for (int j = 0; j < U; ++j)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) to[j][i] = from[j][i];
+}
+
+// Quantisation, NV. A warp works through rows with the next one on its way while it computes ([9331, 2048] bf16 19.4 -> @@ us against a warp per
+// row); a block that holds one row together does not.
 template <typename T, int U, bool BLOCK_ROW>
-__global__ void __launch_bounds__(kFp4RowWarps * 32)
+__global__ void __launch_bounds__(kFp4RowWarps * 32, U == 1 ? 4 : U == 2 ? 3 : 2)
 quant_nvfp4_kernel(const T *in, uint8_t *codes, uint8_t *scale, float *row_scale, int rows, int units, int tiles) {
     __shared__ uint32_t shared[kFp4RowWarps];
     dependency_wait();
     const int lanes = BLOCK_ROW ? blockDim.x : 32;
     const int lane = BLOCK_ROW ? threadIdx.x : threadIdx.x & 31;
-    const int64_t row = BLOCK_ROW ? int64_t(blockIdx.x) : int64_t(blockIdx.x) * kFp4RowWarps + (threadIdx.x >> 5);
+    const int step = BLOCK_ROW ? rows : int(gridDim.x) * kFp4RowWarps;
+    int row = BLOCK_ROW ? int(blockIdx.x) : int(blockIdx.x) * kFp4RowWarps + (int(threadIdx.x) >> 5);
     if (row >= rows) return;
-    uint32_t raw[U][8];
+    uint32_t raw[U][8], ahead[U][8];
+    load_row<U>(in, row, units, lane, lanes, raw);
+    for (; row < rows; row += step) {
+        if (row + step < rows) load_row<U>(in, row + step, units, lane, lanes, ahead);
+        uint32_t bmax[U], amax = 0;
 #pragma unroll
-    for (int j = 0; j < U; ++j) {
-        if (lane + j * lanes < units) load32(in + (row * units + lane + j * lanes) * 16, raw[j]);
-        else
+        for (int j = 0; j < U; ++j) {
+            float2 v[8];
+            unpack16<T>(raw[j], v);
+            bmax[j] = max_bits16(v);
+            amax = max(amax, bmax[j]);
+        }
+        const float g = nv_row_scale(row_max<BLOCK_ROW>(amax, shared));
+        if (lane == 0) row_scale[row] = g;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) raw[j][i] = 0;
-    }
-    uint32_t bmax[U], amax = 0;
-#pragma unroll
-    for (int j = 0; j < U; ++j) {
-        float2 v[8];
-        unpack16<T>(raw[j], v);
-        bmax[j] = max_bits16(v);
-        amax = max(amax, bmax[j]);
-    }
-    const float g = nv_row_scale(row_max<BLOCK_ROW>(amax, shared));
-    if (lane == 0) row_scale[row] = g;
-#pragma unroll
-    for (int j = 0; j < U; ++j) {
-        const int at = lane + j * lanes;
-        if (at >= units) break;
-        float2 v[8];
-        unpack16<T>(raw[j], v);
-        uint32_t s8;
-        *reinterpret_cast<uint2 *>(codes + (row * units + at) * 8) = nv_codes(v, bmax[j], g, s8);
-        scale[scale_byte(row, at, tiles)] = uint8_t(s8);
-        if (at == units - 1) pad_scales(scale, row, units, tiles);
+        for (int j = 0; j < U; ++j) {
+            const int at = lane + j * lanes;
+            if (at >= units) break;
+            float2 v[8];
+            unpack16<T>(raw[j], v);
+            uint32_t s8;
+            *reinterpret_cast<uint2 *>(codes + (int64_t(row) * units + at) * 8) = nv_codes(v, bmax[j], g, s8);
+            scale[scale_byte(row, at, tiles)] = uint8_t(s8);
+            if (at == units - 1) pad_scales(scale, row, units, tiles);
+        }
+        copy_row<U>(raw, ahead);
     }
 }
 
@@ -281,7 +306,9 @@ quant_nvfp4_kernel(const T *in, uint8_t *codes, uint8_t *scale, float *row_scale
 __device__ __forceinline__ float inv_rms(double sum, double inv_n, float eps) {
     const double a = fma(sum, inv_n, double(eps));
     if (!(a > 1e-37 && a < 1e38)) return float(1.0 / sqrt(a));  // no f32 holds it: rows of very large or very small bf16 values, NaN
-    const double r = double(rsqrtf(float(a)));
+    float approx;
+    asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(approx) : "f"(float(a)));
+    const double r = double(approx);
     return float(fma(r, fma(-0.5 * a * r, r, 0.5), r));
 }
 
@@ -294,138 +321,167 @@ struct RmsnormBlockDev {
     float alpha, eps;
 };
 
+// A unit of a weight vector.
+template <typename T>
+__device__ __forceinline__ void load_weight(const void *w, int64_t at, uint32_t (&raw)[8]) {
+    const uint4 *q = reinterpret_cast<const uint4 *>(static_cast<const T *>(w) + at * 16);
+    const uint4 a = load16_keep(q), b = load16_keep(q + 1);
+    raw[0] = a.x; raw[1] = a.y; raw[2] = a.z; raw[3] = a.w;
+    raw[4] = b.x; raw[5] = b.y; raw[6] = b.z; raw[7] = b.w;
+}
+// Adds the squares of a unit to four sums (one chain of 64-bit additions after the other would take longer than the loads).
+template <typename T>
+__device__ __forceinline__ void add_squares(const uint32_t (&raw)[8], double (&s)[4]) {
+    float2 v[8];
+    unpack16<T>(raw, v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        s[2 * (i & 1)] = fma(double(v[i].x), double(v[i].x), s[2 * (i & 1)]);
+        s[2 * (i & 1) + 1] = fma(double(v[i].y), double(v[i].y), s[2 * (i & 1) + 1]);
+    }
+}
+
 template <typename T, int OUT, int U, bool BLOCK_ROW>
-__global__ void __launch_bounds__(kFp4RowWarps * 32)
+__global__ void __launch_bounds__(kFp4RowWarps * 32, U == 1 ? 3 : U == 2 ? 2 : 1)
 rmsnorm_block_kernel(const RmsnormBlockDev p) {
     __shared__ double sums[2][kFp4RowWarps];
     __shared__ uint32_t maxima[kFp4RowWarps];
     dependency_wait();
     const int lanes = BLOCK_ROW ? blockDim.x : 32;
     const int lane = BLOCK_ROW ? threadIdx.x : threadIdx.x & 31;
-    const int64_t row = BLOCK_ROW ? int64_t(blockIdx.x) : int64_t(blockIdx.x) * kFp4RowWarps + (threadIdx.x >> 5);
+    const int step = BLOCK_ROW ? p.rows : int(gridDim.x) * kFp4RowWarps;
+    int row = BLOCK_ROW ? int(blockIdx.x) : int(blockIdx.x) * kFp4RowWarps + (int(threadIdx.x) >> 5);
     if (row >= p.rows) return;
     const int units = p.units;
     const double inv_n = 1.0 / (double(units) * 16.0);
-    uint32_t y[U][8], res[U][8];
-#pragma unroll
-    for (int j = 0; j < U; ++j) {
-        const int at = lane + j * lanes;
-        if (at < units) {
-            load32(static_cast<const T *>(p.x) + (row * units + at) * 16, y[j]);
-            load32(static_cast<const T *>(p.residual) + (row * units + at) * 16, res[j]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) y[j][i] = res[j][i] = 0;
-        }
+    // Weights come from L1 in front of the sums that they wait for, where registers allow it; a warp that walks rows of one unit
+    // per lane keeps those that all rows share.
+    constexpr bool kKeep = U == 1 && !BLOCK_ROW, kEarly = U <= 2;
+    uint32_t post[kEarly ? U : 1][8], gate[kEarly ? U : 1][8], pre[kEarly ? U : 1][8];
+    const int first = min(lane, units - 1);
+    if constexpr (kKeep) {
+        if (p.w_post) load_weight<T>(p.w_post, first, post[0]);
+        if (p.gate && p.seqlen == 0) load_weight<T>(p.gate, first, gate[0]);
+        if constexpr (OUT != kFp4None) load_weight<T>(p.w_pre, first, pre[0]);
     }
-    // A unit of a weight vector.
-    auto weight = [&](const void *w, int at, float2 (&v)[8]) {
-        uint32_t raw[8];
-        const uint4 *q = reinterpret_cast<const uint4 *>(static_cast<const T *>(w) + int64_t(at) * 16);
-        const uint4 a = load16_keep(q), b = load16_keep(q + 1);
-        raw[0] = a.x; raw[1] = a.y; raw[2] = a.z; raw[3] = a.w;
-        raw[4] = b.x; raw[5] = b.y; raw[6] = b.z; raw[7] = b.w;
-        unpack16<T>(raw, v);
-    };
-    auto squares = [&](const uint32_t (&raw)[8], double s) {
-        float2 v[8];
-        unpack16<T>(raw, v);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            s = fma(double(v[i].x), double(v[i].x), s);
-            s = fma(double(v[i].y), double(v[i].y), s);
+    uint32_t x[U][8], res[U][8], x_ahead[U][8], res_ahead[U][8];
+    load_row<U>(p.x, row, units, lane, lanes, x);
+    load_row<U>(p.residual, row, units, lane, lanes, res);
+    for (; row < p.rows; row += step) {
+        if (row + step < p.rows) {
+            load_row<U>(p.x, row + step, units, lane, lanes, x_ahead);
+            load_row<U>(p.residual, row + step, units, lane, lanes, res_ahead);
         }
-        return s;
-    };
-
-    float rx = 1.f;
-    if (p.w_post) {
-        double s = 0;
-#pragma unroll
-        for (int j = 0; j < U; ++j) s = squares(y[j], s);
-        rx = inv_rms(row_sum<BLOCK_ROW>(s, sums[0]), inv_n, p.eps);
-    }
-    const int64_t gate_row = p.seqlen > 0 ? (row / p.seqlen) * units * 16 : 0;
-    double s = 0;
-#pragma unroll
-    for (int j = 0; j < U; ++j) {
-        const int at = lane + j * lanes;
-        if (at >= units) break;
-        float2 v[8], w[8], r[8];
-        unpack16<T>(y[j], v);
-        unpack16<T>(res[j], r);
-        if (p.w_post) {
-            weight(p.w_post, at, w);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = mul2(mul2(v[i], make_float2(rx, rx)), w[i]);
-        }
-        if (p.gate) {
-            weight(static_cast<const T *>(p.gate) + gate_row, at, w);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = mul2(w[i], v[i]);
-        }
-        const float2 one = make_float2(1.f, 1.f), alpha = make_float2(p.alpha, p.alpha);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) y[j][i] = pack2(fma2(mul2(alpha, r[i]), one, v[i]), T());
-        store32(static_cast<T *>(p.residual_out) + (row * units + at) * 16, y[j]);
-        if constexpr (OUT != kFp4None) s = squares(y[j], s);
-    }
-    if constexpr (OUT != kFp4None) {
-        const float ry = inv_rms(row_sum<BLOCK_ROW>(s, sums[1]), inv_n, p.eps);
-        auto normed = [&](int j, int at, float2 (&v)[8]) {
-            float2 w[8];
-            unpack16<T>(y[j], v);
-            weight(p.w_pre, at, w);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = mul2(mul2(v[i], make_float2(ry, ry)), w[i]);
-        };
-        uint32_t bmax[U], amax = 0;
-        float g = 1.f;
-        if constexpr (OUT == kFp4Nv) {
+        const int64_t gate_at = p.seqlen > 0 ? int64_t(row / p.seqlen) * units : 0, row_unit = int64_t(row) * units;
+        if constexpr (kEarly)
 #pragma unroll
             for (int j = 0; j < U; ++j) {
-                bmax[j] = 0;
-                if (lane + j * lanes < units) {
-                    float2 v[8];
-                    normed(j, lane + j * lanes, v);
-                    bmax[j] = max_bits16(v);
-                }
-                amax = max(amax, bmax[j]);
+                const int at = U == 1 ? first : min(lane + j * lanes, units - 1);
+                if (!kKeep && p.w_post) load_weight<T>(p.w_post, at, post[j]);
+                if (p.gate && (!kKeep || p.seqlen > 0)) load_weight<T>(p.gate, gate_at + at, gate[j]);
             }
-            g = nv_row_scale(row_max<BLOCK_ROW>(amax, maxima));
-            if (lane == 0) p.row_scale[row] = g;
+        float rx = 1.f;
+        if (p.w_post) {
+            double s[4] = {};
+#pragma unroll
+            for (int j = 0; j < U; ++j) add_squares<T>(x[j], s);
+            rx = inv_rms(row_sum<BLOCK_ROW>((s[0] + s[1]) + (s[2] + s[3]), sums[0]), inv_n, p.eps);
         }
+        if constexpr (kEarly && !kKeep && OUT != kFp4None)
+#pragma unroll
+            for (int j = 0; j < U; ++j) load_weight<T>(p.w_pre, min(lane + j * lanes, units - 1), pre[j]);
+        double s[4] = {};
 #pragma unroll
         for (int j = 0; j < U; ++j) {
             const int at = lane + j * lanes;
-            const bool in = at < units;
-            float2 v[8];
-            if (in) normed(j, at, v);
-            if constexpr (OUT == kFp4Plain) {
-                if (!in) break;
-                uint32_t r[8];
+            if (at >= units) break;
+            float2 v[8], w[8], r[8];
+            unpack16<T>(x[j], v);
+            unpack16<T>(res[j], r);
+            if (p.w_post) {
+                if constexpr (!kEarly) load_weight<T>(p.w_post, at, post[0]);
+                unpack16<T>(post[kEarly ? j : 0], w);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) r[i] = pack2(v[i], T());
-                store32(static_cast<T *>(p.out) + (row * units + at) * 16, r);
-            } else {
-                uint8_t *codes = static_cast<uint8_t *>(p.out) + (row * units + at) * 8;
-                if constexpr (OUT == kFp4Mx) {
-                    uint32_t m = in ? max_bits16(v) : 0;
-                    m = max(m, __shfl_xor_sync(kFull, m, 1));
-                    if (!in) continue;
-                    const uint32_t e = mx_exponent(m);
-                    *reinterpret_cast<uint2 *>(codes) = mx_codes(v, e);
-                    if ((at & 1) == 0) p.scale[scale_byte(row, at >> 1, p.tiles)] = uint8_t(e);
-                    if (at == units - 1) pad_scales(p.scale, row, units >> 1, p.tiles);
-                } else {
+                for (int i = 0; i < 8; ++i) v[i] = mul2(mul2(v[i], make_float2(rx, rx)), w[i]);
+            }
+            if (p.gate) {
+                if constexpr (!kEarly) load_weight<T>(p.gate, gate_at + at, gate[0]);
+                unpack16<T>(gate[kEarly ? j : 0], w);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = mul2(w[i], v[i]);
+            }
+            const float2 one = make_float2(1.f, 1.f), alpha = make_float2(p.alpha, p.alpha);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[j][i] = pack2(fma2(mul2(alpha, r[i]), one, v[i]), T());   // the stream
+            store32(static_cast<T *>(p.residual_out) + (row_unit + at) * 16, x[j]);
+            if constexpr (OUT != kFp4None) add_squares<T>(x[j], s);
+        }
+        if constexpr (OUT != kFp4None) {
+            const float ry = inv_rms(row_sum<BLOCK_ROW>((s[0] + s[1]) + (s[2] + s[3]), sums[1]), inv_n, p.eps);
+            auto normed = [&](int j, int at, float2 (&v)[8]) {
+                float2 w[8];
+                unpack16<T>(x[j], v);
+                if constexpr (!kEarly) load_weight<T>(p.w_pre, at, pre[0]);
+                unpack16<T>(pre[kEarly ? j : 0], w);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = mul2(mul2(v[i], make_float2(ry, ry)), w[i]);
+            };
+            // one unit per lane: normed once, kept over the maximum of the row
+            float2 h[8];
+            uint32_t bmax[U], amax = 0;
+            float g = 1.f;
+            if constexpr (U == 1) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) h[i] = make_float2(0.f, 0.f);
+                if (lane < units) normed(0, lane, h);
+            }
+            if constexpr (OUT == kFp4Nv) {
+#pragma unroll
+                for (int j = 0; j < U; ++j) {
+                    bmax[j] = 0;
+                    if (lane + j * lanes < units) {
+                        if constexpr (U > 1) normed(j, lane + j * lanes, h);
+                        bmax[j] = max_bits16(h);
+                    }
+                    amax = max(amax, bmax[j]);
+                }
+                g = nv_row_scale(row_max<BLOCK_ROW>(amax, maxima));
+                if (lane == 0) p.row_scale[row] = g;
+            }
+#pragma unroll
+            for (int j = 0; j < U; ++j) {
+                const int at = lane + j * lanes;
+                const bool in = at < units;
+                if constexpr (U > 1)
+                    if (in) normed(j, at, h);
+                if constexpr (OUT == kFp4Plain) {
                     if (!in) break;
-                    uint32_t s8;
-                    *reinterpret_cast<uint2 *>(codes) = nv_codes(v, bmax[j], g, s8);
-                    p.scale[scale_byte(row, at, p.tiles)] = uint8_t(s8);
-                    if (at == units - 1) pad_scales(p.scale, row, units, p.tiles);
+                    uint32_t r[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) r[i] = pack2(h[i], T());
+                    store32(static_cast<T *>(p.out) + (row_unit + at) * 16, r);
+                } else {
+                    uint8_t *codes = static_cast<uint8_t *>(p.out) + (row_unit + at) * 8;
+                    if constexpr (OUT == kFp4Mx) {
+                        uint32_t m = in ? max_bits16(h) : 0;
+                        m = max(m, __shfl_xor_sync(kFull, m, 1));
+                        if (!in) continue;
+                        const uint32_t e = mx_exponent(m);
+                        *reinterpret_cast<uint2 *>(codes) = mx_codes(h, e);
+                        if ((at & 1) == 0) p.scale[scale_byte(row, at >> 1, p.tiles)] = uint8_t(e);
+                        if (at == units - 1) pad_scales(p.scale, row, units >> 1, p.tiles);
+                    } else {
+                        if (!in) break;
+                        uint32_t s8;
+                        *reinterpret_cast<uint2 *>(codes) = nv_codes(h, bmax[j], g, s8);
+                        p.scale[scale_byte(row, at, p.tiles)] = uint8_t(s8);
+                        if (at == units - 1) pad_scales(p.scale, row, units, p.tiles);
+                    }
                 }
             }
         }
+        copy_row<U>(x, x_ahead);
+        copy_row<U>(res, res_ahead);
     }
 }
 
@@ -446,15 +502,40 @@ inline RowSpread row_spread(int rows, int units) {
     return s;
 }
 
+// Blocks of `kernel` that the device holds at once.
+inline int resident_blocks(const void *kernel, int block) {
+    struct Seen { const void *kernel; int dev, blocks; };
+    static thread_local Seen seen[64] = {};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    Seen &s = seen[(reinterpret_cast<uintptr_t>(kernel) >> 4) & 63];
+    if (s.kernel != kernel || s.dev != dev) {
+        int per_sm = 0;
+        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, block, 0) != cudaSuccess || per_sm < 1) {
+            cudaGetLastError();
+            per_sm = 1;
+        }
+        s = {kernel, dev, per_sm * device_sm_count()};
+    }
+    return s.blocks;
+}
+// Blocks of a row kernel: one per row, or as many of eight warps as the device holds, so spread that each has as many rows as the others.
+inline int row_grid(const void *kernel, const RowSpread &s, int rows) {
+    if (s.block_row) return rows;
+    const int blocks = (rows + kFp4RowWarps - 1) / kFp4RowWarps, most = resident_blocks(kernel, kFp4RowWarps * 32);
+    const int turns = (blocks + most - 1) / most;
+    return (blocks + turns - 1) / turns;
+}
+
 template <typename T>
 int launch_quant_nvfp4(const void *in, void *codes, void *scale, void *row_scale, int rows, int units, cudaStream_t stream) {
     const RowSpread s = row_spread(rows, units);
     const int block = s.block_row ? s.warps * 32 : kFp4RowWarps * 32;
-    const int grid = s.block_row ? rows : (rows + kFp4RowWarps - 1) / kFp4RowWarps;
     using fn = void (*)(const T *, uint8_t *, uint8_t *, float *, int, int, int);
     static constexpr fn kernels[2][3] = {{quant_nvfp4_kernel<T, 1, false>, quant_nvfp4_kernel<T, 2, false>, quant_nvfp4_kernel<T, 4, false>},
                                          {quant_nvfp4_kernel<T, 1, true>, quant_nvfp4_kernel<T, 2, true>, quant_nvfp4_kernel<T, 4, true>}};
-    return launch_dependent(kernels[s.block_row][s.per_lane >> 1], grid, block, 0, stream, static_cast<const T *>(in), static_cast<uint8_t *>(codes),
+    const fn kernel = kernels[s.block_row][s.per_lane >> 1];
+    return launch_dependent(kernel, row_grid(reinterpret_cast<const void *>(kernel), s, rows), block, 0, stream, static_cast<const T *>(in), static_cast<uint8_t *>(codes),
                             static_cast<uint8_t *>(scale), static_cast<float *>(row_scale), rows, units, (units + 3) / 4);
 }
 
@@ -462,12 +543,12 @@ template <typename T, int OUT>
 int launch_rmsnorm_block(const RmsnormBlockDev &p, cudaStream_t stream) {
     const RowSpread s = row_spread(p.rows, p.units);
     const int block = s.block_row ? s.warps * 32 : kFp4RowWarps * 32;
-    const int grid = s.block_row ? p.rows : (p.rows + kFp4RowWarps - 1) / kFp4RowWarps;
     using fn = void (*)(RmsnormBlockDev);
     static constexpr fn kernels[2][3] = {
         {rmsnorm_block_kernel<T, OUT, 1, false>, rmsnorm_block_kernel<T, OUT, 2, false>, rmsnorm_block_kernel<T, OUT, 4, false>},
         {rmsnorm_block_kernel<T, OUT, 1, true>, rmsnorm_block_kernel<T, OUT, 2, true>, rmsnorm_block_kernel<T, OUT, 4, true>}};
-    return launch_dependent(kernels[s.block_row][s.per_lane >> 1], grid, block, 0, stream, p);
+    const fn kernel = kernels[s.block_row][s.per_lane >> 1];
+    return launch_dependent(kernel, row_grid(reinterpret_cast<const void *>(kernel), s, p.rows), block, 0, stream, p);
 }
 template <typename T>
 int launch_rmsnorm_block(const RmsnormBlockDev &p, int out, cudaStream_t stream) {
