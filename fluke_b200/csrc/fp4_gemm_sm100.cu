@@ -627,8 +627,9 @@ gemm_fp4_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
 // columns; only A streams. With so few instructions per tile (8 of 128 cycles at K = 512) what lies between two tiles counts: an
 // MMA chain takes some 450 cycles from its first instruction to its first result, and the hand-over of a buffer as long again. So a
 // tile is two halves of 128 columns (gated: gate and up) with a buffer each out of a ring of three (two where the scales need
-// the room), and the chain never stops. 16 epilogue warps, each 32 rows x 32 columns of a buffer.
-template <int FMT, int KMAX>   // KMAX: ring stages of K that B may have (2 or 4)
+// the room), and the chain does not stop. The issuing warp has some 1000 cycles for a tile: its loops are unrolled, and A comes in
+// slots of 512 values of K with one barrier each. 16 epilogue warps, each 32 rows x 32 columns of a buffer.
+template <int FMT, int KMAX>   // KMAX: stages of K that B may have (2 or 4)
 struct Fp4ResidentLayout {
     static constexpr int kBlock = FMT == FLUKE_SM100_FP4_MX ? 32 : 16;
     static constexpr int kAtoms = kFp4StageK / (4 * kBlock);
@@ -636,15 +637,17 @@ struct Fp4ResidentLayout {
     static constexpr int kSf = kAtoms * 512;                   // scales of 128 rows of a stage
     static constexpr bool kRoom = FMT == FLUKE_SM100_FP4_MX || KMAX == 2;
     static constexpr int kAccs = kRoom ? 3 : 2;
-    static constexpr int kStages = FMT == FLUKE_SM100_FP4_NV && KMAX == 2 ? 4 : 6;
-    static constexpr int kOffB = kStages * kOperand;
+    static constexpr int kSlots = KMAX == 2 ? 4 : 3;           // of two stages of A
+    static constexpr int kOffB = kSlots * 2 * kOperand;
     static constexpr int kOffSf = kOffB + KMAX * kOperand;
-    static constexpr int kOffSfB = kOffSf + kStages * kSf;
+    static constexpr int kOffSfB = kOffSf + kSlots * 2 * kSf;
     static constexpr int kOffStaging = kOffSfB + KMAX * 2 * kSf;
     static constexpr int kOffBars = kOffStaging + 16 * 32 * 64;
-    static constexpr int kBars = 2 * kStages + KMAX + 1 + 2 * kAccs;
+    static constexpr int kBars = 2 * kSlots + KMAX + 1 + 2 * kAccs;
     static constexpr int kDynamic = kOffBars + kBars * 8 + 16 + 1024;
-    static constexpr int kColsSfA = kAccs * 128, kColsSfB = kColsSfA + kStages * kAtoms * 4;
+    // Tensor memory: accumulators; the scales of A, of two tiles in turns (a tile begins when the buffer that the half three, or two, before its
+    // first one filled has been read, so the MMAs of the tile before the last have finished); the scales of B.
+    static constexpr int kColsSfA = kAccs * 128, kSetCols = KMAX * kAtoms * 4, kColsSfB = kColsSfA + 2 * kSetCols;
     static_assert(kOffStaging % 1024 == 0 && kDynamic <= 232448, "shared memory");
     static_assert(kColsSfB + KMAX * kAtoms * 8 <= 512, "tensor memory");
 };
@@ -658,12 +661,12 @@ gemm_fp4_resident_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_
                          const __grid_constant__ CUtensorMap tm_sfb, const __grid_constant__ CUtensorMap tm_sfb2,
                          const __grid_constant__ CUtensorMap tm_out, const Fp4PairDev p) {
     using L = Fp4ResidentLayout<FMT, KMAX>;
-    constexpr int STAGES = L::kStages, ACCS = L::kAccs, BN_OUT = GATED ? 128 : 256;
+    constexpr int SLOTS = L::kSlots, ACCS = L::kAccs, BN_OUT = GATED ? 128 : 256;
     extern __shared__ uint8_t smem_raw[];
     // both CTAs compute the same offset
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem + L::kOffBars);
-    uint64_t *full_bar = bars, *empty_bar = bars + STAGES, *bfull_bar = bars + 2 * STAGES, *bempty_bar = bfull_bar + KMAX;
+    uint64_t *full_bar = bars, *empty_bar = bars + SLOTS, *bfull_bar = bars + 2 * SLOTS, *bempty_bar = bfull_bar + KMAX;
     uint64_t *tfull_bar = bempty_bar + 1, *tempty_bar = tfull_bar + ACCS;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + L::kBars);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
@@ -671,7 +674,7 @@ gemm_fp4_resident_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_
     const int rank = int(blockIdx.x & 1);
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < STAGES; ++s) {
+        for (int s = 0; s < SLOTS; ++s) {
             mbar_init(&full_bar[s], 1);
             mbar_init(&empty_bar[s], 1);
         }
@@ -703,7 +706,7 @@ gemm_fp4_resident_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_
     PairRun run(p);
     if (warp == 0) {
         if (elect_one()) {
-            int stage = 0, cur_n = -1, loads_b = 0;
+            int slot = 0, cur_n = -1, loads_b = 0;
             uint32_t phase = 0;
             bool ok = true;
             for (; run.left > 0 && ok; run.next(p)) {
@@ -727,13 +730,17 @@ gemm_fp4_resident_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_
                         tma_load_2d_pair(ssb, &tm_sfb, bar, ks * L::kSf / 8, n0 >> 7);
                         if constexpr (GATED) tma_load_2d_pair(ssb + L::kSf, &tm_sfb2, bar, ks * L::kSf / 8, n0 >> 7);
                     }
-                    ok = mbar_wait(&empty_bar[stage], phase ^ 1u, abort_flag, 141);
-                    if (!ok) break;
-                    const uint32_t bar = cluster_address(smem_u32(&full_bar[stage]), 0);
-                    if (rank == 0) mbar_arrive_expect_tx(&full_bar[stage], 2 * (L::kOperand + L::kSf));
-                    tma_load_2d_pair(smem + stage * L::kOperand, &tm_a, bar, ks * 128, m0);
-                    tma_load_2d_pair(smem + L::kOffSf + stage * L::kSf, &tm_sfa, bar, ks * L::kSf / 8, m0 >> 7);
-                    if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+                    const int part = ks & 1;
+                    if (part == 0) {
+                        ok = mbar_wait(&empty_bar[slot], phase ^ 1u, abort_flag, 141);
+                        if (!ok) break;
+                        if (rank == 0) mbar_arrive_expect_tx(&full_bar[slot], (ks + 1 < p.stages_k ? 4 : 2) * (L::kOperand + L::kSf));
+                    }
+                    const uint32_t bar = cluster_address(smem_u32(&full_bar[slot]), 0);
+                    tma_load_2d_pair(smem + (2 * slot + part) * L::kOperand, &tm_a, bar, ks * 128, m0);
+                    tma_load_2d_pair(smem + L::kOffSf + (2 * slot + part) * L::kSf, &tm_sfa, bar, ks * L::kSf / 8, m0 >> 7);
+                    if (part == 1 || ks + 1 == p.stages_k)
+                        if (++slot == SLOTS) { slot = 0; phase ^= 1u; }
                 }
             }
             if (!ok) {
@@ -746,62 +753,74 @@ gemm_fp4_resident_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_
     } else if (warp == 1) {
         if (rank == 0) {
             const bool leader = elect_one();
-            int stage0 = 0, cur_n = -1, loads_b = 0, acc = 0;
-            uint32_t phase0 = 0, t_phase = 0;   // of the tile's first stage; of the buffers
+            int slot = 0, cur_n = -1, acc = 0;
+            uint32_t phase = 0, t_phase = 0, b_phase = 1, set = 0;   // of the slots, the buffers, the rows of B; scales of A
             bool ok = true;
             const uint32_t a_lo0 = desc_lo(smem_u32(smem)), b_lo0 = desc_lo(smem_u32(smem) + L::kOffB);
             const uint32_t sa_lo0 = desc_lo(smem_u32(smem) + L::kOffSf), sb_lo0 = desc_lo(smem_u32(smem) + L::kOffSfB);
+            const int mmas = (p.stages_k - 1) * 4 + p.last_steps, stages_k = p.stages_k;
             for (; run.left > 0 && ok; run.next(p)) {
-                const int n = run.n;
-                const bool first_of_n = n != cur_n;
+                const bool first_of_n = run.n != cur_n;
                 if (first_of_n) {
-                    cur_n = n;
-                    ++loads_b;
+                    cur_n = run.n;
+                    b_phase ^= 1u;
                 }
-                for (int half = 0; half < 2 && ok; ++half) {
-                    ok = mbar_wait_warp(&tempty_bar[acc], t_phase ^ 1u, abort_flag, 142);
+                const uint32_t tsa = tmem + L::kColsSfA + set;
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    ok = ok && mbar_wait_warp(&tempty_bar[acc], t_phase ^ 1u, abort_flag, 142);
                     if (!ok) break;
                     tc_fence_after_sync();
-                    int stage = stage0;
-                    uint32_t phase = phase0;
-                    for (int ks = 0; ks < p.stages_k; ++ks) {
-                        const uint32_t tsa = tmem + L::kColsSfA + stage * L::kAtoms * 4, tsb = tmem + L::kColsSfB + ks * L::kAtoms * 8 + half * L::kAtoms * 4;
+                    const uint32_t d = tmem + acc * 128;
+                    int sl = slot;
+                    uint32_t sl_phase = phase;
+#pragma unroll
+                    for (int pair = 0; pair < KMAX / 2; ++pair) {
+                        if (2 * pair >= stages_k) break;
+                        const uint32_t a_lo = a_lo0 + sl * (2 * L::kOperand >> 4), sa_lo = sa_lo0 + sl * (2 * L::kSf >> 4);
                         if (half == 0) {
-                            if (first_of_n) ok = mbar_wait_warp(&bfull_bar[ks], (loads_b - 1) & 1, abort_flag, 143);
-                            ok = ok && mbar_wait_warp(&full_bar[stage], phase, abort_flag, 144);
+                            if (first_of_n) {
+                                ok = mbar_wait_warp(&bfull_bar[2 * pair], b_phase, abort_flag, 143);
+                                if (2 * pair + 1 < stages_k) ok = ok && mbar_wait_warp(&bfull_bar[2 * pair + 1], b_phase, abort_flag, 143);
+                            }
+                            ok = ok && mbar_wait_warp(&full_bar[sl], sl_phase, abort_flag, 144);
                             if (!ok) break;
                             tc_fence_after_sync();
                             if (leader) {
 #pragma unroll
-                                for (int i = 0; i < L::kAtoms; ++i) tc_copy_scales<2>(tsa + i * 4, sa_lo0 + stage * (L::kSf >> 4) + i * 32);
+                                for (int i = 0; i < 2 * L::kAtoms; ++i)
+                                    if (2 * pair + i / L::kAtoms < stages_k) tc_copy_scales<2>(tsa + (2 * pair * L::kAtoms + i) * 4, sa_lo + i * 32);
                                 if (first_of_n)
 #pragma unroll
-                                    for (int i = 0; i < 2 * L::kAtoms; ++i) tc_copy_scales<2>(tsb + i * 4, sb_lo0 + ks * (2 * L::kSf >> 4) + i * 32);
+                                    for (int i = 0; i < 4 * L::kAtoms; ++i)
+                                        if (2 * pair + i / (2 * L::kAtoms) < stages_k)
+                                            tc_copy_scales<2>(tmem + L::kColsSfB + (4 * pair * L::kAtoms + i) * 4, sb_lo0 + (4 * pair * L::kAtoms + i) * 32);
                             }
                         }
-                        const uint32_t a_lo = a_lo0 + stage * (L::kOperand >> 4), b_lo = b_lo0 + ks * (L::kOperand >> 4) + half * (L::kOperand >> 5);
-                        const int steps = ks == p.stages_k - 1 ? p.last_steps : 4;
                         if (leader) {
 #pragma unroll
-                            for (int k = 0; k < 4; ++k) {
+                            for (int i = 0; i < 8; ++i) {
                                 constexpr bool mx = FMT == FLUKE_SM100_FP4_MX;
-                                const int atom = mx ? k / 2 : k, part = mx ? (k & 1) * 2 : 0;
-                                if (k < steps)
-                                    tc_mma_fp4<FMT, 2>(tmem + acc * 128, a_lo + 2 * k, b_lo + 2 * k, make_idesc_fp4<FMT>(256, 128, part),
-                                                         tsa + atom * 4, tsb + atom * 4, (ks | k) != 0);
+                                const int ks = 2 * pair + i / 4, k = i % 4, atom = mx ? k / 2 : k, part = mx ? (k & 1) * 2 : 0;
+                                if (8 * pair + i < mmas)
+                                    tc_mma_fp4<FMT, 2>(d, a_lo + (i / 4) * (L::kOperand >> 4) + 2 * k,
+                                                       b_lo0 + ks * (L::kOperand >> 4) + half * (L::kOperand >> 5) + 2 * k,
+                                                       make_idesc_fp4<FMT>(256, 128, part), tsa + (ks * L::kAtoms + atom) * 4,
+                                                       tmem + L::kColsSfB + (ks * 2 * L::kAtoms + half * L::kAtoms + atom) * 4, (pair | i) != 0);
                             }
-                            if (half == 1) tc_commit_pair(&empty_bar[stage]);
-                            if (ks == p.stages_k - 1) tc_commit_pair(&tfull_bar[acc]);
+                            if (half == 1) tc_commit_pair(&empty_bar[sl]);
                         }
-                        if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+                        if (++sl == SLOTS) { sl = 0; sl_phase ^= 1u; }
                     }
                     if (!ok) break;
+                    if (leader) tc_commit_pair(&tfull_bar[acc]);
                     if (++acc == ACCS) { acc = 0; t_phase ^= 1u; }
                     if (half == 1) {
-                        stage0 = stage;
-                        phase0 = phase;
+                        slot = sl;
+                        phase = sl_phase;
                     }
                 }
+                set ^= L::kSetCols;
                 if (ok && leader && run.left > 1 && run.last_of_n(p)) tc_commit_pair(bempty_bar);
             }
         }
@@ -897,7 +916,7 @@ int launch_dependent_clusters(void (*kernel)(P...), int cluster, dim3 grid, int 
     attr[1].val.clusterDim.y = 1;
     attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 2;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
     const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
     if (e != cudaSuccess) cudaGetLastError();
     return (int)e;
@@ -1001,13 +1020,21 @@ int gemm_fp4_split_launch(const fluke_sm100_gemm_fp4_t *g, cudaStream_t stream) 
     p.a_rows = rows;
     const int64_t tiles = tiles_of(rows);
     if (tiles > (INT32_MAX >> 3) - 1024) return (int)cudaErrorInvalidValue;
-    // as many CTAs per tile as fill the device, each with a stage of K at least
-    int split = int(sms / tiles);
-    if (split > 8) split = 8;
-    if (split > p.stages_k) split = p.stages_k;
-    if (split < 1) split = 1;
-    const int each = (p.stages_k + split - 1) / split;
-    p.split = split = (p.stages_k + each - 1) / each;
+    // CTAs per tile, while they fill the device and each has a stage of K at least: the number with the shortest time by what a stage takes
+    // (0.2 us, 0.35 with two weights) and what a hand-over of the tile's rows does (0.6 us and 18 ns per row). Us per call, 1 : 2 : 4 CTAs per
+    // tile: [1, 4096] x [4096, 4096] 6.6 : 5.1 : 4.5, [333, 2048] x [2048, 512] (24 tiles of 64 rows) 5.1 : 5.7 : 5.6.
+    const int most = g->M < rows ? g->M : rows;
+    int each = p.stages_k;
+    float best = 0.f;
+    for (int c = 1; c <= 8 && c <= p.stages_k && (c == 1 || tiles * c <= sms); ++c) {
+        const int n = (p.stages_k + c - 1) / c;
+        const float us = n * (GATED ? 0.35f : 0.2f) + (c > 1 ? 0.6f + 0.018f * most : 0.f);
+        if (c == 1 || us < best) {
+            best = us;
+            each = n;
+        }
+    }
+    const int split = p.split = (p.stages_k + each - 1) / each;
     p.acc_cols = rows < 32 ? 32 : rows;
     const int stage_bytes = p.a_rows * 128 + kWeights * 128 * 128 + kSf * (kWeights + 1);
     // A longer run of K than that holds streams through a deeper ring: [5, 4096] gated with [8192, 4096] twice 10.2 us at 104 KB, 8.2 at 150.
@@ -1017,7 +1044,7 @@ int gemm_fp4_split_launch(const fluke_sm100_gemm_fp4_t *g, cudaStream_t stream) 
     if (p.stages > scale_stages) p.stages = scale_stages;
     if (p.stages > each) p.stages = each;
     // the sums, and with a split what is received (of one share from every rank) in front of them
-    const int most = g->M < rows ? g->M : rows, sums = kWeights * rows * kFp4SumPitch * 4;
+    const int sums = kWeights * rows * kFp4SumPitch * 4;
     p.sums_at = split > 1 ? (split * kWeights * ((most + split - 1) / split) * kFp4SumPitch * 4 + 1023) / 1024 * 1024 : 0;
     int smem = p.stages * stage_bytes;
     if (smem < p.sums_at + sums) smem = p.sums_at + sums;
