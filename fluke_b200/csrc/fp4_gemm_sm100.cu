@@ -58,6 +58,14 @@ __device__ __forceinline__ void tc_copy_scales(uint32_t taddr, uint32_t lo) {
         asm volatile("{\n.reg .b64 D;\nmov.b64 D, {%1, %2};\ntcgen05.cp.cta_group::2.32x128b.warpx4 [%0], D;\n}\n"
                      ::"r"(taddr), "r"(lo), "r"(kDescHiScales) : "memory");
 }
+// Whether the phase has completed, without waiting.
+__device__ __forceinline__ bool mbar_test(uint64_t *bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile(
+        "{\n.reg .pred P;\nmbarrier.test_wait.parity.shared::cta.b64 P, [%1], %2;\nselp.u32 %0, 1, 0, P;\n}\n"
+        : "=r"(done) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+    return done != 0;
+}
 // mbar_wait() of a whole warp, with the same answer for every lane.
 __device__ __forceinline__ bool mbar_wait_warp(uint64_t *bar, uint32_t parity, volatile int *abort_flag, unsigned int site) {
     return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, site));
@@ -496,16 +504,19 @@ gemm_fp4_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
             const bool leader = elect_one();
             int stage = 0;
             uint32_t phase = 0, t_phase = 0;
-            bool ok = true;
+            bool ok = true, ready = false;
             const uint32_t base_lo = desc_lo(smem_u32(smem)), sf_lo = desc_lo(smem_u32(smem) + L::kOffSf);
             for (; run.left > 0 && ok; run.next(p), t_phase ^= 1u) {
                 ok = mbar_wait_warp(tempty_bar, t_phase ^ 1u, abort_flag, 132);
                 if (!ok) break;
                 tc_fence_after_sync();
                 for (int ks = 0; ks < p.stages_k; ++ks) {
-                    ok = mbar_wait_warp(&full_bar[stage], phase, abort_flag, 134);
+                    if (!ready) ok = mbar_wait_warp(&full_bar[stage], phase, abort_flag, 134);
                     if (!ok) break;
                     tc_fence_after_sync();
+                    // The next stage is asked about here and the answer is looked at behind this stage's MMAs.
+                    const bool wraps = stage + 1 == STAGES;
+                    const bool next = mbar_test(&full_bar[wraps ? 0 : stage + 1], wraps ? phase ^ 1u : phase);
                     const uint32_t a_lo = base_lo + stage * (L::kSlot >> 4), s_lo = sf_lo + stage * (L::kSfSlot >> 4);
                     const uint32_t tsa = tmem + 256 + stage * L::kAtoms * 4, tsb = tmem + L::kColsSfB + stage * L::kAtoms * 8;
                     const int steps = ks == p.stages_k - 1 ? p.last_steps : 4;
@@ -527,7 +538,9 @@ gemm_fp4_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
                         tc_commit_pair(&empty_bar[stage]);
                         if (ks == p.stages_k - 1) tc_commit_pair(tfull_bar);
                     }
-                    if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+                    ready = __all_sync(0xffffffffu, next);
+                    stage = wraps ? 0 : stage + 1;
+                    phase ^= wraps;
                 }
             }
         }
@@ -922,24 +935,26 @@ int launch_dependent_clusters(void (*kernel)(P...), int cluster, dim3 grid, int 
     return (int)e;
 }
 
-// Pairs of KERNEL that run at once on the current device; 0 where they cannot.
+// Clusters of `size` CTAs of KERNEL that run at once with `smem` bytes each; 0 where they cannot. A GPC's SMs bound it as well as
+// their number: 16 clusters of 8 CTAs, one per SM, ran in two rounds.
 template <auto KERNEL>
-int pair_capacity(int threads, int smem) {
-    static int cached[64] = {0};
+int cluster_capacity(int size, int threads, int smem) {
+    static int cached[64][9] = {{0}};
     int dev = 0;
     cudaGetDevice(&dev);
     if (dev < 0 || dev >= 64) dev = 0;
-    if (!cached[dev]) {
+    int &slot = cached[dev][size];
+    if (!slot) {
         int n = 0;
         bool ok = configure_smem<KERNEL>(smem) == 0;
         if (ok) {
             cudaLaunchConfig_t cfg = {};
-            cfg.gridDim = dim3(2);
+            cfg.gridDim = dim3(size);
             cfg.blockDim = dim3(threads);
             cfg.dynamicSmemBytes = smem;
             cudaLaunchAttribute attr[1];
             attr[0].id = cudaLaunchAttributeClusterDimension;
-            attr[0].val.clusterDim.x = 2;
+            attr[0].val.clusterDim.x = size;
             attr[0].val.clusterDim.y = 1;
             attr[0].val.clusterDim.z = 1;
             cfg.attrs = attr;
@@ -947,9 +962,9 @@ int pair_capacity(int threads, int smem) {
             ok = cudaOccupancyMaxActiveClusters(&n, reinterpret_cast<const void *>(KERNEL), &cfg) == cudaSuccess && n > 0;
         }
         cudaGetLastError();
-        cached[dev] = ok ? n + 1 : 1;
+        slot = ok ? n + 1 : 1;
     }
-    return cached[dev] - 1;
+    return slot - 1;
 }
 
 // KMAX: 0 streams B, else the resident form with that many stages.
@@ -962,7 +977,7 @@ int gemm_fp4_pair_launch(const fluke_sm100_gemm_fp4_t *g, cudaStream_t stream) {
         if constexpr (KMAX == 0) return gemm_fp4_pair_kernel<FMT, GATED, T>;
         else return gemm_fp4_resident_kernel<FMT, GATED, KMAX, T>;
     }();
-    const int capacity = pair_capacity<kernel>(kThreads, kSmem);
+    const int capacity = cluster_capacity<kernel>(2, kThreads, kSmem);
     if (capacity < 1) return (int)cudaErrorNotSupported;
     Fp4PairDev p;
     p.M = g->M; p.N = g->N; p.K = g->K;
@@ -998,9 +1013,23 @@ int gemm_fp4_pair_launch(const fluke_sm100_gemm_fp4_t *g, cudaStream_t stream) {
     return launch_dependent_clusters(kernel, 2, pairs * 2, kThreads, kSmem, stream, tm_a, tm_b, tm_b2, tm_sfa, tm_sfb, tm_sfb2, tm_out, p);
 }
 
+// Rows of a per tile of the split form: 64 while those tiles are all resident at once, else 128 (plain form; the gated one keeps to
+// 64); what there is of them, if less.
+template <bool GATED>
+int split_rows(const fluke_sm100_gemm_fp4_t *g) {
+    if (g->M <= 32) return g->M <= 16 ? 16 : 32;
+    return GATED || int64_t((g->M + 63) / 64) * ((g->N + 127) / 128) <= device_sm_count() ? 64 : 128;
+}
+template <bool GATED>
+int64_t split_tiles(const fluke_sm100_gemm_fp4_t *g) {
+    const int rows = split_rows<GATED>(g);
+    return int64_t((g->M + rows - 1) / rows) * ((g->N + 127) / 128);
+}
+
 template <int FMT, bool GATED, typename T>
 int gemm_fp4_split_launch(const fluke_sm100_gemm_fp4_t *g, cudaStream_t stream) {
     constexpr int kAtoms = kFp4StageK / (4 * (FMT == FLUKE_SM100_FP4_MX ? 32 : 16)), kSf = kAtoms * 512, kWeights = GATED ? 2 : 1;
+    constexpr auto kernel = gemm_fp4_split_kernel<FMT, GATED, T>;
     Fp4SplitDev p;
     p.M = g->M; p.N = g->N; p.K = g->K;
     p.n_tiles = (g->N + 127) / 128;
@@ -1012,33 +1041,28 @@ int gemm_fp4_split_launch(const fluke_sm100_gemm_fp4_t *g, cudaStream_t stream) 
     p.sfb2 = static_cast<const uint8_t *>(g->b2_scale);
     p.ga = g->a_row; p.gb = g->b_row; p.gb2 = g->b2_row;
     p.out = g->out;
-    // Rows of a per tile: 128 where that leaves tiles for all SMs, else 64 (a hand-over of fewer rows is cheaper, and smaller tiles keep
-    // the SMs busy without one); what there is of them, if less.
-    const int sms = device_sm_count();
-    auto tiles_of = [&](int r) { return int64_t((g->M + r - 1) / r) * p.n_tiles; };
-    const int rows = g->M <= 16 ? 16 : g->M <= 32 ? 32 : !GATED && tiles_of(128) >= sms ? 128 : 64;
-    p.a_rows = rows;
-    const int64_t tiles = tiles_of(rows);
+    const int rows = p.a_rows = split_rows<GATED>(g), sms = device_sm_count();
+    const int64_t tiles = split_tiles<GATED>(g);
     if (tiles > (INT32_MAX >> 3) - 1024) return (int)cudaErrorInvalidValue;
-    // CTAs per tile, while they fill the device and each has a stage of K at least: the number with the shortest time by what a stage takes
-    // (0.2 us, 0.35 with two weights) and what a hand-over of the tile's rows does (0.6 us and 18 ns per row). Us per call, 1 : 2 : 4 CTAs per
-    // tile: [1, 4096] x [4096, 4096] 6.6 : 5.1 : 4.5, [333, 2048] x [2048, 512] (24 tiles of 64 rows) 5.1 : 5.7 : 5.6.
+    // CTAs per tile, while all of them run at once and each has a stage of K at least: the number with the shortest time by what a stage takes
+    // (0.2 us, 0.35 with two weights) and what a hand-over of the tile's rows does (0.6 us, and 18 ns per row and weight). Us per call, 1 : 2 : 4
+    // CTAs per tile: [1, 4096] x [4096, 4096] 6.6 : 5.1 : 4.5, [333, 2048] x [2048, 512] (24 tiles of 64 rows) 5.1 : 5.7 : 5.6.
     const int most = g->M < rows ? g->M : rows;
     int each = p.stages_k;
     float best = 0.f;
     for (int c = 1; c <= 8 && c <= p.stages_k && (c == 1 || tiles * c <= sms); ++c) {
         const int n = (p.stages_k + c - 1) / c;
-        const float us = n * (GATED ? 0.35f : 0.2f) + (c > 1 ? 0.6f + 0.018f * most : 0.f);
-        if (c == 1 || us < best) {
-            best = us;
-            each = n;
-        }
+        const float us = n * (GATED ? 0.35f : 0.2f) + (c > 1 ? 0.6f + 0.018f * kWeights * most : 0.f);
+        if (c > 1 && (us >= best || tiles > cluster_capacity<kernel>(c, kFp4Threads, kFp4SplitMaxSmem + 1024))) continue;
+        best = us;
+        each = n;
     }
     const int split = p.split = (p.stages_k + each - 1) / each;
     p.acc_cols = rows < 32 ? 32 : rows;
     const int stage_bytes = p.a_rows * 128 + kWeights * 128 * 128 + kSf * (kWeights + 1);
-    // A longer run of K than that holds streams through a deeper ring: [5, 4096] gated with [8192, 4096] twice 10.2 us at 104 KB, 8.2 at 150.
-    p.stages = (each * stage_bytes > kFp4SplitSmem ? kFp4SplitDeep : kFp4SplitSmem) / stage_bytes;
+    // A longer run of K than the ring holds streams through a deeper one, where an SM has no second CTA to run: [5, 4096] gated with
+    // [8192, 4096] twice 10.2 us at 104 KB, 8.2 at 150.
+    p.stages = (each * stage_bytes > kFp4SplitSmem && tiles * split <= sms ? kFp4SplitDeep : kFp4SplitSmem) / stage_bytes;
     const int scale_stages = (kFp4SplitCols - kWeights * p.acc_cols) / (kAtoms * 4 * (kWeights + 1));   // what tensor memory holds
     if (p.stages > kFp4SplitStages) p.stages = kFp4SplitStages;
     if (p.stages > scale_stages) p.stages = scale_stages;
@@ -1056,26 +1080,25 @@ int gemm_fp4_split_launch(const fluke_sm100_gemm_fp4_t *g, cudaStream_t stream) 
     if (!rc) rc = make_tmap_2d(&tm_b, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, g->b, g->N, pitch, pitch, 128, 128, true);
     tm_b2 = tm_b;
     if (GATED && !rc) rc = make_tmap_2d(&tm_b2, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, g->b2, g->N, pitch, pitch, 128, 128, true);
-    if (!rc) rc = configure_smem<gemm_fp4_split_kernel<FMT, GATED, T>>(kFp4SplitMaxSmem + 1024);
+    if (!rc) rc = configure_smem<kernel>(kFp4SplitMaxSmem + 1024);
     if (rc) return rc;
-    return launch_dependent_clusters(gemm_fp4_split_kernel<FMT, GATED, T>, split, dim3(int(tiles) * split), kFp4Threads, smem + 1024, stream, tm_a,
+    return launch_dependent_clusters(kernel, split, dim3(int(tiles) * split), kFp4Threads, smem + 1024, stream, tm_a,
                                      tm_b, tm_b2, p);
 }
 
+// The split form for few rows and for products whose tiles it holds all at once, pairs of SMs for the others. MX, us per call, pairs : split:
+// plain, N = 2048: 512 rows K = 512 5.2 : 4.0, K = 2048 7.1 : 5.7, 3000 rows 7.5 : 10.6, 11.4 : 19.1; gated, N = 2048, 256 rows (64 tiles) K = 1024 6.2 :
+// 5.6, 512 rows (128) K = 512 5.5 : 6.1, K = 2048 7.1 : 7.4.
+template <int FMT, bool GATED, typename T>
+int gemm_fp4_dispatch(const fluke_sm100_gemm_fp4_t *g, cudaStream_t stream) {
+    if (g->M <= 64 || split_tiles<GATED>(g) <= (GATED ? 100 : device_sm_count())) return gemm_fp4_split_launch<FMT, GATED, T>(g, stream);
+    if (g->K <= 512) return gemm_fp4_pair_launch<FMT, GATED, 2, T>(g, stream);
+    if (g->K <= 1024) return gemm_fp4_pair_launch<FMT, GATED, 4, T>(g, stream);
+    return gemm_fp4_pair_launch<FMT, GATED, 0, T>(g, stream);
+}
 template <int FMT, typename T>
 int gemm_fp4_dispatch(const fluke_sm100_gemm_fp4_t *g, cudaStream_t stream) {
-    const int64_t pairs = int64_t((g->M + 255) / 256) * ((g->N + (g->b2 ? 127 : 255)) / (g->b2 ? 128 : 256));
-    if (pairs >= 40 && g->M > 128) {
-        const int kmax = g->K <= 512 ? 2 : g->K <= 1024 ? 4 : 0;
-        if (g->b2)
-            return kmax == 2   ? gemm_fp4_pair_launch<FMT, true, 2, T>(g, stream)
-                   : kmax == 4 ? gemm_fp4_pair_launch<FMT, true, 4, T>(g, stream)
-                               : gemm_fp4_pair_launch<FMT, true, 0, T>(g, stream);
-        return kmax == 2   ? gemm_fp4_pair_launch<FMT, false, 2, T>(g, stream)
-               : kmax == 4 ? gemm_fp4_pair_launch<FMT, false, 4, T>(g, stream)
-                           : gemm_fp4_pair_launch<FMT, false, 0, T>(g, stream);
-    }
-    return g->b2 ? gemm_fp4_split_launch<FMT, true, T>(g, stream) : gemm_fp4_split_launch<FMT, false, T>(g, stream);
+    return g->b2 ? gemm_fp4_dispatch<FMT, true, T>(g, stream) : gemm_fp4_dispatch<FMT, false, T>(g, stream);
 }
 
 }  // namespace
