@@ -208,7 +208,7 @@ dequant_fp4_kernel(const uint8_t *codes, const uint8_t *scale, const float *row_
 // ---- rows held in registers -------------------------------------------------------------------
 // A row belongs to one warp (8 rows to a block) or to one whole block of up to 8 warps; lane l of the row's
 // `lanes` holds units l, l + lanes, ... (U of them).
-constexpr int kFp4RowWarps = 8;
+constexpr int kFp4RowWarps = 8, kFp4NormWarps = 4;   // of a block: at most; of the norms that walk rows
 
 template <bool BLOCK_ROW>
 __device__ __forceinline__ uint32_t row_max(uint32_t m, uint32_t *shared) {
@@ -343,15 +343,15 @@ __device__ __forceinline__ void add_squares(const uint32_t (&raw)[8], double (&s
 
 // FULL: rows of exactly U units per lane of a warp ([32000, 512] 28.3 us without, 25.6 with: no lane has to ask for its end).
 template <typename T, int OUT, int U, bool BLOCK_ROW, bool FULL>
-__global__ void __launch_bounds__(kFp4RowWarps * 32, U == 1 ? 3 : U == 2 ? 2 : 1)
+__global__ void __launch_bounds__(BLOCK_ROW ? kFp4RowWarps * 32 : kFp4NormWarps * 32, BLOCK_ROW ? (U <= 2 ? 2 : 1) : U == 1 ? 5 : U == 2 ? 4 : 2)
 rmsnorm_block_kernel(const RmsnormBlockDev p) {
     __shared__ double sums[2][kFp4RowWarps];
     __shared__ uint32_t maxima[kFp4RowWarps];
     dependency_wait();
     const int lanes = BLOCK_ROW ? blockDim.x : 32;
     const int lane = BLOCK_ROW ? threadIdx.x : threadIdx.x & 31;
-    const int step = BLOCK_ROW ? p.rows : int(gridDim.x) * kFp4RowWarps;
-    int row = BLOCK_ROW ? int(blockIdx.x) : int(blockIdx.x) * kFp4RowWarps + (int(threadIdx.x) >> 5);
+    const int step = BLOCK_ROW ? p.rows : int(gridDim.x) * kFp4NormWarps;
+    int row = BLOCK_ROW ? int(blockIdx.x) : int(blockIdx.x) * kFp4NormWarps + (int(threadIdx.x) >> 5);
     if (row >= p.rows) return;
     const int units = FULL ? 32 * U : p.units;
     const double inv_n = 1.0 / (double(units) * 16.0), eps = double(p.eps);
@@ -359,12 +359,23 @@ rmsnorm_block_kernel(const RmsnormBlockDev p) {
     // per lane keeps those that all rows share.
     constexpr bool kKeep = U == 1 && !BLOCK_ROW, kEarly = U <= 2;
     uint32_t post[kEarly ? U : 1][8], gate[kEarly ? U : 1][8], pre[kEarly ? U : 1][8];
+    float2 post_kept[kKeep ? 8 : 1], gate_kept[kKeep ? 8 : 1], pre_kept[kKeep ? 8 : 1];
     const int first = FULL ? lane : min(lane, units - 1);
     if constexpr (kKeep) {
-        if (p.w_post) load_weight<T>(p.w_post, first, post[0]);
-        if (p.gate && p.seqlen == 0) load_weight<T>(p.gate, first, gate[0]);
-        if constexpr (OUT != kFp4None) load_weight<T>(p.w_pre, first, pre[0]);
+        if (p.w_post) {
+            load_weight<T>(p.w_post, first, post[0]);
+            unpack16<T>(post[0], post_kept);
+        }
+        if (p.gate && p.seqlen == 0) {
+            load_weight<T>(p.gate, first, gate[0]);
+            unpack16<T>(gate[0], gate_kept);
+        }
+        if constexpr (OUT != kFp4None) {
+            load_weight<T>(p.w_pre, first, pre[0]);
+            unpack16<T>(pre[0], pre_kept);
+        }
     }
+    const int tiles = !FULL ? p.tiles : OUT == kFp4Mx ? 4 * U : 8 * U;
     uint32_t x[U][8], res[U][8], x_ahead[U][8], res_ahead[U][8];
     load_row<U, FULL>(p.x, row, units, lane, lanes, x);
     load_row<U, FULL>(p.residual, row, units, lane, lanes, res);
@@ -375,7 +386,10 @@ rmsnorm_block_kernel(const RmsnormBlockDev p) {
             for (int j = 0; j < U; ++j) {
                 const int at = U == 1 ? first : FULL ? lane + j * 32 : min(lane + j * lanes, units - 1);
                 if (!kKeep && p.w_post) load_weight<T>(p.w_post, at, post[j]);
-                if (p.gate && (!kKeep || p.seqlen > 0)) load_weight<T>(p.gate, gate_at + at, gate[j]);
+                if (p.gate && (!kKeep || p.seqlen > 0)) {
+                    load_weight<T>(p.gate, gate_at + at, gate[j]);
+                    if constexpr (kKeep) unpack16<T>(gate[0], gate_kept);
+                }
             }
         float rx = 1.f;
         if (p.w_post) {
@@ -397,15 +411,15 @@ rmsnorm_block_kernel(const RmsnormBlockDev p) {
             unpack16<T>(res[j], r);
             if (p.w_post) {
                 if constexpr (!kEarly) load_weight<T>(p.w_post, at, post[0]);
-                unpack16<T>(post[kEarly ? j : 0], w);
+                if constexpr (!kKeep) unpack16<T>(post[kEarly ? j : 0], w);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = mul2(mul2(v[i], make_float2(rx, rx)), w[i]);
+                for (int i = 0; i < 8; ++i) v[i] = mul2(mul2(v[i], make_float2(rx, rx)), kKeep ? post_kept[kKeep ? i : 0] : w[i]);
             }
             if (p.gate) {
                 if constexpr (!kEarly) load_weight<T>(p.gate, gate_at + at, gate[0]);
-                unpack16<T>(gate[kEarly ? j : 0], w);
+                if constexpr (!kKeep) unpack16<T>(gate[kEarly ? j : 0], w);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = mul2(w[i], v[i]);
+                for (int i = 0; i < 8; ++i) v[i] = mul2(kKeep ? gate_kept[kKeep ? i : 0] : w[i], v[i]);
             }
             const float2 one = make_float2(1.f, 1.f), alpha = make_float2(p.alpha, p.alpha);
 #pragma unroll
@@ -424,9 +438,9 @@ rmsnorm_block_kernel(const RmsnormBlockDev p) {
                 float2 w[8];
                 unpack16<T>(x[j], v);
                 if constexpr (!kEarly) load_weight<T>(p.w_pre, at, pre[0]);
-                unpack16<T>(pre[kEarly ? j : 0], w);
+                if constexpr (!kKeep) unpack16<T>(pre[kEarly ? j : 0], w);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = mul2(mul2(v[i], make_float2(ry, ry)), w[i]);
+                for (int i = 0; i < 8; ++i) v[i] = mul2(mul2(v[i], make_float2(ry, ry)), kKeep ? pre_kept[kKeep ? i : 0] : w[i]);
             };
             // one unit per lane: normed once, kept over the maximum of the row
             float2 h[8];
@@ -470,14 +484,14 @@ rmsnorm_block_kernel(const RmsnormBlockDev p) {
                         if (!in) continue;
                         const uint32_t e = mx_exponent(m);
                         *reinterpret_cast<uint2 *>(codes) = mx_codes(h, e);
-                        if ((at & 1) == 0) p.scale[scale_byte(row, at >> 1, p.tiles)] = uint8_t(e);
-                        if (at == units - 1) pad_scales(p.scale, row, units >> 1, p.tiles);
+                        if ((at & 1) == 0) p.scale[scale_byte(row, at >> 1, tiles)] = uint8_t(e);
+                        if (at == units - 1) pad_scales(p.scale, row, units >> 1, tiles);
                     } else {
                         if (!in) break;
                         uint32_t s8;
                         *reinterpret_cast<uint2 *>(codes) = nv_codes(h, bmax[j], g, s8);
-                        p.scale[scale_byte(row, at, p.tiles)] = uint8_t(s8);
-                        if (at == units - 1) pad_scales(p.scale, row, units, p.tiles);
+                        p.scale[scale_byte(row, at, tiles)] = uint8_t(s8);
+                        if (at == units - 1) pad_scales(p.scale, row, units, tiles);
                     }
                 }
             }
@@ -521,11 +535,11 @@ inline int resident_blocks(const void *kernel, int block) {
     }
     return s.blocks;
 }
-// Blocks of a row kernel: one per row, or as many of eight warps as the device holds (fewer, so that every warp has as many rows as the
+// Blocks of a row kernel: one per row, or as many of `warps` warps as the device holds (fewer, so that every warp has as many rows as the
 // others, leaves some SMs with fewer blocks: [32000, 512] 400 blocks instead of 444, 24.3 : 23.2 us).
-inline int row_grid(const void *kernel, const RowSpread &s, int rows) {
+inline int row_grid(const void *kernel, const RowSpread &s, int rows, int warps) {
     if (s.block_row) return rows;
-    const int blocks = (rows + kFp4RowWarps - 1) / kFp4RowWarps, most = resident_blocks(kernel, kFp4RowWarps * 32);
+    const int blocks = (rows + warps - 1) / warps, most = resident_blocks(kernel, warps * 32);
     return blocks < most ? blocks : most;
 }
 
@@ -537,21 +551,21 @@ int launch_quant_nvfp4(const void *in, void *codes, void *scale, void *row_scale
     static constexpr fn kernels[2][3] = {{quant_nvfp4_kernel<T, 1, false>, quant_nvfp4_kernel<T, 2, false>, quant_nvfp4_kernel<T, 4, false>},
                                          {quant_nvfp4_kernel<T, 1, true>, quant_nvfp4_kernel<T, 2, true>, quant_nvfp4_kernel<T, 4, true>}};
     const fn kernel = kernels[s.block_row][s.per_lane >> 1];
-    return launch_dependent(kernel, row_grid(reinterpret_cast<const void *>(kernel), s, rows), block, 0, stream, static_cast<const T *>(in), static_cast<uint8_t *>(codes),
+    return launch_dependent(kernel, row_grid(reinterpret_cast<const void *>(kernel), s, rows, kFp4RowWarps), block, 0, stream, static_cast<const T *>(in), static_cast<uint8_t *>(codes),
                             static_cast<uint8_t *>(scale), static_cast<float *>(row_scale), rows, units, (units + 3) / 4);
 }
 
 template <typename T, int OUT>
 int launch_rmsnorm_block(const RmsnormBlockDev &p, cudaStream_t stream) {
     const RowSpread s = row_spread(p.rows, p.units);
-    const int block = s.block_row ? s.warps * 32 : kFp4RowWarps * 32;
+    const int block = s.block_row ? s.warps * 32 : kFp4NormWarps * 32;
     using fn = void (*)(RmsnormBlockDev);
     static constexpr fn kernels[3][3] = {
         {rmsnorm_block_kernel<T, OUT, 1, false, false>, rmsnorm_block_kernel<T, OUT, 2, false, false>, rmsnorm_block_kernel<T, OUT, 4, false, false>},
         {rmsnorm_block_kernel<T, OUT, 1, true, false>, rmsnorm_block_kernel<T, OUT, 2, true, false>, rmsnorm_block_kernel<T, OUT, 4, true, false>},
         {rmsnorm_block_kernel<T, OUT, 1, false, true>, rmsnorm_block_kernel<T, OUT, 2, false, true>, rmsnorm_block_kernel<T, OUT, 4, false, true>}};
     const fn kernel = kernels[s.block_row ? 1 : p.units == 32 * s.per_lane ? 2 : 0][s.per_lane >> 1];
-    return launch_dependent(kernel, row_grid(reinterpret_cast<const void *>(kernel), s, p.rows), block, 0, stream, p);
+    return launch_dependent(kernel, row_grid(reinterpret_cast<const void *>(kernel), s, p.rows, kFp4NormWarps), block, 0, stream, p);
 }
 template <typename T>
 int launch_rmsnorm_block(const RmsnormBlockDev &p, int out, cudaStream_t stream) {
