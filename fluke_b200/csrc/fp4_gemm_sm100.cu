@@ -5,17 +5,20 @@
 //
 // The tensor cores take the codes as they are stored and apply the block scales themselves
 // (tcgen05.mma .block_scale, kind mxf4 and mxf4nvf4: 64 values of K per instruction, f32 accumulators in tensor
-// memory), so nothing is decoded on the way: TMA brings 128-byte-swizzled blocks of 256 values of K per row into a ring of
-// stages, bulk copies bring the stage's scale tiles, and tcgen05.cp moves those to tensor memory, where the instruction reads
-// them. Row scales are powers of two and are applied to the accumulators, which is exact.
+// memory), so nothing is decoded on the way: TMA brings 128-byte-swizzled blocks of 256 values of K per row and the scale tiles that
+// belong to them, and tcgen05.cp moves those to tensor memory, where the instruction reads them. Row scales are powers of two and are
+// applied to the accumulators, which is exact.
 //
-//   warp 0      loader (one thread)
-//   warp 1      tensor memory, scale copies and MMAs (one thread)
-//   warps 2-3   idle
-//   warps 4-11  epilogue: two warps per quadrant of tensor-memory lanes, thread = row
+// Three forms, by what bounds them (gemm_fp4_dispatch chooses):
+//   split      few rows or few tiles: latency, and reading the weights. One tile per CTA, K split over a cluster.
+//   resident   many tiles, K <= 1024: writing the output. Pairs of SMs, the weight's rows stay on chip.
+//   pair       many tiles, longer K: the MMAs, under the power limit. Pairs of SMs, both operands stream.
+// In each warp 0 loads (one thread), warp 1 owns tensor memory and issues scale copies and MMAs, warps 2-3 are idle and the others are the
+// epilogue. An MMA of 128 (pair: 256) x 256 x 64 takes 128 cycles, one of half the columns 64, with or without the scale copies
+// between them; the first result comes some 450 cycles after the first instruction.
 //
 // The scale tiles of a stage have tensor-memory columns of their own: they are overwritten when the stage is filled
-// again, which the MMAs that read them have announced.
+// again, which the MMAs that read them have announced (resident: see its layout).
 
 namespace fluke_sm100 {
 namespace {
