@@ -208,7 +208,7 @@ dequant_fp4_kernel(const uint8_t *codes, const uint8_t *scale, const float *row_
 // ---- rows held in registers -------------------------------------------------------------------
 // A row belongs to one warp (8 rows to a block) or to one whole block of up to 8 warps; lane l of the row's
 // `lanes` holds units l, l + lanes, ... (U of them).
-constexpr int kFp4RowWarps = 8, kFp4NormWarps = 4;   // of a block: at most; of the norms that walk rows
+constexpr int kFp4RowWarps = 16, kFp4WalkWarps = 8, kFp4NormWarps = 4;   // of a block that holds a row, at most; of blocks that walk rows
 
 template <bool BLOCK_ROW>
 __device__ __forceinline__ uint32_t row_max(uint32_t m, uint32_t *shared) {
@@ -259,14 +259,14 @@ __device__ __forceinline__ void copy_row(uint32_t (&to)[U][8], const uint32_t (&
 // row; 9.9 with the quotients of nv_codes and the three-operand maximum, 0.76 of the copy rate); a block that holds one row together does not. Two
 // or four warps to such a row instead of one: 10.8, 11.8.
 template <typename T, int U, bool BLOCK_ROW>
-__global__ void __launch_bounds__(kFp4RowWarps * 32, U == 1 ? 4 : U == 2 ? 3 : 2)
+__global__ void __launch_bounds__(BLOCK_ROW ? kFp4RowWarps * 32 : kFp4WalkWarps * 32, BLOCK_ROW ? 1 : U == 1 ? 4 : U == 2 ? 3 : 2)
 quant_nvfp4_kernel(const T *in, uint8_t *codes, uint8_t *scale, float *row_scale, int rows, int units, int tiles) {
     __shared__ uint32_t shared[kFp4RowWarps];
     dependency_wait();
     const int lanes = BLOCK_ROW ? blockDim.x : 32;
     const int lane = BLOCK_ROW ? threadIdx.x : threadIdx.x & 31;
-    const int step = BLOCK_ROW ? rows : int(gridDim.x) * kFp4RowWarps;
-    int row = BLOCK_ROW ? int(blockIdx.x) : int(blockIdx.x) * kFp4RowWarps + (int(threadIdx.x) >> 5);
+    const int step = BLOCK_ROW ? rows : int(gridDim.x) * kFp4WalkWarps;
+    int row = BLOCK_ROW ? int(blockIdx.x) : int(blockIdx.x) * kFp4WalkWarps + (int(threadIdx.x) >> 5);
     if (row >= rows) return;
     uint32_t raw[U][8], ahead[U][8];
     load_row<U>(in, row, units, lane, lanes, raw);
@@ -304,8 +304,8 @@ quant_nvfp4_kernel(const T *in, uint8_t *codes, uint8_t *scale, float *row_scale
 // rounded once to f32: what is quantised behind them lies next to borders, and like this the result depends on
 // the values alone, not on how a row is spread over lanes. One Newton step from the hardware's reciprocal root r, with 1 - a r^2 in 64
 // bits, leaves a relative error of 1e-13 before that rounding.
-// Bound by instructions: [32000, 512] to mxfp4 22.1 us (16.4 at the copy rate), some 450 instructions per row and warp; without any access to
-// memory 19.7, without the 64-bit sums as well 13.7. Rows brought ahead by bulk copies into shared memory instead of registers: 24.8 against 23.2.
+// Bound by instructions: [32000, 512] to mxfp4 21.3 us (16.4 at the copy rate). With a warp per row it was 23.2 us and some 450 instructions per row;
+// without any access to memory 19.7, without the 64-bit sums as well 13.7. Rows brought ahead by bulk copies into shared memory instead of registers: 24.8.
 __device__ __forceinline__ float inv_rms(double sum, double inv_n, double eps) {
     const double a = fma(sum, inv_n, eps);
     const float f = float(a);
@@ -344,163 +344,258 @@ __device__ __forceinline__ void add_squares(const uint32_t (&raw)[8], double (&s
     }
 }
 
-// FULL: rows of exactly U units per lane of a warp ([32000, 512] 28.3 us without, 25.6 with: no lane has to ask for its end).
-template <typename T, int OUT, int U, bool BLOCK_ROW, bool FULL>
-__global__ void __launch_bounds__(BLOCK_ROW ? kFp4RowWarps * 32 : kFp4NormWarps * 32, BLOCK_ROW ? (U <= 2 ? 2 : 1) : U == 1 ? 5 : U == 2 ? 4 : 2)
-rmsnorm_block_kernel(const RmsnormBlockDev p) {
-    __shared__ double sums[2][kFp4RowWarps];
-    __shared__ uint32_t maxima[kFp4RowWarps];
-    dependency_wait();
-    const int lanes = BLOCK_ROW ? blockDim.x : 32;
-    const int lane = BLOCK_ROW ? threadIdx.x : threadIdx.x & 31;
-    const int step = BLOCK_ROW ? p.rows : int(gridDim.x) * kFp4NormWarps;
-    int row = BLOCK_ROW ? int(blockIdx.x) : int(blockIdx.x) * kFp4NormWarps + (int(threadIdx.x) >> 5);
-    if (row >= p.rows) return;
-    const int units = FULL ? 32 * U : p.units;
-    const double inv_n = 1.0 / (double(units) * 16.0), eps = double(p.eps);
-    // Weights come from L1 in front of the sums that they wait for, where registers allow it; a warp that walks rows of one unit
-    // per lane keeps those that all rows share.
-    constexpr bool kKeep = U == 1 && !BLOCK_ROW, kEarly = U <= 2;
-    uint32_t post[kEarly ? U : 1][8], gate[kEarly ? U : 1][8], pre[kEarly ? U : 1][8];
-    float2 post_kept[kKeep ? 8 : 1], gate_kept[kKeep ? 8 : 1], pre_kept[kKeep ? 8 : 1];
-    const int first = FULL ? lane : min(lane, units - 1);
-    if constexpr (kKeep) {
-        if (p.w_post) {
-            load_weight<T>(p.w_post, first, post[0]);
-            unpack16<T>(post[0], post_kept);
-        }
-        if (p.gate && p.seqlen == 0) {
-            load_weight<T>(p.gate, first, gate[0]);
-            unpack16<T>(gate[0], gate_kept);
-        }
-        if constexpr (OUT != kFp4None) {
-            load_weight<T>(p.w_pre, first, pre[0]);
-            unpack16<T>(pre[0], pre_kept);
+// What both forms of the norms do with a unit. y = round16(alpha res + gate ((x rx) post)); the stream's unit replaces x.
+template <typename T>
+__device__ __forceinline__ void stream_unit(uint32_t (&x)[8], const uint32_t (&res)[8], bool normed, float rx, const float2 (&post)[8], bool gated,
+                                            const float2 (&gate)[8], float alpha) {
+    float2 v[8], r[8];
+    unpack16<T>(x, v);
+    unpack16<T>(res, r);
+    if (normed)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = mul2(mul2(v[i], make_float2(rx, rx)), post[i]);
+    if (gated)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = mul2(gate[i], v[i]);
+    const float2 one = make_float2(1.f, 1.f), a2 = make_float2(alpha, alpha);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = pack2(fma2(mul2(a2, r[i]), one, v[i]), T());
+}
+// h = (y ry) pre
+template <typename T>
+__device__ __forceinline__ void normed_unit(const uint32_t (&y)[8], float ry, const float2 (&pre)[8], float2 (&h)[8]) {
+    unpack16<T>(y, h);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) h[i] = mul2(mul2(h[i], make_float2(ry, ry)), pre[i]);
+}
+// Writes unit `at` of the next block's input; all lanes of a warp come here (MX: the pair of lanes that shares a block), `in` is whether
+// the unit is one of the row.
+template <typename T, int OUT>
+__device__ __forceinline__ void write_unit(const RmsnormBlockDev &p, int64_t row, int at, int units, int tiles, bool in, const float2 (&h)[8],
+                                           uint32_t bmax, float g) {
+    if constexpr (OUT == kFp4Plain) {
+        if (!in) return;
+        uint32_t r[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) r[i] = pack2(h[i], T());
+        store32(static_cast<T *>(p.out) + (row * units + at) * 16, r);
+    } else {
+        uint8_t *codes = static_cast<uint8_t *>(p.out) + (row * units + at) * 8;
+        if constexpr (OUT == kFp4Mx) {
+            uint32_t m = in ? max_bits16(h) : 0;
+            m = max(m, __shfl_xor_sync(kFull, m, 1));
+            if (!in) return;
+            const uint32_t e = mx_exponent(m);
+            *reinterpret_cast<uint2 *>(codes) = mx_codes(h, e);
+            if ((at & 1) == 0) p.scale[scale_byte(row, at >> 1, tiles)] = uint8_t(e);
+            if (at == units - 1) pad_scales(p.scale, row, units >> 1, tiles);
+        } else {
+            if (!in) return;
+            uint32_t s8;
+            *reinterpret_cast<uint2 *>(codes) = nv_codes(h, bmax, g, s8);
+            p.scale[scale_byte(row, at, tiles)] = uint8_t(s8);
+            if (at == units - 1) pad_scales(p.scale, row, units, tiles);
         }
     }
-    const int tiles = !FULL ? p.tiles : OUT == kFp4Mx ? 4 * U : 8 * U;
-    uint32_t x[U][8], res[U][8], x_ahead[U][8], res_ahead[U][8];
-    load_row<U, FULL>(p.x, row, units, lane, lanes, x);
-    load_row<U, FULL>(p.residual, row, units, lane, lanes, res);
-    for (; row < p.rows; row += step) {
-        const int64_t gate_at = p.seqlen > 0 ? int64_t(row / p.seqlen) * units : 0, row_unit = int64_t(row) * units;
-        if constexpr (kEarly)
+}
+
+// Rows of up to 2048 values: LANES lanes (half a warp or one) hold a row, lane l units l, l + LANES, ... (U of them), and a block's warps walk
+// rows. The weights that all rows share lie in shared memory as f32, which saves a conversion per value and row. FULL: rows of exactly
+// LANES * U units, where no lane has to ask for its end. The next rows are asked for while these are computed with two units per lane (us,
+// with : without: [32000, 512] to mxfp4 21.3 : 23.8, [9331, 1024] 13.2 : 14.2; one unit [16384, 256] 7.1 : 6.6, whose registers carry six blocks without),
+// and behind the other loads: a use of those waits for every load in front of it.
+template <typename T, int OUT, int LANES, int U, bool FULL>
+__global__ void __launch_bounds__(kFp4NormWarps * 32, U == 1 ? 6 : 4)
+rmsnorm_rows_kernel(const RmsnormBlockDev p) {
+    constexpr bool kAhead = U == 2;
+    constexpr int kGroups = 32 / LANES;   // rows of a warp at a time
+    // unit u's four pieces of four values are `units` pieces apart: lanes that read the same piece of neighbouring units meet no bank twice
+    extern __shared__ float4 weights[];
+    const int units = FULL ? LANES * U : p.units, tiles = !FULL ? p.tiles : OUT == kFp4Mx ? (units / 2 + 3) / 4 : (units + 3) / 4;
+    const bool own_gate = p.gate && p.seqlen > 0;
+    float4 *const post = weights, *const gate = weights + 4 * units, *const pre = weights + 8 * units;
+    dependency_wait();
+    for (int w = 0; w < 3; ++w) {
+        const void *src = w == 0 ? p.w_post : w == 1 ? (own_gate ? nullptr : p.gate) : OUT != kFp4None ? p.w_pre : nullptr;
+        if (src)
+            for (int u = threadIdx.x; u < units; u += kFp4NormWarps * 32) {
+                uint32_t raw[8];
+                float2 v[8];
+                load_weight<T>(src, u, raw);
+                unpack16<T>(raw, v);
 #pragma unroll
-            for (int j = 0; j < U; ++j) {
-                const int at = U == 1 ? first : FULL ? lane + j * 32 : min(lane + j * lanes, units - 1);
-                if (!kKeep && p.w_post) load_weight<T>(p.w_post, at, post[j]);
-                if (p.gate && (!kKeep || p.seqlen > 0)) {
-                    load_weight<T>(p.gate, gate_at + at, gate[j]);
-                    if constexpr (kKeep) unpack16<T>(gate[0], gate_kept);
-                }
+                for (int c = 0; c < 4; ++c) weights[(w * 4 + c) * units + u] = make_float4(v[2 * c].x, v[2 * c].y, v[2 * c + 1].x, v[2 * c + 1].y);
             }
+    }
+    __syncthreads();
+    auto weight = [&](const float4 *w, int at, float2 (&v)[8]) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            const float4 q = w[c * units + at];
+            v[2 * c] = make_float2(q.x, q.y);
+            v[2 * c + 1] = make_float2(q.z, q.w);
+        }
+    };
+    const int lane = threadIdx.x & (LANES - 1), group = (threadIdx.x & 31) / LANES;
+    const double inv_n = 1.0 / (double(units) * 16.0), eps = double(p.eps);
+    auto sum_of = [&](const double (&s)[4]) {
+        double t = (s[0] + s[1]) + (s[2] + s[3]);
+#pragma unroll
+        for (int d = LANES / 2; d > 0; d >>= 1) t += __shfl_xor_sync(kFull, t, d);
+        return t;
+    };
+    const int step = int(gridDim.x) * kFp4NormWarps * kGroups;
+    uint32_t x[U][8], res[U][8], x_ahead[kAhead ? U : 1][8], res_ahead[kAhead ? U : 1][8];
+    // `first` is the row of the warp's first group: the loop is the same for all lanes, rows behind the last are zeros and not written
+    int first = (int(blockIdx.x) * kFp4NormWarps + (int(threadIdx.x) >> 5)) * kGroups;
+    auto load = [&](int row, auto &a, auto &b) {
+        const int have = row < p.rows ? units : 0;
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+            const int at = lane + j * LANES;
+            if (FULL ? row < p.rows : at < have) {
+                load32(static_cast<const T *>(p.x) + (int64_t(row) * units + at) * 16, a[j]);
+                load32(static_cast<const T *>(p.residual) + (int64_t(row) * units + at) * 16, b[j]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) a[j][i] = b[j][i] = 0;
+            }
+        }
+    };
+    if (kAhead && first < p.rows) load(first + group, x, res);
+    for (; first < p.rows; first += step) {
+        const int row = first + group;
+        const bool live = row < p.rows;
+        if constexpr (!kAhead) load(row, x, res);
+        const int64_t gate_at = own_gate && live ? int64_t(row / p.seqlen) * units : 0;
         float rx = 1.f;
         if (p.w_post) {
             double s[4] = {};
 #pragma unroll
             for (int j = 0; j < U; ++j) add_squares<T>(x[j], s);
-            rx = inv_rms(row_sum<BLOCK_ROW>((s[0] + s[1]) + (s[2] + s[3]), sums[0]), inv_n, eps);
+            rx = inv_rms(sum_of(s), inv_n, eps);
         }
-        if constexpr (kEarly && !kKeep && OUT != kFp4None)
-#pragma unroll
-            for (int j = 0; j < U; ++j) load_weight<T>(p.w_pre, FULL ? lane + j * 32 : min(lane + j * lanes, units - 1), pre[j]);
         double s[4] = {};
 #pragma unroll
         for (int j = 0; j < U; ++j) {
-            const int at = lane + j * lanes;
-            if (!FULL && at >= units) break;
-            float2 v[8], w[8], r[8];
-            unpack16<T>(x[j], v);
-            unpack16<T>(res[j], r);
-            if (p.w_post) {
-                if constexpr (!kEarly) load_weight<T>(p.w_post, at, post[0]);
-                if constexpr (!kKeep) unpack16<T>(post[kEarly ? j : 0], w);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = mul2(mul2(v[i], make_float2(rx, rx)), kKeep ? post_kept[kKeep ? i : 0] : w[i]);
+            const int at = lane + j * LANES;
+            const bool in = FULL ? live : live && at < units;
+            const int safe = FULL || at < units ? at : 0;
+            float2 wp[8], wg[8];
+            if (p.w_post) weight(post, safe, wp);
+            if (own_gate) {
+                uint32_t raw[8];
+                load_weight<T>(p.gate, gate_at + safe, raw);
+                unpack16<T>(raw, wg);
+            } else if (p.gate) {
+                weight(gate, safe, wg);
             }
-            if (p.gate) {
-                if constexpr (!kEarly) load_weight<T>(p.gate, gate_at + at, gate[0]);
-                if constexpr (!kKeep) unpack16<T>(gate[kEarly ? j : 0], w);
+            stream_unit<T>(x[j], res[j], p.w_post != nullptr, rx, wp, p.gate != nullptr, wg, p.alpha);
+            if (!FULL && at >= units)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = mul2(kKeep ? gate_kept[kKeep ? i : 0] : w[i], v[i]);
-            }
-            const float2 one = make_float2(1.f, 1.f), alpha = make_float2(p.alpha, p.alpha);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x[j][i] = pack2(fma2(mul2(alpha, r[i]), one, v[i]), T());   // the stream
-            store32(static_cast<T *>(p.residual_out) + (row_unit + at) * 16, x[j]);
+                for (int i = 0; i < 8; ++i) x[j][i] = 0;
+            if (in) store32(static_cast<T *>(p.residual_out) + (int64_t(row) * units + at) * 16, x[j]);
             if constexpr (OUT != kFp4None) add_squares<T>(x[j], s);
         }
-        // The next row is asked for behind the last of this row's other loads: a use of those waits for every load in front of it.
-        if (row + step < p.rows) {
-            load_row<U, FULL>(p.x, row + step, units, lane, lanes, x_ahead);
-            load_row<U, FULL>(p.residual, row + step, units, lane, lanes, res_ahead);
-        }
+        if constexpr (kAhead)
+            if (first + step < p.rows) load(row + step, x_ahead, res_ahead);
         if constexpr (OUT != kFp4None) {
-            const float ry = inv_rms(row_sum<BLOCK_ROW>((s[0] + s[1]) + (s[2] + s[3]), sums[1]), inv_n, eps);
-            auto normed = [&](int j, int at, float2 (&v)[8]) {
-                float2 w[8];
-                unpack16<T>(x[j], v);
-                if constexpr (!kEarly) load_weight<T>(p.w_pre, at, pre[0]);
-                if constexpr (!kKeep) unpack16<T>(pre[kEarly ? j : 0], w);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = mul2(mul2(v[i], make_float2(ry, ry)), kKeep ? pre_kept[kKeep ? i : 0] : w[i]);
-            };
-            // one unit per lane: normed once, kept over the maximum of the row
-            float2 h[8];
+            const float ry = inv_rms(sum_of(s), inv_n, eps);
+            float2 h[8], wn[8];
             uint32_t bmax[U], amax = 0;
             float g = 1.f;
-            if constexpr (U == 1) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) h[i] = make_float2(0.f, 0.f);
-                if (FULL || lane < units) normed(0, lane, h);
-            }
+            auto unit = [&](int j) {
+                const int at = lane + j * LANES;
+                weight(pre, FULL || at < units ? at : 0, wn);
+                normed_unit<T>(x[j], ry, wn, h);
+            };
             if constexpr (OUT == kFp4Nv) {
 #pragma unroll
                 for (int j = 0; j < U; ++j) {
-                    bmax[j] = 0;
-                    if (FULL || lane + j * lanes < units) {
-                        if constexpr (U > 1) normed(j, lane + j * lanes, h);
-                        bmax[j] = max_bits16(h);
-                    }
+                    unit(j);
+                    bmax[j] = FULL || lane + j * LANES < units ? max_bits16(h) : 0;
                     amax = max(amax, bmax[j]);
                 }
-                g = nv_row_scale(row_max<BLOCK_ROW>(amax, maxima));
-                if (lane == 0) p.row_scale[row] = g;
+                amax = __reduce_max_sync(LANES == 32 ? kFull : 0xFFFFu << (threadIdx.x & 16), amax);
+                g = nv_row_scale(amax);
+                if (lane == 0 && live) p.row_scale[row] = g;
             }
 #pragma unroll
             for (int j = 0; j < U; ++j) {
-                const int at = lane + j * lanes;
-                const bool in = FULL || at < units;
-                if constexpr (U > 1)
-                    if (in) normed(j, at, h);
-                if constexpr (OUT == kFp4Plain) {
-                    if (!in) break;
-                    uint32_t r[8];
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) r[i] = pack2(h[i], T());
-                    store32(static_cast<T *>(p.out) + (row_unit + at) * 16, r);
-                } else {
-                    uint8_t *codes = static_cast<uint8_t *>(p.out) + (row_unit + at) * 8;
-                    if constexpr (OUT == kFp4Mx) {
-                        uint32_t m = in ? max_bits16(h) : 0;
-                        m = max(m, __shfl_xor_sync(kFull, m, 1));
-                        if (!in) continue;
-                        const uint32_t e = mx_exponent(m);
-                        *reinterpret_cast<uint2 *>(codes) = mx_codes(h, e);
-                        if ((at & 1) == 0) p.scale[scale_byte(row, at >> 1, tiles)] = uint8_t(e);
-                        if (at == units - 1) pad_scales(p.scale, row, units >> 1, tiles);
-                    } else {
-                        if (!in) break;
-                        uint32_t s8;
-                        *reinterpret_cast<uint2 *>(codes) = nv_codes(h, bmax[j], g, s8);
-                        p.scale[scale_byte(row, at, tiles)] = uint8_t(s8);
-                        if (at == units - 1) pad_scales(p.scale, row, units, tiles);
-                    }
-                }
+                const int at = lane + j * LANES;
+                if (OUT != kFp4Nv || U > 1) unit(j);
+                write_unit<T, OUT>(p, row, at, units, tiles, FULL ? live : live && at < units, h, OUT == kFp4Nv ? bmax[j] : 0, g);
             }
         }
-        copy_row<U>(x, x_ahead);
-        copy_row<U>(res, res_ahead);
+        if constexpr (kAhead) {
+            copy_row<U>(x, x_ahead);
+            copy_row<U>(res, res_ahead);
+        }
+    }
+}
+
+// A row held by a block: few rows, or more than 2048 values.
+template <typename T, int OUT, int U>
+__global__ void __launch_bounds__(kFp4RowWarps * 32, 1)
+rmsnorm_block_kernel(const RmsnormBlockDev p) {
+    __shared__ double sums[2][kFp4RowWarps];
+    __shared__ uint32_t maxima[kFp4RowWarps];
+    dependency_wait();
+    const int lanes = blockDim.x, lane = threadIdx.x, units = p.units;
+    const int64_t row = blockIdx.x;
+    const double inv_n = 1.0 / (double(units) * 16.0), eps = double(p.eps);
+    uint32_t x[U][8], res[U][8], post[U][8], gate[U][8], pre[U][8];
+    load_row<U>(p.x, row, units, lane, lanes, x);
+    load_row<U>(p.residual, row, units, lane, lanes, res);
+    const int64_t gate_at = p.seqlen > 0 ? row / p.seqlen * units : 0;
+    auto weights = [&](const void *w, int64_t base, uint32_t (&raw)[U][8]) {
+#pragma unroll
+        for (int j = 0; j < U; ++j) load_weight<T>(w, base + min(lane + j * lanes, units - 1), raw[j]);
+    };
+    if (p.w_post) weights(p.w_post, 0, post);
+    if (p.gate) weights(p.gate, gate_at, gate);
+    if constexpr (OUT != kFp4None) weights(p.w_pre, 0, pre);
+    float rx = 1.f;
+    if (p.w_post) {
+        double s[4] = {};
+#pragma unroll
+        for (int j = 0; j < U; ++j) add_squares<T>(x[j], s);
+        rx = inv_rms(row_sum<true>((s[0] + s[1]) + (s[2] + s[3]), sums[0]), inv_n, eps);
+    }
+    double s[4] = {};
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+        const int at = lane + j * lanes;
+        if (at >= units) break;
+        float2 wp[8], wg[8];
+        if (p.w_post) unpack16<T>(post[j], wp);
+        if (p.gate) unpack16<T>(gate[j], wg);
+        stream_unit<T>(x[j], res[j], p.w_post != nullptr, rx, wp, p.gate != nullptr, wg, p.alpha);
+        store32(static_cast<T *>(p.residual_out) + (row * units + at) * 16, x[j]);
+        if constexpr (OUT != kFp4None) add_squares<T>(x[j], s);
+    }
+    if constexpr (OUT != kFp4None) {
+        const float ry = inv_rms(row_sum<true>((s[0] + s[1]) + (s[2] + s[3]), sums[1]), inv_n, eps);
+        float2 h[U][8];
+        uint32_t bmax[U], amax = 0;
+        float g = 1.f;
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+            float2 wn[8];
+            unpack16<T>(pre[j], wn);
+            normed_unit<T>(x[j], ry, wn, h[j]);
+            bmax[j] = lane + j * lanes < units ? max_bits16(h[j]) : 0;
+            amax = max(amax, bmax[j]);
+        }
+        if constexpr (OUT == kFp4Nv) {
+            g = nv_row_scale(row_max<true>(amax, maxima));
+            if (lane == 0) p.row_scale[row] = g;
+        }
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+            const int at = lane + j * lanes;
+            write_unit<T, OUT>(p, row, at, units, p.tiles, at < units, h[j], bmax[j], g);
+        }
     }
 }
 
@@ -510,65 +605,77 @@ struct RowSpread { int per_lane, warps; bool block_row; };
 inline RowSpread row_spread(int rows, int units) {
     const bool few = rows < 4 * device_sm_count();
     RowSpread s = {1, 1, false};
-    if (few && units > 32) {
+    if (units > 128 || (few && units > 32)) {
         s.block_row = true;
-        s.warps = (units + 31) / 32 < kFp4RowWarps ? (units + 31) / 32 : kFp4RowWarps;
-    } else if (units > 128) {
-        s.block_row = true;
-        s.warps = units > 512 ? 8 : units > 256 ? 4 : 2;
+        s.per_lane = few && units <= 32 * kFp4RowWarps ? 1 : units <= 256 ? 2 : 4;
+        s.warps = (units + 32 * s.per_lane - 1) / (32 * s.per_lane);
     }
     while (s.per_lane * s.warps * 32 < units) s.per_lane *= 2;
     return s;
 }
-
 // Blocks of `kernel` that the device holds at once.
-inline int resident_blocks(const void *kernel, int block) {
-    struct Seen { const void *kernel; int dev, blocks; };
+inline int resident_blocks(const void *kernel, int block, int smem = 0) {
+    struct Seen { const void *kernel; int dev, smem, blocks; };
     static thread_local Seen seen[64] = {};
     int dev = 0;
     cudaGetDevice(&dev);
     Seen &s = seen[(reinterpret_cast<uintptr_t>(kernel) >> 4) & 63];
-    if (s.kernel != kernel || s.dev != dev) {
+    if (s.kernel != kernel || s.dev != dev || s.smem != smem) {
         int per_sm = 0;
-        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, block, 0) != cudaSuccess || per_sm < 1) {
+        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, block, smem) != cudaSuccess || per_sm < 1) {
             cudaGetLastError();
             per_sm = 1;
         }
-        s = {kernel, dev, per_sm * device_sm_count()};
+        s = {kernel, dev, smem, per_sm * device_sm_count()};
     }
     return s.blocks;
 }
-// Blocks of a row kernel: one per row, or as many of `warps` warps as the device holds (fewer, so that every warp has as many rows as the
-// others, leaves some SMs with fewer blocks: [32000, 512] 400 blocks instead of 444, 24.3 : 23.2 us).
-inline int row_grid(const void *kernel, const RowSpread &s, int rows, int warps) {
-    if (s.block_row) return rows;
-    const int blocks = (rows + warps - 1) / warps, most = resident_blocks(kernel, warps * 32);
-    return blocks < most ? blocks : most;
-}
-
 template <typename T>
 int launch_quant_nvfp4(const void *in, void *codes, void *scale, void *row_scale, int rows, int units, cudaStream_t stream) {
     const RowSpread s = row_spread(rows, units);
-    const int block = s.block_row ? s.warps * 32 : kFp4RowWarps * 32;
     using fn = void (*)(const T *, uint8_t *, uint8_t *, float *, int, int, int);
     static constexpr fn kernels[2][3] = {{quant_nvfp4_kernel<T, 1, false>, quant_nvfp4_kernel<T, 2, false>, quant_nvfp4_kernel<T, 4, false>},
                                          {quant_nvfp4_kernel<T, 1, true>, quant_nvfp4_kernel<T, 2, true>, quant_nvfp4_kernel<T, 4, true>}};
     const fn kernel = kernels[s.block_row][s.per_lane >> 1];
-    return launch_dependent(kernel, row_grid(reinterpret_cast<const void *>(kernel), s, rows, kFp4RowWarps), block, 0, stream, static_cast<const T *>(in), static_cast<uint8_t *>(codes),
-                            static_cast<uint8_t *>(scale), static_cast<float *>(row_scale), rows, units, (units + 3) / 4);
+    // a block per row, or as many blocks of walking warps as the device holds
+    int grid = rows, block = s.warps * 32;
+    if (!s.block_row) {
+        block = kFp4WalkWarps * 32;
+        const int blocks = (rows + kFp4WalkWarps - 1) / kFp4WalkWarps, most = resident_blocks(reinterpret_cast<const void *>(kernel), block);
+        grid = blocks < most ? blocks : most;
+    }
+    return launch_dependent(kernel, grid, block, 0, stream, static_cast<const T *>(in), static_cast<uint8_t *>(codes), static_cast<uint8_t *>(scale),
+                            static_cast<float *>(row_scale), rows, units, (units + 3) / 4);
 }
 
+template <typename T, int OUT, int LANES, int U, bool FULL>
+int launch_rmsnorm_rows(const RmsnormBlockDev &p, cudaStream_t stream) {
+    constexpr auto kernel = rmsnorm_rows_kernel<T, OUT, LANES, U, FULL>;
+    const int smem = 12 * p.units * int(sizeof(float4)), block = kFp4NormWarps * 32;
+    constexpr int kRows = kFp4NormWarps * 32 / LANES;
+    const int blocks = (p.rows + kRows - 1) / kRows, most = resident_blocks(reinterpret_cast<const void *>(kernel), block, smem);
+    return launch_dependent(kernel, blocks < most ? blocks : most, block, smem, stream, p);
+}
+template <typename T, int OUT, int LANES, int U>
+int launch_rmsnorm_rows(const RmsnormBlockDev &p, cudaStream_t stream) {
+    return p.units == LANES * U ? launch_rmsnorm_rows<T, OUT, LANES, U, true>(p, stream) : launch_rmsnorm_rows<T, OUT, LANES, U, false>(p, stream);
+}
+// Few rows: a block each, as many warps as the row has units for. Else half a warp per row up to 768 values (a sum over 16 lanes serves two rows at
+// once), a warp up to 2048, and a block of warps with two units per lane beyond.
 template <typename T, int OUT>
 int launch_rmsnorm_block(const RmsnormBlockDev &p, cudaStream_t stream) {
-    const RowSpread s = row_spread(p.rows, p.units);
-    const int block = s.block_row ? s.warps * 32 : kFp4NormWarps * 32;
-    using fn = void (*)(RmsnormBlockDev);
-    static constexpr fn kernels[3][3] = {
-        {rmsnorm_block_kernel<T, OUT, 1, false, false>, rmsnorm_block_kernel<T, OUT, 2, false, false>, rmsnorm_block_kernel<T, OUT, 4, false, false>},
-        {rmsnorm_block_kernel<T, OUT, 1, true, false>, rmsnorm_block_kernel<T, OUT, 2, true, false>, rmsnorm_block_kernel<T, OUT, 4, true, false>},
-        {rmsnorm_block_kernel<T, OUT, 1, false, true>, rmsnorm_block_kernel<T, OUT, 2, false, true>, rmsnorm_block_kernel<T, OUT, 4, false, true>}};
-    const fn kernel = kernels[s.block_row ? 1 : p.units == 32 * s.per_lane ? 2 : 0][s.per_lane >> 1];
-    return launch_dependent(kernel, row_grid(reinterpret_cast<const void *>(kernel), s, p.rows, kFp4NormWarps), block, 0, stream, p);
+    const int units = p.units;
+    const bool few = p.rows < 4 * device_sm_count();
+    if (units > 128 || (few && units > 16)) {
+        const int each = !few || units > 32 * kFp4RowWarps ? 2 : 1, warps = (units + 32 * each - 1) / (32 * each);
+        return launch_dependent(each == 1 ? rmsnorm_block_kernel<T, OUT, 1> : rmsnorm_block_kernel<T, OUT, 2>, p.rows, warps * 32, 0, stream, p);
+    }
+    if (units <= 16) return launch_rmsnorm_rows<T, OUT, 16, 1>(p, stream);
+    if (units <= 32) return launch_rmsnorm_rows<T, OUT, 16, 2>(p, stream);
+    if (units <= 48) return launch_rmsnorm_rows<T, OUT, 16, 3>(p, stream);
+    if (units <= 64) return launch_rmsnorm_rows<T, OUT, 32, 2>(p, stream);
+    if (units <= 96) return launch_rmsnorm_rows<T, OUT, 32, 3>(p, stream);
+    return launch_rmsnorm_rows<T, OUT, 32, 4>(p, stream);
 }
 template <typename T>
 int launch_rmsnorm_block(const RmsnormBlockDev &p, int out, cudaStream_t stream) {
