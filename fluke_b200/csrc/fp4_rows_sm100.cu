@@ -206,42 +206,36 @@ dequant_fp4_kernel(const uint8_t *codes, const uint8_t *scale, const float *row_
 }
 
 // ---- rows held in registers -------------------------------------------------------------------
-// A row belongs to one warp (8 rows to a block) or to one whole block of up to 8 warps; lane l of the row's
-// `lanes` holds units l, l + lanes, ... (U of them).
+// A row belongs to half a warp or a warp (blocks whose warps walk rows), or to a block of up to 16 warps; lane l of the row's `lanes`
+// holds units l, l + lanes, ... (U of them). Maximum and sum of a block's row:
 constexpr int kFp4RowWarps = 16, kFp4WalkWarps = 8, kFp4NormWarps = 4;   // of a block that holds a row, at most; of blocks that walk rows
 
-template <bool BLOCK_ROW>
 __device__ __forceinline__ uint32_t row_max(uint32_t m, uint32_t *shared) {
     m = __reduce_max_sync(kFull, m);
-    if constexpr (BLOCK_ROW) {
-        const int warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-        if ((threadIdx.x & 31) == 0) shared[warp] = m;
-        __syncthreads();
-        m = 0;
-        for (int w = 0; w < warps; ++w) m = max(m, shared[w]);
-    }
+    const int warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    if ((threadIdx.x & 31) == 0) shared[warp] = m;
+    __syncthreads();
+    m = 0;
+    for (int w = 0; w < warps; ++w) m = max(m, shared[w]);
     return m;
 }
-template <bool BLOCK_ROW>
 __device__ __forceinline__ double row_sum(double s, double *shared) {
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(kFull, s, d);
-    if constexpr (BLOCK_ROW) {
-        const int warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-        if ((threadIdx.x & 31) == 0) shared[warp] = s;
-        __syncthreads();
-        s = 0;
-        for (int w = 0; w < warps; ++w) s += shared[w];
-    }
+    const int warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    if ((threadIdx.x & 31) == 0) shared[warp] = s;
+    __syncthreads();
+    s = 0;
+    for (int w = 0; w < warps; ++w) s += shared[w];
     return s;
 }
 
-// The units of a row that this lane holds; zeros behind the end.
-template <int U, bool FULL = false>
-__device__ __forceinline__ void load_row(const void *base, int64_t row, int units, int lane, int lanes, uint32_t (&raw)[U][8]) {
+// The units of a row that this lane holds; zeros from unit `have` on.
+template <int U>
+__device__ __forceinline__ void load_row(const void *base, int64_t row, int have, int units, int lane, int lanes, uint32_t (&raw)[U][8]) {
 #pragma unroll
     for (int j = 0; j < U; ++j) {
-        if (FULL || lane + j * lanes < units) load32(static_cast<const uint8_t *>(base) + (row * units + lane + j * lanes) * 32, raw[j]);
+        if (lane + j * lanes < have) load32(static_cast<const uint8_t *>(base) + (row * units + lane + j * lanes) * 32, raw[j]);
         else
 #pragma unroll
             for (int i = 0; i < 8; ++i) raw[j][i] = 0;
@@ -255,23 +249,24 @@ __device__ __forceinline__ void copy_row(uint32_t (&to)[U][8], const uint32_t (&
         for (int i = 0; i < 8; ++i) to[j][i] = from[j][i];
 }
 
-// Quantisation, NV. A warp works through rows with the next one on its way while it computes ([9331, 2048] bf16 19.4 -> 12.2 us against a warp per
-// row; 9.9 with the quotients of nv_codes and the three-operand maximum, 0.76 of the copy rate); a block that holds one row together does not. Two
-// or four warps to such a row instead of one: 10.8, 11.8.
-template <typename T, int U, bool BLOCK_ROW>
-__global__ void __launch_bounds__(BLOCK_ROW ? kFp4RowWarps * 32 : kFp4WalkWarps * 32, BLOCK_ROW ? 1 : U == 1 ? 4 : U == 2 ? 3 : 2)
-quant_nvfp4_kernel(const T *in, uint8_t *codes, uint8_t *scale, float *row_scale, int rows, int units, int tiles) {
-    __shared__ uint32_t shared[kFp4RowWarps];
+// Quantisation, NV. LANES lanes (half a warp or one) hold a row, and a warp works through rows with the next ones on their way while it computes
+// ([9331, 2048] bf16 19.4 -> 12.2 us against a warp per row; 9.9 with the quotients of nv_codes and the three-operand maximum, 0.76 of the copy
+// rate). Two or four warps to such a row instead of one: 10.8, 11.8. Half a warp: [16384, 256] 4.7 -> 3.3, [32000, 512] 9.0 -> 8.5, [16384, 768] 7.8 -> 6.8.
+template <typename T, int LANES, int U>
+__global__ void __launch_bounds__(kFp4WalkWarps * 32, U == 1 ? 4 : U == 2 ? 3 : 2)
+quant_nvfp4_rows_kernel(const T *in, uint8_t *codes, uint8_t *scale, float *row_scale, int rows, int units, int tiles) {
+    constexpr int kGroups = 32 / LANES;   // rows of a warp at a time
     dependency_wait();
-    const int lanes = BLOCK_ROW ? blockDim.x : 32;
-    const int lane = BLOCK_ROW ? threadIdx.x : threadIdx.x & 31;
-    const int step = BLOCK_ROW ? rows : int(gridDim.x) * kFp4WalkWarps;
-    int row = BLOCK_ROW ? int(blockIdx.x) : int(blockIdx.x) * kFp4WalkWarps + (int(threadIdx.x) >> 5);
-    if (row >= rows) return;
+    const int lane = threadIdx.x & (LANES - 1), group = (threadIdx.x & 31) / LANES;
+    const int step = int(gridDim.x) * kFp4WalkWarps * kGroups;
+    // the loop is the same for all lanes of a warp; rows behind the last are zeros and not written
+    int first = (int(blockIdx.x) * kFp4WalkWarps + (int(threadIdx.x) >> 5)) * kGroups;
     uint32_t raw[U][8], ahead[U][8];
-    load_row<U>(in, row, units, lane, lanes, raw);
-    for (; row < rows; row += step) {
-        if (row + step < rows) load_row<U>(in, row + step, units, lane, lanes, ahead);
+    auto load = [&](int row, uint32_t (&r)[U][8]) { load_row<U>(in, row, row < rows ? units : 0, units, lane, LANES, r); };
+    if (first < rows) load(first + group, raw);
+    for (; first < rows; first += step) {
+        const int row = first + group, mine = row < rows ? units : 0;
+        if (first + step < rows) load(row + step, ahead);
         uint32_t bmax[U], amax = 0;
 #pragma unroll
         for (int j = 0; j < U; ++j) {
@@ -280,12 +275,12 @@ quant_nvfp4_kernel(const T *in, uint8_t *codes, uint8_t *scale, float *row_scale
             bmax[j] = max_bits16(v);
             amax = max(amax, bmax[j]);
         }
-        const float g = nv_row_scale(row_max<BLOCK_ROW>(amax, shared));
-        if (lane == 0) row_scale[row] = g;
+        const float g = nv_row_scale(__reduce_max_sync(LANES == 32 ? kFull : 0xFFFFu << (threadIdx.x & 16), amax));
+        if (lane == 0 && mine) row_scale[row] = g;
 #pragma unroll
         for (int j = 0; j < U; ++j) {
-            const int at = lane + j * lanes;
-            if (at >= units) break;
+            const int at = lane + j * LANES;
+            if (at >= mine) break;
             float2 v[8];
             unpack16<T>(raw[j], v);
             uint32_t s8;
@@ -294,6 +289,37 @@ quant_nvfp4_kernel(const T *in, uint8_t *codes, uint8_t *scale, float *row_scale
             if (at == units - 1) pad_scales(scale, row, units, tiles);
         }
         copy_row<U>(raw, ahead);
+    }
+}
+// A row held by a block.
+template <typename T, int U>
+__global__ void __launch_bounds__(kFp4RowWarps * 32, 1)
+quant_nvfp4_block_kernel(const T *in, uint8_t *codes, uint8_t *scale, float *row_scale, int units, int tiles) {
+    __shared__ uint32_t shared[kFp4RowWarps];
+    dependency_wait();
+    const int lane = threadIdx.x, lanes = blockDim.x;
+    const int64_t row = blockIdx.x;
+    uint32_t raw[U][8], bmax[U], amax = 0;
+    load_row<U>(in, row, units, units, lane, lanes, raw);
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+        float2 v[8];
+        unpack16<T>(raw[j], v);
+        bmax[j] = max_bits16(v);
+        amax = max(amax, bmax[j]);
+    }
+    const float g = nv_row_scale(row_max(amax, shared));
+    if (lane == 0) row_scale[row] = g;
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+        const int at = lane + j * lanes;
+        if (at >= units) break;
+        float2 v[8];
+        unpack16<T>(raw[j], v);
+        uint32_t s8;
+        *reinterpret_cast<uint2 *>(codes + (row * units + at) * 8) = nv_codes(v, bmax[j], g, s8);
+        scale[scale_byte(row, at, tiles)] = uint8_t(s8);
+        if (at == units - 1) pad_scales(scale, row, units, tiles);
     }
 }
 
@@ -545,8 +571,8 @@ rmsnorm_block_kernel(const RmsnormBlockDev p) {
     const int64_t row = blockIdx.x;
     const double inv_n = 1.0 / (double(units) * 16.0), eps = double(p.eps);
     uint32_t x[U][8], res[U][8], post[U][8], gate[U][8], pre[U][8];
-    load_row<U>(p.x, row, units, lane, lanes, x);
-    load_row<U>(p.residual, row, units, lane, lanes, res);
+    load_row<U>(p.x, row, units, units, lane, lanes, x);
+    load_row<U>(p.residual, row, units, units, lane, lanes, res);
     const int64_t gate_at = p.seqlen > 0 ? row / p.seqlen * units : 0;
     auto weights = [&](const void *w, int64_t base, uint32_t (&raw)[U][8]) {
 #pragma unroll
@@ -560,7 +586,7 @@ rmsnorm_block_kernel(const RmsnormBlockDev p) {
         double s[4] = {};
 #pragma unroll
         for (int j = 0; j < U; ++j) add_squares<T>(x[j], s);
-        rx = inv_rms(row_sum<true>((s[0] + s[1]) + (s[2] + s[3]), sums[0]), inv_n, eps);
+        rx = inv_rms(row_sum((s[0] + s[1]) + (s[2] + s[3]), sums[0]), inv_n, eps);
     }
     double s[4] = {};
 #pragma unroll
@@ -575,7 +601,7 @@ rmsnorm_block_kernel(const RmsnormBlockDev p) {
         if constexpr (OUT != kFp4None) add_squares<T>(x[j], s);
     }
     if constexpr (OUT != kFp4None) {
-        const float ry = inv_rms(row_sum<true>((s[0] + s[1]) + (s[2] + s[3]), sums[1]), inv_n, eps);
+        const float ry = inv_rms(row_sum((s[0] + s[1]) + (s[2] + s[3]), sums[1]), inv_n, eps);
         float2 h[U][8];
         uint32_t bmax[U], amax = 0;
         float g = 1.f;
@@ -588,7 +614,7 @@ rmsnorm_block_kernel(const RmsnormBlockDev p) {
             amax = max(amax, bmax[j]);
         }
         if constexpr (OUT == kFp4Nv) {
-            g = nv_row_scale(row_max<true>(amax, maxima));
+            g = nv_row_scale(row_max(amax, maxima));
             if (lane == 0) p.row_scale[row] = g;
         }
 #pragma unroll
@@ -599,20 +625,6 @@ rmsnorm_block_kernel(const RmsnormBlockDev p) {
     }
 }
 
-// How a row of `units` is spread: one warp, or a block of `warps`, and the units of a lane. With few rows a row is spread over as
-// many warps as it has units for.
-struct RowSpread { int per_lane, warps; bool block_row; };
-inline RowSpread row_spread(int rows, int units) {
-    const bool few = rows < 4 * device_sm_count();
-    RowSpread s = {1, 1, false};
-    if (units > 128 || (few && units > 32)) {
-        s.block_row = true;
-        s.per_lane = few && units <= 32 * kFp4RowWarps ? 1 : units <= 256 ? 2 : 4;
-        s.warps = (units + 32 * s.per_lane - 1) / (32 * s.per_lane);
-    }
-    while (s.per_lane * s.warps * 32 < units) s.per_lane *= 2;
-    return s;
-}
 // Blocks of `kernel` that the device holds at once.
 inline int resident_blocks(const void *kernel, int block, int smem = 0) {
     struct Seen { const void *kernel; int dev, smem, blocks; };
@@ -630,22 +642,32 @@ inline int resident_blocks(const void *kernel, int block, int smem = 0) {
     }
     return s.blocks;
 }
+template <typename T, int LANES, int U>
+int launch_quant_nvfp4_rows(const T *in, uint8_t *codes, uint8_t *scale, float *row_scale, int rows, int units, cudaStream_t stream) {
+    constexpr auto kernel = quant_nvfp4_rows_kernel<T, LANES, U>;
+    constexpr int kBlock = kFp4WalkWarps * 32, kRows = kFp4WalkWarps * 32 / LANES;
+    const int blocks = (rows + kRows - 1) / kRows, most = resident_blocks(reinterpret_cast<const void *>(kernel), kBlock);
+    return launch_dependent(kernel, blocks < most ? blocks : most, kBlock, 0, stream, in, codes, scale, row_scale, rows, units, (units + 3) / 4);
+}
+template <typename T, int U>
+int launch_quant_nvfp4_block(const T *in, uint8_t *codes, uint8_t *scale, float *row_scale, int rows, int units, cudaStream_t stream) {
+    return launch_dependent(quant_nvfp4_block_kernel<T, U>, rows, (units + 32 * U - 1) / (32 * U) * 32, 0, stream, in, codes, scale, row_scale, units,
+                            (units + 3) / 4);
+}
+// Few rows: a block each, as many warps as the row has units for. Else half a warp per row up to 768 values, a warp up to 2048, and a block of warps
+// with two units per lane, from 4096 values on four ([4096, 4096] two : four 10.2 : 11.3 us, [1024, 16384] 15.7 : 12.1).
 template <typename T>
-int launch_quant_nvfp4(const void *in, void *codes, void *scale, void *row_scale, int rows, int units, cudaStream_t stream) {
-    const RowSpread s = row_spread(rows, units);
-    using fn = void (*)(const T *, uint8_t *, uint8_t *, float *, int, int, int);
-    static constexpr fn kernels[2][3] = {{quant_nvfp4_kernel<T, 1, false>, quant_nvfp4_kernel<T, 2, false>, quant_nvfp4_kernel<T, 4, false>},
-                                         {quant_nvfp4_kernel<T, 1, true>, quant_nvfp4_kernel<T, 2, true>, quant_nvfp4_kernel<T, 4, true>}};
-    const fn kernel = kernels[s.block_row][s.per_lane >> 1];
-    // a block per row, or as many blocks of walking warps as the device holds
-    int grid = rows, block = s.warps * 32;
-    if (!s.block_row) {
-        block = kFp4WalkWarps * 32;
-        const int blocks = (rows + kFp4WalkWarps - 1) / kFp4WalkWarps, most = resident_blocks(reinterpret_cast<const void *>(kernel), block);
-        grid = blocks < most ? blocks : most;
-    }
-    return launch_dependent(kernel, grid, block, 0, stream, static_cast<const T *>(in), static_cast<uint8_t *>(codes), static_cast<uint8_t *>(scale),
-                            static_cast<float *>(row_scale), rows, units, (units + 3) / 4);
+int launch_quant_nvfp4(const T *in, uint8_t *codes, uint8_t *scale, float *row_scale, int rows, int units, cudaStream_t s) {
+    const bool few = rows < 4 * device_sm_count();
+    if (few && units > 16 && units <= 32 * kFp4RowWarps) return launch_quant_nvfp4_block<T, 1>(in, codes, scale, row_scale, rows, units, s);
+    if (units > 256) return launch_quant_nvfp4_block<T, 4>(in, codes, scale, row_scale, rows, units, s);
+    if (units > 128) return launch_quant_nvfp4_block<T, 2>(in, codes, scale, row_scale, rows, units, s);
+    if (units <= 16) return launch_quant_nvfp4_rows<T, 16, 1>(in, codes, scale, row_scale, rows, units, s);
+    if (units <= 32) return launch_quant_nvfp4_rows<T, 16, 2>(in, codes, scale, row_scale, rows, units, s);
+    if (units <= 48) return launch_quant_nvfp4_rows<T, 16, 3>(in, codes, scale, row_scale, rows, units, s);
+    if (units <= 64) return launch_quant_nvfp4_rows<T, 32, 2>(in, codes, scale, row_scale, rows, units, s);
+    if (units <= 96) return launch_quant_nvfp4_rows<T, 32, 3>(in, codes, scale, row_scale, rows, units, s);
+    return launch_quant_nvfp4_rows<T, 32, 4>(in, codes, scale, row_scale, rows, units, s);
 }
 
 template <typename T, int OUT, int LANES, int U, bool FULL>
@@ -706,9 +728,12 @@ extern "C" int fluke_sm100_quant_fp4(const void *in, void *codes, void *scale, v
     if (!aligned32(in) || !aligned16(codes) || !aligned16(scale)) return (int)cudaErrorMisalignedAddress;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const int units = cols / 16;
-    if (format == FLUKE_SM100_FP4_NV)
-        return bf16 ? launch_quant_nvfp4<__nv_bfloat16>(in, codes, scale, row_scale, rows, units, s)
-                    : launch_quant_nvfp4<__half>(in, codes, scale, row_scale, rows, units, s);
+    if (format == FLUKE_SM100_FP4_NV) {
+        uint8_t *c = static_cast<uint8_t *>(codes), *b = static_cast<uint8_t *>(scale);
+        float *r = static_cast<float *>(row_scale);
+        return bf16 ? launch_quant_nvfp4(static_cast<const __nv_bfloat16 *>(in), c, b, r, rows, units, s)
+                    : launch_quant_nvfp4(static_cast<const __half *>(in), c, b, r, rows, units, s);
+    }
     const int64_t total = int64_t(rows) * units;
     if (format != FLUKE_SM100_FP4_MX || total > INT32_MAX) return (int)cudaErrorInvalidValue;
     const int grid = int((total + 255) / 256), tiles = fp4_tiles(cols, format);
