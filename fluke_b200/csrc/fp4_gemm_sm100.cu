@@ -1114,7 +1114,7 @@ int gemm_fp4_dispatch(const fluke_sm100_gemm_fp4_t *g, cudaStream_t stream) {
 
 extern "C" int fluke_sm100_gemm_fp4(const fluke_sm100_gemm_fp4_t *g, void *stream) {
     using namespace fluke_sm100;
-    if (!g || !fp4_shape_ok(g->M, g->K) || g->N <= 0 || g->N % 8 != 0) return (int)cudaErrorInvalidValue;
+    if (!g || !fp4_shape_ok(g->M, g->K) || g->N <= 0 || g->N > kFp4MaxSize || g->N % 8 != 0) return (int)cudaErrorInvalidValue;
     if (g->format != FLUKE_SM100_FP4_MX && g->format != FLUKE_SM100_FP4_NV) return (int)cudaErrorInvalidValue;
     if (g->M == 0) return 0;
     const bool nv = g->format == FLUKE_SM100_FP4_NV;

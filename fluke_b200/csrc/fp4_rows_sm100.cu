@@ -712,7 +712,9 @@ int launch_rmsnorm_block(const RmsnormBlockDev &p, int out, cudaStream_t stream)
 // Sizes and addresses that every kernel here needs: rows of whole blocks (and of whole 16-byte pieces as codes, which the
 // products ask for), 16-bit tensors on 32 bytes, codes and scales on 16.
 inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-inline bool fp4_shape_ok(int rows, int cols) { return rows >= 0 && cols >= 32 && cols % 32 == 0; }
+// kFp4MaxSize: the next tile's end and a grid's step from the last row still fit 32 bits.
+constexpr int kFp4MaxSize = INT32_MAX - (1 << 20);
+inline bool fp4_shape_ok(int rows, int cols) { return rows >= 0 && rows <= kFp4MaxSize && cols >= 32 && cols <= kFp4MaxSize && cols % 32 == 0; }
 inline int fp4_tiles(int cols, int format) { return (cols / (format == FLUKE_SM100_FP4_MX ? 32 : 16) + 3) / 4; }
 
 }  // namespace

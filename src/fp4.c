@@ -8,7 +8,7 @@
 
 size_t fluke_fp4_scale_bytes(int rows, int cols, int format) {
     size_t block = format == FLUKE_FP4_MX ? 32 : 16, tiles;
-    if (rows <= 0 || cols <= 0 || (format != FLUKE_FP4_MX && format != FLUKE_FP4_NV)) return 0;
+    if (rows <= 0 || cols <= 0 || cols % 32 != 0 || (format != FLUKE_FP4_MX && format != FLUKE_FP4_NV)) return 0;
     tiles = ((size_t)cols + 4 * block - 1) / (4 * block);
     return ((size_t)rows + 127) / 128 * tiles * 512;
 }

@@ -96,6 +96,28 @@ def test_c_entries_refuse(flib):
     assert flib.fluke_gated_mlp_nvfp4_gpu(P, P, P, P, P, P, P, P, P, 0, 4, 64, 64, 0) == invalid
 
 
+def test_sizes_next_to_the_largest_int_are_refused(flib):
+    # rounding such a size up to a tile, or a step from the last row, does not fit 32 bits
+    most, wide = (1 << 31) - 1, (1 << 31) - 32
+    for rows_ in (most, most - 127, most - (1 << 20) + 1):
+        assert flib.fluke_quant_mxfp4_gpu(P, P, P, rows_, 32, 0) == 1
+        assert flib.fluke_quant_nvfp4_gpu(P, P, P, P, rows_, 32, 0) == 1
+        assert flib.fluke_dequant_nvfp4_gpu(P, P, P, P, rows_, 32, 0) == 1
+        assert flib.fluke_gemm_mxfp4_gpu(P, P, P, P, P, rows_, 8, 32, 0) == 1
+        b = L.fluke_rmsnorm_block_t(rows_, 32, 0, 0, P, P, P, P, P, 1.0, 1e-5, P, 0, P, P, P)
+        assert flib.fluke_rmsnorm_block_gpu(ctypes.byref(b)) == 1
+    assert flib.fluke_gemm_mxfp4_gpu(P, P, P, P, P, 1, most - 7, 32, 0) == 1
+    assert flib.fluke_gemm_mxfp4_gpu(P, P, P, P, P, 1, 8, wide, 0) == 1
+    assert flib.fluke_gated_mlp_mxfp4_gpu(P, P, P, P, P, P, P, 1, most - 7, 32, 0) == 1
+    assert flib.fluke_quant_mxfp4_gpu(P, P, P, 1, wide, 0) == 1
+
+
+def test_scale_bytes_of_columns_that_no_operator_takes(flib):
+    for fmt in (1, 2):
+        assert flib.fluke_fp4_scale_bytes(4, 48, fmt) == 0
+        assert flib.fluke_fp4_scale_bytes(4, 31, fmt) == 0
+
+
 def test_c_entry_of_the_norms_refuses(flib):
     def call(**change):
         b = L.fluke_rmsnorm_block_t(4, 64, 0, 0, P, P, P, P, P, 1.0, 1e-5, P, 0, P, P, P)
