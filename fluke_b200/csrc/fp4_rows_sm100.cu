@@ -332,6 +332,7 @@ quant_nvfp4_block_kernel(const T *in, uint8_t *codes, uint8_t *scale, float *row
 // bits, leaves a relative error of 1e-13 before that rounding.
 // Bound by instructions: [32000, 512] to mxfp4 21.3 us (16.4 at the copy rate). With a warp per row it was 23.2 us and some 450 instructions per row;
 // without any access to memory 19.7, without the 64-bit sums as well 13.7. Rows brought ahead by bulk copies into shared memory instead of registers: 24.8.
+// Squares exact in 32 bits and moved to 64 by a shift of their bits instead of conversions: 22.4 -> 26.2.
 __device__ __forceinline__ float inv_rms(double sum, double inv_n, double eps) {
     const double a = fma(sum, inv_n, eps);
     const float f = float(a);
