@@ -776,6 +776,17 @@ extern "C" int fluke_sm100_rmsnorm_block(const fluke_sm100_rmsnorm_block_t *b, v
     if (!aligned32(b->x, b->residual, b->residual_out, quant ? nullptr : b->out) || (quant && !(aligned16(b->out) && aligned16(b->scale))) ||
         !aligned32(b->w_post, b->gate, b->w_pre))
         return (int)cudaErrorMisalignedAddress;
+    // A row is read before it is written, but rows come in any order: an output lies where an input of the same rows does, or apart from it.
+    const uint64_t bytes = uint64_t(b->rows) * b->cols * 2, out_bytes = b->out_format == kFp4None ? 0 : quant ? bytes / 4 : bytes;
+    auto apart = [](const void *a, uint64_t na, const void *c, uint64_t nc) {
+        const uint64_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(c);
+        return na == 0 || nc == 0 || x + na <= y || y + nc <= x;
+    };
+    for (const void *in : {b->x, b->residual}) {
+        if (b->residual_out != in && !apart(b->residual_out, bytes, in, bytes)) return (int)cudaErrorInvalidValue;
+        if ((quant || b->out != in) && !apart(b->out, out_bytes, in, bytes)) return (int)cudaErrorInvalidValue;
+    }
+    if (!apart(b->out, out_bytes, b->residual_out, bytes)) return (int)cudaErrorInvalidValue;
     RmsnormBlockDev p;
     p.x = b->x; p.residual = b->residual; p.w_post = b->w_post; p.gate = b->gate; p.w_pre = b->w_pre;
     p.residual_out = b->residual_out; p.out = b->out;

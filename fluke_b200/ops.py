@@ -207,7 +207,7 @@ def rmsnorm_block(x, residual, post_weight, gate, pre_weight, alpha, eps, seqlen
     """Norms around a block: stream = alpha * residual + gate * norm(x, post_weight), then norm(stream, pre_weight)
     for the next block, as 16-bit values (quant None) or quantised ("mxfp4", "nvfp4"). gate [cols], or
     [ceil(rows / seqlen), cols] with seqlen > 0. post_weight, gate and pre_weight may be None. Returns the
-    stream (written to `residual_out`, which may be `residual`, or to a new tensor) followed by the
+    stream (written to `residual_out`, which may be `residual` or `x`, or to a new tensor) followed by the
     next block's input: (stream, out), (stream, codes, scale[, row_scale]), or (stream,) without pre_weight."""
     if quant not in _QUANT:
         raise ValueError(f"quant is None, 'mxfp4' or 'nvfp4', not {quant!r}")

@@ -591,9 +591,9 @@ typedef struct {
     const void *gate;           /* or NULL                                                          */
     const void *pre_weight;     /* [hidden_dim] or NULL                                             */
     float alpha, eps;
-    void *residual_out;         /* [n_tokens, hidden_dim]; may be residual itself                   */
+    void *residual_out;         /* [n_tokens, hidden_dim]; may be residual or x itself              */
     int out_format;             /* 0: 16 bits, FLUKE_FP4_MX, FLUKE_FP4_NV                           */
-    void *out;                  /* 16-bit values or codes                                           */
+    void *out;                  /* 16-bit values (may be x or residual itself) or codes; apart from residual_out */
     void *scale;                /* quantised: block scales                                          */
     void *row_scale;            /* nvfp4: f32 [n_tokens]                                            */
 } fluke_rmsnorm_block_t;

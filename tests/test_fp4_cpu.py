@@ -135,6 +135,19 @@ def test_c_entry_of_the_norms_refuses(flib):
         assert call(**change) == 716, change
 
 
+def test_norms_refuse_outputs_that_overlap_other_rows(flib):
+    # [4, 64]: 512 bytes. A row's output may take the place of its own input, not of another row's.
+    def call(**change):
+        b = L.fluke_rmsnorm_block_t(4, 64, 0, 0, P, P + 4096, P + 8192, 0, P + 8192, 1.0, 1e-5, P + 16384, 0, P + 20480, P + 24576, P + 28672)
+        for k, v in change.items():
+            setattr(b, k, v)
+        return flib.fluke_rmsnorm_block_gpu(ctypes.byref(b))
+    for change in (dict(residual_out=P + 128), dict(residual_out=P + 4096 + 128), dict(residual_out=P + 4096 - 128), dict(residual=P + 16384 + 384),
+                   dict(out=P + 128), dict(out=P + 4096 - 32), dict(out=P + 16384), dict(out=P + 16384 + 384),
+                   dict(out_format=1, out=P), dict(out_format=1, out=P + 4096), dict(out_format=2, out=P + 16384 + 496)):
+        assert call(**change) == 1, change
+
+
 def test_operators_refuse_cpu_tensors():
     x = torch.zeros(4, 64, dtype=torch.float16)
     codes, scale = prep.quantize_mxfp4(x)

@@ -3,11 +3,13 @@
 Codes, scales, row scales and what is read back are compared bit for bit, and so are the stream and the
 next input of the fused norms (their operations are defined one by one). Products are held to half
 a step of the 16-bit type plus the bound of an f32 sum of K products, K * 2^-24 * sum |a b|."""
+import ctypes
+
 import numpy as np
 import pytest
 import torch
 
-from fluke_b200 import ops
+from fluke_b200 import lib as L, ops
 from oracle import fp4
 
 pytestmark = pytest.mark.gpu
@@ -254,6 +256,26 @@ def test_norms_in_place_on_the_stream(m, k, quant):
     assert got[0].data_ptr() == res.data_ptr()
     same = lambda a, b: torch.equal(bits(a), bits(b)) if a.dim() != 3 else torch.equal(*(torch.from_numpy(fp4.untile_scales(v.cpu().numpy(), m, k // 32)) for v in (a, b)))
     assert all(same(a, b) for a, b in zip(want, got))
+
+
+@pytest.mark.parametrize("m,k", [(7, 1024), (1300, 512), (1300, 2080)])
+def test_norms_in_place_of_the_input(flib, m, k):
+    g = torch.Generator(device=DEV).manual_seed(m)
+    t = lambda *s: torch.randn(*s, generator=g, device=DEV).half()
+    x, res, w = t(m, k), t(m, k), t(k)
+    want = ops.rmsnorm_block(x, res, w, None, w, 0.5, 1e-5)
+    a = x.clone()
+    got = ops.rmsnorm_block(a, res, w, None, w, 0.5, 1e-5, residual_out=a)
+    assert got[0].data_ptr() == a.data_ptr() and all(torch.equal(bits(u), bits(v)) for u, v in zip(want, got))
+    a, r = x.clone(), res.clone()   # the stream in the place of the residual, the next input in that of x
+    torch.cuda.synchronize()
+    b = L.fluke_rmsnorm_block_t(m, k, 0, 0, a.data_ptr(), r.data_ptr(), w.data_ptr(), 0, w.data_ptr(), 0.5, 1e-5, r.data_ptr(), 0, a.data_ptr(), 0, 0)
+    assert flib.fluke_rmsnorm_block_gpu(ctypes.byref(b)) == 0
+    torch.cuda.synchronize()
+    assert torch.equal(bits(r), bits(want[0])) and torch.equal(bits(a), bits(want[1]))
+    with pytest.raises(RuntimeError):
+        rows_ = torch.zeros(m + 1, k, dtype=torch.float16, device=DEV)
+        ops.rmsnorm_block(x, rows_[1:], w, None, w, 0.5, 1e-5, residual_out=rows_[:-1])
 
 
 def test_nothing_is_written_behind_the_rows(flib):
