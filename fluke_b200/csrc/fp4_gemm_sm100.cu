@@ -621,7 +621,8 @@ gemm_fp4_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) {
-                    tma_store_2d(&tm_out, staging, c0, m0);
+                    if (p.passes_by) tma_store_2d(&tm_out, staging, c0, m0, l2_evict_first());
+                    else tma_store_2d(&tm_out, staging, c0, m0);
                     tma_store_commit();
                 }
             }
@@ -994,7 +995,8 @@ int gemm_fp4_pair_launch(const fluke_sm100_gemm_fp4_t *g, cudaStream_t stream) {
     p.stages_k = (g->K + kFp4StageK - 1) / kFp4StageK;
     p.last_steps = (g->K - (p.stages_k - 1) * kFp4StageK + 63) / 64;
     p.ga = g->a_row; p.gb = g->b_row; p.gb2 = g->b2_row;
-    // such lines drive out what the next kernels read: gated [32000, 512] x 2 [2048, 512] (131 MB) 36.8 : 36.5 us, in a long loop 44.5 : 43.3
+    // such lines drive out what the next kernels read: gated [32000, 512] x 2 [2048, 512] (131 MB) 36.8 : 36.5 us, in a long loop 44.5 : 43.3;
+    // streamed [8192, 4096] x [8192, 4096] (134 MB) 110.0 : 109.6, 127.8 : 127.0
     p.passes_by = int64_t(g->M) * g->N * 2 > int64_t(device_l2_bytes()) / 8 * 7;
     CUtensorMap tm_a, tm_b, tm_b2, tm_sfa, tm_sfb, tm_sfb2, tm_out;
     const uint64_t pitch = uint64_t(g->K) / 2, sf_words = uint64_t(fp4_tiles(g->K, FMT)) * 64;
