@@ -1,0 +1,64 @@
+"""4-bit operators where ordinary values do not take them, against oracle/fp4.py as in test_fp4_gpu.py."""
+import numpy as np
+import pytest
+import torch
+
+from fluke_b200 import ops
+from oracle import fp4
+from test_fp4_gpu import DEV, GATED, TYPES, half_step, on_gpu
+
+pytestmark = pytest.mark.gpu
+
+# (rows, weight rows, K) of the split, the resident and the streamed form of the products
+FORMS = [(5, 264, 96), (64, 136, 2080), (2600, 1032, 96), (2600, 1032, 1024), (2600, 1032, 2080)]
+
+
+def one_term(m, n, k, fmt, values, weights):
+    """a with values[r % len] and b with weights[c % len] in the last column and zeros elsewhere: sums are single products, which f32 holds."""
+    a, b = np.zeros((m, k), np.float32), np.zeros((n, k), np.float32)
+    a[:, -1] = np.resize(np.asarray(values, np.float32), m)
+    b[:, -1] = np.resize(np.asarray(weights, np.float32), n)
+    return fp4.quantise(a, fmt), fp4.quantise(b, fmt)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("fmt", ["mx", "nv"])
+@pytest.mark.parametrize("m,n,k", FORMS)
+def test_gates_at_which_silu_is_small(m, n, k, fmt, dtype):
+    """Gates from -80 (bf16; -12 in f16) to 40, under an up that brings the result back into the type. Gate and up are exact, so what is left is the rounding and the
+    relative error of silu * up in f32: ex2.approx 2^-22 and its argument's 2^-23 |g|, 1 + exp(-g) 2^-24, rcp.approx 2^-23 and two products of
+    2^-24 each, below (|g| + 5) 2^-23. Some gates lie below -87, where silu may be zero: it is less than 2^-119 there."""
+    low, high = (80, 40) if dtype == "bf16" else (12, 12)
+    steps = np.concatenate(([-1000, -100], -np.geomspace(low, 1e-3, 61), np.geomspace(1e-3, high, 30)))
+    up = np.exp2(np.round(np.where(steps < -1, np.minimum(-steps * 1.4427, 115), 1))) if dtype == "bf16" else np.where(np.arange(len(steps)) % 2, 8.0, -3.0)
+    a, b = one_term(m, n, k, fmt, (1.0, 0.75, 0.5, 1.0), steps)
+    u = one_term(m, n, k, fmt, (1.0,), up)[1]
+    va, vb, vu = (fp4.values(*q, fmt) for q in (a, b, u))
+    gate, lift = np.outer(va[:, -1], vb[:, -1]), np.outer(va[:, -1], vu[:, -1])
+    want = gate * np.exp(np.minimum(gate, 0)) / (1 + np.exp(-np.abs(gate))) * lift
+    got = GATED[fmt](*on_gpu(a), *on_gpu(b), *on_gpu(u), dtype=TYPES[dtype]).cpu().double().numpy()
+    err = np.abs(want) * (np.abs(gate) + 5) * 2.0 ** -23
+    tol = half_step(np.abs(want) + err, dtype) + err + np.where(gate < -87, np.abs(lift) * 2.0 ** -119, 0)
+    assert (np.abs(got - want) <= tol).all(), (np.abs(got - want) / tol).max()
+
+
+@pytest.mark.parametrize("fmt", ["mx", "nv"])
+@pytest.mark.parametrize("m,n,k", FORMS)
+def test_a_weight_row_without_a_value_stays_alone(m, n, k, fmt):
+    """A gate row, an up row with an infinity: its column is NaN, the neighbours are what they are without it."""
+    g = torch.Generator().manual_seed(n)
+    a, b, u = (fp4.quantise(torch.randn(r, k, generator=g).numpy(), fmt) for r in (m, n, n))
+    want = GATED[fmt](*on_gpu(a), *on_gpu(b), *on_gpu(u), dtype=torch.bfloat16)
+
+    def spoiled(q, rows_):
+        codes, scale, row = (None if t is None else t.copy() for t in q)
+        for r in rows_:
+            codes[r, :fp4.BLOCK[fmt]], scale[r, 0] = 0, 255 if fmt == "mx" else 0x7F
+            if row is not None:
+                row[r] = np.nan
+        return codes, scale, row
+    got = GATED[fmt](*on_gpu(a), *on_gpu(spoiled(b, (6, 37))), *on_gpu(spoiled(u, (101, n - 2))), dtype=torch.bfloat16)
+    bad = torch.zeros(n, dtype=torch.bool)
+    bad[[6, 37, 101, n - 2]] = True
+    assert torch.isnan(got[:, bad.to(DEV)]).all()
+    assert torch.equal(got[:, ~bad.to(DEV)], want[:, ~bad.to(DEV)])
