@@ -6,8 +6,8 @@
 // The tensor cores take the codes as they are stored and apply the block scales themselves
 // (tcgen05.mma .block_scale, kind mxf4 and mxf4nvf4: 64 values of K per instruction, f32 accumulators in tensor
 // memory), so nothing is decoded on the way: TMA brings 128-byte-swizzled blocks of 256 values of K per row and the scale tiles that
-// belong to them, and tcgen05.cp moves those to tensor memory, where the instruction reads them. Row scales are powers of two and are
-// applied to the accumulators, which is exact.
+// belong to them, and tcgen05.cp moves those to tensor memory, where the instruction reads them. Row scales are applied to the
+// accumulators (scale_rows); the quantiser's are powers of two, for which that is exact.
 //
 // Three forms, by what bounds them (gemm_fp4_dispatch chooses):
 //   split      few rows or few tiles: latency, and reading the weights. One tile per CTA, K split over a cluster.
@@ -102,6 +102,25 @@ __device__ __forceinline__ void cluster_sync_threads() {
 // The two halves of it; without ordering memory.
 __device__ __forceinline__ void cluster_arrive_relaxed() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
+// acc * ga * gb for two columns of a row (NV), in an order that leaves f32 only where the result does: ga is given as low * high, min(ga, 1) and max(ga, 1).
+// A sum that is not zero is a multiple of 2^-20 and the quantiser's scales are at least 2^-100, so acc * low is exact; and where high is above one (low is one),
+// a product with gb that overflows does so for good. With ga as one factor a row of 1e36 times weights of 0.01 overflowed at acc * ga. The resident form, bound
+// by its epilogue, leaves the third product out where no row of a warp has a scale above one (amax above 2688): always : where needed [32000, 512] x [1536, 512] 31.1 : 28.5 us,
+// gated with 2 [2048, 512] 70 : 60.
+struct RowScale {
+    float2 low, high;
+    __device__ __forceinline__ explicit RowScale(float ga) {
+        const bool small = ga < 1.f;   // a NaN is high
+        low = small ? make_float2(ga, ga) : make_float2(1.f, 1.f);
+        high = small ? make_float2(1.f, 1.f) : make_float2(ga, ga);
+    }
+};
+template <bool HIGH = true>   // false: high is one
+__device__ __forceinline__ float2 scale_rows(float2 acc, const RowScale &ga, float2 gb) {
+    const float2 v = mul2(mul2(acc, ga.low), gb);
+    return HIGH ? mul2(v, ga.high) : v;
+}
+
 __device__ __forceinline__ float ex2_approx(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -335,16 +354,14 @@ gemm_fp4_split_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_con
                     v[i >> 1][(i & 1) * 4 + 3] += x.w;
                 }
             const int out_row = m0 + row0 + row;
-            float ga = 1.f;
-            if constexpr (FMT == FLUKE_SM100_FP4_NV) ga = p.ga[out_row];
+            const RowScale ga(FMT == FLUKE_SM100_FP4_NV ? p.ga[out_row] : 1.f);
             uint32_t w[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 float2 y = make_float2(v[0][2 * i], v[0][2 * i + 1]), u = make_float2(v[kWeights - 1][2 * i], v[kWeights - 1][2 * i + 1]);
                 if constexpr (FMT == FLUKE_SM100_FP4_NV) {
-                    const float2 ga2 = make_float2(ga, ga);
-                    y = mul2(mul2(y, ga2), *reinterpret_cast<const float2 *>(p.gb + col + 2 * i));
-                    if constexpr (GATED) u = mul2(mul2(u, ga2), *reinterpret_cast<const float2 *>(p.gb2 + col + 2 * i));
+                    y = scale_rows(y, ga, *reinterpret_cast<const float2 *>(p.gb + col + 2 * i));
+                    if constexpr (GATED) u = scale_rows(u, ga, *reinterpret_cast<const float2 *>(p.gb2 + col + 2 * i));
                 }
                 if constexpr (GATED) y = silu_times(y, u);
                 w[i] = pack2(y, T());
@@ -589,7 +606,7 @@ gemm_fp4_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
             __syncwarp();
             if (lane == 0) mbar_arrive_cluster(tempty);
             if (m0 >= p.M) continue;
-            const float2 ga2 = make_float2(ga, ga);
+            const RowScale ga2(ga);
 #pragma unroll
             for (int g = 0; g < (GATED ? 1 : 2); ++g) {
                 const int c0 = n0 + (GATED ? half * 64 : half * 128 + g * 64);
@@ -616,11 +633,11 @@ gemm_fp4_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
                                 gb = *reinterpret_cast<const float4 *>(p.gb + col);
                                 if (GATED) gu = *reinterpret_cast<const float4 *>(p.gb2 + col);
                             }
-                            v[0] = mul2(mul2(v[0], ga2), make_float2(gb.x, gb.y));
-                            v[1] = mul2(mul2(v[1], ga2), make_float2(gb.z, gb.w));
+                            v[0] = scale_rows(v[0], ga2, make_float2(gb.x, gb.y));
+                            v[1] = scale_rows(v[1], ga2, make_float2(gb.z, gb.w));
                             if constexpr (GATED) {
-                                u[0] = mul2(mul2(u[0], ga2), make_float2(gu.x, gu.y));
-                                u[1] = mul2(mul2(u[1], ga2), make_float2(gu.z, gu.w));
+                                u[0] = scale_rows(u[0], ga2, make_float2(gu.x, gu.y));
+                                u[1] = scale_rows(u[1], ga2, make_float2(gu.z, gu.w));
                             }
                         }
 #pragma unroll
@@ -884,7 +901,6 @@ gemm_fp4_resident_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_
             const int n = run.n, m0 = run.m * 256 + rank * 128 + q * 32, n0 = n * BN_OUT;
             float ga = 1.f;
             if (FMT == FLUKE_SM100_FP4_NV && m0 + lane < p.M) ga = p.ga[m0 + lane];
-            const float2 ga2 = make_float2(ga, ga);
 #pragma unroll 1
             for (int half = 0; half < (GATED ? 1 : 2) && ok; ++half) {
                 uint32_t a[32], u[GATED ? 32 : 1];
@@ -895,25 +911,43 @@ gemm_fp4_resident_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_
                 if (m0 >= p.M || c0 >= p.N) continue;
                 if (lane == 0) tma_store_wait_read<0>();
                 __syncwarp();
+                const RowScale ga2(ga);
+                auto finish = [&](auto high) {   // high: some row of the warp has a scale above one
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    uint32_t w[4];
+                    for (int j = 0; j < 4; ++j) {
+                        float2 v[4];
+                        [[maybe_unused]] float2 up[4];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int c = 8 * j + 2 * i;
-                        float2 v = make_float2(__uint_as_float(a[c]), __uint_as_float(a[c + 1])), up;
-                        if constexpr (GATED) up = make_float2(__uint_as_float(u[c]), __uint_as_float(u[c + 1]));
-                        if constexpr (FMT == FLUKE_SM100_FP4_NV) {
-                            const bool in = c0 + c < p.N;  // N is even
-                            const float2 zero = make_float2(0.f, 0.f);
-                            v = mul2(mul2(v, ga2), in ? *reinterpret_cast<const float2 *>(p.gb + c0 + c) : zero);
-                            if constexpr (GATED) up = mul2(mul2(up, ga2), in ? *reinterpret_cast<const float2 *>(p.gb2 + c0 + c) : zero);
+                        for (int i = 0; i < 4; ++i) {
+                            v[i] = make_float2(__uint_as_float(a[8 * j + 2 * i]), __uint_as_float(a[8 * j + 2 * i + 1]));
+                            if constexpr (GATED) up[i] = make_float2(__uint_as_float(u[8 * j + 2 * i]), __uint_as_float(u[8 * j + 2 * i + 1]));
                         }
-                        if constexpr (GATED) v = silu_times(v, up);
-                        w[i] = pack2(v, T());
+                        auto scale = [&](float2 (&x)[4], const float *g) {   // eight columns; N is a multiple of eight
+                            float4 lo = make_float4(0.f, 0.f, 0.f, 0.f), hi = lo;
+                            if (c0 + 8 * j < p.N) {
+                                lo = *reinterpret_cast<const float4 *>(g + c0 + 8 * j);
+                                hi = *reinterpret_cast<const float4 *>(g + c0 + 8 * j + 4);
+                            }
+                            x[0] = scale_rows<high>(x[0], ga2, make_float2(lo.x, lo.y));
+                            x[1] = scale_rows<high>(x[1], ga2, make_float2(lo.z, lo.w));
+                            x[2] = scale_rows<high>(x[2], ga2, make_float2(hi.x, hi.y));
+                            x[3] = scale_rows<high>(x[3], ga2, make_float2(hi.z, hi.w));
+                        };
+                        if constexpr (FMT == FLUKE_SM100_FP4_NV) {
+                            scale(v, p.gb);
+                            if constexpr (GATED) scale(up, p.gb2);
+                        }
+                        uint32_t w[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            if constexpr (GATED) v[i] = silu_times(v[i], up[i]);
+                            w[i] = pack2(v[i], T());
+                        }
+                        *reinterpret_cast<uint4 *>(staging + tile_offset<32>(lane, j)) = make_uint4(w[0], w[1], w[2], w[3]);
                     }
-                    *reinterpret_cast<uint4 *>(staging + tile_offset<32>(lane, j)) = make_uint4(w[0], w[1], w[2], w[3]);
-                }
+                };
+                if (FMT == FLUKE_SM100_FP4_NV && __any_sync(0xffffffffu, !(ga <= 1.f))) finish(std::true_type());
+                else finish(std::false_type());
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) {

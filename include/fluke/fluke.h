@@ -559,7 +559,8 @@ int fluke_dequant_mxfp4_gpu(const void *in, const void *scale, void *out, int n_
 int fluke_dequant_nvfp4_gpu(const void *in, const void *scale, const void *row_scale, void *out, int n_tokens,
                             int hidden_dim, int dtype);
 
-/* out [M,N] = a [M,K] @ b [N,K]^T, f32 accumulation, rounded once. K % 32 == 0, N % 8 == 0, any M. */
+/* out [M,N] = a [M,K] @ b [N,K]^T, f32 accumulation, rounded once. K % 32 == 0, N % 8 == 0, any M. Row scales may be any positive
+ * f32: powers of two, as the quantiser gives them, are applied exactly wherever the result is a number of f32. */
 int fluke_gemm_mxfp4_gpu(void *out, const void *a, const void *a_scale, const void *b, const void *b_scale, int M, int N,
                          int K, int dtype);
 int fluke_gemm_nvfp4_gpu(void *out, const void *a, const void *a_scale, const void *a_row, const void *b,

@@ -5,7 +5,7 @@ import torch
 
 from fluke_b200 import ops
 from oracle import fp4
-from test_fp4_gpu import DEV, GATED, TYPES, half_step, on_gpu
+from test_fp4_gpu import DEV, GATED, GEMM, TYPES, half_step, on_gpu
 
 pytestmark = pytest.mark.gpu
 
@@ -62,3 +62,67 @@ def test_a_weight_row_without_a_value_stays_alone(m, n, k, fmt):
     bad[[6, 37, 101, n - 2]] = True
     assert torch.isnan(got[:, bad.to(DEV)]).all()
     assert torch.equal(got[:, ~bad.to(DEV)], want[:, ~bad.to(DEV)])
+
+
+def random_rows(seed, m, k, scale, fmt="nv"):
+    x = torch.randn(m, k, generator=torch.Generator().manual_seed(seed))
+    x[m // 3] = 0
+    return fp4.quantise((x * scale).bfloat16().double().numpy(), fmt)
+
+
+def gated_bound(va, vb, vu, gate, up, k):
+    """Of silu(gate) * up with sums of K products in f32 (the derivative of silu is below 1.1)."""
+    dg, du = (k * 2.0 ** -24 * (np.abs(va) @ np.abs(w).T) for w in (vb, vu))
+    silu = gate * np.exp(np.minimum(gate, 0)) / (1 + np.exp(-np.abs(gate)))
+    return silu * up, np.abs(up) * 1.1 * dg + np.abs(silu) * du + 1.1 * dg * du + np.abs(silu * up) * (np.minimum(np.abs(gate), 87) + 5) * 2.0 ** -23
+
+
+def close(got, want, tol, dtype):
+    """Within tol and half a step, or infinite where the type holds no such number (from half a step above its largest one on)."""
+    top = torch.finfo(TYPES[dtype]).max * (1 + torch.finfo(TYPES[dtype]).eps / 4)
+    return ((np.abs(got - want) <= tol + half_step(want, dtype)) | (np.isinf(got) & (got * want > 0) & (np.abs(want) + tol >= top))).all()
+
+
+@pytest.mark.parametrize("sa,sb", [(1e36, 0.01), (0.01, 1e36), (1e37, 1e-30), (1e-30, 1e37), (1e-22, 1e-12)])
+@pytest.mark.parametrize("m,n,k", FORMS)
+def test_row_scales_that_are_far_apart(m, n, k, sa, sb):
+    """nvfp4 rows and weights of very different magnitudes: finite results stay finite, in either operand's favour."""
+    a, b = random_rows(m, m, k, sa), random_rows(n + 1, n, k, sb)
+    va, vb = fp4.values(*a, "nv"), fp4.values(*b, "nv")
+    want = va @ vb.T
+    assert np.abs(want).max() < 3e38
+    got = GEMM["nv"](*on_gpu(a), *on_gpu(b), dtype=torch.bfloat16).cpu().double().numpy()
+    tol = half_step(want, "bf16") + k * 2.0 ** -24 * (np.abs(va) @ np.abs(vb).T)
+    assert (np.abs(got - want) <= tol).all()
+    # gates of that size, finite and mostly far below zero or above, under an up near one; rows of zeros give a gate of zero
+    u = random_rows(n + 2, n, k, 1.0 / sa)
+    vu = fp4.values(*u, "nv")
+    up = va @ vu.T
+    want, tol = gated_bound(va, vb, vu, va @ vb.T, up, k)
+    keep = np.abs(want) < 3e38
+    got = GATED["nv"](*on_gpu(a), *on_gpu(b), *on_gpu(u), dtype=torch.bfloat16).cpu().double().numpy()
+    assert np.isfinite(got[keep]).all() and (np.abs(got - want) <= tol + half_step(want, "bf16"))[keep].all()
+
+
+@pytest.mark.parametrize("m,n,k", FORMS)
+def test_an_up_of_any_size_under_a_gate_of_zero(m, n, k):
+    a, b, u = random_rows(1, m, k, 1e36), random_rows(2, n, k, 0.0), random_rows(3, n, k, 0.01)
+    got = GATED["nv"](*on_gpu(a), *on_gpu(b), *on_gpu(u), dtype=torch.bfloat16)
+    assert (got == 0).all()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("m,n,k", FORMS)
+def test_row_scales_that_are_no_powers_of_two(m, n, k, dtype):
+    """Published nvfp4 weights carry one f32 per tensor: repeated per row it is a row scale like any other (two more roundings of 2^-24)."""
+    a, b, u = random_rows(1, m, k, 1.0), random_rows(2, n, k, 1.0 / k ** 0.5), random_rows(3, n, k, 1.0 / k ** 0.5)
+    g = np.random.default_rng(4)
+    a = (a[0], a[1], (a[2] * g.uniform(0.5, 2, m)).astype(np.float32))
+    b, u = ((q[0], q[1], np.full(n, q[2].max() * f, np.float32)) for q, f in ((b, 0.7), (u, 1.3)))
+    va, vb, vu = (fp4.values(*q, "nv") for q in (a, b, u))
+    gate, up = va @ vb.T, va @ vu.T
+    got = GEMM["nv"](*on_gpu(a), *on_gpu(b), dtype=TYPES[dtype]).cpu().double().numpy()
+    assert close(got, gate, k * 2.0 ** -24 * (np.abs(va) @ np.abs(vb).T) + np.abs(gate) * 2.0 ** -23, dtype)
+    want, tol = gated_bound(va, vb, vu, gate, up, k + 2)   # two more roundings in either sum
+    got = GATED["nv"](*on_gpu(a), *on_gpu(b), *on_gpu(u), dtype=TYPES[dtype]).cpu().double().numpy()
+    assert close(got, want, tol, dtype)
