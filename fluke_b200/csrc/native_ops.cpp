@@ -407,7 +407,7 @@ struct Fp4 {
 Fp4 fp4_matrix(PyObject *codes, PyObject *scale, PyObject *row, bool nv, const char *what, const at::Tensor *like) {
     const at::Tensor &c = required(codes, 2), &s = required(scale);
     const at::Tensor *r = nv ? &required(row) : nullptr;
-    if (!nv && row != Py_None) refuse("fluke_b200.ops: %s has row scales, a has none", what);
+    if (!nv && row != Py_None) refuse("fluke_b200.ops: row scales of %s, mxfp4 has none", what);
     const int64_t rows = c.size(0), cols = 2 * c.size(1), block = nv ? 16 : 32;
     if (!like) like = &c;
     expect(c, what, at::kByte, c.sizes(), *like);
@@ -459,9 +459,9 @@ PyObject *quant_fp4(Args a) {
     return wrap_all({&codes, &scale, nv ? &row : nullptr});
 }
 
-// codes, scale, row_scale or None (mxfp4), dtype
+// codes, scale, row_scale (mxfp4: None), dtype, nv
 PyObject *dequant_fp4(Args a) {
-    const bool nv = a[2] != Py_None;
+    const bool nv = truth(a[4]);
     const Fp4 q = fp4_matrix(a[0], a[1], a[2], nv, "the codes", nullptr);
     const at::ScalarType dtype = out_type(a[3]);
     const int type = activation_type(dtype);
@@ -474,9 +474,9 @@ PyObject *dequant_fp4(Args a) {
     return wrap(out);
 }
 
-// a: codes, scale, row scale or None (mxfp4); b the same; up the same or three times None; dtype
+// a: codes, scale, row scale (mxfp4: None); b the same; up the same (not gated: three times None); dtype, nv, gated
 PyObject *gemm_fp4(Args v) {
-    const bool nv = v[2] != Py_None, gated = v[6] != Py_None;
+    const bool nv = truth(v[10]), gated = truth(v[11]);
     const at::ScalarType dtype = out_type(v[9]);
     const int type = activation_type(dtype);
     const Fp4 a = fp4_matrix(v[0], v[1], v[2], nv, "a", nullptr), b = fp4_matrix(v[3], v[4], v[5], nv, gated ? "gate" : "b", &a.codes);
@@ -573,7 +573,7 @@ PyMethodDef methods[] = {
     {"bind", bind, METH_O, nullptr}, {"names", names, METH_NOARGS, nullptr},
     FAST(rmsnorm, 6), FAST(rmsnorm_quant, 7), FAST(quant, 4), FAST(dequant_transpose, 3), FAST(rotary_emb, 11), FAST(rotary_qkv, 4),
     FAST(silu_mul, 1), FAST(flstm_step, 4), FAST(qkv_rotary, 11), FAST(gated_mlp, 10), FAST(gemm_i8, 5), FAST(gemm_fp8, 4),
-    FAST(down_proj, 6), FAST(lstm_step, 6), FAST(quant_fp4, 2), FAST(dequant_fp4, 4), FAST(gemm_fp4, 10), FAST(rmsnorm_block, 10), {nullptr, nullptr, 0, nullptr}};
+    FAST(down_proj, 6), FAST(lstm_step, 6), FAST(quant_fp4, 2), FAST(dequant_fp4, 5), FAST(gemm_fp4, 12), FAST(rmsnorm_block, 10), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

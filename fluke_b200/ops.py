@@ -178,29 +178,29 @@ def quant_nvfp4(x):
 
 
 def dequant_mxfp4(codes, scale, dtype=torch.float16):
-    return _N.dequant_fp4(codes, scale, None, dtype)
+    return _N.dequant_fp4(codes, scale, None, dtype, False)
 
 
 def dequant_nvfp4(codes, scale, row_scale, dtype=torch.float16):
-    return _N.dequant_fp4(codes, scale, row_scale, dtype)
+    return _N.dequant_fp4(codes, scale, row_scale, dtype, True)
 
 
 def gemm_mxfp4(a, a_scale, b, b_scale, dtype=torch.float16):
     """[M, N] = a [M, K] @ b [N, K]^T of two quantised matrices."""
-    return _N.gemm_fp4(a, a_scale, None, b, b_scale, None, None, None, None, dtype)
+    return _N.gemm_fp4(a, a_scale, None, b, b_scale, None, None, None, None, dtype, False, False)
 
 
 def gemm_nvfp4(a, a_scale, a_row, b, b_scale, b_row, dtype=torch.float16):
-    return _N.gemm_fp4(a, a_scale, a_row, b, b_scale, b_row, None, None, None, dtype)
+    return _N.gemm_fp4(a, a_scale, a_row, b, b_scale, b_row, None, None, None, dtype, True, False)
 
 
 def gated_mlp_mxfp4(a, a_scale, gate, gate_scale, up, up_scale, dtype=torch.float16):
     """[M, N] = silu(a @ gate^T) * (a @ up^T), gate and up [N, K]."""
-    return _N.gemm_fp4(a, a_scale, None, gate, gate_scale, None, up, up_scale, None, dtype)
+    return _N.gemm_fp4(a, a_scale, None, gate, gate_scale, None, up, up_scale, None, dtype, False, True)
 
 
 def gated_mlp_nvfp4(a, a_scale, a_row, gate, gate_scale, gate_row, up, up_scale, up_row, dtype=torch.float16):
-    return _N.gemm_fp4(a, a_scale, a_row, gate, gate_scale, gate_row, up, up_scale, up_row, dtype)
+    return _N.gemm_fp4(a, a_scale, a_row, gate, gate_scale, gate_row, up, up_scale, up_row, dtype, True, True)
 
 
 def rmsnorm_block(x, residual, post_weight, gate, pre_weight, alpha, eps, seqlen=0, quant=None, residual_out=None):

@@ -126,3 +126,15 @@ def test_row_scales_that_are_no_powers_of_two(m, n, k, dtype):
     want, tol = gated_bound(va, vb, vu, gate, up, k + 2)   # two more roundings in either sum
     got = GATED["nv"](*on_gpu(a), *on_gpu(b), *on_gpu(u), dtype=TYPES[dtype]).cpu().double().numpy()
     assert close(got, want, tol, dtype)
+
+
+def test_a_missing_part_is_not_another_operator():
+    """Without row scales nvfp4 bytes are not mxfp4 bytes (up to 64 columns their scales have the same shape), and without an up there is no gated product."""
+    x, w = (torch.randn(8, 64, device=DEV).half() for _ in range(2))
+    nv, wn, mx, wm = ops.quant_nvfp4(x), ops.quant_nvfp4(w), ops.quant_mxfp4(x), ops.quant_mxfp4(w)
+    for call in (lambda: ops.dequant_nvfp4(*nv[:2], None), lambda: ops.gemm_nvfp4(*nv[:2], None, *wn[:2], None), lambda: ops.gemm_nvfp4(*nv, *wn[:2], None),
+                 lambda: ops.gemm_nvfp4(*nv[:2], None, *wn), lambda: ops.gated_mlp_nvfp4(*nv[:2], None, *wn[:2], None, *wn[:2], None),
+                 lambda: ops.gated_mlp_nvfp4(*nv, *wn, *wn[:2], None), lambda: ops.gated_mlp_nvfp4(*nv, *wn, None, None, None),
+                 lambda: ops.gated_mlp_mxfp4(*mx, *wm, None, None), lambda: ops.gated_mlp_mxfp4(*mx, *wm, None, wm[1]), lambda: ops.gemm_mxfp4(*mx, None, None)):
+        with pytest.raises((TypeError, ValueError)):
+            call()
