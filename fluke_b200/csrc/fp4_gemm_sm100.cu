@@ -20,6 +20,8 @@
 // The scale tiles of a stage have tensor-memory columns of their own: they are overwritten when the stage is filled
 // again, which the MMAs that read them have announced (resident: see its layout).
 
+#include "kept.h"
+
 namespace fluke_sm100 {
 namespace {
 
@@ -992,16 +994,15 @@ int launch_dependent_clusters(void (*kernel)(P...), int cluster, dim3 grid, int 
     return (int)e;
 }
 
-// Clusters of `size` CTAs of KERNEL that run at once with `smem` bytes each; 0 where they cannot. A GPC's SMs bound it as well as
-// their number: 16 clusters of 8 CTAs, one per SM, ran in two rounds.
+// Clusters of `size` CTAs of KERNEL that run at once with `smem` bytes each; 0 where they cannot or the device does not say. A GPC's SMs bound it as
+// well as their number: 16 clusters of 8 CTAs, one per SM, ran in two rounds.
 template <auto KERNEL>
 int cluster_capacity(int size, int threads, int smem) {
-    static int cached[64][9] = {{0}};
+    static std::atomic<int> cached[64][9];
     int dev = 0;
     cudaGetDevice(&dev);
     if (dev < 0 || dev >= 64) dev = 0;
-    int &slot = cached[dev][size];
-    if (!slot) {
+    return kept(cached[dev][size], [&] {
         int n = 0;
         bool ok = configure_smem<KERNEL>(smem) == 0;
         if (ok) {
@@ -1016,12 +1017,11 @@ int cluster_capacity(int size, int threads, int smem) {
             attr[0].val.clusterDim.z = 1;
             cfg.attrs = attr;
             cfg.numAttrs = 1;
-            ok = cudaOccupancyMaxActiveClusters(&n, reinterpret_cast<const void *>(KERNEL), &cfg) == cudaSuccess && n > 0;
+            ok = cudaOccupancyMaxActiveClusters(&n, reinterpret_cast<const void *>(KERNEL), &cfg) == cudaSuccess;
         }
         cudaGetLastError();
-        slot = ok ? n + 1 : 1;
-    }
-    return slot - 1;
+        return ok ? n : 0;
+    });
 }
 
 // KMAX: 0 streams B, else the resident form with that many stages.

@@ -637,7 +637,7 @@ inline int resident_blocks(const void *kernel, int block, int smem = 0) {
         int per_sm = 0;
         if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, block, smem) != cudaSuccess || per_sm < 1) {
             cudaGetLastError();
-            per_sm = 1;
+            return device_sm_count();   // one per SM; the next call asks again
         }
         s = {kernel, dev, smem, per_sm * device_sm_count()};
     }
