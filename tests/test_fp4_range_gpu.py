@@ -138,3 +138,79 @@ def test_a_missing_part_is_not_another_operator():
                  lambda: ops.gated_mlp_mxfp4(*mx, *wm, None, None), lambda: ops.gated_mlp_mxfp4(*mx, *wm, None, wm[1]), lambda: ops.gemm_mxfp4(*mx, None, None)):
         with pytest.raises((TypeError, ValueError)):
             call()
+
+
+# ---- rows that walk: more rows than are resident at once, every width of lane and unit -----------
+
+def sample(m):
+    """Rows of the first turn, of later ones and of the ragged end."""
+    return np.unique(np.concatenate((np.arange(20), np.random.default_rng(m).integers(0, m, 90), np.arange(m - 20, m))))
+
+
+def stream_of(m, k, t, seed):
+    """Normal values with some large channels; rows and blocks of zeros and rows without a value among them."""
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    x = torch.randn(m, k, generator=g, device=DEV)
+    x[:, torch.rand(k, generator=g, device=DEV) < 0.02] *= 20
+    x[5], x[m - 2, :32], x[m - 7, k - 1], x[m - 11, 40 % k] = 0, 0, float("inf"), float("nan")
+    return x.to(t)
+
+
+def check_rows(got, want, fmt, rows_, m, k):
+    codes, scales, row = want
+    blocks = k // fp4.BLOCK[fmt]
+    assert np.array_equal(got[0][torch.from_numpy(rows_).to(DEV)].cpu().numpy(), fp4.pack(codes))
+    tiles = fp4.untile_scales(got[1].cpu().numpy(), m, got[1].shape[1] * 4)[rows_]
+    assert np.array_equal(tiles[:, :blocks], scales) and not tiles[:, blocks:].any()
+    if fmt == "nv":
+        assert np.array_equal(got[2].cpu().numpy()[rows_], row, equal_nan=True)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("m,k", [(20011, 32), (20011, 256), (9331, 480), (9331, 512), (9331, 736), (9331, 768), (9331, 992), (9331, 1024), (9331, 1504), (9331, 1536), (9331, 2016),
+                                 (9331, 2048), (700, 2080), (700, 4096), (700, 4128), (700, 16384)])
+def test_nvfp4_quantiser_of_many_rows(m, k, dtype):
+    x, rows_ = stream_of(m, k, TYPES[dtype], k), sample(m)
+    check_rows(ops.quant_nvfp4(x), fp4.quantise(x[torch.from_numpy(rows_).to(DEV)].cpu().double().numpy(), "nv"), "nv", rows_, m, k)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("fmt", [None, "mx", "nv"])
+@pytest.mark.parametrize("m,k,seqlen", [(20011, 32, 0), (9331, 256, 1333), (9331, 480, 0), (9331, 512, 1333), (9331, 736, 1), (9331, 768, 0), (9331, 992, 1333), (9331, 1024, 7),
+                                        (9331, 1504, 0), (9331, 1536, 1333), (9331, 2016, 1000), (9331, 2048, 0), (700, 2080, 100), (700, 4096, 7), (700, 16384, 1)])
+def test_norms_of_many_rows(m, k, seqlen, fmt, dtype):
+    """In place of the residual, which a later turn of the same warp must not have read too late."""
+    t = TYPES[dtype]
+    x, res = stream_of(m, k, t, k), stream_of(m, k, t, k + 1)
+    g = torch.Generator(device=DEV).manual_seed(k + 2)
+    post, pre = ((1 + 0.1 * torch.randn(k, generator=g, device=DEV)).to(t) for _ in range(2))
+    gate = (0.5 * torch.randn(-(-m // seqlen) if seqlen else 1, k, generator=g, device=DEV)).to(t)
+    rows_ = sample(m)
+    at = torch.from_numpy(rows_).to(DEV)
+    num = lambda v: v.float().cpu().numpy()
+    round16 = lambda v: torch.from_numpy(v).to(t).float().numpy()
+    own = num(gate[at // seqlen] if seqlen else gate.expand(len(rows_), k))
+    stream, h = fp4.rmsnorm_block(num(x[at]), num(res[at]), num(post), own, num(pre), 0.75, 1e-5, 1, round16)
+    got = ops.rmsnorm_block(x, res, post, gate, pre, 0.75, 1e-5, seqlen=seqlen, quant=None if fmt is None else fmt + "fp4", residual_out=res)
+    assert np.array_equal(num(got[0][at]), stream, equal_nan=True)
+    if fmt is None:
+        assert np.array_equal(num(got[1][at]), round16(h), equal_nan=True)
+    else:
+        check_rows(got[1:], fp4.quantise(h, fmt), fmt, rows_, m, k)
+
+
+@pytest.mark.parametrize("fmt", ["mx", "nv"])
+@pytest.mark.parametrize("m,k", [(7, 1024), (1300, 512), (9331, 1056)])
+def test_quantised_norms_in_place_of_the_input(m, k, fmt):
+    """Codes, every block scale and row scales of a call whose stream goes to x, against those of a call with a stream of its own."""
+    g = torch.Generator(device=DEV).manual_seed(m)
+    t = lambda *s: torch.randn(*s, generator=g, device=DEV).bfloat16()
+    x, res, w, gate = t(m, k), t(m, k), t(k), t(-(-m // 100), k)
+    want = ops.rmsnorm_block(x, res, w, gate, w, 0.5, 1e-5, seqlen=100, quant=fmt + "fp4")
+    got = ops.rmsnorm_block(x, res, w, gate, w, 0.5, 1e-5, seqlen=100, quant=fmt + "fp4", residual_out=x)
+    assert got[0].data_ptr() == x.data_ptr()
+    blocks = k // fp4.BLOCK[fmt]
+    for a, b in zip(want, got):
+        if a.dim() == 3:
+            a, b = (torch.from_numpy(fp4.untile_scales(v.cpu().numpy(), m, blocks).copy()) for v in (a, b))
+        assert torch.equal(a.cpu().view(torch.uint8), b.cpu().view(torch.uint8))
