@@ -157,10 +157,10 @@ __device__ __forceinline__ void unpack16(const uint32_t (&r)[8], float2 (&v)[8])
 
 // ---- quantisation, MX -------------------------------------------------------------------------
 // Blocks do not depend on their row: thread = unit, a block is two neighbouring lanes (rows are whole blocks, so
-// a pair never straddles two). Bound by memory: 2 bytes in and 0.53 out per value; [32000, 512] 7.0 us, 0.91 of the measured copy rate.
+// a pair never straddles two; row0 is the row of the first unit). Bound by memory: 2 bytes in and 0.53 out per value; [32000, 512] 7.0 us, 0.91 of the measured copy rate.
 template <typename T>
 __global__ void __launch_bounds__(256)
-quant_mxfp4_kernel(const T *in, uint8_t *codes, uint8_t *scale, uint32_t units, uint32_t units_per_row, int tiles) {
+quant_mxfp4_kernel(const T *in, uint8_t *codes, uint8_t *scale, uint32_t units, uint32_t units_per_row, int tiles, uint32_t row0) {
     dependency_wait();
     const uint32_t u = blockIdx.x * 256u + threadIdx.x;
     const bool live = u < units;
@@ -173,7 +173,7 @@ quant_mxfp4_kernel(const T *in, uint8_t *codes, uint8_t *scale, uint32_t units, 
     if (!live) return;
     const uint32_t e = mx_exponent(m);
     *reinterpret_cast<uint2 *>(codes + int64_t(u) * 8) = mx_codes(v, e);
-    const uint32_t row = u / units_per_row, at = u - row * units_per_row;
+    const uint32_t r = u / units_per_row, at = u - r * units_per_row, row = row0 + r;
     if ((at & 1u) == 0) scale[scale_byte(row, int(at >> 1), tiles)] = uint8_t(e);
     if (at == units_per_row - 1) pad_scales(scale, row, int(units_per_row >> 1), tiles);
 }
@@ -183,13 +183,13 @@ quant_mxfp4_kernel(const T *in, uint8_t *codes, uint8_t *scale, uint32_t units, 
 template <typename T, bool MX>
 __global__ void __launch_bounds__(256)
 dequant_fp4_kernel(const uint8_t *codes, const uint8_t *scale, const float *row_scale, T *out, uint32_t units, uint32_t units_per_row,
-                   int tiles) {
+                   int tiles, uint32_t row0) {
     dependency_wait();
     const uint32_t u = blockIdx.x * 256u + threadIdx.x;
     if (u >= units) return;
     const uint32_t row = u / units_per_row, at = u - row * units_per_row;
     const uint2 c = *reinterpret_cast<const uint2 *>(codes + int64_t(u) * 8);
-    const uint32_t s8 = scale[scale_byte(row, int(MX ? at >> 1 : at), tiles)];
+    const uint32_t s8 = scale[scale_byte(int64_t(row0) + row, int(MX ? at >> 1 : at), tiles)];
     const float s = MX ? e8m0_value(s8) : e4m3_value(s8), g = MX ? 1.f : row_scale[row];
     const float2 s2 = make_float2(s, s), g2 = make_float2(g, g);
     float2 lo[4], hi[4];
@@ -716,6 +716,18 @@ inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 
 // kFp4MaxSize: the next tile's end and a grid's step from the last row still fit 32 bits.
 constexpr int kFp4MaxSize = INT32_MAX - (1 << 20);
 inline bool fp4_shape_ok(int rows, int cols) { return rows >= 0 && rows <= kFp4MaxSize && cols >= 32 && cols <= kFp4MaxSize && cols % 32 == 0; }
+// Kernels whose thread is a unit count units in 32 bits: launch(first row, rows) for runs of rows of at most INT32_MAX units (one run, as a rule).
+template <typename F>
+int in_row_runs(int rows, int units, F launch) {
+    const int most = INT32_MAX / units;
+    for (int row = 0; row < rows;) {
+        const int n = rows - row < most ? rows - row : most, rc = launch(row, n);
+        if (rc) return rc;
+        row += n;
+    }
+    return 0;
+}
+inline int unit_blocks(int rows, int units) { return int((int64_t(rows) * units + 255) / 256); }
 inline int fp4_tiles(int cols, int format) { return (cols / (format == FLUKE_SM100_FP4_MX ? 32 : 16) + 3) / 4; }
 
 }  // namespace
@@ -737,14 +749,17 @@ extern "C" int fluke_sm100_quant_fp4(const void *in, void *codes, void *scale, v
         return bf16 ? launch_quant_nvfp4(static_cast<const __nv_bfloat16 *>(in), c, b, r, rows, units, s)
                     : launch_quant_nvfp4(static_cast<const __half *>(in), c, b, r, rows, units, s);
     }
-    const int64_t total = int64_t(rows) * units;
-    if (format != FLUKE_SM100_FP4_MX || total > INT32_MAX) return (int)cudaErrorInvalidValue;
-    const int grid = int((total + 255) / 256), tiles = fp4_tiles(cols, format);
-    if (bf16)
-        return launch_dependent(quant_mxfp4_kernel<__nv_bfloat16>, grid, 256, 0, s, static_cast<const __nv_bfloat16 *>(in),
-                                static_cast<uint8_t *>(codes), static_cast<uint8_t *>(scale), uint32_t(total), uint32_t(units), tiles);
-    return launch_dependent(quant_mxfp4_kernel<__half>, grid, 256, 0, s, static_cast<const __half *>(in), static_cast<uint8_t *>(codes),
-                            static_cast<uint8_t *>(scale), uint32_t(total), uint32_t(units), tiles);
+    if (format != FLUKE_SM100_FP4_MX) return (int)cudaErrorInvalidValue;
+    const int tiles = fp4_tiles(cols, format);
+    return in_row_runs(rows, units, [&](int row0, int n) {
+        auto run = [&](auto *x) {
+            using T = std::remove_const_t<std::remove_pointer_t<decltype(x)>>;
+            return launch_dependent(quant_mxfp4_kernel<T>, unit_blocks(n, units), 256, 0, s, x + int64_t(row0) * cols,
+                                    static_cast<uint8_t *>(codes) + int64_t(row0) * (cols / 2), static_cast<uint8_t *>(scale), uint32_t(n) * uint32_t(units),
+                                    uint32_t(units), tiles, uint32_t(row0));
+        };
+        return bf16 ? run(static_cast<const __nv_bfloat16 *>(in)) : run(static_cast<const __half *>(in));
+    });
 }
 
 extern "C" int fluke_sm100_dequant_fp4(const void *codes, const void *scale, const void *row_scale, void *out, int rows, int cols, int format,
@@ -753,16 +768,18 @@ extern "C" int fluke_sm100_dequant_fp4(const void *codes, const void *scale, con
     if (rows == 0) return 0;
     if (!out || !codes || !scale || (format == FLUKE_SM100_FP4_NV && !row_scale)) return (int)cudaErrorInvalidValue;
     if (!aligned32(out) || !aligned16(codes) || !aligned16(scale)) return (int)cudaErrorMisalignedAddress;
-    const int64_t total = int64_t(rows) * (cols / 16);
-    if (total > INT32_MAX) return (int)cudaErrorInvalidValue;
     const bool mx = format == FLUKE_SM100_FP4_MX;
-    auto run = [&](auto *o) {
-        using T = std::remove_pointer_t<decltype(o)>;
-        return launch_dependent(mx ? dequant_fp4_kernel<T, true> : dequant_fp4_kernel<T, false>, int((total + 255) / 256), 256, 0,
-                                static_cast<cudaStream_t>(stream), static_cast<const uint8_t *>(codes), static_cast<const uint8_t *>(scale),
-                                static_cast<const float *>(row_scale), o, uint32_t(total), uint32_t(cols / 16), fp4_tiles(cols, format));
-    };
-    return bf16 ? run(static_cast<__nv_bfloat16 *>(out)) : run(static_cast<__half *>(out));
+    const int units = cols / 16;
+    return in_row_runs(rows, units, [&](int row0, int n) {
+        auto run = [&](auto *o) {
+            using T = std::remove_pointer_t<decltype(o)>;
+            return launch_dependent(mx ? dequant_fp4_kernel<T, true> : dequant_fp4_kernel<T, false>, unit_blocks(n, units), 256, 0,
+                                    static_cast<cudaStream_t>(stream), static_cast<const uint8_t *>(codes) + int64_t(row0) * (cols / 2),
+                                    static_cast<const uint8_t *>(scale), mx ? nullptr : static_cast<const float *>(row_scale) + row0, o + int64_t(row0) * cols,
+                                    uint32_t(n) * uint32_t(units), uint32_t(units), fp4_tiles(cols, format), uint32_t(row0));
+        };
+        return bf16 ? run(static_cast<__nv_bfloat16 *>(out)) : run(static_cast<__half *>(out));
+    });
 }
 
 extern "C" int fluke_sm100_rmsnorm_block(const fluke_sm100_rmsnorm_block_t *b, void *stream) {

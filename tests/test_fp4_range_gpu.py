@@ -214,3 +214,28 @@ def test_quantised_norms_in_place_of_the_input(m, k, fmt):
         if a.dim() == 3:
             a, b = (torch.from_numpy(fp4.untile_scales(v.cpu().numpy(), m, blocks).copy()) for v in (a, b))
         assert torch.equal(a.cpu().view(torch.uint8), b.cpu().view(torch.uint8))
+
+
+@pytest.mark.parametrize("fmt", ["mx", "nv"])
+def test_more_than_2_pow_31_units(flib, fmt):
+    """[4194433, 8192]: 2^31 + 66048 units of 16 values, which the mxfp4 quantiser and both read-backs work through in two runs of rows. 69 GB, read back in place."""
+    m, k = (1 << 22) + 129, 8192
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < 110e9:
+        pytest.skip("needs 110 GB of free memory")
+    x = torch.empty(m, k, dtype=torch.bfloat16, device=DEV)
+    x.normal_(generator=torch.Generator(device=DEV).manual_seed(1))
+    rows_ = np.concatenate((np.arange(3), np.arange((1 << 22) - 140, (1 << 22) - 120), np.arange((1 << 22) - 3, (1 << 22) + 3), np.arange(m - 3, m)))
+    at = torch.from_numpy(rows_).to(DEV)
+    want = fp4.quantise(x[at].cpu().double().numpy(), fmt)
+    q = ops.quant_mxfp4(x) if fmt == "mx" else ops.quant_nvfp4(x)
+    assert np.array_equal(q[0][at].cpu().numpy(), fp4.pack(want[0]))
+    x.fill_(float("nan"))
+    torch.cuda.synchronize()
+    args = [t.data_ptr() for t in (*q, x)]
+    assert (flib.fluke_dequant_mxfp4_gpu if fmt == "mx" else flib.fluke_dequant_nvfp4_gpu)(*args, m, k, 1) == 0
+    torch.cuda.synchronize()
+    assert np.array_equal(x[at].cpu().double().numpy(), fp4.values(*want, fmt))
+    assert not torch.isnan(x[:, 0]).any() and not torch.isnan(x[:, -1]).any()
+    del x, q
+    torch.cuda.empty_cache()
