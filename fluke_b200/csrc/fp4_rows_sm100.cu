@@ -793,17 +793,27 @@ extern "C" int fluke_sm100_rmsnorm_block(const fluke_sm100_rmsnorm_block_t *b, v
     if (!aligned32(b->x, b->residual, b->residual_out, quant ? nullptr : b->out) || (quant && !(aligned16(b->out) && aligned16(b->scale))) ||
         !aligned32(b->w_post, b->gate, b->w_pre))
         return (int)cudaErrorMisalignedAddress;
-    // A row is read before it is written, but rows come in any order: an output lies where an input of the same rows does, or apart from it.
-    const uint64_t bytes = uint64_t(b->rows) * b->cols * 2, out_bytes = b->out_format == kFp4None ? 0 : quant ? bytes / 4 : bytes;
-    auto apart = [](const void *a, uint64_t na, const void *c, uint64_t nc) {
-        const uint64_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(c);
-        return na == 0 || nc == 0 || x + na <= y || y + nc <= x;
+    // A row is read before it is written, but rows come in any order: the stream and a 16-bit result lie where x or the residual of the same rows does, or apart
+    // from everything; what all rows read, and scales, lie apart from everything.
+    const uint64_t row_bytes = uint64_t(b->cols) * 2, bytes = b->rows * row_bytes, out_bytes = b->out_format == kFp4None ? 0 : quant ? bytes / 4 : bytes;
+    const uint64_t gates = b->seqlen > 0 ? (uint64_t(b->rows) + b->seqlen - 1) / b->seqlen : 1;
+    const uint64_t scale_bytes = quant ? (uint64_t(b->rows) + 127) / 128 * fp4_tiles(b->cols, b->out_format) * 512 : 0;
+    struct Range { const void *at; uint64_t n; };
+    auto apart = [](Range a, Range c) {
+        const uint64_t x = reinterpret_cast<uintptr_t>(a.at), y = reinterpret_cast<uintptr_t>(c.at);
+        return a.n == 0 || c.n == 0 || x + a.n <= y || y + c.n <= x;
     };
-    for (const void *in : {b->x, b->residual}) {
-        if (b->residual_out != in && !apart(b->residual_out, bytes, in, bytes)) return (int)cudaErrorInvalidValue;
-        if ((quant || b->out != in) && !apart(b->out, out_bytes, in, bytes)) return (int)cudaErrorInvalidValue;
+    const Range in[] = {{b->x, bytes}, {b->residual, bytes}, {b->w_post, b->w_post ? row_bytes : 0}, {b->gate, b->gate ? gates * row_bytes : 0},
+                        {b->w_pre, b->out_format != kFp4None ? row_bytes : 0}};
+    const Range out[] = {{b->residual_out, bytes}, {b->out, out_bytes}, {b->scale, scale_bytes}, {b->row_scale, b->out_format == kFp4Nv ? uint64_t(b->rows) * 4 : 0}};
+    for (int o = 0; o < 4; ++o) {
+        for (int i = 0; i < 5; ++i) {
+            const bool in_place = i < 2 && out[o].at == in[i].at && (o == 0 || (o == 1 && !quant));
+            if (!in_place && !apart(out[o], in[i])) return (int)cudaErrorInvalidValue;
+        }
+        for (int other = 0; other < o; ++other)
+            if (!apart(out[o], out[other])) return (int)cudaErrorInvalidValue;
     }
-    if (!apart(b->out, out_bytes, b->residual_out, bytes)) return (int)cudaErrorInvalidValue;
     RmsnormBlockDev p;
     p.x = b->x; p.residual = b->residual; p.w_post = b->w_post; p.gate = b->gate; p.w_pre = b->w_pre;
     p.residual_out = b->residual_out; p.out = b->out;

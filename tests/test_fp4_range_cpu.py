@@ -1,6 +1,9 @@
 """Host-side parts of the 4-bit operators that need no GPU."""
+import ctypes
 import os
 import subprocess
+
+from fluke_b200 import lib as L
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
@@ -11,3 +14,32 @@ def test_a_failed_capacity_query_is_asked_again(tmp_path):
     subprocess.run([os.environ.get("CXX", "g++"), "-std=c++17", "-O1", "-pthread", os.path.join(ROOT, "tests", "csrc", "kept_test.cpp"), "-o", exe], check=True)
     out = subprocess.run([exe], check=True, capture_output=True, text=True, timeout=60).stdout
     assert out.split() == ["0/1", "-1/2", "7/3", "7/3", "7/3", "0"]
+
+
+P = 1 << 20   # an address that is aligned and never followed: every call below is refused before a launch
+
+
+def test_norms_refuse_outputs_over_what_every_row_reads(flib):
+    """[256, 64], a gate per 100 rows: 32768 bytes of rows, 128 of a weight, 384 of gates, 8192 of codes, 1024 of scales, 1024 of row scales."""
+    at = {name: P + i * 65536 for i, name in enumerate(("x", "residual", "post_weight", "gate", "pre_weight", "residual_out", "out", "scale", "row_scale"))}
+
+    def call(**change):
+        b = L.fluke_rmsnorm_block_t()
+        for k, v in {**at, **dict(n_tokens=256, hidden_dim=64, seqlen=100, alpha=1.0, eps=1e-5), **change}.items():
+            setattr(b, k, v)
+        return flib.fluke_rmsnorm_block_gpu(ctypes.byref(b))
+
+    def over(out, n_out, other, n_other, fmt):
+        for delta in (0, -(n_out - 32), n_other - 32):   # the same start, the output's last and first bytes
+            assert call(**{"out_format": fmt, out: at[other] + delta}) == 1, (out, other, delta, fmt)
+    for fmt, n_out, n_scale in ((0, 32768, 0), (1, 8192, 1024), (2, 8192, 1024)):
+        assert not n_scale or flib.fluke_fp4_scale_bytes(256, 64, fmt) == n_scale
+        for other, n in (("post_weight", 128), ("gate", 384), ("pre_weight", 128)):
+            over("residual_out", 32768, other, n, fmt)
+            over("out", n_out, other, n, fmt)
+        if n_scale:
+            for other, n in (("x", 32768), ("residual", 32768), ("post_weight", 128), ("gate", 384), ("residual_out", 32768), ("out", n_out)):
+                over("scale", n_scale, other, n, fmt)
+        if fmt == 2:
+            for other, n in (("x", 32768), ("pre_weight", 128), ("gate", 384), ("residual_out", 32768), ("out", n_out), ("scale", n_scale)):
+                over("row_scale", 1024, other, n, fmt)
