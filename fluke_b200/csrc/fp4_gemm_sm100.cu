@@ -1173,7 +1173,7 @@ extern "C" int fluke_sm100_gemm_fp4(const fluke_sm100_gemm_fp4_t *g, void *strea
     if (!g->a || !g->a_scale || !g->b || !g->b_scale || !g->out || (g->b2 && !g->b2_scale)) return (int)cudaErrorInvalidValue;
     if (nv && (!g->a_row || !g->b_row || (g->b2 && !g->b2_row))) return (int)cudaErrorInvalidValue;
     if (!aligned16(g->a) || !aligned16(g->a_scale) || !aligned16(g->b) || !aligned16(g->b_scale) || !aligned16(g->b2) || !aligned16(g->b2_scale) ||
-        !aligned16(g->out) || (nv && (!aligned16(g->b_row) || !aligned16(g->b2_row))))
+        !aligned16(g->out) || (nv && (!aligned4(g->a_row) || !aligned16(g->b_row) || !aligned16(g->b2_row))))
         return (int)cudaErrorMisalignedAddress;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (nv) return g->bf16 ? gemm_fp4_dispatch<FLUKE_SM100_FP4_NV, __nv_bfloat16>(g, s) : gemm_fp4_dispatch<FLUKE_SM100_FP4_NV, __half>(g, s);

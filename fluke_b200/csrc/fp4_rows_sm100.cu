@@ -713,6 +713,7 @@ int launch_rmsnorm_block(const RmsnormBlockDev &p, int out, cudaStream_t stream)
 // Sizes and addresses that every kernel here needs: rows of whole blocks (and of whole 16-byte pieces as codes, which the
 // products ask for), 16-bit tensors on 32 bytes, codes and scales on 16.
 inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+inline bool aligned4(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
 // kFp4MaxSize: the next tile's end and a grid's step from the last row still fit 32 bits.
 constexpr int kFp4MaxSize = INT32_MAX - (1 << 20);
 inline bool fp4_shape_ok(int rows, int cols) { return rows >= 0 && rows <= kFp4MaxSize && cols >= 32 && cols <= kFp4MaxSize && cols % 32 == 0; }
@@ -740,7 +741,7 @@ extern "C" int fluke_sm100_quant_fp4(const void *in, void *codes, void *scale, v
     if (!fp4_shape_ok(rows, cols) || (format == FLUKE_SM100_FP4_NV && cols > FLUKE_SM100_FP4_MAX_ROW)) return (int)cudaErrorInvalidValue;
     if (rows == 0) return 0;
     if (!in || !codes || !scale || (format == FLUKE_SM100_FP4_NV && !row_scale)) return (int)cudaErrorInvalidValue;
-    if (!aligned32(in) || !aligned16(codes) || !aligned16(scale)) return (int)cudaErrorMisalignedAddress;
+    if (!aligned32(in) || !aligned16(codes) || !aligned16(scale) || (format == FLUKE_SM100_FP4_NV && !aligned4(row_scale))) return (int)cudaErrorMisalignedAddress;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const int units = cols / 16;
     if (format == FLUKE_SM100_FP4_NV) {
@@ -767,7 +768,7 @@ extern "C" int fluke_sm100_dequant_fp4(const void *codes, const void *scale, con
     if (!fp4_shape_ok(rows, cols) || (format != FLUKE_SM100_FP4_MX && format != FLUKE_SM100_FP4_NV)) return (int)cudaErrorInvalidValue;
     if (rows == 0) return 0;
     if (!out || !codes || !scale || (format == FLUKE_SM100_FP4_NV && !row_scale)) return (int)cudaErrorInvalidValue;
-    if (!aligned32(out) || !aligned16(codes) || !aligned16(scale)) return (int)cudaErrorMisalignedAddress;
+    if (!aligned32(out) || !aligned16(codes) || !aligned16(scale) || (format == FLUKE_SM100_FP4_NV && !aligned4(row_scale))) return (int)cudaErrorMisalignedAddress;
     const bool mx = format == FLUKE_SM100_FP4_MX;
     const int units = cols / 16;
     return in_row_runs(rows, units, [&](int row0, int n) {
@@ -791,7 +792,7 @@ extern "C" int fluke_sm100_rmsnorm_block(const fluke_sm100_rmsnorm_block_t *b, v
     if (b->out_format != kFp4None && (!b->w_pre || !b->out)) return (int)cudaErrorInvalidValue;
     if ((quant && !b->scale) || (b->out_format == kFp4Nv && !b->row_scale)) return (int)cudaErrorInvalidValue;
     if (!aligned32(b->x, b->residual, b->residual_out, quant ? nullptr : b->out) || (quant && !(aligned16(b->out) && aligned16(b->scale))) ||
-        !aligned32(b->w_post, b->gate, b->w_pre))
+        !aligned32(b->w_post, b->gate, b->w_pre) || (b->out_format == kFp4Nv && !aligned4(b->row_scale)))
         return (int)cudaErrorMisalignedAddress;
     // A row is read before it is written, but rows come in any order: the stream and a 16-bit result lie where x or the residual of the same rows does, or apart
     // from everything; what all rows read, and scales, lie apart from everything.

@@ -542,8 +542,9 @@ int fluke_factored_lstm_layer_i8_noalloc_gpu(const fluke_flstm_layer_t *layer);
  * (r % 32) * 16 + (r / 32 % 4) * 4 + c % 4. The quantisers write zeros for blocks behind the end of a
  * row up to a multiple of 4 (the products read them) and leave rows behind the last as they were.
  * cols is a multiple of 32; rows and cols are below 2^31 - 2^20. 16-bit tensors start on 32 bytes;
- * codes, scales, row scales of weights and outputs of products on 16. Outputs lie apart from each
- * other and from inputs, except where it is said (the norms refuse what does not).
+ * codes, scales, row scales of weights and outputs of products on 16, other row scales on 4.
+ * Outputs lie apart from each other and from inputs, except where it is said (the norms refuse
+ * what does not).
  * ---------------------------------------------------------------------------------- */
 enum { FLUKE_F16 = 0, FLUKE_BF16 = 1 };
 enum { FLUKE_FP4_MX = 1, FLUKE_FP4_NV = 2 };

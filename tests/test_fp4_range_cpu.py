@@ -43,3 +43,14 @@ def test_norms_refuse_outputs_over_what_every_row_reads(flib):
         if fmt == 2:
             for other, n in (("x", 32768), ("pre_weight", 128), ("gate", 384), ("residual_out", 32768), ("out", n_out), ("scale", n_scale)):
                 over("row_scale", 1024, other, n, fmt)
+
+
+def test_row_scales_on_odd_addresses_are_refused(flib):
+    """Row scales are f32: an address that is no multiple of 4 faults on the device. cudaErrorMisalignedAddress (716) before a launch."""
+    Q = P + 2
+    assert flib.fluke_quant_nvfp4_gpu(P, P, P, Q, 4, 64, 0) == 716
+    assert flib.fluke_dequant_nvfp4_gpu(P, P, Q, P, 4, 64, 0) == 716
+    assert flib.fluke_gemm_nvfp4_gpu(P, P, P, Q, P, P, P, 4, 64, 64, 0) == 716
+    assert flib.fluke_gated_mlp_nvfp4_gpu(P, P, P, Q, P, P, P, P, P, P, 4, 64, 64, 0) == 716
+    b = L.fluke_rmsnorm_block_t(4, 64, 0, 0, P, P + 4096, P + 8192, 0, P + 8192, 1.0, 1e-5, P + 16384, 2, P + 20480, P + 24576, P + 28674)
+    assert flib.fluke_rmsnorm_block_gpu(ctypes.byref(b)) == 716
