@@ -126,8 +126,10 @@ __device__ __forceinline__ uint2 nv_codes(const float2 (&v)[8], uint32_t bmax_bi
         s8 = 0x7F;
         return make_uint2(0, 0);
     }
-    // Two quotients, each correctly rounded: with the correctly rounded reciprocal of a divisor of four significant bits one exact
-    // residual is enough (every one of the 2^23 mantissas tried against all eight divisors). First bmax / (6 g), g a power of two.
+    // Two quotients, each correctly rounded: q = v r with the correctly rounded reciprocal r of the divisor, then q + (v - q s) r with an exact residual, one fused
+    // operation each (P. Markstein, IBM J. Res. Dev. 34, 1990). In general that leaves the last quotient to be proved; for the divisors here, six and four
+    // significant bits, every mantissa was tried (tests/test_fp4_range_cpu.py). No step leaves the normal numbers where a code depends on it: s g is at
+    // least 2^-109 and a value below a quarter of it is zero. First bmax / (6 g), g a power of two.
     const float b = __uint_as_float(bmax_bits) * __uint_as_float((254u << 23) - __float_as_uint(g));
     constexpr float kSixth = 1.0f / 6.0f;
     float t = b * kSixth;

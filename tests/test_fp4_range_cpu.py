@@ -3,7 +3,11 @@ import ctypes
 import os
 import subprocess
 
-from fluke_b200 import lib as L
+import numpy as np
+import pytest
+import torch
+
+from fluke_b200 import lib as L, prep
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
@@ -54,3 +58,35 @@ def test_row_scales_on_odd_addresses_are_refused(flib):
     assert flib.fluke_gated_mlp_nvfp4_gpu(P, P, P, Q, P, P, P, P, P, P, 4, 64, 64, 0) == 716
     b = L.fluke_rmsnorm_block_t(4, 64, 0, 0, P, P + 4096, P + 8192, 0, P + 8192, 1.0, 1e-5, P + 16384, 2, P + 20480, P + 24576, P + 28674)
     assert flib.fluke_rmsnorm_block_gpu(ctypes.byref(b)) == 716
+
+
+def fma32(a, b, c):
+    """Correctly rounded f32 a * b + c where 64 bits hold it exactly, which the asserts of its callers' operands say."""
+    return (a.astype(np.longdouble) * np.longdouble(b) + c.astype(np.longdouble)).astype(np.float32)
+
+
+@pytest.mark.skipif(np.finfo(np.longdouble).nmant < 63, reason="needs 64-bit mantissas")
+@pytest.mark.parametrize("divisor", [6.0] + [1 + i / 8 for i in range(8)])
+def test_every_quotient_of_the_nvfp4_quantiser(divisor):
+    """x / 6 and x / s with s of four significant bits, as nv_codes computes them (fp4_rows_sm100.cu: a correctly rounded reciprocal and one residual), for
+    every f32 mantissa against the correctly rounded division. Exponents only shift both sides."""
+    d = np.float32(divisor)
+    r = np.float32(1) / d
+    for part in range(8):
+        x = ((np.arange(1 << 20, dtype=np.uint32) + np.uint32(part << 20)) | np.uint32(0x3F800000)).view(np.float32)
+        want = x / d
+        # the reciprocal's sign is turned for s, so that a zero keeps its sign; the signs of 6 are written the other way round
+        q = x * r if divisor == 6 else x * -r
+        residual = fma32(q, -d if divisor == 6 else d, x)
+        # the residual has few bits, so its product with r and the sum with q fit 64
+        assert (np.abs(residual) < 2.0 ** -20).all() and (residual * np.float32(2.0 ** 30) == np.rint(residual * np.float32(2.0 ** 30))).all()
+        got = fma32(residual, r if divisor == 6 else -r, q)
+        assert np.array_equal(got if divisor == 6 else -got, want)
+
+
+def test_preparation_of_no_rows():
+    z = torch.zeros(0, 96)
+    codes, scale = prep.quantize_mxfp4(z)
+    assert codes.shape == (0, 48) and scale.shape == (0, 1, 512)
+    codes, scale, row = prep.quantize_nvfp4(z)
+    assert codes.shape == (0, 48) and scale.shape == (0, 2, 512) and row.shape == (0,)

@@ -239,3 +239,24 @@ def test_more_than_2_pow_31_units(flib, fmt):
     assert not torch.isnan(x[:, 0]).any() and not torch.isnan(x[:, -1]).any()
     del x, q
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_quotients_of_every_16_bit_mantissa(dtype):
+    """Rows whose blocks have each of the eight mantissas of an e4m3 scale, with every mantissa of the type in four binades under it, and every block maximum."""
+    t = TYPES[dtype]
+    bits_ = 10 if dtype == "f16" else 7
+    mantissas = 1 + torch.arange(1 << bits_) / (1 << bits_)
+    values = torch.cat([mantissas * 2.0 ** e for e in (-2, -1, 0, 1)] + [-mantissas])   # below 4
+    values = torch.cat((values, torch.zeros(-len(values) % 15)))
+    blocks = []
+    for eighth in range(8):   # a block maximum of 6 (1 + i / 8) gives the scale 1 + i / 8 in a row of scale 1
+        blocks.append(torch.cat((torch.full((len(values) // 15, 1), 6 * (1 + eighth / 8)), values.view(-1, 15)), 1))
+    tops = torch.cat([mantissas * 2.0 ** e for e in (-8, -3, 0, 2, 7, 11)])
+    blocks.append(torch.cat((tops.clamp_max(2688)[:, None], torch.rand(len(tops), 15, generator=torch.Generator().manual_seed(1)) * tops[:, None]), 1))
+    x = torch.cat(blocks)
+    x = torch.cat((x, torch.zeros(-len(x) % 63, 16))).view(-1, 63 * 16)
+    x = torch.cat((torch.full((len(x), 16), 2688.0), x), 1).to(t)   # the row's scale is 1 (some of the last rows hold larger values)
+    want = fp4.quantise(x.double().numpy(), "nv")
+    assert (want[2][:len(values) * 8 // 15 // 63] == 1).all()
+    check_rows(ops.quant_nvfp4(x.to(DEV)), want, "nv", np.arange(len(x)), *x.shape)
