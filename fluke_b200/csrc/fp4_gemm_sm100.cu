@@ -11,7 +11,7 @@
 //
 // Three forms, by what bounds them (gemm_fp4_dispatch chooses):
 //   split      few rows or few tiles: latency, and reading the weights. One tile per CTA, K split over a cluster.
-//   resident   many tiles, K <= 1024: writing the output. Pairs of SMs, the weight's rows stay on chip.
+//   resident   many tiles, K <= 1024: writing the output (gated: the epilogue's SiLU). Pairs of SMs, the weight's rows stay on chip.
 //   pair       many tiles, longer K: the MMAs, under the power limit. Pairs of SMs, both operands stream.
 // In each warp 0 loads (one thread), warp 1 owns tensor memory and issues scale copies and MMAs, warps 2-3 are idle and the others are the
 // epilogue. An MMA of 128 (pair: 256) x 256 x 64 takes 128 cycles, one of half the columns 64, with or without the scale copies
@@ -136,7 +136,7 @@ __device__ __forceinline__ float rcp_approx(float x) {
 // silu(g) * u = g / (1 + exp(-g)) * u, which cancels for no gate (h + h tanh(h), h = g / 2, does for a negative one, and the hardware's tanh has 11 bits: at a
 // gate of -8 it was off by up to 70 %). Relative error below (|g| + 5) 2^-23: ex2.approx 2^-22, its argument 2^-23 of itself, rcp.approx 2^-23, the other
 // operations 2^-24 each. Below a gate of -87 silu, less than 2^-119 there, is zero. Two operations of the special-function unit per value instead of one: gated
-// [32000, 512] x 2 [2048, 512] mx 36.0 -> 48.0 us, nv 53.4 -> 61.9, [1803, 2048] x 2 [4096, 2048] nv 18.4 -> 18.7, few rows as before. A reciprocal for two
+// [32000, 512] x 2 [2048, 512] mx 36.0 -> 48.0 us, nv 53.4 -> 61.9, [1803, 2048] x 2 [4096, 2048] nv 18.4 -> 18.7, mx [300, 512] 5.8 -> 6.2, few rows as before. A reciprocal for two
 // values, where no gate of a lane's 32 is below -43 (a product of two of 1 + exp(-g) overflows otherwise), mx 44.7 but nv 65.8, whose registers do not hold the test; for
 // four values 45.9 and 68.9; every second exp(-g) as a polynomial instead 49.3 and 76.8.
 __device__ __forceinline__ float2 silu_times(float2 g, float2 u) {
@@ -392,8 +392,8 @@ gemm_fp4_split_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_con
 // would need on its own, which is what bounds large products (L2 to SM).
 //
 // The accumulators take 256 of the 512 tensor-memory columns, the scales most of the others, so there is no second
-// buffer: the epilogue warps take all of their part into registers (some 150 cycles), hand the columns back and do the arithmetic
-// and the stores while the MMAs of the next tile run.
+// buffer: the epilogue warps take all of their part into registers (some 150 cycles; 128 of them, for which the compiler spills 12 at most), hand the columns back
+// and do the arithmetic and the stores while the MMAs of the next tile run.
 //
 // A pair works through a contiguous run of the tiles in n-major order.
 template <int FMT>
@@ -1045,8 +1045,8 @@ int gemm_fp4_pair_launch(const fluke_sm100_gemm_fp4_t *g, cudaStream_t stream) {
     p.stages_k = (g->K + kFp4StageK - 1) / kFp4StageK;
     p.last_steps = (g->K - (p.stages_k - 1) * kFp4StageK + 63) / 64;
     p.ga = g->a_row; p.gb = g->b_row; p.gb2 = g->b2_row;
-    // such lines drive out what the next kernels read: gated [32000, 512] x 2 [2048, 512] (131 MB) 36.8 : 36.5 us, in a long loop 44.5 : 43.3;
-    // streamed [8192, 4096] x [8192, 4096] (134 MB) 110.0 : 109.6, 127.8 : 127.0
+    // such lines drive out what the next kernels read: gated [32000, 512] x 2 [2048, 512] (131 MB) 48.9 : 47.8 us, in a long loop 50.6 : 49.6;
+    // streamed [8192, 4096] x [8192, 4096] (134 MB) 106.6 : 106.3
     p.passes_by = int64_t(g->M) * g->N * 2 > int64_t(device_l2_bytes()) / 8 * 7;
     CUtensorMap tm_a, tm_b, tm_b2, tm_sfa, tm_sfb, tm_sfb2, tm_out;
     const uint64_t pitch = uint64_t(g->K) / 2, sf_words = uint64_t(fp4_tiles(g->K, FMT)) * 64;
@@ -1147,8 +1147,8 @@ int gemm_fp4_split_launch(const fluke_sm100_gemm_fp4_t *g, cudaStream_t stream) 
 }
 
 // The split form for few rows and for products whose tiles it holds all at once, pairs of SMs for the others. MX, us per call, pairs : split:
-// plain, N = 2048: 512 rows K = 512 5.2 : 4.0, K = 2048 7.1 : 5.7, 3000 rows 7.5 : 10.6, 11.4 : 19.1; gated, N = 2048, 256 rows (64 tiles) K = 1024 6.2 :
-// 5.6, 512 rows (128) K = 512 5.5 : 6.1, K = 2048 7.1 : 7.4.
+// plain, N = 2048: 512 rows K = 512 5.2 : 4.0, K = 2048 7.1 : 5.7, 3000 rows 7.5 : 10.6, 11.4 : 19.1; gated, N = 2048, 256 rows (64 tiles) K = 1024 6.3 :
+// 5.7, 384 rows (96) 6.5 : 5.8, 512 rows (128) K = 512 5.8 : 6.4, K = 2048 7.4 : 7.5.
 template <int FMT, bool GATED, typename T>
 int gemm_fp4_dispatch(const fluke_sm100_gemm_fp4_t *g, cudaStream_t stream) {
     if (g->M <= 64 || split_tiles<GATED>(g) <= (GATED ? 100 : device_sm_count())) return gemm_fp4_split_launch<FMT, GATED, T>(g, stream);

@@ -253,7 +253,7 @@ __device__ __forceinline__ void copy_row(uint32_t (&to)[U][8], const uint32_t (&
 
 // Quantisation, NV. LANES lanes (half a warp or one) hold a row, and a warp works through rows with the next ones on their way while it computes
 // ([9331, 2048] bf16 19.4 -> 12.2 us against a warp per row; 9.9 with the quotients of nv_codes and the three-operand maximum, 0.76 of the copy
-// rate). Two or four warps to such a row instead of one: 10.8, 11.8. Half a warp: [16384, 256] 4.7 -> 3.3, [32000, 512] 9.0 -> 8.5, [16384, 768] 7.8 -> 6.8.
+// rate; with four units per lane two registers spill at 128). Two or four warps to such a row instead of one: 10.8, 11.8. Half a warp: [16384, 256] 4.7 -> 3.3, [32000, 512] 9.0 -> 8.5, [16384, 768] 7.8 -> 6.8.
 template <typename T, int LANES, int U>
 __global__ void __launch_bounds__(kFp4WalkWarps * 32, U == 1 ? 4 : U == 2 ? 3 : 2)
 quant_nvfp4_rows_kernel(const T *in, uint8_t *codes, uint8_t *scale, float *row_scale, int rows, int units, int tiles) {
@@ -432,7 +432,7 @@ __device__ __forceinline__ void write_unit(const RmsnormBlockDev &p, int64_t row
 // rows. The weights that all rows share lie in shared memory as f32, which saves a conversion per value and row. FULL: rows of exactly
 // LANES * U units, where no lane has to ask for its end. The next rows are asked for while these are computed with two units per lane (us,
 // with : without: [32000, 512] to mxfp4 21.3 : 23.8, [9331, 1024] 13.2 : 14.2; one unit [16384, 256] 7.1 : 6.6, whose registers carry six blocks without),
-// and behind the other loads: a use of those waits for every load in front of it.
+// and behind the other loads: a use of those waits for every load in front of it. At 128 registers (four blocks) forms of four units and some of two spill up to 14.
 template <typename T, int OUT, int LANES, int U, bool FULL>
 __global__ void __launch_bounds__(kFp4NormWarps * 32, U == 1 ? 6 : 4)
 rmsnorm_rows_kernel(const RmsnormBlockDev p) {
