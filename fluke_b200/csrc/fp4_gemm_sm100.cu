@@ -71,7 +71,7 @@ __device__ __forceinline__ bool mbar_test(uint64_t *bar, uint32_t parity) {
         : "=r"(done) : "r"(smem_u32(bar)), "r"(parity) : "memory");
     return done != 0;
 }
-// mbar_wait() of a whole warp, with the same answer for every lane.
+// mbar_wait() of a whole warp, with the same answer for every lane: where one lane gives up, no other goes on to an instruction that takes the warp.
 __device__ __forceinline__ bool mbar_wait_warp(uint64_t *bar, uint32_t parity, volatile int *abort_flag, unsigned int site) {
     return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, site));
 }
@@ -295,7 +295,7 @@ gemm_fp4_split_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_con
     bool ok = true;
     if (warp >= 4) {
         const int q = warp & 3, half = (warp - 4) >> 2;
-        ok = mbar_wait(&done_bar, 0, abort_flag, 123);
+        ok = mbar_wait_warp(&done_bar, 0, abort_flag, 123);
         if (ok) {
             tc_fence_after_sync();
             // eight columns per turn: this code runs once, and more of it would cost more to fetch than to execute
@@ -337,7 +337,7 @@ gemm_fp4_split_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_con
                               sums + (w * p.a_rows + lane * share) * kFp4SumPitch, theirs * kFp4SumPitch * 4,
                               cluster_address(smem_u32(&sums_bar), lane));
         }
-        if (warp >= 4 && ok && mine > 0) ok = mbar_wait(&sums_bar, 0, abort_flag, 124);
+        if (warp >= 4 && ok && mine > 0) ok = mbar_wait_warp(&sums_bar, 0, abort_flag, 124);
     }
     if (warp >= 4 && ok) {
         // eight output columns of a row per turn
@@ -595,7 +595,7 @@ gemm_fp4_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
             const int n = run.n, m0 = run.m * 256 + rank * 128 + q * 32, n0 = n * BN_OUT;
             float ga = 1.f;
             if (FMT == FLUKE_SM100_FP4_NV && m0 + lane < p.M) ga = p.ga[m0 + lane];
-            ok = mbar_wait(tfull_bar, t_phase, abort_flag, 135);
+            ok = mbar_wait_warp(tfull_bar, t_phase, abort_flag, 135);
             if (!ok) break;
             tc_fence_after_sync();
             const uint32_t t_row = tmem + (uint32_t(q * 32) << 16);
@@ -889,7 +889,7 @@ gemm_fp4_resident_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_
         const uint64_t evict_first = l2_evict_first();
         // The warp's 32 x 32 cells of the next buffer, which is handed back.
         auto take = [&](uint32_t (&a)[32]) {
-            if (!mbar_wait(&tfull_bar[acc], t_phase, abort_flag, 145)) return false;
+            if (!mbar_wait_warp(&tfull_bar[acc], t_phase, abort_flag, 145)) return false;
             tc_fence_after_sync();
             tmem_ld_32x32(t_row + acc * 128, a);
             tmem_ld_wait();
