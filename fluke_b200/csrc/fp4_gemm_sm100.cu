@@ -107,7 +107,7 @@ __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.w
 // acc * ga * gb for two columns of a row (NV), in an order that leaves f32 only where the result does: ga is given as low * high, min(ga, 1) and max(ga, 1).
 // A sum that is not zero is a multiple of 2^-20 and the quantiser's scales are at least 2^-100, so acc * low is exact; and where high is above one (low is one),
 // a product with gb that overflows does so for good. With ga as one factor a row of 1e36 times weights of 0.01 overflowed at acc * ga. The resident form, bound
-// by its epilogue, leaves the third product out where no row of a warp has a scale above one (amax above 2688): always : where needed [32000, 512] x [1536, 512] 31.1 : 28.5 us,
+// by its epilogue, leaves the third product out where no row of a warp has a scale above one (amax above 2688): always : where needed [32000, 512] x [1536, 512] 31.1 : 28.3 us,
 // gated with 2 [2048, 512] 70 : 60.
 struct RowScale {
     float2 low, high;
@@ -136,8 +136,8 @@ __device__ __forceinline__ float rcp_approx(float x) {
 // silu(g) * u = g / (1 + exp(-g)) * u, which cancels for no gate (h + h tanh(h), h = g / 2, does for a negative one, and the hardware's tanh has 11 bits: at a
 // gate of -8 it was off by up to 70 %). Relative error below (|g| + 5) 2^-23: ex2.approx 2^-22, its argument 2^-23 of itself, rcp.approx 2^-23, the other
 // operations 2^-24 each. Below a gate of -87 silu, less than 2^-119 there, is zero. Two operations of the special-function unit per value instead of one: gated
-// [32000, 512] x 2 [2048, 512] mx 36.0 -> 48.0 us, nv 53.4 -> 61.9, [1803, 2048] x 2 [4096, 2048] nv 18.4 -> 18.7, mx [300, 512] 5.8 -> 6.2, few rows as before. A reciprocal for two
-// values, where no gate of a lane's 32 is below -43 (a product of two of 1 + exp(-g) overflows otherwise), mx 44.7 but nv 65.8, whose registers do not hold the test; for
+// [32000, 512] x 2 [2048, 512] mx 34.9 -> 43.8 us, nv 50.5 -> 55.6, [1803, 2048] x 2 [4096, 2048] nv 17.3 -> 17.6, mx [300, 512] 5.8 -> 6.0, few rows as before. Where this form
+// took 48.0 (mx) and 61.9 (nv), before the epilogue's waits were made uniform: a reciprocal for two values, where no gate of a lane's 32 is below -43 (a product of two of 1 + exp(-g) overflows otherwise), 44.7 and 65.8, whose registers do not hold the test; for
 // four values 45.9 and 68.9; every second exp(-g) as a polynomial instead 49.3 and 76.8.
 __device__ __forceinline__ float2 silu_times(float2 g, float2 u) {
     const float2 t = mul2(g, make_float2(-1.44269504f, -1.44269504f));
