@@ -136,9 +136,10 @@ __device__ __forceinline__ float rcp_approx(float x) {
 // silu(g) * u = g / (1 + exp(-g)) * u, which cancels for no gate (h + h tanh(h), h = g / 2, does for a negative one, and the hardware's tanh has 11 bits: at a
 // gate of -8 it was off by up to 70 %). Relative error below (|g| + 5) 2^-23: ex2.approx 2^-22, its argument 2^-23 of itself, rcp.approx 2^-23, the other
 // operations 2^-24 each. Below a gate of -87 silu, less than 2^-119 there, is zero. Two operations of the special-function unit per value instead of one: gated
-// [32000, 512] x 2 [2048, 512] mx 34.9 -> 43.8 us, nv 50.5 -> 55.6, [1803, 2048] x 2 [4096, 2048] nv 17.3 -> 17.6, mx [300, 512] 5.8 -> 6.0, few rows as before. Where this form
-// took 48.0 (mx) and 61.9 (nv), before the epilogue's waits were made uniform: a reciprocal for two values, where no gate of a lane's 32 is below -43 (a product of two of 1 + exp(-g) overflows otherwise), 44.7 and 65.8, whose registers do not hold the test; for
-// four values 45.9 and 68.9; every second exp(-g) as a polynomial instead 49.3 and 76.8.
+// [32000, 512] x 2 [2048, 512] mx 34.9 -> 43.8 us, nv 50.5 -> 55.6, [1803, 2048] x 2 [4096, 2048] nv 17.3 -> 17.6, mx [300, 512] 5.8 -> 6.0, few rows as before.
+// Where this form took 48.0 (mx) and 61.9 (nv), before the epilogue's waits were made uniform: a reciprocal for two values, where no gate of a lane's 32 is
+// below -43 (a product of two of 1 + exp(-g) overflows otherwise), 44.7 and 65.8, whose registers do not hold the test; for four values 45.9 and 68.9; every
+// second exp(-g) as a polynomial 49.3 and 76.8.
 __device__ __forceinline__ float2 silu_times(float2 g, float2 u) {
     const float2 t = mul2(g, make_float2(-1.44269504f, -1.44269504f));
     const float2 d = add2(make_float2(ex2_approx(t.x), ex2_approx(t.y)), make_float2(1.f, 1.f));
