@@ -128,7 +128,8 @@ int fluke_sm100_dequant_fp4(const void *codes, const void *scale, const void *ro
 typedef struct {
     int rows, cols, seqlen;     /* seqlen: rows that share a row of gate; 0 = one row for all     */
     int bf16;                   /* type of every 16-bit tensor here: 0 f16, 1 bf16                */
-    int out_format;             /* 0: 16 bits, enum fluke_sm100_fp4, 3: no output but the stream  */
+    int out_format;             /* 0: 16 bits, enum fluke_sm100_fp4, 3: no output but the stream, */
+                                /* 4 int8 and 5 e4m3 under a scale per row                        */
     const void *x, *residual, *w_post, *gate, *w_pre;   /* w_post and gate may be null            */
     void *residual_out;         /* may be residual                                                */
     void *out, *scale;
@@ -148,6 +149,40 @@ typedef struct {
     void *out;
 } fluke_sm100_gemm_fp4_t;
 int fluke_sm100_gemm_fp4(const fluke_sm100_gemm_fp4_t *g, void *stream);
+
+/* ---- 16-bit product with an epilogue -------------------------------------------------------- */
+
+typedef struct {
+    int bf16;                   /* type of every tensor here: 0 f16, 1 bf16                        */
+    int activation;             /* FLUKE_ACT_* of <fluke/fluke.h>                                   */
+    int M, N, K;                /* out [M,N]; x [M,K]; w [N,K]                                    */
+    const void *x, *w;
+    const void *bias;           /* [N] or null                                                    */
+    const void *residual;       /* [M,N] or null; may be out                                      */
+    void *out;
+    long long ld_x, ld_residual, ld_out;    /* values between rows, multiples of 8                */
+    float alpha;
+} fluke_sm100_linear_t;
+int fluke_sm100_linear(const fluke_sm100_linear_t *g, void *stream);
+
+/* ---- gated linear recurrence ---------------------------------------------------------------- */
+
+#define FLUKE_SM100_RECURRENCE_KEPT 64      /* steps between the states that the forward pass keeps */
+typedef struct {
+    int bf16;                   /* type of the 16-bit tensors: 0 f16, 1 bf16                       */
+    int T, B, H, reverse;
+    const void *gate, *value, *grad;        /* [T,B,H] by their strides; grad: backward            */
+    void *out, *grad_gate, *grad_value;     /* forward; backward; backward                         */
+    long long gate_step, gate_chunk, value_step, value_chunk, grad_step, grad_chunk;
+    long long out_step, out_chunk, grad_gate_step, grad_gate_chunk, grad_value_step, grad_value_chunk;
+    const int *lengths;         /* [B] or null                                                    */
+    const float *h0;            /* [B,H] or null                                                  */
+    float *h_last;              /* [B,H] or null; may be h0                                       */
+    float *states;              /* [ceil(T / KEPT),B,H]: written forward (or null), read backward */
+    const float *grad_last;     /* [B,H] or null                                                  */
+    float *grad_h0;             /* [B,H] or null; may be grad_last                                */
+} fluke_sm100_recurrence_t;
+int fluke_sm100_recurrence(const fluke_sm100_recurrence_t *r, int backward, void *stream);
 
 /* ---- factored LSTM ------------------------------------------------------------------------ */
 

@@ -5,6 +5,8 @@
 #include "gemm_sm100.cu"
 #include "fp4_rows_sm100.cu"
 #include "fp4_gemm_sm100.cu"
+#include "linear_sm100.cu"
+#include "recurrence_sm100.cu"
 #include "lstm_sm100.cu"
 #include "lstm_persist_sm100.cu"
 #include "lstm_cluster_sm100.cu"

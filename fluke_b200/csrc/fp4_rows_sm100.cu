@@ -22,7 +22,9 @@
 namespace fluke_sm100 {
 namespace {
 
-enum Fp4Out { kFp4Plain = 0, kFp4Mx = 1, kFp4Nv = 2, kFp4None = 3 };
+enum Fp4Out { kFp4Plain = 0, kFp4Mx = 1, kFp4Nv = 2, kFp4None = 3, kRowI8 = 4, kRowE4 = 5 };
+// Outputs that need the largest magnitude of the whole row first.
+__host__ __device__ constexpr bool by_row(int out) { return out == kFp4Nv || out == kRowI8 || out == kRowE4; }
 
 __device__ __forceinline__ float2 unpack2(uint32_t v, __half) { return half2_bits_to_float2(v); }
 __device__ __forceinline__ float2 unpack2(uint32_t v, __nv_bfloat16) {
@@ -149,6 +151,42 @@ __device__ __forceinline__ uint2 nv_codes(const float2 (&v)[8], uint32_t bmax_bi
     }
     return make_uint2(e2m1x8(q[0], q[1], q[2], q[3]) ^ 0x88888888u, e2m1x8(q[4], q[5], q[6], q[7]) ^ 0x88888888u);
 }
+
+// 8-bit values under an f32 scale per row, its largest magnitude (at least 1e-12) over the largest code (127, or 448 in e4m3): value = v * (most / largest), rounded to
+// nearest with ties to even. A row with an infinity or a NaN has no value: its scale is NaN and its codes are zero.
+struct RowScale8 {
+    float scale, factor;
+    __device__ __forceinline__ RowScale8(uint32_t amax_bits, float most) {
+        const float top = fmaxf(__uint_as_float(amax_bits), 1e-12f);
+        const bool bad = amax_bits >= kInfBits;
+        scale = bad ? __uint_as_float(0x7FFFFFFFu) : __fdiv_rn(top, most);
+        factor = bad ? 0.f : __fdiv_rn(most, top);
+    }
+};
+// 16 of them. A factor of zero: a row without a value.
+template <int OUT>
+__device__ __forceinline__ uint4 row_codes(const float2 (&v)[8], float factor) {
+    uint32_t w[4] = {0, 0, 0, 0};
+    if (factor == 0.f) return make_uint4(0, 0, 0, 0);
+    const float2 f2 = make_float2(factor, factor);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 a = mul2(v[2 * i], f2), b = mul2(v[2 * i + 1], f2);
+        if constexpr (OUT == kRowE4) {
+            uint16_t lo, hi;
+            asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(a.y), "f"(a.x));
+            asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(b.y), "f"(b.x));
+            w[i] = uint32_t(lo) | (uint32_t(hi) << 16);
+        } else {
+            // 127 (most / largest) largest may round up to just above 127, never to 127.5
+            const int q0 = __float2int_rn(a.x), q1 = __float2int_rn(a.y), q2 = __float2int_rn(b.x), q3 = __float2int_rn(b.y);
+            w[i] = __byte_perm(__byte_perm(q0, q1, 0x0040), __byte_perm(q2, q3, 0x0040), 0x5410);
+        }
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+template <int OUT>
+constexpr float kRowMost = OUT == kRowI8 ? 127.f : 448.f;
 
 // A unit: 16 consecutive values of a row, 32 bytes in 16 bits and 8 as codes.
 template <typename T>
@@ -408,6 +446,8 @@ __device__ __forceinline__ void write_unit(const RmsnormBlockDev &p, int64_t row
 #pragma unroll
         for (int i = 0; i < 8; ++i) r[i] = pack2(h[i], T());
         store32(static_cast<T *>(p.out) + (row * units + at) * 16, r);
+    } else if constexpr (OUT == kRowI8 || OUT == kRowE4) {
+        if (in) *reinterpret_cast<uint4 *>(static_cast<uint8_t *>(p.out) + (row * units + at) * 16) = row_codes<OUT>(h, g);
     } else {
         uint8_t *codes = static_cast<uint8_t *>(p.out) + (row * units + at) * 8;
         if constexpr (OUT == kFp4Mx) {
@@ -538,7 +578,7 @@ rmsnorm_rows_kernel(const RmsnormBlockDev p) {
                 weight(pre, FULL || at < units ? at : 0, wn);
                 normed_unit<T>(x[j], ry, wn, h);
             };
-            if constexpr (OUT == kFp4Nv) {
+            if constexpr (by_row(OUT)) {
 #pragma unroll
                 for (int j = 0; j < U; ++j) {
                     unit(j);
@@ -546,13 +586,19 @@ rmsnorm_rows_kernel(const RmsnormBlockDev p) {
                     amax = max(amax, bmax[j]);
                 }
                 amax = __reduce_max_sync(LANES == 32 ? kFull : 0xFFFFu << (threadIdx.x & 16), amax);
-                g = nv_row_scale(amax);
-                if (lane == 0 && live) p.row_scale[row] = g;
+                if constexpr (OUT == kFp4Nv) {
+                    g = nv_row_scale(amax);
+                    if (lane == 0 && live) p.row_scale[row] = g;
+                } else {
+                    const RowScale8 r8(amax, kRowMost<OUT>);
+                    g = r8.factor;
+                    if (lane == 0 && live) p.row_scale[row] = r8.scale;
+                }
             }
 #pragma unroll
             for (int j = 0; j < U; ++j) {
                 const int at = lane + j * LANES;
-                if (OUT != kFp4Nv || U > 1) unit(j);
+                if (!by_row(OUT) || U > 1) unit(j);
                 write_unit<T, OUT>(p, row, at, units, tiles, FULL ? live : live && at < units, h, OUT == kFp4Nv ? bmax[j] : 0, g);
             }
         }
@@ -619,6 +665,10 @@ rmsnorm_block_kernel(const RmsnormBlockDev p) {
         if constexpr (OUT == kFp4Nv) {
             g = nv_row_scale(row_max(amax, maxima));
             if (lane == 0) p.row_scale[row] = g;
+        } else if constexpr (by_row(OUT)) {
+            const RowScale8 r8(row_max(amax, maxima), kRowMost<OUT>);
+            g = r8.factor;
+            if (lane == 0) p.row_scale[row] = r8.scale;
         }
 #pragma unroll
         for (int j = 0; j < U; ++j) {
@@ -708,6 +758,8 @@ int launch_rmsnorm_block(const RmsnormBlockDev &p, int out, cudaStream_t stream)
         case kFp4Plain: return launch_rmsnorm_block<T, kFp4Plain>(p, stream);
         case kFp4Mx: return launch_rmsnorm_block<T, kFp4Mx>(p, stream);
         case kFp4Nv: return launch_rmsnorm_block<T, kFp4Nv>(p, stream);
+        case kRowI8: return launch_rmsnorm_block<T, kRowI8>(p, stream);
+        case kRowE4: return launch_rmsnorm_block<T, kRowE4>(p, stream);
         default: return launch_rmsnorm_block<T, kFp4None>(p, stream);
     }
 }
@@ -787,20 +839,21 @@ extern "C" int fluke_sm100_dequant_fp4(const void *codes, const void *scale, con
 
 extern "C" int fluke_sm100_rmsnorm_block(const fluke_sm100_rmsnorm_block_t *b, void *stream) {
     if (!b || !fp4_shape_ok(b->rows, b->cols) || b->cols > FLUKE_SM100_FP4_MAX_ROW || b->seqlen < 0) return (int)cudaErrorInvalidValue;
-    if (b->out_format < kFp4Plain || b->out_format > kFp4None) return (int)cudaErrorInvalidValue;
+    if (b->out_format < kFp4Plain || b->out_format > kRowE4) return (int)cudaErrorInvalidValue;
     if (b->rows == 0) return 0;
-    const bool quant = b->out_format == kFp4Mx || b->out_format == kFp4Nv;
+    const bool fp4 = b->out_format == kFp4Mx || b->out_format == kFp4Nv, rows8 = b->out_format == kRowI8 || b->out_format == kRowE4;
+    const bool quant = fp4 || rows8, row_scales = by_row(b->out_format);
     if (!b->x || !b->residual || !b->residual_out) return (int)cudaErrorInvalidValue;
     if (b->out_format != kFp4None && (!b->w_pre || !b->out)) return (int)cudaErrorInvalidValue;
-    if ((quant && !b->scale) || (b->out_format == kFp4Nv && !b->row_scale)) return (int)cudaErrorInvalidValue;
-    if (!aligned32(b->x, b->residual, b->residual_out, quant ? nullptr : b->out) || (quant && !(aligned16(b->out) && aligned16(b->scale))) ||
-        !aligned32(b->w_post, b->gate, b->w_pre) || (b->out_format == kFp4Nv && !aligned4(b->row_scale)))
+    if ((fp4 && !b->scale) || (row_scales && !b->row_scale)) return (int)cudaErrorInvalidValue;
+    if (!aligned32(b->x, b->residual, b->residual_out, quant ? nullptr : b->out) || (quant && !aligned16(b->out)) || (fp4 && !aligned16(b->scale)) ||
+        !aligned32(b->w_post, b->gate, b->w_pre) || (row_scales && !aligned4(b->row_scale)))
         return (int)cudaErrorMisalignedAddress;
     // A row is read before it is written, but rows come in any order: the stream and a 16-bit result lie where x or the residual of the same rows does, or apart
     // from everything; what all rows read, and scales, lie apart from everything.
-    const uint64_t row_bytes = uint64_t(b->cols) * 2, bytes = b->rows * row_bytes, out_bytes = b->out_format == kFp4None ? 0 : quant ? bytes / 4 : bytes;
+    const uint64_t row_bytes = uint64_t(b->cols) * 2, bytes = b->rows * row_bytes, out_bytes = b->out_format == kFp4None ? 0 : rows8 ? bytes / 2 : quant ? bytes / 4 : bytes;
     const uint64_t gates = b->seqlen > 0 ? (uint64_t(b->rows) + b->seqlen - 1) / b->seqlen : 1;
-    const uint64_t scale_bytes = quant ? (uint64_t(b->rows) + 127) / 128 * fp4_tiles(b->cols, b->out_format) * 512 : 0;
+    const uint64_t scale_bytes = fp4 ? (uint64_t(b->rows) + 127) / 128 * fp4_tiles(b->cols, b->out_format) * 512 : 0;
     struct Range { const void *at; uint64_t n; };
     auto apart = [](Range a, Range c) {
         const uint64_t x = reinterpret_cast<uintptr_t>(a.at), y = reinterpret_cast<uintptr_t>(c.at);
@@ -808,7 +861,7 @@ extern "C" int fluke_sm100_rmsnorm_block(const fluke_sm100_rmsnorm_block_t *b, v
     };
     const Range in[] = {{b->x, bytes}, {b->residual, bytes}, {b->w_post, b->w_post ? row_bytes : 0}, {b->gate, b->gate ? gates * row_bytes : 0},
                         {b->w_pre, b->out_format != kFp4None ? row_bytes : 0}};
-    const Range out[] = {{b->residual_out, bytes}, {b->out, out_bytes}, {b->scale, scale_bytes}, {b->row_scale, b->out_format == kFp4Nv ? uint64_t(b->rows) * 4 : 0}};
+    const Range out[] = {{b->residual_out, bytes}, {b->out, out_bytes}, {b->scale, scale_bytes}, {b->row_scale, row_scales ? uint64_t(b->rows) * 4 : 0}};
     for (int o = 0; o < 4; ++o) {
         for (int i = 0; i < 5; ++i) {
             const bool in_place = i < 2 && out[o].at == in[i].at && (o == 0 || (o == 1 && !quant));

@@ -35,7 +35,8 @@ namespace {
     X(fluke_gated_mlp_fp8_plain_gpu) X(fluke_gemm_i8_gpu) X(fluke_gemm_fp8_gpu) X(fluke_down_proj_i8_gpu) \
     X(fluke_down_proj_fp8_gpu) X(fluke_factored_lstm_step_i8_gpu) X(fluke_factored_lstm_step_fp8_gpu) X(fluke_last_error) \
     X(fluke_fp4_scale_bytes) X(fluke_quant_mxfp4_gpu) X(fluke_quant_nvfp4_gpu) X(fluke_dequant_mxfp4_gpu) X(fluke_dequant_nvfp4_gpu) \
-    X(fluke_gemm_mxfp4_gpu) X(fluke_gemm_nvfp4_gpu) X(fluke_gated_mlp_mxfp4_gpu) X(fluke_gated_mlp_nvfp4_gpu) X(fluke_rmsnorm_block_gpu)
+    X(fluke_gemm_mxfp4_gpu) X(fluke_gemm_nvfp4_gpu) X(fluke_gated_mlp_mxfp4_gpu) X(fluke_gated_mlp_nvfp4_gpu) X(fluke_rmsnorm_block_gpu) \
+    X(fluke_linear_gpu) X(fluke_linear_recurrence_gpu) X(fluke_linear_recurrence_backward_gpu)
 
 struct Entry {
 #define X(name) decltype(&::name) name = nullptr;
@@ -523,19 +524,140 @@ PyObject *rmsnorm_block(Args a) {
         required(a[9]);
         expect(stream, "residual_out", type, {m, k}, x);
     }
-    if (pre) out = format == 0 ? empty_on(x, {m, k}, type) : empty_on(x, {m, k / 2}, at::kByte);
-    if (format != 0) scale = new_scale(x, m, k, format == FLUKE_FP4_NV);
-    if (format == FLUKE_FP4_NV) row = empty_on(x, {m}, at::kFloat);
+    const bool fp4 = format == FLUKE_FP4_MX || format == FLUKE_FP4_NV, by_row = format != 0 && format != FLUKE_FP4_MX;
+    if (pre) out = format == 0 ? empty_on(x, {m, k}, type) : fp4 ? empty_on(x, {m, k / 2}, at::kByte) : empty_on(x, {m, k}, format == FLUKE_ROW_INT8 ? at::kChar : at::kByte);
+    if (fp4) scale = new_scale(x, m, k, format == FLUKE_FP4_NV);
+    if (by_row) row = empty_on(x, {m}, at::kFloat);
     b.n_tokens = m; b.hidden_dim = k; b.seqlen = gate ? seqlen : 0;
     b.x = ptr(x); b.residual = ptr(res); b.post_weight = ptr(post); b.gate = ptr(gate); b.pre_weight = ptr(pre);
     b.alpha = real(a[5]); b.eps = real(a[6]);
     b.residual_out = ptr(stream);
     b.out_format = format;
     if (pre) b.out = ptr(out);
-    if (format != 0) b.scale = ptr(scale);
-    if (format == FLUKE_FP4_NV) b.row_scale = ptr(row);
+    if (fp4) b.scale = ptr(scale);
+    if (by_row) b.row_scale = ptr(row);
     check(on_device(x, [&] { return L.fluke_rmsnorm_block_gpu(&b); }), "fluke_rmsnorm_block_gpu");
-    return wrap_all({&stream, pre ? &out : nullptr, format != 0 ? &scale : nullptr, format == FLUKE_FP4_NV ? &row : nullptr});
+    return wrap_all({&stream, pre ? &out : nullptr, fp4 ? &scale : nullptr, by_row ? &row : nullptr});
+}
+
+// ---- 16-bit product with an epilogue, gated linear recurrence --------------------------------------
+
+// A tensor on the GPU whose last dimension is dense, with this many dimensions.
+const at::Tensor &rows_of(PyObject *o, const char *what, int64_t dims) {
+    const at::Tensor &t = tensor(o);
+    if (!t.is_cuda()) {
+        PyErr_SetString(PyExc_RuntimeError, "fluke_b200.ops needs CUDA tensors (there is no CPU fallback)");
+        throw Failed();
+    }
+    if (t.dim() != dims) refuse("fluke_b200.ops: %s has %lld dimensions, %lld are needed", what, (long long)t.dim(), (long long)dims);
+    if (t.size(dims - 1) > 1 && t.stride(dims - 1) != 1) refuse("fluke_b200.ops: the rows of %s are not dense", what);
+    return t;
+}
+// Distance between rows; one row has any.
+long long pitch(const at::Tensor &t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
+
+// x, weight, bias, activation, residual, alpha, out
+PyObject *linear(Args a) {
+    const at::Tensor &x = rows_of(a[0], "x", 2), &w = required(a[1], 2);
+    const at::Tensor *bias = input(a[2]), *res = a[4] == Py_None ? nullptr : &rows_of(a[4], "residual", 2);
+    const at::ScalarType type = x.scalar_type();
+    fluke_linear_t l = {};
+    l.dtype = activation_type(type);
+    l.M = small(x.size(0), "rows"); l.K = small(x.size(1), "columns"); l.N = small(w.size(0), "columns");
+    if (l.K % 8 != 0 || l.K == 0) refuse("fluke_b200.ops: rows of %d values, a multiple of 8 is needed", l.K);
+    if (l.N % 8 != 0 || l.N == 0) refuse("fluke_b200.ops: a weight of %d rows, a multiple of 8 is needed", l.N);
+    expect(w, "weight", type, {l.N, l.K}, x);
+    if (bias) expect(*bias, "bias", type, {l.N}, x);
+    if (res) expect(*res, "residual", type, {l.M, l.N}, x);
+    at::Tensor out;
+    if (a[6] == Py_None) {
+        out = empty_on(x, {l.M, l.N}, type);
+    } else {
+        out = rows_of(a[6], "out", 2);
+        expect(out, "out", type, {l.M, l.N}, x);
+    }
+    l.activation = integer(a[3]);
+    l.x = ptr(x); l.weight = ptr(w); l.bias = ptr(bias); l.residual = ptr(res); l.out = ptr(out);
+    l.ld_x = pitch(x); l.ld_residual = res ? pitch(*res) : 0; l.ld_out = pitch(out);
+    l.alpha = real(a[5]);
+    check(on_device(x, [&] { return L.fluke_linear_gpu(&l); }), "fluke_linear_gpu");
+    return wrap(out);
+}
+
+// Strides of a tensor [T, B, H]; a dimension of one element has any.
+long long step_of(const at::Tensor &t) { return t.size(0) > 1 ? t.stride(0) : t.size(2); }
+long long chunk_of(const at::Tensor &t) { return t.size(1) > 1 ? t.stride(1) : t.size(2); }
+// A new tensor [T, B, H] with the leading dimensions in `like`'s order.
+at::Tensor new_steps(const at::Tensor &like) {
+    const int64_t t = like.size(0), b = like.size(1), h = like.size(2);
+    if (t > 1 && b > 1 && like.stride(1) > like.stride(0)) return empty_on(like, {b, t, h}, like.scalar_type()).transpose(0, 1);
+    return empty_on(like, {t, b, h}, like.scalar_type());
+}
+const at::Tensor *state_of(PyObject *o, const char *what, const at::Tensor &like) {
+    const at::Tensor *t = input(o);
+    if (t) expect(*t, what, at::kFloat, {like.size(1), like.size(2)}, like);
+    return t;
+}
+const at::Tensor *lengths_of(PyObject *o, const at::Tensor &like) {
+    const at::Tensor *t = input(o);
+    if (t) expect(*t, "lengths", at::kInt, {like.size(1)}, like);
+    return t;
+}
+template <typename R>
+void steps_of(R &r, const at::Tensor &gate, const at::Tensor &value) {
+    r.dtype = activation_type(gate.scalar_type());
+    r.T = small(gate.size(0), "steps"); r.B = small(gate.size(1), "chunks"); r.H = small(gate.size(2), "channels");
+    if (r.H % 2 != 0) refuse("fluke_b200.ops: %d channels, an even number is needed", r.H);
+    expect(value, "value", gate.scalar_type(), gate.sizes(), gate);
+    r.gate = ptr(gate); r.value = ptr(value);
+    r.gate_step = step_of(gate); r.gate_chunk = chunk_of(gate);
+    r.value_step = step_of(value); r.value_chunk = chunk_of(value);
+}
+
+// gate, value, h0, lengths, reverse, save, out, h_last
+PyObject *linear_recurrence(Args a) {
+    const at::Tensor &gate = rows_of(a[0], "gate", 3), &value = rows_of(a[1], "value", 3);
+    fluke_linear_recurrence_t r = {};
+    steps_of(r, gate, value);
+    const at::Tensor *h0 = state_of(a[2], "h0", gate), *lengths = lengths_of(a[3], gate);
+    const bool save = truth(a[5]);
+    at::Tensor out, last, states;
+    if (a[6] == Py_None) {
+        out = new_steps(value);
+    } else {
+        out = rows_of(a[6], "out", 3);
+        expect(out, "out", gate.scalar_type(), gate.sizes(), gate);
+    }
+    if (a[7] == Py_None) last = empty_on(gate, {r.B, r.H}, at::kFloat);
+    else {
+        state_of(a[7], "h_last", gate);
+        last = tensor(a[7]);
+    }
+    if (save) states = empty_on(gate, {(int64_t(r.T) + 63) / 64, r.B, r.H}, at::kFloat);
+    r.reverse = truth(a[4]);
+    r.out = ptr(out); r.out_step = step_of(out); r.out_chunk = chunk_of(out);
+    r.lengths = ptr(lengths); r.h0 = ptr(h0); r.h_last = ptr(last);
+    r.states = save ? ptr(states) : nullptr;
+    check(on_device(gate, [&] { return L.fluke_linear_recurrence_gpu(&r); }), "fluke_linear_recurrence_gpu");
+    return wrap_all({&out, &last, save ? &states : nullptr});
+}
+
+// grad, gate, value, states, grad_last, lengths, reverse
+PyObject *linear_recurrence_backward(Args a) {
+    const at::Tensor &grad = rows_of(a[0], "grad", 3), &gate = rows_of(a[1], "gate", 3), &value = rows_of(a[2], "value", 3), &states = required(a[3]);
+    fluke_linear_recurrence_grad_t r = {};
+    steps_of(r, gate, value);
+    expect(grad, "grad", gate.scalar_type(), gate.sizes(), gate);
+    expect(states, "states", at::kFloat, {(int64_t(r.T) + 63) / 64, r.B, r.H}, gate);
+    const at::Tensor *grad_last = state_of(a[4], "grad_last", gate), *lengths = lengths_of(a[5], gate);
+    at::Tensor dg = new_steps(gate), dv = new_steps(value), dh = empty_on(gate, {r.B, r.H}, at::kFloat);
+    r.reverse = truth(a[6]);
+    r.grad = ptr(grad); r.grad_step = step_of(grad); r.grad_chunk = chunk_of(grad);
+    r.grad_gate = ptr(dg); r.grad_gate_step = step_of(dg); r.grad_gate_chunk = chunk_of(dg);
+    r.grad_value = ptr(dv); r.grad_value_step = step_of(dv); r.grad_value_chunk = chunk_of(dv);
+    r.lengths = ptr(lengths); r.states = ptr(states); r.grad_last = ptr(grad_last); r.grad_h0 = ptr(dh);
+    check(on_device(gate, [&] { return L.fluke_linear_recurrence_backward_gpu(&r); }), "fluke_linear_recurrence_backward_gpu");
+    return wrap_all({&dg, &dv, &dh});
 }
 
 // {name: address} of the loaded library's entry points
@@ -573,7 +695,8 @@ PyMethodDef methods[] = {
     {"bind", bind, METH_O, nullptr}, {"names", names, METH_NOARGS, nullptr},
     FAST(rmsnorm, 6), FAST(rmsnorm_quant, 7), FAST(quant, 4), FAST(dequant_transpose, 3), FAST(rotary_emb, 11), FAST(rotary_qkv, 4),
     FAST(silu_mul, 1), FAST(flstm_step, 4), FAST(qkv_rotary, 11), FAST(gated_mlp, 10), FAST(gemm_i8, 5), FAST(gemm_fp8, 4),
-    FAST(down_proj, 6), FAST(lstm_step, 6), FAST(quant_fp4, 2), FAST(dequant_fp4, 5), FAST(gemm_fp4, 12), FAST(rmsnorm_block, 10), {nullptr, nullptr, 0, nullptr}};
+    FAST(down_proj, 6), FAST(lstm_step, 6), FAST(quant_fp4, 2), FAST(dequant_fp4, 5), FAST(gemm_fp4, 12), FAST(rmsnorm_block, 10),
+    FAST(linear, 7), FAST(linear_recurrence, 8), FAST(linear_recurrence_backward, 7), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -15,7 +15,7 @@ import sys
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 SO_PATH = os.path.join(ROOT, "lib", "libfluke.so")
 
-P, I, F, Z = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_size_t
+P, I, F, Z, LL = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_size_t, ctypes.c_longlong
 
 
 class fluke_dims_t(ctypes.Structure):
@@ -44,7 +44,30 @@ class fluke_rmsnorm_block_t(ctypes.Structure):
                 ("alpha", F), ("eps", F), ("residual_out", P), ("out_format", I), ("out", P), ("scale", P), ("row_scale", P)]
 
 
+class fluke_linear_t(ctypes.Structure):
+    _fields_ = [("M", I), ("N", I), ("K", I), ("dtype", I), ("activation", I),
+                ("x", P), ("weight", P), ("bias", P), ("residual", P), ("out", P),
+                ("ld_x", LL), ("ld_residual", LL), ("ld_out", LL), ("alpha", F)]
+
+
+class fluke_linear_recurrence_t(ctypes.Structure):
+    _fields_ = [("T", I), ("B", I), ("H", I), ("dtype", I), ("reverse", I),
+                ("gate", P), ("value", P), ("out", P),
+                ("gate_step", LL), ("gate_chunk", LL), ("value_step", LL), ("value_chunk", LL), ("out_step", LL), ("out_chunk", LL),
+                ("lengths", P), ("h0", P), ("h_last", P), ("states", P)]
+
+
+class fluke_linear_recurrence_grad_t(ctypes.Structure):
+    _fields_ = [("T", I), ("B", I), ("H", I), ("dtype", I), ("reverse", I),
+                ("gate", P), ("value", P), ("grad", P), ("grad_gate", P), ("grad_value", P),
+                ("gate_step", LL), ("gate_chunk", LL), ("value_step", LL), ("value_chunk", LL), ("grad_step", LL), ("grad_chunk", LL),
+                ("grad_gate_step", LL), ("grad_gate_chunk", LL), ("grad_value_step", LL), ("grad_value_chunk", LL),
+                ("lengths", P), ("states", P), ("grad_last", P), ("grad_h0", P)]
+
+
 FP4_MX, FP4_NV = 1, 2
+ROW_INT8, ROW_FP8 = 4, 5
+ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu": 3, "tanh": 4, "sigmoid": 5}
 
 # name -> (restype, argtypes). The first ten are exactly fluke_lib._SIGNATURES of the reference.
 VOID_SIGNATURES = {
@@ -116,6 +139,10 @@ SIGNATURES = {
     "fluke_gated_mlp_mxfp4_gpu": (I, [P] * 7 + [I] * 4),
     "fluke_gated_mlp_nvfp4_gpu": (I, [P] * 10 + [I] * 4),
     "fluke_rmsnorm_block_gpu": (I, [ctypes.POINTER(fluke_rmsnorm_block_t)]),
+    # 16-bit product with an epilogue, gated linear recurrence
+    "fluke_linear_gpu": (I, [ctypes.POINTER(fluke_linear_t)]),
+    "fluke_linear_recurrence_gpu": (I, [ctypes.POINTER(fluke_linear_recurrence_t)]),
+    "fluke_linear_recurrence_backward_gpu": (I, [ctypes.POINTER(fluke_linear_recurrence_grad_t)]),
     # internal status word (bounded device waits)
     "fluke_sm100_read_status": (I, [ctypes.POINTER(ctypes.c_uint), I]),
     "fluke_sm100_copy_rows_async": (I, [P, ctypes.c_size_t, P, ctypes.c_size_t, ctypes.c_size_t, ctypes.c_size_t, I, P]),

@@ -205,16 +205,46 @@ def gated_mlp_nvfp4(a, a_scale, a_row, gate, gate_scale, gate_row, up, up_scale,
 
 def rmsnorm_block(x, residual, post_weight, gate, pre_weight, alpha, eps, seqlen=0, quant=None, residual_out=None):
     """Norms around a block: stream = alpha * residual + gate * norm(x, post_weight), then norm(stream, pre_weight)
-    for the next block, as 16-bit values (quant None) or quantised ("mxfp4", "nvfp4"). gate [cols], or
+    for the next block, as 16-bit values (quant None) or quantised: "mxfp4", "nvfp4", or "int8" (int8 codes) and "fp8"
+    (e4m3 bytes) under an f32 scale per row, as the 8-bit products take them. gate [cols], or
     [ceil(rows / seqlen), cols] with seqlen > 0. post_weight, gate and pre_weight may be None. Returns the
     stream (written to `residual_out`, which may be `residual` or `x`, or to a new tensor) followed by the
-    next block's input: (stream, out), (stream, codes, scale[, row_scale]), or (stream,) without pre_weight."""
+    next block's input: (stream, out), (stream, codes, scale[, row_scale]) with the row scales alone for 8 bits, or (stream,) without
+    pre_weight."""
     if quant not in _QUANT:
-        raise ValueError(f"quant is None, 'mxfp4' or 'nvfp4', not {quant!r}")
+        raise ValueError(f"quant is None, 'mxfp4', 'nvfp4', 'int8' or 'fp8', not {quant!r}")
     return _N.rmsnorm_block(x, residual, post_weight, gate, pre_weight, alpha, eps, seqlen, _QUANT[quant], residual_out)
 
 
-_QUANT = {None: 0, "mxfp4": _lib.FP4_MX, "nvfp4": _lib.FP4_NV}
+_QUANT = {None: 0, "mxfp4": _lib.FP4_MX, "nvfp4": _lib.FP4_NV, "int8": _lib.ROW_INT8, "fp8": _lib.ROW_FP8}
+
+
+# ---- 16-bit product with an epilogue, gated linear recurrence (additive) ----------------------
+# f16 or bf16; inputs may be views whose last dimension is dense (columns of a wider tensor, transposed leading
+# dimensions). A wrong type, shape, device, stride or alignment raises; the calls run on the tensors' device.
+
+def linear(x, weight, bias=None, activation=None, residual=None, alpha=1.0, out=None):
+    """[M, N] = activation(x [M, K] @ weight [N, K]^T + bias [N]) + alpha * residual [M, N], rounded once. activation: None,
+    "relu", "silu", "gelu", "tanh" or "sigmoid". K and N are multiples of 8, rows begin on 16 bytes. `out` may be
+    `residual`, else it lies apart from the inputs."""
+    if activation not in _lib.ACTIVATIONS:
+        raise ValueError(f"activation is None, 'relu', 'silu', 'gelu', 'tanh' or 'sigmoid', not {activation!r}")
+    return _N.linear(x, weight, bias, _lib.ACTIVATIONS[activation], residual, alpha, out)
+
+
+def linear_recurrence(gate, value, h0=None, lengths=None, reverse=False, save=False, out=None, h_last=None):
+    """h_t = f_t h_{t-1} + (1 - f_t) value_t with f = sigmoid(gate), per chunk and channel of gate and value [T, B, H], over t = 0 ..
+    T-1, or T-1 .. 0 with `reverse`. h0 f32 [B, H] (None: zeros). With lengths (int32 [B]) the steps t >= lengths[b] are not
+    taken and their output is zero. Returns (out, h_last), out as `value` in type and, where it is new, in the order of
+    its leading dimensions, h_last f32 [B, H] (may be given, as h0 itself too); with `save` also the states that
+    linear_recurrence_backward needs."""
+    return _N.linear_recurrence(gate, value, h0, lengths, reverse, save, out, h_last)
+
+
+def linear_recurrence_backward(grad, gate, value, states, grad_last=None, lengths=None, reverse=False):
+    """Gradients (of gate, of value, of h0) from those of out (grad [T, B, H]) and of h_last (f32 [B, H] or None: zeros), with
+    the inputs of the forward call and the states it saved."""
+    return _N.linear_recurrence_backward(grad, gate, value, states, grad_last, lengths, reverse)
 
 
 # ---- factored LSTM (additive) ---------------------------------------------------------------

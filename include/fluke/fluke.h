@@ -548,6 +548,9 @@ int fluke_factored_lstm_layer_i8_noalloc_gpu(const fluke_flstm_layer_t *layer);
  * ---------------------------------------------------------------------------------- */
 enum { FLUKE_F16 = 0, FLUKE_BF16 = 1 };
 enum { FLUKE_FP4_MX = 1, FLUKE_FP4_NV = 2 };
+/* 8-bit output of the norms around a block, for the 8-bit products: scale[row] = max(amax, 1e-12) / 127 (int8) or / 448 (e4m3),
+ * code = v * (127 or 448 / max(amax, 1e-12)) to the nearest, ties to even. A row with an infinity or a NaN has the scale NaN and zeros. */
+enum { FLUKE_ROW_INT8 = 4, FLUKE_ROW_FP8 = 5 };
 
 /* Bytes of the block scales of a [rows, cols] matrix; 0 for sizes or a format that there is not. */
 size_t fluke_fp4_scale_bytes(int rows, int cols, int format);
@@ -596,12 +599,78 @@ typedef struct {
     const void *pre_weight;     /* [hidden_dim] or NULL                                             */
     float alpha, eps;
     void *residual_out;         /* [n_tokens, hidden_dim]; may be residual or x itself              */
-    int out_format;             /* 0: 16 bits, FLUKE_FP4_MX, FLUKE_FP4_NV                           */
+    int out_format;             /* 0: 16 bits, FLUKE_FP4_MX, FLUKE_FP4_NV, FLUKE_ROW_INT8, FLUKE_ROW_FP8 */
     void *out;                  /* 16-bit values (may be x or residual itself) or codes; apart from residual_out */
-    void *scale;                /* quantised: block scales                                          */
-    void *row_scale;            /* nvfp4: f32 [n_tokens]                                            */
+    void *scale;                /* mxfp4, nvfp4: block scales                                       */
+    void *row_scale;            /* nvfp4, int8, e4m3: f32 [n_tokens]                                */
 } fluke_rmsnorm_block_t;
 int fluke_rmsnorm_block_gpu(const fluke_rmsnorm_block_t *block);
+
+/* ------------------------------------------------------------------------------------
+ * Part 7 -- around and instead of the quantised products (no counterpart in the reference): a 16-bit product with its
+ * epilogue, and a gated linear recurrence with its gradients. All return 0 or a CUDA error code (fluke_last_error() tells it
+ * in words), check sizes, strides and alignment before they launch, and take f16 or bf16 tensors by `dtype`.
+ * ---------------------------------------------------------------------------------- */
+
+/* out = activation(x @ weight^T + bias) + alpha * residual, sums and what follows in f32, rounded once:
+ *     relu max(v, 0), silu v / (1 + exp(-v)), gelu v Phi(v) with the normal distribution Phi, tanh, sigmoid 1 / (1 + exp(-v)).
+ * Rows of x, residual and out may be apart (columns of a wider tensor). K and N are multiples of 8, row distances multiples
+ * of 8 and at least the row's length, all tensors start on 16 bytes. The output lies apart from everything but a residual in the same place. */
+enum { FLUKE_ACT_NONE = 0, FLUKE_ACT_RELU = 1, FLUKE_ACT_SILU = 2, FLUKE_ACT_GELU = 3, FLUKE_ACT_TANH = 4, FLUKE_ACT_SIGMOID = 5 };
+typedef struct {
+    int M, N, K;
+    int dtype;                  /* of every tensor                                                  */
+    int activation;
+    const void *x;              /* [M, K]                                                           */
+    const void *weight;         /* [N, K], dense                                                    */
+    const void *bias;           /* [N] or NULL                                                      */
+    const void *residual;       /* [M, N] or NULL                                                   */
+    void *out;                  /* [M, N]; may be residual                                          */
+    long long ld_x, ld_residual, ld_out;    /* values from row to row                               */
+    float alpha;                /* of residual                                                      */
+} fluke_linear_t;
+int fluke_linear_gpu(const fluke_linear_t *linear);
+
+/* Gated linear recurrence over time, per chunk and channel, in processing order (t = 0 .. T-1, or T-1 .. 0 with `reverse`):
+ *     h_t = f_t h_{t-1} + (1 - f_t) value_t,   f_t = sigmoid(gate_t),   out_t = h_t
+ * in f32 from h0 (zeros where it is NULL), out rounded to 16 bits; h_last is the state behind the last step. The state of a
+ * stream is carried from call to call by h0 and h_last, down to single steps. Gate, value and out are [T, B, H] by their strides
+ * (values between steps and between chunks: time- or batch-major, or columns of wider rows), with H values in a row. H and the
+ * strides are even, the strides at least H, 16-bit tensors start on 4 bytes, f32 ones on 8. With `lengths` (int32 [B], limited to 0 .. T) the steps t >= lengths[b]
+ * of chunk b are not taken: out is zero there, whatever the inputs hold. `states` receives what the gradients need: the
+ * state in front of every 64th step, f32 [ceil(T / 64), B, H]. Outputs lie apart from inputs and from each other, but for h_last
+ * in the place of h0. Results do not depend on how the work is spread beyond the rounding of f32, and are the same from call to call. */
+typedef struct {
+    int T, B, H;
+    int dtype;                  /* of gate, value, out                                              */
+    int reverse;
+    const void *gate, *value;
+    void *out;
+    long long gate_step, gate_chunk, value_step, value_chunk, out_step, out_chunk;
+    const void *lengths;        /* or NULL                                                          */
+    const void *h0;             /* f32 [B, H] or NULL                                               */
+    void *h_last;               /* f32 [B, H] or NULL; may be h0                                    */
+    void *states;               /* or NULL                                                          */
+} fluke_linear_recurrence_t;
+int fluke_linear_recurrence_gpu(const fluke_linear_recurrence_t *r);
+
+/* Its gradients: those of gate, value and h0, from the gradients of out (grad) and of h_last (grad_last, zeros where it is NULL) and the
+ * states that the forward call kept. With e_t the gradient of h_t: grad_value = (1 - f_t) e_t, grad_gate = e_t (h_{t-1} - value_t) f_t (1 - f_t),
+ * and f_t e_t reaches h_{t-1}. Zero behind a chunk's length. Computed in f32, grad_gate and grad_value rounded to 16 bits. */
+typedef struct {
+    int T, B, H;
+    int dtype;                  /* of gate, value, grad, grad_gate, grad_value                      */
+    int reverse;
+    const void *gate, *value, *grad;
+    void *grad_gate, *grad_value;
+    long long gate_step, gate_chunk, value_step, value_chunk, grad_step, grad_chunk;
+    long long grad_gate_step, grad_gate_chunk, grad_value_step, grad_value_chunk;
+    const void *lengths;        /* as in the forward call                                           */
+    const void *states;         /* from the forward call                                            */
+    const void *grad_last;      /* f32 [B, H] or NULL                                               */
+    void *grad_h0;              /* f32 [B, H] or NULL; may be grad_last                             */
+} fluke_linear_recurrence_grad_t;
+int fluke_linear_recurrence_backward_gpu(const fluke_linear_recurrence_grad_t *r);
 
 #endif /* HAVE_CUDA || HAVE_ROCM */
 

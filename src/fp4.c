@@ -91,7 +91,8 @@ int fluke_rmsnorm_block_gpu(const fluke_rmsnorm_block_t *b) {
     s.bf16 = b->dtype == FLUKE_BF16;
     /* without the second norm only the stream is written, whatever the format */
     s.out_format = b->pre_weight ? b->out_format : 3;
-    if (b->out_format != 0 && b->out_format != FLUKE_FP4_MX && b->out_format != FLUKE_FP4_NV)
+    if (b->out_format != 0 && b->out_format != FLUKE_FP4_MX && b->out_format != FLUKE_FP4_NV &&
+        b->out_format != FLUKE_ROW_INT8 && b->out_format != FLUKE_ROW_FP8)
         return fluke_host_note_error(1);
     s.x = b->x; s.residual = b->residual; s.residual_out = b->residual_out;
     s.w_post = b->post_weight; s.gate = b->gate; s.w_pre = b->pre_weight;
