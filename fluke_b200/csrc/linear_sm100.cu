@@ -280,6 +280,244 @@ linear_split_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
     }
 }
 
+// ---- many tiles: pairs of SMs -------------------------------------------------------------------
+// A pair of CTAs (cluster of 2) works on tiles of 256 rows of x by BN columns with tcgen05 cta_group::2. Each CTA loads its own 128
+// rows of x and half of the weight's rows and holds its 128 rows of the sums; the first CTA issues for both. The sums have two
+// buffers in tensor memory, so that the epilogue of a tile runs under the MMAs of the next. The tiles of a residual come by TMA into the
+// staging that the output leaves from, ahead of the sums.
+//
+// In each CTA warp 0 loads (one thread), warp 1 owns tensor memory and (first CTA) issues MMAs, warps 2-3 are idle and the others are
+// the epilogue: 32 rows x BN / 2 columns each.
+//
+// Pairs take tiles in turns, and the tiles are ordered in bands of kLinBand rows of tiles, column by column: what runs at the same time shares
+// rows of x and of the weight in L2.
+constexpr int kLinBand = 8;
+template <int BN>
+struct LinPairLayout {
+    static constexpr int kOperandX = 128 * 128, kOperandW = BN / 2 * 128;
+    static constexpr int kSlot = kOperandX + kOperandW;
+    static constexpr int kStages = BN == 256 ? 5 : 7;
+    static constexpr int kGroups = BN / 128;                   // of 64 columns, per epilogue warp
+    static constexpr int kOffStaging = kStages * kSlot;
+    static constexpr int kOffBars = kOffStaging + 8 * kGroups * 32 * 128;
+    static constexpr int kBars = 2 * kStages + 4 + 8 * kGroups;
+    static constexpr int kDynamic = kOffBars + kBars * 8 + 16 + 1024;
+    static_assert(kOffStaging % 1024 == 0 && kDynamic <= 232448, "shared memory");
+};
+
+struct LinPairDev {
+    int M, N;
+    int m_tiles, n_tiles, tiles, stages_k;
+    int last_steps;                   // MMAs of the last stage
+    int passes_by;                    // the output is larger than what L2 can keep, its lines go first
+    const void *bias;
+    int residual;
+    float alpha;
+};
+
+__device__ __forceinline__ void lin_tile(const LinPairDev &p, int t, int &m, int &n) {
+    const int band = t / (kLinBand * p.n_tiles), at = t - band * kLinBand * p.n_tiles;
+    const int rows = min(kLinBand, p.m_tiles - band * kLinBand);
+    n = at / rows;
+    m = band * kLinBand + at - n * rows;
+}
+
+template <typename T, int ACT, int BN>
+__global__ void __launch_bounds__(kLinThreads, 1)
+linear_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_res,
+                   const __grid_constant__ CUtensorMap tm_out, const LinPairDev p) {
+    using L = LinPairLayout<BN>;
+    constexpr int STAGES = L::kStages;
+    extern __shared__ uint8_t smem_raw[];
+    // both CTAs compute the same offset
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + L::kOffBars);
+    uint64_t *full_bar = bars, *empty_bar = bars + STAGES, *tfull_bar = bars + 2 * STAGES, *tempty_bar = tfull_bar + 2, *res_bar = tempty_bar + 2;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + L::kBars);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+    const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x) >> 5, 0), lane = threadIdx.x & 31;
+    const int rank = int(blockIdx.x & 1), pair = int(blockIdx.x >> 1), pairs = int(gridDim.x >> 1);
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) {
+            mbar_init(&full_bar[s], 1);
+            mbar_init(&empty_bar[s], 1);
+        }
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(&tfull_bar[s], 1);
+            mbar_init(&tempty_bar[s], 16);
+        }
+        for (int s = 0; s < 8 * L::kGroups; ++s) mbar_init(&res_bar[s], 1);
+        *abort_flag = 0;
+        fence_barrier_init();
+        tma_prefetch_desc(&tm_x);
+        tma_prefetch_desc(&tm_w);
+        tma_prefetch_desc(&tm_out);
+        if (p.residual) tma_prefetch_desc(&tm_res);
+    }
+    if (warp == 1) {
+        tmem_alloc(tmem_slot, 2 * BN, PairTag());
+        dependency_trigger();
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    cluster_sync_threads();  // the partner's barriers are set up, its tensor memory is there
+    tc_fence_after_sync();
+    const uint32_t tmem = *tmem_slot;
+    dependency_wait();
+
+    bool ok = true;
+    if (warp == 0) {
+        if (elect_one()) {
+            int stage = 0;
+            uint32_t phase = 0;
+            for (int t = pair; t < p.tiles && ok; t += pairs) {
+                int m, n;
+                lin_tile(p, t, m, n);
+                const int m0 = m * 256 + rank * 128, n0 = n * BN + rank * (BN / 2);
+                for (int ks = 0; ks < p.stages_k; ++ks) {
+                    ok = mbar_wait(&empty_bar[stage], phase ^ 1u, abort_flag, 160);
+                    if (!ok) break;
+                    uint8_t *sx = smem + stage * L::kSlot, *sw = sx + L::kOperandX;
+                    const uint32_t bar = cluster_address(smem_u32(&full_bar[stage]), 0);
+                    if (rank == 0) mbar_arrive_expect_tx(&full_bar[stage], 2 * L::kSlot);
+                    tma_load_2d_pair(sx, &tm_x, bar, ks * kLinStageK, m0);
+                    tma_load_2d_pair(sw, &tm_w, bar, ks * kLinStageK, n0);
+                    if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+                }
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        if (rank == 0) {
+            const bool leader = elect_one();
+            int stage = 0;
+            uint32_t phase = 0, buf = 0, t_phase = 0;
+            bool ready = false;
+            const uint32_t base_lo = desc_lo(smem_u32(smem));
+            for (int t = pair; t < p.tiles && ok; t += pairs) {
+                ok = mbar_wait_warp(&tempty_bar[buf], t_phase ^ 1u, abort_flag, 161);
+                if (!ok) break;
+                tc_fence_after_sync();
+                const uint32_t d = tmem + buf * BN;
+                for (int ks = 0; ks < p.stages_k; ++ks) {
+                    if (!ready) ok = mbar_wait_warp(&full_bar[stage], phase, abort_flag, 162);
+                    if (!ok) break;
+                    tc_fence_after_sync();
+                    // The next stage is asked about here and the answer is looked at behind this stage's MMAs.
+                    const bool wraps = stage + 1 == STAGES;
+                    const bool next = mbar_test(&full_bar[wraps ? 0 : stage + 1], wraps ? phase ^ 1u : phase);
+                    const uint32_t x_lo = base_lo + stage * (L::kSlot >> 4);
+                    const int steps = ks == p.stages_k - 1 ? p.last_steps : 4;
+                    if (leader) {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            if (k < steps) tc_mma_f16<2>(d, x_lo + 2 * k, x_lo + (L::kOperandX >> 4) + 2 * k, make_idesc_16<T>(256, BN), (ks | k) != 0);
+                        tc_commit_pair(&empty_bar[stage]);
+                        if (ks == p.stages_k - 1) tc_commit_pair(&tfull_bar[buf]);
+                    }
+                    ready = __all_sync(0xffffffffu, next);
+                    stage = wraps ? 0 : stage + 1;
+                    phase ^= wraps;
+                }
+                buf ^= 1u;
+                t_phase ^= buf ^ 1u;   // a buffer's phase advances when both have been used
+            }
+        }
+        __syncwarp();
+    } else if (warp >= 4) {
+        const int q = warp & 3, half = (warp - 4) >> 2;
+        uint8_t *staging = smem + L::kOffStaging + (warp - 4) * (L::kGroups * 32 * 128);
+        uint64_t *loaded = res_bar + (warp - 4) * L::kGroups;
+        const uint32_t tempty = cluster_address(smem_u32(tempty_bar), 0);
+        const T *bias = static_cast<const T *>(p.bias);
+        uint32_t buf = 0, t_phase = 0, res_phase = 0;   // res_phase: a bit per group
+        for (int t = pair; t < p.tiles && ok; t += pairs) {
+            int m, n;
+            lin_tile(p, t, m, n);
+            const int m0 = m * 256 + rank * 128 + q * 32, c0 = n * BN + half * (BN / 2);
+            const bool rows = m0 < p.M;
+            // The staging of a group is free when its last store has read it; every group of every tile commits one, if an empty one.
+            if (lane == 0) {
+#pragma unroll
+                for (int g = 0; g < L::kGroups; ++g) {
+                    if (g + 1 < L::kGroups) tma_store_wait_read<L::kGroups - 1>();
+                    else tma_store_wait_read<0>();
+                    if (p.residual && rows && c0 + g * 64 < p.N) {
+                        mbar_arrive_expect_tx(&loaded[g], 32 * 128);
+                        tma_load_2d(staging + g * (32 * 128), &tm_res, &loaded[g], c0 + g * 64, m0);
+                    }
+                }
+            }
+            __syncwarp();
+            ok = mbar_wait_warp(&tfull_bar[buf], t_phase, abort_flag, 163);
+            if (!ok) break;
+            tc_fence_after_sync();
+            const uint32_t t_row = tmem + (uint32_t(q * 32) << 16) + buf * BN + half * (BN / 2);
+#pragma unroll
+            for (int g = 0; g < L::kGroups; ++g) {
+                uint32_t a[2][32];
+                tmem_ld_32x32(t_row + g * 64, a[0]);
+                tmem_ld_32x32(t_row + g * 64 + 32, a[1]);
+                tmem_ld_wait();
+                if (g + 1 == L::kGroups) {
+                    tc_fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_cluster(tempty + buf * 8);
+                }
+                const int c = c0 + g * 64;
+                const bool live = rows && c < p.N;
+                uint8_t *stage_row = staging + g * (32 * 128);
+                if (live) {
+                    if (p.residual) {
+                        ok = mbar_wait_warp(&loaded[g], (res_phase >> g) & 1u, abort_flag, 164);
+                        if (!ok) break;
+                        res_phase ^= 1u << g;
+                    }
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        uint4 *cell = reinterpret_cast<uint4 *>(stage_row + sw128_offset(lane, j));
+                        uint4 b, r;
+                        if (bias) b = c + 8 * j < p.N ? *reinterpret_cast<const uint4 *>(bias + c + 8 * j) : make_uint4(0, 0, 0, 0);
+                        if (p.residual) r = *cell;
+                        float v[8];
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(a[j >> 2][(j & 3) * 8 + i]);
+                        *cell = finish8<T, ACT>(v, bias ? &b : nullptr, p.residual ? &r : nullptr, p.alpha);
+                    }
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                }
+                if (lane == 0) {
+                    if (live) {
+                        if (p.passes_by) tma_store_2d(&tm_out, stage_row, c, m0, l2_evict_first());
+                        else tma_store_2d(&tm_out, stage_row, c, m0);
+                    }
+                    tma_store_commit();
+                }
+            }
+            buf ^= 1u;
+            t_phase ^= buf ^ 1u;
+        }
+        if (lane == 0) tma_store_wait_all<0>();
+        __syncwarp();
+    }
+    if (!ok) {
+        // loads in flight get a bounded chance to land before the shared memory is released
+        const long long t0 = clock64();
+        while (clock64() - t0 < (1ll << 22)) { }
+    }
+
+    __syncwarp();
+    tc_fence_before_sync();
+    __syncthreads();
+    cluster_sync_threads();  // nothing of the partner still arrives here or reads this CTA's operands
+    if (warp == 1) {
+        tc_fence_after_sync();
+        tmem_dealloc(tmem, 2 * BN, PairTag());
+    }
+}
+
 inline LinEpilogue lin_epilogue(const fluke_sm100_linear_t *g) {
     return {g->bias, g->residual, g->out, g->ld_residual, g->ld_out, g->alpha};
 }
@@ -342,9 +580,40 @@ int linear_split_launch(const fluke_sm100_linear_t *g, cudaStream_t stream) {
     return launch_dependent_clusters(kernel, split, dim3(int(tiles) * split), kLinThreads, smem + 1024, stream, tm_x, tm_w, p);
 }
 
+template <typename T, int ACT, int BN>
+int linear_pair_launch(const fluke_sm100_linear_t *g, cudaStream_t stream) {
+    using L = LinPairLayout<BN>;
+    constexpr auto kernel = linear_pair_kernel<T, ACT, BN>;
+    const int capacity = cluster_capacity<kernel>(2, kLinThreads, L::kDynamic);
+    if (capacity < 1) return (int)cudaErrorNotSupported;
+    LinPairDev p;
+    p.M = g->M; p.N = g->N;
+    p.m_tiles = (g->M + 255) / 256;
+    p.n_tiles = (g->N + BN - 1) / BN;
+    const int64_t tiles = int64_t(p.m_tiles) * p.n_tiles;
+    if (tiles > INT32_MAX - 1024 || int64_t(kLinBand) * p.n_tiles > INT32_MAX) return (int)cudaErrorInvalidValue;
+    p.tiles = int(tiles);
+    p.stages_k = (g->K + kLinStageK - 1) / kLinStageK;
+    p.last_steps = (g->K - (p.stages_k - 1) * kLinStageK + 15) / 16;
+    p.passes_by = int64_t(g->M) * g->N * 2 > int64_t(device_l2_bytes()) / 8 * 7;
+    p.bias = g->bias;
+    p.residual = g->residual != nullptr;
+    p.alpha = g->alpha;
+    CUtensorMap tm_x, tm_w, tm_res, tm_out;
+    int rc = lin_operand(&tm_x, g->x, g->M, g->K, g->ld_x, 128);
+    if (!rc) rc = lin_operand(&tm_w, g->w, g->N, g->K, g->K, BN / 2);
+    if (!rc) rc = lin_operand(&tm_out, g->out, g->M, g->N, g->ld_out, 32);
+    tm_res = tm_out;
+    if (!rc && g->residual) rc = lin_operand(&tm_res, g->residual, g->M, g->N, g->ld_residual, 32);
+    if (rc) return rc;
+    const int pairs = p.tiles < capacity ? p.tiles : capacity;
+    return launch_dependent_clusters(kernel, 2, pairs * 2, kLinThreads, L::kDynamic, stream, tm_x, tm_w, tm_res, tm_out, p);
+}
+
 template <typename T, int ACT>
 int linear_dispatch(const fluke_sm100_linear_t *g, cudaStream_t stream) {
-    return linear_split_launch<T, ACT>(g, stream);
+    if (g->M <= 64 || lin_split_tiles(g) <= device_sm_count()) return linear_split_launch<T, ACT>(g, stream);
+    return linear_pair_launch<T, ACT, 256>(g, stream);
 }
 template <typename T>
 int linear_dispatch(const fluke_sm100_linear_t *g, cudaStream_t stream) {
