@@ -21,6 +21,7 @@ namespace {
 
 constexpr int kRecSteps = 8;          // of a lane
 constexpr int kRecKept = FLUKE_SM100_RECURRENCE_KEPT;   // steps between kept states
+constexpr int kRecThreads = 256;       // at most; fewer for a few steps
 constexpr int kRecMostCluster = 8;
 
 struct RecIn {
@@ -43,253 +44,320 @@ struct RecDev {
     float *states;                    // written forwards (or null), read backwards
 };
 
-__device__ __forceinline__ uint32_t ld_pair(const void *p, int64_t at) {
+__device__ __forceinline__ uint32_t ld_pair(const char *p) {
     uint32_t v;
-    asm volatile("ld.global.L1::no_allocate.b32 %0, [%1];" : "=r"(v) : "l"(static_cast<const uint16_t *>(p) + at) : "memory");
+    asm volatile("ld.global.L1::no_allocate.b32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
     return v;
 }
-__device__ __forceinline__ void st_pair(void *p, int64_t at, uint32_t v) {
-    *reinterpret_cast<uint32_t *>(static_cast<uint16_t *>(p) + at) = v;
+// -1 / (1 + exp(g)): relative error below 2^-21 and, of the argument's rounding, |g| 2^-24; zero above 87, where it is below 2^-125. Its sign
+// saves the negations: packed operations have none.
+__device__ __forceinline__ float2 gate_less_one(float2 g) {
+    const float2 a = mul2(g, make_float2(1.44269504f, 1.44269504f)), one = make_float2(-1.f, -1.f);
+    const float2 d = fma2(make_float2(ex2_approx(a.x), ex2_approx(a.y)), one, one);
+    return make_float2(rcp_approx(d.x), rcp_approx(d.y));
 }
-// 1 / (1 + exp(g)): relative error below 2^-21 and, of the argument's rounding, |g| 2^-24; zero above 87, where it is below 2^-125.
-__device__ __forceinline__ float2 one_minus_gate(float2 g) {
-    const float2 a = mul2(g, make_float2(1.44269504f, 1.44269504f));
+// 1 / (1 + exp(-g)), alike.
+__device__ __forceinline__ float2 gate_of(float2 g) {
+    const float2 a = mul2(g, make_float2(-1.44269504f, -1.44269504f));
     const float2 d = add2(make_float2(ex2_approx(a.x), ex2_approx(a.y)), make_float2(1.f, 1.f));
     return make_float2(rcp_approx(d.x), rcp_approx(d.y));
 }
-// a + c (b - a)
-__device__ __forceinline__ float2 towards(float2 a, float2 c, float2 b) { return fma2(c, fma2(a, make_float2(-1.f, -1.f), b), a); }
-// a - c a
-__device__ __forceinline__ float2 less(float2 a, float2 c) { return fma2(make_float2(-c.x, -c.y), a, a); }
-// a + (b - c a): what a run (c, b) makes of a
-__device__ __forceinline__ float2 through(float2 a, float2 c, float2 b) { return add2(a, fma2(make_float2(-c.x, -c.y), a, b)); }
+// With m = -c: a + c (b - a), and a - c a.
+__device__ __forceinline__ float2 towards(float2 a, float2 m, float2 b) { return fma2(m, fma2(b, make_float2(-1.f, -1.f), a), a); }
+__device__ __forceinline__ float2 less(float2 a, float2 m) { return fma2(m, a, a); }
+// C of a run and one more step; a run's C is kept as its negative as well.
+__device__ __forceinline__ float2 longer(float2 M, float2 m) { return fma2(m, add2(M, make_float2(1.f, 1.f)), M); }
+// a + (b - C a): what a run makes of a
+__device__ __forceinline__ float2 through(float2 a, float2 M, float2 b) { return add2(a, fma2(M, a, b)); }
+__device__ __forceinline__ float2 low(float4 q) { return make_float2(q.x, q.y); }
+__device__ __forceinline__ float2 high(float4 q) { return make_float2(q.z, q.w); }
+__device__ __forceinline__ float4 both(float2 a, float2 b) { return make_float4(a.x, a.y, b.x, b.y); }
+// Stores into the shared memory of a CTA of the cluster.
+__device__ __forceinline__ void tell(const float4 *to, int rank, float2 a, float2 b) {
+    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(cluster_address(smem_u32(to), rank)), "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y) : "memory");
+}
 
-// Where a thread works: its chunk, its two channels and which run of a tile it holds.
+// Where a thread works. Processing goes through steps s = 0 .. T-1, time through s or T - 1 - s; a tensor is walked from its first step in
+// processing order. What lies in [from, to) is inside the chunk.
 template <int LANES>
 struct RecPlace {
-    int b, rank, channel, lane, run, runs;
-    bool in;                          // the channels exist
+    int b, rank, channel, lane, run, runs, from, to;
+    bool in;                          // the channels exist (else the last two are read, and nothing is written)
+    int64_t state;
     __device__ __forceinline__ explicit RecPlace(const RecDev &p) {
-        constexpr int kPerWarp = 32 / LANES;
         const int slab = int(blockIdx.x) / p.split;
         rank = int(blockIdx.x) - slab * p.split;
         b = slab / p.slabs;
         lane = threadIdx.x & (LANES - 1);
         channel = (slab - b * p.slabs) * (2 * LANES) + 2 * lane;
+        in = channel < p.H;
+        channel = min(channel, p.H - 2);
         run = int(threadIdx.x) / LANES;
         runs = int(blockDim.x) / LANES;
-        (void)kPerWarp;
-        in = channel < p.H;
+        state = int64_t(b) * p.H + channel;
+    }
+    __device__ __forceinline__ void measure(const RecDev &p) {   // reads global memory
+        const int length = p.lengths ? min(max(p.lengths[b], 0), p.T) : p.T;
+        from = p.reverse ? p.T - length : 0;
+        to = p.reverse ? p.T : length;
     }
 };
-__device__ __forceinline__ int rec_length(const RecDev &p, int b) {
-    return p.lengths ? min(max(p.lengths[b], 0), p.T) : p.T;
+// A tensor from step s on: bytes between steps, in processing order.
+struct RecWalk {
+    const char *at;
+    int64_t step;
+    template <int LANES, typename X>
+    __device__ __forceinline__ RecWalk(const RecDev &p, const X &x, const RecPlace<LANES> &w, int s) {
+        step = (p.reverse ? -x.step : x.step) * 2;
+        at = static_cast<const char *>(x.at) + (w.b * x.chunk + w.channel + (p.reverse ? p.T - 1 : 0) * x.step) * 2 + s * step;
+    }
+    __device__ __forceinline__ const char *operator[](int k) const { return at + k * step; }
+    __device__ __forceinline__ char *out(int k) const { return const_cast<char *>(at + k * step); }
+};
+__device__ __forceinline__ float2 ld_state(const float *s, int64_t at) {
+    return s ? *reinterpret_cast<const float2 *>(s + at) : make_float2(0.f, 0.f);
 }
-__device__ __forceinline__ float2 ld_state(const float *s, int64_t at, bool in) {
-    return s && in ? *reinterpret_cast<const float2 *>(s + at) : make_float2(0.f, 0.f);
-}
+__device__ __forceinline__ void st_state(float *s, int64_t at, float2 v) { *reinterpret_cast<float2 *>(s + at) = v; }
 
 // Forwards. LANES: lanes that share a run, with two channels each.
-template <typename T, int LANES>
-__global__ void __launch_bounds__(512)
+template <typename T, int LANES, bool CLUSTER>
+__global__ void __launch_bounds__(kRecThreads, 3)
 recurrence_kernel(const RecDev p) {
-    __shared__ float4 run_of[2][512 / LANES][LANES];            // C and V of every run of the tile
-    __shared__ float4 tile_of[2][kRecMostCluster][LANES];       // of every CTA's tile
-    const RecPlace<LANES> w(p);
+    constexpr int kRuns = kRecThreads / LANES;
+    __shared__ float4 run_of[2][kRuns][LANES];                             // -C and V of every run of the tile
+    __shared__ float4 tile_of[2][CLUSTER ? kRecMostCluster : 1][LANES];    // of every CTA's tile
+    __shared__ float2 carried[2][LANES];                                   // the state in front of the tile
+    RecPlace<LANES> w(p);
+    const bool last_run = w.run == w.runs - 1;
+    int s0 = (w.rank * w.runs + w.run) * kRecSteps;
+    const int stride = p.split * w.runs * kRecSteps;                       // steps of a round
+    RecWalk gate(p, p.gate, w, s0), value(p, p.value, w, s0), out(p, p.out, w, s0);
+    if (CLUSTER) cluster_arrive_relaxed();   // this CTA runs: awaited before others are told anything
     dependency_wait();
-    const int length = rec_length(p, w.b), tile = w.runs * kRecSteps;
-    const int64_t state_at = int64_t(w.b) * p.H + w.channel;
-    float2 carry = ld_state(p.h0, state_at, w.in);
-    // A step's place: processing goes through s = 0, 1, ..., time through s or T - 1 - s.
-    auto time_of = [&](int s) { return p.reverse ? p.T - 1 - s : s; };
-    const int64_t gate0 = w.b * p.gate.chunk + w.channel, value0 = w.b * p.value.chunk + w.channel, out0 = w.b * p.out.chunk + w.channel;
+    w.measure(p);
+    float2 h = ld_state(p.h0, w.state), carry = h;
     uint32_t g[kRecSteps], v[kRecSteps];
-    auto load = [&](int s0) {
+    auto load = [&](int s) {
+        if (s + kRecSteps <= p.T) {
 #pragma unroll
-        for (int k = 0; k < kRecSteps; ++k) {
-            const int t = time_of(s0 + k);
-            const bool ask = w.in && s0 + k < p.T;
-            g[k] = ask ? ld_pair(p.gate.at, gate0 + t * p.gate.step) : 0;
-            v[k] = ask ? ld_pair(p.value.at, value0 + t * p.value.step) : 0;
-        }
-    };
-    int s0 = w.rank * tile + w.run * kRecSteps;
-    load(s0);
-    for (int round = 0; round < p.rounds; ++round, s0 += p.split * tile) {
-        const int par = round & 1;
-        float2 c[kRecSteps], x[kRecSteps], C = make_float2(0.f, 0.f), V = C;
-#pragma unroll
-        for (int k = 0; k < kRecSteps; ++k) {
-            // behind a chunk's end nothing changes, whatever stands there
-            const bool live = s0 + k < p.T && time_of(s0 + k) < length;
-            c[k] = one_minus_gate(unpack2(g[k], T()));
-            x[k] = unpack2(v[k], T());
-            if (!live) c[k] = x[k] = make_float2(0.f, 0.f);
-            V = towards(V, c[k], x[k]);
-            C = towards(C, c[k], make_float2(1.f, 1.f));
-        }
-        load(s0 + p.split * tile);
-        run_of[par][w.run][w.lane] = make_float4(C.x, C.y, V.x, V.y);
-        __syncthreads();
-        float2 h;
-        if (p.split == 1) {
-            h = carry;
-            for (int r = 0; r < w.runs; ++r) {
-                if (r == w.run) h = carry;
-                const float4 q = run_of[par][r][w.lane];
-                carry = through(carry, make_float2(q.x, q.y), make_float2(q.z, q.w));
+            for (int k = 0; k < kRecSteps; ++k) {
+                g[k] = ld_pair(gate[k]);
+                v[k] = ld_pair(value[k]);
             }
         } else {
-            float2 before_c = make_float2(0.f, 0.f), before_v = before_c;
-            C = V = before_c;
-            for (int r = 0; r < w.runs; ++r) {
-                if (r == w.run) {
-                    before_c = C;
-                    before_v = V;
-                }
-                const float4 q = run_of[par][r][w.lane];
-                V = through(V, make_float2(q.x, q.y), make_float2(q.z, q.w));
-                C = towards(C, make_float2(q.x, q.y), make_float2(1.f, 1.f));
+#pragma unroll
+            for (int k = 0; k < kRecSteps; ++k) {
+                g[k] = s + k < p.T ? ld_pair(gate[k]) : 0;
+                v[k] = s + k < p.T ? ld_pair(value[k]) : 0;
             }
-            // every CTA is told by as many threads as it has lanes of a run
-            if (w.run < p.split) {
-                const uint32_t to = cluster_address(smem_u32(&tile_of[par][w.rank][w.lane]), w.run);
-                asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(to), "f"(C.x), "f"(C.y), "f"(V.x), "f"(V.y) : "memory");
-            }
-            cluster_sync_threads();
-            h = carry;
-            for (int r = 0; r < p.split; ++r) {
-                if (r == w.rank) h = carry;
-                const float4 q = tile_of[par][r][w.lane];
-                carry = through(carry, make_float2(q.x, q.y), make_float2(q.z, q.w));
-            }
-            h = through(h, before_c, before_v);
         }
-        if (w.in && s0 < p.T && p.states && s0 % kRecKept == 0)
-            *reinterpret_cast<float2 *>(p.states + int64_t(s0 / kRecKept) * p.B * p.H + state_at) = h;
+        gate.at += stride * gate.step;
+        value.at += stride * value.step;
+    };
+    load(s0);
+    if (CLUSTER) cluster_wait();
+    if (!CLUSTER && last_run) carried[0][w.lane] = h;
+    for (int round = 0; round < p.rounds; ++round, s0 += stride) {
+        const int par = round & 1;
+        const bool all = s0 >= w.from && s0 + kRecSteps <= w.to;           // of the run's steps lie inside the chunk
+        float2 m[kRecSteps], M = make_float2(0.f, 0.f), V = M;
+        uint32_t values[kRecSteps];
 #pragma unroll
         for (int k = 0; k < kRecSteps; ++k) {
-            h = towards(h, c[k], x[k]);
-            const int t = time_of(s0 + k);
-            if (w.in && s0 + k < p.T) st_pair(p.out.at, out0 + t * p.out.step, t < length ? pack2(h, T()) : 0);
+            m[k] = gate_less_one(unpack2(g[k], T()));
+            values[k] = v[k];
         }
+        if (!all)
+            // behind a chunk's end nothing changes, whatever stands there
+#pragma unroll
+            for (int k = 0; k < kRecSteps; ++k)
+                if (s0 + k < w.from || s0 + k >= w.to) {
+                    m[k] = make_float2(0.f, 0.f);
+                    values[k] = 0;
+                }
+        if (round + 1 < p.rounds) load(s0 + stride);
+#pragma unroll
+        for (int k = 0; k < kRecSteps; ++k) {
+            V = towards(V, m[k], unpack2(values[k], T()));
+            M = longer(M, m[k]);
+        }
+        if (!CLUSTER) {
+            run_of[par][w.run][w.lane] = both(M, V);
+            __syncthreads();
+            h = carried[par][w.lane];
+            for (int r = 0; r < w.run; ++r) {
+                const float4 q = run_of[par][r][w.lane];
+                h = through(h, low(q), high(q));
+            }
+        } else {
+            run_of[par][w.run][w.lane] = both(M, V);
+            __syncthreads();
+            float2 before_m = make_float2(0.f, 0.f), before_v = before_m;
+            for (int r = 0; r < w.run; ++r) {
+                const float4 q = run_of[par][r][w.lane];
+                before_v = through(before_v, low(q), high(q));
+                before_m = longer(before_m, low(q));
+            }
+            if (last_run)
+                for (int r = 0; r < p.split; ++r) tell(&tile_of[par][w.rank][w.lane], r, longer(before_m, M), through(before_v, M, V));
+            cluster_sync_threads();
+            for (int r = 0; r < p.split; ++r) {
+                const float4 q = tile_of[par][r][w.lane];
+                if (r == w.rank) h = carry;
+                carry = through(carry, low(q), high(q));
+            }
+            h = through(h, before_m, before_v);
+        }
+        if (p.states && s0 % kRecKept == 0 && w.in && s0 < p.T) st_state(p.states, int64_t(s0 / kRecKept) * p.B * p.H + w.state, h);
+        if (all) {
+#pragma unroll
+            for (int k = 0; k < kRecSteps; ++k) {
+                h = towards(h, m[k], unpack2(values[k], T()));
+                if (w.in) *reinterpret_cast<uint32_t *>(out.out(k)) = pack2(h, T());
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < kRecSteps; ++k) {
+                h = towards(h, m[k], unpack2(values[k], T()));
+                if (w.in && s0 + k < p.T) *reinterpret_cast<uint32_t *>(out.out(k)) = s0 + k >= w.from && s0 + k < w.to ? pack2(h, T()) : 0;
+            }
+        }
+        out.at += stride * out.step;
+        if (!CLUSTER && last_run) carried[par ^ 1][w.lane] = h;
     }
-    // every thread of the cluster has read h0, which may be the same, in front of the last barrier
-    if (w.rank == 0 && w.run == 0 && w.in && p.h_last) *reinterpret_cast<float2 *>(p.h_last + state_at) = carry;
+    // Only threads that have read h0 themselves, or are behind a barrier that all who do have passed, write what may lie in its place.
+    if (p.h_last && w.in && (CLUSTER ? w.rank == 0 && w.run == 0 : last_run)) st_state(p.h_last, w.state, CLUSTER ? carry : h);
 }
 
 // Backwards: tiles, and the runs of a tile, are joined from the last to the first.
-template <typename T, int LANES>
-__global__ void __launch_bounds__(512)
+template <typename T, int LANES, bool CLUSTER>
+__global__ void __launch_bounds__(kRecThreads, 2)
 recurrence_backward_kernel(const RecDev p) {
-    __shared__ float4 run_of[2][512 / LANES][LANES];            // C and V of every run of the tile
-    __shared__ float2 run_back[2][512 / LANES][LANES];          // D
-    __shared__ float4 tile_of[2][kRecMostCluster][LANES];       // C and D of every CTA's tile
-    const RecPlace<LANES> w(p);
+    constexpr int kRuns = kRecThreads / LANES;
+    __shared__ float4 run_of[2][kRuns][LANES];                             // -C and V of every run of the tile
+    __shared__ float2 run_back[2][kRuns][LANES];                           // D
+    __shared__ float4 tile_of[2][CLUSTER ? kRecMostCluster : 1][LANES];    // -C and D of every CTA's tile
+    __shared__ float2 carried[2][LANES];                                   // what reaches the tile from the steps behind it
+    RecPlace<LANES> w(p);
+    const bool first_run = w.run == 0;
+    const int stride = p.split * w.runs * kRecSteps;                       // steps of a round
+    int tile0 = ((p.rounds - 1) * p.split + w.rank) * w.runs * kRecSteps, s0 = tile0 + w.run * kRecSteps;
+    RecWalk gate(p, p.gate, w, s0), value(p, p.value, w, s0), grad(p, p.grad, w, s0), dgate(p, p.grad_gate, w, s0), dvalue(p, p.grad_value, w, s0);
+    if (CLUSTER) cluster_arrive_relaxed();   // this CTA runs: awaited before others are told anything
     dependency_wait();
-    const int length = rec_length(p, w.b), tile = w.runs * kRecSteps;
-    const int64_t state_at = int64_t(w.b) * p.H + w.channel;
-    float2 carry = ld_state(p.grad_last, state_at, w.in);
-    auto time_of = [&](int s) { return p.reverse ? p.T - 1 - s : s; };
-    const int64_t gate0 = w.b * p.gate.chunk + w.channel, value0 = w.b * p.value.chunk + w.channel, grad0 = w.b * p.grad.chunk + w.channel;
-    const int64_t dg0 = w.b * p.grad_gate.chunk + w.channel, dv0 = w.b * p.grad_value.chunk + w.channel;
+    w.measure(p);
+    float2 x = ld_state(p.grad_last, w.state), carry = x, kept;
     uint32_t g[kRecSteps], v[kRecSteps], dy[kRecSteps];
-    float2 kept;                                                // the state in front of the tile
-    auto load = [&](int s0) {
+    auto load = [&](int s, int tile) {
+        if (s + kRecSteps <= p.T) {
 #pragma unroll
-        for (int k = 0; k < kRecSteps; ++k) {
-            const int t = time_of(s0 + k);
-            const bool ask = w.in && s0 >= 0 && s0 + k < p.T;
-            g[k] = ask ? ld_pair(p.gate.at, gate0 + t * p.gate.step) : 0;
-            v[k] = ask ? ld_pair(p.value.at, value0 + t * p.value.step) : 0;
-            dy[k] = ask ? ld_pair(p.grad.at, grad0 + t * p.grad.step) : 0;
+            for (int k = 0; k < kRecSteps; ++k) {
+                g[k] = ld_pair(gate[k]);
+                v[k] = ld_pair(value[k]);
+                dy[k] = ld_pair(grad[k]);
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < kRecSteps; ++k) {
+                g[k] = s + k < p.T ? ld_pair(gate[k]) : 0;
+                v[k] = s + k < p.T ? ld_pair(value[k]) : 0;
+                dy[k] = s + k < p.T ? ld_pair(grad[k]) : 0;
+            }
         }
-        const int first = s0 - w.run * kRecSteps;
-        kept = ld_state(p.states, int64_t(first / kRecKept) * p.B * p.H + state_at, w.in && first >= 0 && first < p.T);
+        // the state in front of the tile
+        kept = tile < p.T ? ld_state(p.states, int64_t(tile / kRecKept) * p.B * p.H + w.state) : make_float2(0.f, 0.f);
+        gate.at -= stride * gate.step;
+        value.at -= stride * value.step;
+        grad.at -= stride * grad.step;
     };
-    int s0 = ((p.rounds - 1) * p.split + w.rank) * tile + w.run * kRecSteps;
-    load(s0);
-    for (int round = p.rounds - 1; round >= 0; --round, s0 -= p.split * tile) {
+    if (p.rounds > 0) load(s0, tile0);
+    if (CLUSTER) cluster_wait();
+    if (!CLUSTER && first_run) carried[(p.rounds - 1) & 1][w.lane] = x;
+    for (int round = p.rounds - 1; round >= 0; --round, s0 -= stride, tile0 -= stride) {
         const int par = round & 1;
-        float2 c[kRecSteps], C = make_float2(0.f, 0.f), V = C, D = C, h = kept;
-        uint32_t gate[kRecSteps], value[kRecSteps], grad[kRecSteps];
+        const bool all = s0 >= w.from && s0 + kRecSteps <= w.to;
+        float2 m[kRecSteps], M = make_float2(0.f, 0.f), V = M, D = M, h = kept;
+        uint32_t gates[kRecSteps], values[kRecSteps], grads[kRecSteps];
 #pragma unroll
         for (int k = 0; k < kRecSteps; ++k) {
-            const bool live = s0 + k < p.T && time_of(s0 + k) < length;
-            gate[k] = g[k];
-            value[k] = live ? v[k] : 0;
-            grad[k] = live ? dy[k] : 0;
-            c[k] = one_minus_gate(unpack2(g[k], T()));
-            if (!live) c[k] = make_float2(0.f, 0.f);
-            V = towards(V, c[k], unpack2(value[k], T()));
-            C = towards(C, c[k], make_float2(1.f, 1.f));
+            gates[k] = g[k];
+            values[k] = v[k];
+            grads[k] = dy[k];
+            m[k] = gate_less_one(unpack2(g[k], T()));
+        }
+        if (!all)
+#pragma unroll
+            for (int k = 0; k < kRecSteps; ++k)
+                if (s0 + k < w.from || s0 + k >= w.to) {
+                    m[k] = make_float2(0.f, 0.f);
+                    gates[k] = values[k] = grads[k] = 0;
+                }
+        if (round > 0) load(s0 - stride, tile0 - stride);
+#pragma unroll
+        for (int k = 0; k < kRecSteps; ++k) {
+            V = towards(V, m[k], unpack2(values[k], T()));
+            M = longer(M, m[k]);
         }
 #pragma unroll
-        for (int k = kRecSteps - 1; k >= 0; --k) D = less(add2(D, unpack2(grad[k], T())), c[k]);
-        load(s0 - p.split * tile);
-        run_of[par][w.run][w.lane] = make_float4(C.x, C.y, V.x, V.y);
+        for (int k = kRecSteps - 1; k >= 0; --k) D = less(add2(D, unpack2(grads[k], T())), m[k]);
+        run_of[par][w.run][w.lane] = both(M, V);
         run_back[par][w.run][w.lane] = D;
         __syncthreads();
         for (int r = 0; r < w.run; ++r) {
             const float4 q = run_of[par][r][w.lane];
-            h = through(h, make_float2(q.x, q.y), make_float2(q.z, q.w));
+            h = through(h, low(q), high(q));
         }
-        float2 x;
-        if (p.split == 1) {
-            x = carry;
-            for (int r = w.runs - 1; r >= 0; --r) {
-                if (r == w.run) x = carry;
-                const float2 q = *reinterpret_cast<const float2 *>(&run_of[par][r][w.lane]);
-                carry = through(carry, q, run_back[par][r][w.lane]);
-            }
+        if (!CLUSTER) {
+            x = carried[par][w.lane];
+            for (int r = w.runs - 1; r > w.run; --r) x = through(x, low(run_of[par][r][w.lane]), run_back[par][r][w.lane]);
         } else {
-            float2 behind_c = make_float2(0.f, 0.f), behind_d = behind_c;
-            C = D = behind_c;
-            for (int r = w.runs - 1; r >= 0; --r) {
-                if (r == w.run) {
-                    behind_c = C;
-                    behind_d = D;
-                }
-                const float2 q = *reinterpret_cast<const float2 *>(&run_of[par][r][w.lane]);
-                D = through(D, q, run_back[par][r][w.lane]);
-                C = towards(C, q, make_float2(1.f, 1.f));
+            float2 behind_m = make_float2(0.f, 0.f), behind_d = behind_m;
+            for (int r = w.runs - 1; r > w.run; --r) {
+                const float2 q = low(run_of[par][r][w.lane]);
+                behind_d = through(behind_d, q, run_back[par][r][w.lane]);
+                behind_m = longer(behind_m, q);
             }
-            if (w.run < p.split) {
-                const uint32_t to = cluster_address(smem_u32(&tile_of[par][w.rank][w.lane]), w.run);
-                asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(to), "f"(C.x), "f"(C.y), "f"(D.x), "f"(D.y) : "memory");
-            }
+            if (first_run)
+                for (int r = 0; r < p.split; ++r) tell(&tile_of[par][w.rank][w.lane], r, longer(behind_m, M), through(behind_d, M, D));
             cluster_sync_threads();
-            x = carry;
             for (int r = p.split - 1; r >= 0; --r) {
-                if (r == w.rank) x = carry;
                 const float4 q = tile_of[par][r][w.lane];
-                carry = through(carry, make_float2(q.x, q.y), make_float2(q.z, q.w));
+                if (r == w.rank) x = carry;
+                carry = through(carry, low(q), high(q));
             }
-            x = through(x, behind_c, behind_d);
+            x = through(x, behind_m, behind_d);
         }
-        float2 before[kRecSteps];                               // h - v in front of each step
+        float2 before[kRecSteps];                               // v - h in front of each step
 #pragma unroll
         for (int k = 0; k < kRecSteps; ++k) {
-            const float2 u = unpack2(value[k], T());
-            before[k] = fma2(u, make_float2(-1.f, -1.f), h);
-            h = towards(h, c[k], u);
+            const float2 u = unpack2(values[k], T());
+            before[k] = fma2(h, make_float2(-1.f, -1.f), u);
+            h = towards(h, m[k], u);
         }
 #pragma unroll
         for (int k = kRecSteps - 1; k >= 0; --k) {
-            const float2 e = add2(x, unpack2(grad[k], T())), ce = mul2(c[k], e);
+            const float2 e = add2(x, unpack2(grads[k], T())), ce = mul2(m[k], e);   // -c e
+            x = add2(e, ce);
             // f by itself: one minus c has no digits left where c is near one
-            const float2 raw = unpack2(gate[k], T()), f = one_minus_gate(make_float2(-raw.x, -raw.y));
-            x = less(e, c[k]);
-            const bool live = s0 + k < p.T && time_of(s0 + k) < length;
-            const float2 dg = mul2(mul2(ce, before[k]), f);
-            const int t = time_of(s0 + k);
-            if (w.in && s0 + k < p.T) {
-                st_pair(p.grad_gate.at, dg0 + t * p.grad_gate.step, live ? pack2(dg, T()) : 0);
-                st_pair(p.grad_value.at, dv0 + t * p.grad_value.step, live ? pack2(ce, T()) : 0);
+            const uint32_t dg = pack2(mul2(mul2(ce, before[k]), gate_of(unpack2(gates[k], T()))), T()), dv = pack2(ce, T()) ^ 0x80008000u;
+            if (all) {
+                if (w.in) {
+                    *reinterpret_cast<uint32_t *>(dgate.out(k)) = dg;
+                    *reinterpret_cast<uint32_t *>(dvalue.out(k)) = dv;
+                }
+            } else {
+                const bool live = s0 + k >= w.from && s0 + k < w.to;
+                if (w.in && s0 + k < p.T) {
+                    *reinterpret_cast<uint32_t *>(dgate.out(k)) = live ? dg : 0;
+                    *reinterpret_cast<uint32_t *>(dvalue.out(k)) = live ? dv : 0;
+                }
             }
         }
+        dgate.at -= stride * dgate.step;
+        dvalue.at -= stride * dvalue.step;
+        if (!CLUSTER && first_run) carried[par ^ 1][w.lane] = x;
     }
-    if (w.rank == 0 && w.run == 0 && w.in && p.grad_h0) *reinterpret_cast<float2 *>(p.grad_h0 + state_at) = carry;
+    if (p.grad_h0 && w.in && (CLUSTER ? w.rank == 0 : true) && first_run) st_state(p.grad_h0, w.state, CLUSTER ? carry : x);
 }
 
 // How a call is spread: lanes per run, threads per CTA, CTAs per cluster.
@@ -299,13 +367,12 @@ struct RecPlan {
 // Returns false for more CTAs than a grid has.
 inline bool rec_plan(RecDev *p, RecPlan *plan) {
     plan->lanes = p->H <= 32 ? 16 : 32;
-    const int per_warp = 32 / plan->lanes;
     // no more warps than the steps fill
-    int warps = 8;
-    while (warps > 1 && (warps / 2) * per_warp * kRecSteps >= p->T) warps /= 2;
+    int warps = kRecThreads / 32;
+    while (warps > 1 && (warps / 2) * (32 / plan->lanes) * kRecSteps >= p->T) warps /= 2;
     plan->threads = warps * 32;
     plan->split = 1;
-    const int tile = warps * per_warp * kRecSteps;
+    const int tile = plan->threads / plan->lanes * kRecSteps;
     p->slabs = (p->H + 2 * plan->lanes - 1) / (2 * plan->lanes);
     p->split = plan->split;
     const int64_t tiles = (int64_t(p->T) + tile - 1) / tile, blocks = int64_t(p->B) * p->slabs * plan->split;
@@ -314,13 +381,17 @@ inline bool rec_plan(RecDev *p, RecPlan *plan) {
     return blocks <= INT32_MAX;
 }
 
+template <typename T, int LANES, bool CLUSTER>
+int recurrence_launch(const RecDev &p, const RecPlan &plan, bool backward, cudaStream_t stream) {
+    return launch_dependent_clusters(backward ? recurrence_backward_kernel<T, LANES, CLUSTER> : recurrence_kernel<T, LANES, CLUSTER>, plan.split, dim3(plan.blocks),
+                                     plan.threads, 0, stream, p);
+}
 template <typename T>
 int recurrence_launch(RecDev p, bool backward, cudaStream_t stream) {
     RecPlan plan;
     if (!rec_plan(&p, &plan)) return (int)cudaErrorInvalidValue;
-    auto kernel = plan.lanes == 16 ? (backward ? recurrence_backward_kernel<T, 16> : recurrence_kernel<T, 16>)
-                                   : (backward ? recurrence_backward_kernel<T, 32> : recurrence_kernel<T, 32>);
-    return launch_dependent_clusters(kernel, plan.split, dim3(plan.blocks), plan.threads, 0, stream, p);
+    if (plan.split > 1) return plan.lanes == 16 ? recurrence_launch<T, 16, true>(p, plan, backward, stream) : recurrence_launch<T, 32, true>(p, plan, backward, stream);
+    return plan.lanes == 16 ? recurrence_launch<T, 16, false>(p, plan, backward, stream) : recurrence_launch<T, 32, false>(p, plan, backward, stream);
 }
 
 // A tensor [T, B, H] by its strides: rows of H values that begin on 4 bytes.
