@@ -167,7 +167,7 @@ int fluke_sm100_linear(const fluke_sm100_linear_t *g, void *stream);
 
 /* ---- gated linear recurrence ---------------------------------------------------------------- */
 
-#define FLUKE_SM100_RECURRENCE_KEPT 64      /* steps between the states that the forward pass keeps */
+#define FLUKE_SM100_RECURRENCE_KEPT 16      /* steps between the states that the forward pass keeps */
 typedef struct {
     int bf16;                   /* type of the 16-bit tensors: 0 f16, 1 bf16                       */
     int T, B, H, reverse;

@@ -633,7 +633,7 @@ PyObject *linear_recurrence(Args a) {
         state_of(a[7], "h_last", gate);
         last = tensor(a[7]);
     }
-    if (save) states = empty_on(gate, {(int64_t(r.T) + 63) / 64, r.B, r.H}, at::kFloat);
+    if (save) states = empty_on(gate, {(int64_t(r.T) + 15) / 16, r.B, r.H}, at::kFloat);
     r.reverse = truth(a[4]);
     r.out = ptr(out); r.out_step = step_of(out); r.out_chunk = chunk_of(out);
     r.lengths = ptr(lengths); r.h0 = ptr(h0); r.h_last = ptr(last);
@@ -648,7 +648,7 @@ PyObject *linear_recurrence_backward(Args a) {
     fluke_linear_recurrence_grad_t r = {};
     steps_of(r, gate, value);
     expect(grad, "grad", gate.scalar_type(), gate.sizes(), gate);
-    expect(states, "states", at::kFloat, {(int64_t(r.T) + 63) / 64, r.B, r.H}, gate);
+    expect(states, "states", at::kFloat, {(int64_t(r.T) + 15) / 16, r.B, r.H}, gate);
     const at::Tensor *grad_last = state_of(a[4], "grad_last", gate), *lengths = lengths_of(a[5], gate);
     at::Tensor dg = new_steps(gate), dv = new_steps(value), dh = empty_on(gate, {r.B, r.H}, at::kFloat);
     r.reverse = truth(a[6]);

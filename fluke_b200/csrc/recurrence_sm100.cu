@@ -10,18 +10,17 @@
 // Backwards, with e_t the gradient of h_t and x_t what reaches step t from the steps behind it:
 //     e_t = dy_t + x_t,    x_{t-1} = e_t - c_t e_t,    dv_t = c_t e_t,    dg_t = e_t (h_{t-1} - v_t) f_t c_t
 // a run of steps acts on x as x_out = x_in + (D - C x_in), C as above. The states h_{t-1} are computed again, from those that the forward
-// pass keeps of every 64th step (4 bytes per 64 values): that reads 6 and writes 4 bytes per value, where states kept in full would be read as well, and rounded.
+// pass keeps of every 16th step (4 bytes per 16 values): that reads 6 and writes 4 bytes per value, where states kept in full would be read as well, and rounded.
 //
-// Both are bound by memory: a lane holds two channels of eight steps in registers, a warp reads rows of 64 channels (128 bytes)
-// or two runs of 32, all of a tile's loads are asked for a tile ahead, and what joins the runs goes through shared memory. Where chunks
-// and channels fill too few SMs, the tiles of a chunk are spread over a cluster, whose CTAs tell each other what their runs do.
+// Both are bound by memory, or else by instructions: two for every tensor and value would already be half of what an SM issues in that time. A warp takes
+// rows of 64 channels, a lane two of them; its run is some steps of a tile, and what joins the runs goes through shared memory.
 
 namespace fluke_sm100 {
 namespace {
 
 constexpr int kRecSteps = 8;          // of a lane
 constexpr int kRecKept = FLUKE_SM100_RECURRENCE_KEPT;   // steps between kept states
-constexpr int kRecThreads = 256;       // at most; fewer for a few steps
+constexpr int kRecThreads = 256;      // of the form that goes through registers
 constexpr int kRecMostCluster = 8;
 
 struct RecIn {
@@ -34,8 +33,10 @@ struct RecOut {
 };
 struct RecDev {
     int T, B, H;
-    int reverse, split, rounds;       // CTAs of a cluster; tiles of each
-    int slabs;                        // runs of channels per chunk
+    int reverse;
+    int slabs;                        // runs of channels per chunk, a warp's each
+    int split, segment;               // CTAs of a cluster; steps of a warp
+    int rounds, runs;                 // (through registers) tiles, and warps per tile
     const int *lengths;
     RecIn gate, value, grad;          // grad: backwards
     RecOut out, grad_gate, grad_value;
@@ -73,27 +74,66 @@ __device__ __forceinline__ float2 low(float4 q) { return make_float2(q.x, q.y); 
 __device__ __forceinline__ float2 high(float4 q) { return make_float2(q.z, q.w); }
 __device__ __forceinline__ float4 both(float2 a, float2 b) { return make_float4(a.x, a.y, b.x, b.y); }
 // Stores into the shared memory of a CTA of the cluster.
-__device__ __forceinline__ void tell(const float4 *to, int rank, float2 a, float2 b) {
+__device__ __forceinline__ void tell(const float2 *to, int rank, float2 a, float2 b) {
     asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(cluster_address(smem_u32(to), rank)), "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y) : "memory");
 }
+__device__ __forceinline__ void tell(const float *to, int rank, float a, float b) {
+    asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(cluster_address(smem_u32(to), rank)), "f"(a), "f"(b) : "memory");
+}
+// The same operations for one channel.
+__device__ __forceinline__ float gate_less_one(float g) { return rcp_approx(fmaf(ex2_approx(g * 1.44269504f), -1.f, -1.f)); }
+__device__ __forceinline__ float towards(float a, float m, float b) { return fmaf(m, a - b, a); }
+__device__ __forceinline__ float less(float a, float m) { return fmaf(m, a, a); }
+__device__ __forceinline__ float longer(float M, float m) { return fmaf(m, M + 1.f, M); }
+__device__ __forceinline__ float through(float a, float M, float b) { return a + fmaf(M, a, b); }
+__device__ __forceinline__ float plus(float a, float b) { return a + b; }
+__device__ __forceinline__ float minus(float a, float b) { return a - b; }
+__device__ __forceinline__ float times(float a, float b) { return a * b; }
+__device__ __forceinline__ float add_times(float a, float b, float c) { return fmaf(a, b, c); }
+__device__ __forceinline__ float2 plus(float2 a, float2 b) { return add2(a, b); }
+__device__ __forceinline__ float2 minus(float2 a, float2 b) { return fma2(b, make_float2(-1.f, -1.f), a); }
+__device__ __forceinline__ float2 times(float2 a, float2 b) { return mul2(a, b); }
+__device__ __forceinline__ float2 add_times(float2 a, float2 b, float2 c) { return fma2(a, b, c); }
+template <typename F> __device__ __forceinline__ F zero_of();
+template <> __device__ __forceinline__ float zero_of<float>() { return 0.f; }
+template <> __device__ __forceinline__ float2 zero_of<float2>() { return make_float2(0.f, 0.f); }
+// -c = -1 / (1 + E), and -f = -E / (1 + E), with E = exp(g). f is not one minus c, which has no digits left where c is near one. An infinite E has c = 0, and any
+// finite f then gives the gradient of zero.
+__device__ __forceinline__ float gate_less_one(float g, float &f) {
+    const float E = ex2_approx(g * 1.44269504f), m = rcp_approx(fmaf(E, -1.f, -1.f));
+    f = fminf(E, 3.0e38f) * m;
+    return m;
+}
+__device__ __forceinline__ float2 gate_less_one(float2 g, float2 &f) {
+    const float2 a = mul2(g, make_float2(1.44269504f, 1.44269504f)), one = make_float2(-1.f, -1.f);
+    const float2 E = make_float2(ex2_approx(a.x), ex2_approx(a.y)), d = fma2(E, one, one), m = make_float2(rcp_approx(d.x), rcp_approx(d.y));
+    f = mul2(make_float2(fminf(E.x, 3.0e38f), fminf(E.y, 3.0e38f)), m);
+    return m;
+}
+// 16-bit values of a lane, one or two.
+template <typename T> __device__ __forceinline__ float2 widen(uint32_t v) { return unpack2(v, T()); }
+template <typename T> __device__ __forceinline__ float widen(uint16_t v) { return unpack2(v, T()).x; }
+template <typename T> __device__ __forceinline__ uint32_t narrow(float2 v) { return pack2(v, T()); }
+template <typename T> __device__ __forceinline__ uint16_t narrow(float v) { return uint16_t(pack2(make_float2(v, 0.f), T())); }
+template <typename Raw> __device__ __forceinline__ Raw sign_bits() { return Raw(0x80008000u); }
+// Gates of plus infinity, whose 1 - f is zero.
+template <typename Raw> __device__ __forceinline__ Raw closed_gates(__half) { return Raw(0x7C007C00u); }
+template <typename Raw> __device__ __forceinline__ Raw closed_gates(__nv_bfloat16) { return Raw(0x7F807F80u); }
 
-// Where a thread works. Processing goes through steps s = 0 .. T-1, time through s or T - 1 - s; a tensor is walked from its first step in
-// processing order. What lies in [from, to) is inside the chunk.
-template <int LANES>
+// Where a warp works: 64 channels of a chunk, and of them the steps of one run of each tile. Processing goes through steps s = 0 .. T-1, time through s
+// or T - 1 - s; a tensor is walked in processing order. What lies in [from, to) is inside the chunk.
 struct RecPlace {
-    int b, rank, channel, lane, run, runs, from, to;
+    int b, channel, lane, from, to;
     bool in;                          // the channels exist (else the last two are read, and nothing is written)
     int64_t state;
-    __device__ __forceinline__ explicit RecPlace(const RecDev &p) {
-        const int slab = int(blockIdx.x) / p.split;
-        rank = int(blockIdx.x) - slab * p.split;
+    __device__ __forceinline__ RecPlace(const RecDev &p, int slab) {
         b = slab / p.slabs;
-        lane = threadIdx.x & (LANES - 1);
-        channel = (slab - b * p.slabs) * (2 * LANES) + 2 * lane;
-        in = channel < p.H;
+        in = b < p.B;
+        b = min(b, p.B - 1);
+        lane = threadIdx.x & 31;
+        channel = (slab % p.slabs) * 64 + 2 * lane;
+        in = in && channel < p.H;
         channel = min(channel, p.H - 2);
-        run = int(threadIdx.x) / LANES;
-        runs = int(blockDim.x) / LANES;
         state = int64_t(b) * p.H + channel;
     }
     __device__ __forceinline__ void measure(const RecDev &p) {   // reads global memory
@@ -101,232 +141,148 @@ struct RecPlace {
         from = p.reverse ? p.T - length : 0;
         to = p.reverse ? p.T : length;
     }
+    __device__ __forceinline__ bool inside(int s) const { return s >= from && s < to; }
 };
 // A tensor from step s on: bytes between steps, in processing order.
 struct RecWalk {
-    const char *at;
+    char *at;
     int64_t step;
-    template <int LANES, typename X>
-    __device__ __forceinline__ RecWalk(const RecDev &p, const X &x, const RecPlace<LANES> &w, int s) {
+    template <typename X>
+    __device__ __forceinline__ RecWalk(const RecDev &p, const X &x, const RecPlace &w, int s) {
         step = (p.reverse ? -x.step : x.step) * 2;
-        at = static_cast<const char *>(x.at) + (w.b * x.chunk + w.channel + (p.reverse ? p.T - 1 : 0) * x.step) * 2 + s * step;
+        at = const_cast<char *>(static_cast<const char *>(x.at)) + (w.b * x.chunk + w.channel + (p.reverse ? p.T - 1 : 0) * x.step) * 2 + s * step;
     }
-    __device__ __forceinline__ const char *operator[](int k) const { return at + k * step; }
-    __device__ __forceinline__ char *out(int k) const { return const_cast<char *>(at + k * step); }
+    __device__ __forceinline__ char *operator[](int k) const { return at + k * step; }
 };
-__device__ __forceinline__ float2 ld_state(const float *s, int64_t at) {
-    return s ? *reinterpret_cast<const float2 *>(s + at) : make_float2(0.f, 0.f);
+__device__ __forceinline__ void st_pair(char *p, uint32_t v) { *reinterpret_cast<uint32_t *>(p) = v; }
+template <int CH = 2> struct RecLane;
+template <> struct RecLane<1> { typedef float F; typedef uint16_t Raw; };
+template <> struct RecLane<2> { typedef float2 F; typedef uint32_t Raw; };
+template <int CH = 2>
+__device__ __forceinline__ typename RecLane<CH>::F ld_state(const float *s, int64_t at) {
+    using F = typename RecLane<CH>::F;
+    return s ? *reinterpret_cast<const F *>(s + at) : zero_of<F>();
 }
-__device__ __forceinline__ void st_state(float *s, int64_t at, float2 v) { *reinterpret_cast<float2 *>(s + at) = v; }
+template <typename F>
+__device__ __forceinline__ void st_state(float *s, int64_t at, F v) { *reinterpret_cast<F *>(s + at) = v; }
 
-// Forwards. LANES: lanes that share a run, with two channels each.
-template <typename T, int LANES, bool CLUSTER>
+// ---- through registers ----------------------------------------------------------------------------
+// For a few steps, and for strides or addresses that TMA does not take. A CTA's warps are runs of a tile (p.runs of them) of as many chunks or
+// channels as that leaves; the next tile's loads are asked for while this one is computed.
+template <typename T>
 __global__ void __launch_bounds__(kRecThreads, 3)
-recurrence_kernel(const RecDev p) {
-    constexpr int kRuns = kRecThreads / LANES;
-    __shared__ float4 run_of[2][kRuns][LANES];                             // -C and V of every run of the tile
-    __shared__ float4 tile_of[2][CLUSTER ? kRecMostCluster : 1][LANES];    // of every CTA's tile
-    __shared__ float2 carried[2][LANES];                                   // the state in front of the tile
-    RecPlace<LANES> w(p);
-    const bool last_run = w.run == w.runs - 1;
-    int s0 = (w.rank * w.runs + w.run) * kRecSteps;
-    const int stride = p.split * w.runs * kRecSteps;                       // steps of a round
+recurrence_direct_kernel(const RecDev p) {
+    __shared__ float4 run_of[2][kRecThreads / 32][32];                     // -C and V of every run
+    __shared__ float2 carried[2][kRecThreads / 32][32];                    // the state in front of the tile, by the last run's warp
+    const int warp = threadIdx.x >> 5, run = warp & (p.runs - 1), first = warp - run, last = first + p.runs - 1;
+    RecPlace w(p, int(blockIdx.x) * (kRecThreads / 32 / p.runs) + warp / p.runs);
+    const int stride = p.runs * kRecSteps;
+    int s0 = run * kRecSteps;
     RecWalk gate(p, p.gate, w, s0), value(p, p.value, w, s0), out(p, p.out, w, s0);
-    if (CLUSTER) cluster_arrive_relaxed();   // this CTA runs: awaited before others are told anything
     dependency_wait();
     w.measure(p);
-    float2 h = ld_state(p.h0, w.state), carry = h;
+    float2 h = ld_state(p.h0, w.state);
     uint32_t g[kRecSteps], v[kRecSteps];
     auto load = [&](int s) {
-        if (s + kRecSteps <= p.T) {
 #pragma unroll
-            for (int k = 0; k < kRecSteps; ++k) {
-                g[k] = ld_pair(gate[k]);
-                v[k] = ld_pair(value[k]);
-            }
-        } else {
-#pragma unroll
-            for (int k = 0; k < kRecSteps; ++k) {
-                g[k] = s + k < p.T ? ld_pair(gate[k]) : 0;
-                v[k] = s + k < p.T ? ld_pair(value[k]) : 0;
-            }
+        for (int k = 0; k < kRecSteps; ++k) {
+            g[k] = s + k < p.T ? ld_pair(gate[k]) : 0;
+            v[k] = s + k < p.T ? ld_pair(value[k]) : 0;
         }
         gate.at += stride * gate.step;
         value.at += stride * value.step;
     };
     load(s0);
-    if (CLUSTER) cluster_wait();
-    if (!CLUSTER && last_run) carried[0][w.lane] = h;
+    if (warp == last) carried[0][warp][w.lane] = h;
     for (int round = 0; round < p.rounds; ++round, s0 += stride) {
         const int par = round & 1;
-        const bool all = s0 >= w.from && s0 + kRecSteps <= w.to;           // of the run's steps lie inside the chunk
         float2 m[kRecSteps], M = make_float2(0.f, 0.f), V = M;
         uint32_t values[kRecSteps];
 #pragma unroll
         for (int k = 0; k < kRecSteps; ++k) {
-            m[k] = gate_less_one(unpack2(g[k], T()));
-            values[k] = v[k];
-        }
-        if (!all)
             // behind a chunk's end nothing changes, whatever stands there
-#pragma unroll
-            for (int k = 0; k < kRecSteps; ++k)
-                if (s0 + k < w.from || s0 + k >= w.to) {
-                    m[k] = make_float2(0.f, 0.f);
-                    values[k] = 0;
-                }
-        if (round + 1 < p.rounds) load(s0 + stride);
-#pragma unroll
-        for (int k = 0; k < kRecSteps; ++k) {
+            const bool live = w.inside(s0 + k);
+            m[k] = live ? gate_less_one(unpack2(g[k], T())) : make_float2(0.f, 0.f);
+            values[k] = live ? v[k] : 0;
             V = towards(V, m[k], unpack2(values[k], T()));
             M = longer(M, m[k]);
         }
-        if (!CLUSTER) {
-            run_of[par][w.run][w.lane] = both(M, V);
-            __syncthreads();
-            h = carried[par][w.lane];
-            for (int r = 0; r < w.run; ++r) {
-                const float4 q = run_of[par][r][w.lane];
-                h = through(h, low(q), high(q));
-            }
-        } else {
-            run_of[par][w.run][w.lane] = both(M, V);
-            __syncthreads();
-            float2 before_m = make_float2(0.f, 0.f), before_v = before_m;
-            for (int r = 0; r < w.run; ++r) {
-                const float4 q = run_of[par][r][w.lane];
-                before_v = through(before_v, low(q), high(q));
-                before_m = longer(before_m, low(q));
-            }
-            if (last_run)
-                for (int r = 0; r < p.split; ++r) tell(&tile_of[par][w.rank][w.lane], r, longer(before_m, M), through(before_v, M, V));
-            cluster_sync_threads();
-            for (int r = 0; r < p.split; ++r) {
-                const float4 q = tile_of[par][r][w.lane];
-                if (r == w.rank) h = carry;
-                carry = through(carry, low(q), high(q));
-            }
-            h = through(h, before_m, before_v);
+        if (round + 1 < p.rounds) load(s0 + stride);
+        run_of[par][warp][w.lane] = both(M, V);
+        __syncthreads();
+        h = carried[par][last][w.lane];
+        for (int r = first; r < warp; ++r) {
+            const float4 q = run_of[par][r][w.lane];
+            h = through(h, low(q), high(q));
         }
         if (p.states && s0 % kRecKept == 0 && w.in && s0 < p.T) st_state(p.states, int64_t(s0 / kRecKept) * p.B * p.H + w.state, h);
-        if (all) {
 #pragma unroll
-            for (int k = 0; k < kRecSteps; ++k) {
-                h = towards(h, m[k], unpack2(values[k], T()));
-                if (w.in) *reinterpret_cast<uint32_t *>(out.out(k)) = pack2(h, T());
-            }
-        } else {
-#pragma unroll
-            for (int k = 0; k < kRecSteps; ++k) {
-                h = towards(h, m[k], unpack2(values[k], T()));
-                if (w.in && s0 + k < p.T) *reinterpret_cast<uint32_t *>(out.out(k)) = s0 + k >= w.from && s0 + k < w.to ? pack2(h, T()) : 0;
-            }
+        for (int k = 0; k < kRecSteps; ++k) {
+            h = towards(h, m[k], unpack2(values[k], T()));
+            if (w.in && s0 + k < p.T) st_pair(out[k], w.inside(s0 + k) ? pack2(h, T()) : 0);
         }
         out.at += stride * out.step;
-        if (!CLUSTER && last_run) carried[par ^ 1][w.lane] = h;
+        if (warp == last) carried[par ^ 1][warp][w.lane] = h;
     }
-    // Only threads that have read h0 themselves, or are behind a barrier that all who do have passed, write what may lie in its place.
-    if (p.h_last && w.in && (CLUSTER ? w.rank == 0 && w.run == 0 : last_run)) st_state(p.h_last, w.state, CLUSTER ? carry : h);
+    // by the threads that have read h0, which may be the same
+    if (p.h_last && w.in && warp == last) st_state(p.h_last, w.state, h);
 }
 
 // Backwards: tiles, and the runs of a tile, are joined from the last to the first.
-template <typename T, int LANES, bool CLUSTER>
+template <typename T>
 __global__ void __launch_bounds__(kRecThreads, 2)
-recurrence_backward_kernel(const RecDev p) {
-    constexpr int kRuns = kRecThreads / LANES;
-    __shared__ float4 run_of[2][kRuns][LANES];                             // -C and V of every run of the tile
-    __shared__ float2 run_back[2][kRuns][LANES];                           // D
-    __shared__ float4 tile_of[2][CLUSTER ? kRecMostCluster : 1][LANES];    // -C and D of every CTA's tile
-    __shared__ float2 carried[2][LANES];                                   // what reaches the tile from the steps behind it
-    RecPlace<LANES> w(p);
-    const bool first_run = w.run == 0;
-    const int stride = p.split * w.runs * kRecSteps;                       // steps of a round
-    int tile0 = ((p.rounds - 1) * p.split + w.rank) * w.runs * kRecSteps, s0 = tile0 + w.run * kRecSteps;
+recurrence_direct_backward_kernel(const RecDev p) {
+    __shared__ float4 run_of[2][kRecThreads / 32][32];                     // -C and V of every run
+    __shared__ float2 run_back[2][kRecThreads / 32][32], carried[2][kRecThreads / 32][32];   // D; what reaches the tile from behind, by the first run's warp
+    const int warp = threadIdx.x >> 5, run = warp & (p.runs - 1), first = warp - run, last = first + p.runs - 1;
+    RecPlace w(p, int(blockIdx.x) * (kRecThreads / 32 / p.runs) + warp / p.runs);
+    const int stride = p.runs * kRecSteps;
+    int tile0 = (p.rounds - 1) * stride, s0 = tile0 + run * kRecSteps;
     RecWalk gate(p, p.gate, w, s0), value(p, p.value, w, s0), grad(p, p.grad, w, s0), dgate(p, p.grad_gate, w, s0), dvalue(p, p.grad_value, w, s0);
-    if (CLUSTER) cluster_arrive_relaxed();   // this CTA runs: awaited before others are told anything
     dependency_wait();
     w.measure(p);
-    float2 x = ld_state(p.grad_last, w.state), carry = x, kept;
+    float2 x = ld_state(p.grad_last, w.state), kept = make_float2(0.f, 0.f);
     uint32_t g[kRecSteps], v[kRecSteps], dy[kRecSteps];
     auto load = [&](int s, int tile) {
-        if (s + kRecSteps <= p.T) {
 #pragma unroll
-            for (int k = 0; k < kRecSteps; ++k) {
-                g[k] = ld_pair(gate[k]);
-                v[k] = ld_pair(value[k]);
-                dy[k] = ld_pair(grad[k]);
-            }
-        } else {
-#pragma unroll
-            for (int k = 0; k < kRecSteps; ++k) {
-                g[k] = s + k < p.T ? ld_pair(gate[k]) : 0;
-                v[k] = s + k < p.T ? ld_pair(value[k]) : 0;
-                dy[k] = s + k < p.T ? ld_pair(grad[k]) : 0;
-            }
+        for (int k = 0; k < kRecSteps; ++k) {
+            g[k] = s + k < p.T ? ld_pair(gate[k]) : 0;
+            v[k] = s + k < p.T ? ld_pair(value[k]) : 0;
+            dy[k] = s + k < p.T ? ld_pair(grad[k]) : 0;
         }
-        // the state in front of the tile
-        kept = tile < p.T ? ld_state(p.states, int64_t(tile / kRecKept) * p.B * p.H + w.state) : make_float2(0.f, 0.f);
+        kept = ld_state(p.states, int64_t(tile / kRecKept) * p.B * p.H + w.state);   // the state in front of the tile
         gate.at -= stride * gate.step;
         value.at -= stride * value.step;
         grad.at -= stride * grad.step;
     };
     if (p.rounds > 0) load(s0, tile0);
-    if (CLUSTER) cluster_wait();
-    if (!CLUSTER && first_run) carried[(p.rounds - 1) & 1][w.lane] = x;
+    if (warp == first) carried[(p.rounds - 1) & 1][warp][w.lane] = x;
     for (int round = p.rounds - 1; round >= 0; --round, s0 -= stride, tile0 -= stride) {
         const int par = round & 1;
-        const bool all = s0 >= w.from && s0 + kRecSteps <= w.to;
         float2 m[kRecSteps], M = make_float2(0.f, 0.f), V = M, D = M, h = kept;
         uint32_t gates[kRecSteps], values[kRecSteps], grads[kRecSteps];
 #pragma unroll
         for (int k = 0; k < kRecSteps; ++k) {
+            const bool live = w.inside(s0 + k);
             gates[k] = g[k];
-            values[k] = v[k];
-            grads[k] = dy[k];
-            m[k] = gate_less_one(unpack2(g[k], T()));
-        }
-        if (!all)
-#pragma unroll
-            for (int k = 0; k < kRecSteps; ++k)
-                if (s0 + k < w.from || s0 + k >= w.to) {
-                    m[k] = make_float2(0.f, 0.f);
-                    gates[k] = values[k] = grads[k] = 0;
-                }
-        if (round > 0) load(s0 - stride, tile0 - stride);
-#pragma unroll
-        for (int k = 0; k < kRecSteps; ++k) {
+            values[k] = live ? v[k] : 0;
+            grads[k] = live ? dy[k] : 0;
+            m[k] = live ? gate_less_one(unpack2(g[k], T())) : make_float2(0.f, 0.f);
             V = towards(V, m[k], unpack2(values[k], T()));
             M = longer(M, m[k]);
         }
+        if (round > 0) load(s0 - stride, tile0 - stride);
 #pragma unroll
         for (int k = kRecSteps - 1; k >= 0; --k) D = less(add2(D, unpack2(grads[k], T())), m[k]);
-        run_of[par][w.run][w.lane] = both(M, V);
-        run_back[par][w.run][w.lane] = D;
+        run_of[par][warp][w.lane] = both(M, V);
+        run_back[par][warp][w.lane] = D;
         __syncthreads();
-        for (int r = 0; r < w.run; ++r) {
+        for (int r = first; r < warp; ++r) {
             const float4 q = run_of[par][r][w.lane];
             h = through(h, low(q), high(q));
         }
-        if (!CLUSTER) {
-            x = carried[par][w.lane];
-            for (int r = w.runs - 1; r > w.run; --r) x = through(x, low(run_of[par][r][w.lane]), run_back[par][r][w.lane]);
-        } else {
-            float2 behind_m = make_float2(0.f, 0.f), behind_d = behind_m;
-            for (int r = w.runs - 1; r > w.run; --r) {
-                const float2 q = low(run_of[par][r][w.lane]);
-                behind_d = through(behind_d, q, run_back[par][r][w.lane]);
-                behind_m = longer(behind_m, q);
-            }
-            if (first_run)
-                for (int r = 0; r < p.split; ++r) tell(&tile_of[par][w.rank][w.lane], r, longer(behind_m, M), through(behind_d, M, D));
-            cluster_sync_threads();
-            for (int r = p.split - 1; r >= 0; --r) {
-                const float4 q = tile_of[par][r][w.lane];
-                if (r == w.rank) x = carry;
-                carry = through(carry, low(q), high(q));
-            }
-            x = through(x, behind_m, behind_d);
-        }
+        x = carried[par][first][w.lane];
+        for (int r = last; r > warp; --r) x = through(x, low(run_of[par][r][w.lane]), run_back[par][r][w.lane]);
         float2 before[kRecSteps];                               // v - h in front of each step
 #pragma unroll
         for (int k = 0; k < kRecSteps; ++k) {
@@ -340,58 +296,411 @@ recurrence_backward_kernel(const RecDev p) {
             x = add2(e, ce);
             // f by itself: one minus c has no digits left where c is near one
             const uint32_t dg = pack2(mul2(mul2(ce, before[k]), gate_of(unpack2(gates[k], T()))), T()), dv = pack2(ce, T()) ^ 0x80008000u;
-            if (all) {
-                if (w.in) {
-                    *reinterpret_cast<uint32_t *>(dgate.out(k)) = dg;
-                    *reinterpret_cast<uint32_t *>(dvalue.out(k)) = dv;
-                }
-            } else {
-                const bool live = s0 + k >= w.from && s0 + k < w.to;
-                if (w.in && s0 + k < p.T) {
-                    *reinterpret_cast<uint32_t *>(dgate.out(k)) = live ? dg : 0;
-                    *reinterpret_cast<uint32_t *>(dvalue.out(k)) = live ? dv : 0;
-                }
+            if (w.in && s0 + k < p.T) {
+                const bool live = w.inside(s0 + k);
+                st_pair(dgate[k], live ? dg : 0);
+                st_pair(dvalue[k], live ? dv : 0);
             }
         }
         dgate.at -= stride * dgate.step;
         dvalue.at -= stride * dvalue.step;
-        if (!CLUSTER && first_run) carried[par ^ 1][w.lane] = x;
+        if (warp == first) carried[par ^ 1][warp][w.lane] = x;
     }
-    if (p.grad_h0 && w.in && (CLUSTER ? w.rank == 0 : true) && first_run) st_state(p.grad_h0, w.state, CLUSTER ? carry : x);
+    if (p.grad_h0 && w.in && warp == first) st_state(p.grad_h0, w.state, x);
 }
 
-// How a call is spread: lanes per run, threads per CTA, CTAs per cluster.
-struct RecPlan {
-    int lanes, threads, split, blocks;
+// ---- a warp by itself -----------------------------------------------------------------------------
+// A warp takes 64 channels of a chunk (CH = 2 per lane) or 32 (CH = 1) through all steps, in tiles of 16 that asynchronous copies of 16 bytes per lane
+// bring into a ring of its own. No warp waits for another, and a step costs its two chained operations and the gate: some 20 instructions for 64 values
+// forwards, four of them of the special-function unit, which takes 8 cycles each: 32 of a scheduler's cycles.
+//
+// SEGMENTED: where chunks and channels are fewer than that needs, the warps of a CTA (and the CTAs of a cluster) take segments of the steps. Each
+// first finds what its segment does as one run; the runs are joined once, and then the segment is walked from the state in front of it. Its tiles are read a second time,
+// from L2 as a rule.
+constexpr int kRecTile = 16;
+static_assert(kRecKept == kRecTile, "a tile begins with a kept state");
+
+template <int CH, int TENSORS, int WARPS, int STAGES, bool SEGMENTED>
+struct RecLayout {
+    static constexpr int kRow = 64 * CH, kTensor = kRecTile * kRow, kStage = TENSORS * kTensor, kRing = STAGES * kStage;
+    static constexpr int kOffRuns = WARPS * kRing;                                         // (segmented) WARPS x 32 lanes of two values
+    static constexpr int kOffTotals = kOffRuns + (SEGMENTED ? WARPS * 32 * 8 * CH : 0);    // kRecMostCluster x 32
+    static constexpr int kDynamic = kOffTotals + (SEGMENTED ? kRecMostCluster * 32 * 8 * CH : 0);
 };
-// Returns false for more CTAs than a grid has.
-inline bool rec_plan(RecDev *p, RecPlan *plan) {
-    plan->lanes = p->H <= 32 ? 16 : 32;
-    // no more warps than the steps fill
-    int warps = kRecThreads / 32;
-    while (warps > 1 && (warps / 2) * (32 / plan->lanes) * kRecSteps >= p->T) warps /= 2;
-    plan->threads = warps * 32;
-    plan->split = 1;
-    const int tile = plan->threads / plan->lanes * kRecSteps;
-    p->slabs = (p->H + 2 * plan->lanes - 1) / (2 * plan->lanes);
-    p->split = plan->split;
-    const int64_t tiles = (int64_t(p->T) + tile - 1) / tile, blocks = int64_t(p->B) * p->slabs * plan->split;
-    p->rounds = int((tiles + plan->split - 1) / plan->split);
-    plan->blocks = int(blocks);
-    return blocks <= INT32_MAX;
+
+// Where such a warp works.
+template <int CH>
+struct RecWarp {
+    int b, channel0, channel, lane, from, to;
+    bool in;
+    int64_t state;
+    __device__ __forceinline__ RecWarp(const RecDev &p, int slab) {
+        b = slab / p.slabs;
+        lane = threadIdx.x & 31;
+        channel0 = (slab - b * p.slabs) * (32 * CH);
+        channel = channel0 + CH * lane;
+        in = channel < p.H;
+        state = int64_t(b) * p.H + min(channel, p.H - CH);
+    }
+    __device__ __forceinline__ void measure(const RecDev &p) {   // reads global memory
+        const int length = p.lengths ? min(max(p.lengths[b], 0), p.T) : p.T;
+        from = p.reverse ? p.T - length : 0;
+        to = p.reverse ? p.T : length;
+    }
+    __device__ __forceinline__ bool inside(int s) const { return s >= from && s < to; }
+    __device__ __forceinline__ bool tile_inside(int s) const { return s >= from && s + kRecTile <= to; }
+};
+__device__ __forceinline__ void copy16(uint32_t to, const void *from, uint32_t bytes) {   // zeros behind `bytes`
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// The copies of a tensor's tiles: which 16 bytes of which rows are this lane's. Rows lie in processing order.
+template <int CH>
+struct RecCopy {
+    static constexpr int kPieces = 4 * CH, kRows = 32 / kPieces, kTurns = kRecTile / kRows;   // 16 bytes each, per row; rows at a time
+    const char *at;                   // of this lane's row of the first tile
+    int64_t step;                     // bytes from step to step, in processing order
+    uint32_t to, bytes;               // shared address in a tile, bytes that the piece has (0: none)
+    int row;
+    template <typename X>
+    __device__ __forceinline__ RecCopy(const RecDev &p, const X &x, const RecWarp<CH> &w, uint32_t tile0) {
+        const int piece = w.lane % kPieces;
+        row = w.lane / kPieces;
+        step = (p.reverse ? -x.step : x.step) * 2;
+        const int channel = w.channel0 + piece * 8, have = min(max(p.H - channel, 0), 8);
+        bytes = have * 2;
+        at = static_cast<const char *>(x.at) + (w.b * x.chunk + (have > 0 ? channel : 0) + (p.reverse ? p.T - 1 : 0) * x.step) * 2 + row * step;
+        to = tile0 + row * (64 * CH) + piece * 16;
+    }
+    // Steps s .. s + 15, those that the tensor has
+    __device__ __forceinline__ void tile(const RecDev &p, int s, uint32_t offset) const {
+        const char *src = at + s * step;
+        if (s + kRecTile <= p.T) {
+#pragma unroll
+            for (int i = 0; i < kTurns; ++i) copy16(to + offset + i * (kRows * 64 * CH), src + i * (kRows * step), bytes);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kTurns; ++i) {
+                const bool has = s + row + i * kRows < p.T;
+                copy16(to + offset + i * (kRows * 64 * CH), has ? src + i * (kRows * step) : at, has ? bytes : 0);
+            }
+        }
+    }
+};
+// Where a lane's channels of step s go.
+template <int CH>
+struct RecPut {
+    char *at;
+    int64_t step;
+    template <typename X>
+    __device__ __forceinline__ RecPut(const RecDev &p, const X &x, const RecWarp<CH> &w) {
+        step = (p.reverse ? -x.step : x.step) * 2;
+        at = static_cast<char *>(x.at) + (w.b * x.chunk + w.channel + (p.reverse ? p.T - 1 : 0) * x.step) * 2;
+    }
+};
+
+template <typename T, int CH, int WARPS, int STAGES, bool SEGMENTED>
+__global__ void __launch_bounds__(WARPS * 32)
+recurrence_warp_kernel(const RecDev p) {
+    using L = RecLayout<CH, 2, WARPS, STAGES, SEGMENTED>;
+    using F = typename RecLane<CH>::F;
+    using Raw = typename RecLane<CH>::Raw;
+    extern __shared__ __align__(128) uint8_t smem[];
+    const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x) >> 5, 0);
+    const int rank = SEGMENTED ? int(blockIdx.x) % p.split : 0, slab = SEGMENTED ? int(blockIdx.x) / p.split : int(blockIdx.x) * WARPS + warp;
+    if (SEGMENTED && p.split > 1) cluster_arrive_relaxed();   // this CTA runs: awaited before others are told anything
+    dependency_wait();
+    if (slab >= p.B * p.slabs) return;
+    RecWarp<CH> w(p, slab);
+    // the steps of this warp, in processing order, and their tiles; a segment's are walked twice
+    const int segment = rank * WARPS + warp, first = SEGMENTED ? int(min(int64_t(segment) * p.segment, int64_t(p.T))) : 0, end = SEGMENTED ? min(first + p.segment, p.T) : p.T;
+    const int n = (end - first + kRecTile - 1) / kRecTile, visits = SEGMENTED ? 2 * n : n;
+    uint8_t *ring = smem + warp * L::kRing;
+    const RecCopy<CH> gates(p, p.gate, w, smem_u32(ring)), values(p, p.value, w, smem_u32(ring) + L::kTensor);
+    int put_stage = 0, put = 0, stage = 0;
+    // Every turn asks for a tile, or for nothing behind the last: the copies of the turn STAGES - 1 before this one have then arrived.
+    auto ask = [&] {
+        if (put < visits) {
+            const int s = first + (SEGMENTED && put >= n ? put - n : put) * kRecTile;
+            gates.tile(p, s, put_stage * L::kStage);
+            values.tile(p, s, put_stage * L::kStage);
+        }
+        copy_commit();
+        ++put;
+        if (++put_stage == STAGES) put_stage = 0;
+    };
+    for (int i = 0; i < STAGES - 1; ++i) ask();
+    w.measure(p);
+    F h = ld_state<CH>(p.h0, w.state);
+    Raw g[kRecTile], v[kRecTile];
+    auto take = [&](int s) {
+        copy_wait<STAGES - 2>();
+        __syncwarp();                 // all lanes' copies; and all lanes have read the tile whose place the next one takes
+        ask();
+        const uint8_t *tile = ring + stage * L::kStage + w.lane * sizeof(Raw);
+#pragma unroll
+        for (int k = 0; k < kRecTile; ++k) {
+            g[k] = *reinterpret_cast<const Raw *>(tile + k * L::kRow);
+            v[k] = *reinterpret_cast<const Raw *>(tile + k * L::kRow + L::kTensor);
+        }
+        if (!w.tile_inside(s)) {
+            // behind a chunk's end nothing changes, whatever stands there
+#pragma unroll
+            for (int k = 0; k < kRecTile; ++k)
+                if (!w.inside(s + k)) {
+                    g[k] = closed_gates<Raw>(T());
+                    v[k] = 0;
+                }
+        }
+        if (++stage == STAGES) stage = 0;
+    };
+    if (SEGMENTED) {
+        F M = zero_of<F>(), V = M;
+        for (int i = 0; i < n; ++i) {
+            take(first + i * kRecTile);
+            F m[kRecTile];
+#pragma unroll
+            for (int k = 0; k < kRecTile; ++k) m[k] = gate_less_one(widen<T>(g[k]));
+#pragma unroll
+            for (int k = 0; k < kRecTile; ++k) {
+                V = towards(V, m[k], widen<T>(v[k]));
+                M = longer(M, m[k]);
+            }
+        }
+        F *runs = reinterpret_cast<F *>(smem + L::kOffRuns), *totals = reinterpret_cast<F *>(smem + L::kOffTotals);
+        runs[(warp * 32 + w.lane) * 2] = M;
+        runs[(warp * 32 + w.lane) * 2 + 1] = V;
+        __syncthreads();
+        F before_m = zero_of<F>(), before_v = before_m;
+#pragma unroll 4
+        for (int r = 0; r < warp; ++r) {
+            const F qm = runs[(r * 32 + w.lane) * 2], qv = runs[(r * 32 + w.lane) * 2 + 1];
+            before_v = through(before_v, qm, qv);
+            before_m = longer(before_m, qm);
+        }
+        if (p.split > 1) {
+            cluster_wait();
+            if (warp == WARPS - 1)
+                for (int r = 0; r < p.split; ++r) tell(totals + (rank * 32 + w.lane) * 2, r, longer(before_m, M), through(before_v, M, V));
+            cluster_sync_threads();
+            for (int r = 0; r < rank; ++r) h = through(h, totals[(r * 32 + w.lane) * 2], totals[(r * 32 + w.lane) * 2 + 1]);
+        }
+        h = through(h, before_m, before_v);
+    }
+    const RecPut<CH> out(p, p.out, w);
+    for (int i = 0; i < n; ++i) {
+        const int s = first + i * kRecTile;
+        take(s);
+        if (p.states && w.in) st_state(p.states, int64_t(s / kRecKept) * p.B * p.H + w.state, h);
+        // Gates, then the chain, then the stores: alone on its scheduler, a warp is as fast as what it has to issue side by side.
+        F m[kRecTile];
+#pragma unroll
+        for (int k = 0; k < kRecTile; ++k) m[k] = gate_less_one(widen<T>(g[k]));
+#pragma unroll
+        for (int k = 0; k < kRecTile; ++k) {
+            h = towards(h, m[k], widen<T>(v[k]));
+            v[k] = narrow<T>(h);
+        }
+        char *to = out.at + s * out.step;
+        if (w.tile_inside(s)) {
+            if (w.in)
+#pragma unroll
+                for (int k = 0; k < kRecTile; ++k, to += out.step) *reinterpret_cast<Raw *>(to) = v[k];
+        } else {
+#pragma unroll
+            for (int k = 0; k < kRecTile; ++k, to += out.step)
+                if (w.in && s + k < p.T) *reinterpret_cast<Raw *>(to) = w.inside(s + k) ? v[k] : Raw(0);
+        }
+    }
+    // By threads that have read h0 themselves, or are behind a barrier that all who do have passed: it may lie in the same place.
+    if (p.h_last && w.in && (!SEGMENTED || segment == p.split * WARPS - 1)) st_state(p.h_last, w.state, h);
 }
 
-template <typename T, int LANES, bool CLUSTER>
-int recurrence_launch(const RecDev &p, const RecPlan &plan, bool backward, cudaStream_t stream) {
-    return launch_dependent_clusters(backward ? recurrence_backward_kernel<T, LANES, CLUSTER> : recurrence_kernel<T, LANES, CLUSTER>, plan.split, dim3(plan.blocks),
-                                     plan.threads, 0, stream, p);
+// Backwards: steps are walked from the last to the first. In a tile the states are computed again from the one that the forward pass kept.
+template <typename T, int CH, int WARPS, int STAGES, bool SEGMENTED>
+__global__ void __launch_bounds__(WARPS * 32)
+recurrence_warp_backward_kernel(const RecDev p) {
+    using L = RecLayout<CH, 3, WARPS, STAGES, SEGMENTED>;
+    using F = typename RecLane<CH>::F;
+    using Raw = typename RecLane<CH>::Raw;
+    extern __shared__ __align__(128) uint8_t smem[];
+    const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x) >> 5, 0);
+    const int rank = SEGMENTED ? int(blockIdx.x) % p.split : 0, slab = SEGMENTED ? int(blockIdx.x) / p.split : int(blockIdx.x) * WARPS + warp;
+    if (SEGMENTED && p.split > 1) cluster_arrive_relaxed();   // this CTA runs: awaited before others are told anything
+    dependency_wait();
+    if (slab >= p.B * p.slabs) return;
+    RecWarp<CH> w(p, slab);
+    const int segment = rank * WARPS + warp, first = SEGMENTED ? int(min(int64_t(segment) * p.segment, int64_t(p.T))) : 0, end = SEGMENTED ? min(first + p.segment, p.T) : p.T;
+    const int n = (end - first + kRecTile - 1) / kRecTile, visits = SEGMENTED ? 2 * n : n;
+    uint8_t *ring = smem + warp * L::kRing;
+    const uint32_t ring0 = smem_u32(ring);
+    const RecCopy<CH> gates(p, p.gate, w, ring0), values(p, p.value, w, ring0 + L::kTensor), grads(p, p.grad, w, ring0 + 2 * L::kTensor);
+    int put_stage = 0, put = 0, stage = 0;
+    auto ask = [&] {
+        if (put < visits) {
+            const bool run_only = SEGMENTED && put < n;   // the first walk takes no values
+            const int s = first + (n - 1 - (SEGMENTED && !run_only ? put - n : put)) * kRecTile;
+            gates.tile(p, s, put_stage * L::kStage);
+            if (!run_only) values.tile(p, s, put_stage * L::kStage);
+            grads.tile(p, s, put_stage * L::kStage);
+        }
+        copy_commit();
+        ++put;
+        if (++put_stage == STAGES) put_stage = 0;
+    };
+    for (int i = 0; i < STAGES - 1; ++i) ask();
+    w.measure(p);
+    F x = ld_state<CH>(p.grad_last, w.state);
+    // the next tile, `values_too` or only gates and gradients
+    Raw g[kRecTile], v[kRecTile], dy[kRecTile];
+    auto take = [&](int s, auto values_too) {
+        copy_wait<STAGES - 2>();
+        __syncwarp();                 // all lanes' copies; and all lanes have read the tile whose place the next one takes
+        ask();
+        const uint8_t *tile = ring + stage * L::kStage + w.lane * sizeof(Raw);
+#pragma unroll
+        for (int k = 0; k < kRecTile; ++k) {
+            g[k] = *reinterpret_cast<const Raw *>(tile + k * L::kRow);
+            if constexpr (decltype(values_too)::value) v[k] = *reinterpret_cast<const Raw *>(tile + k * L::kRow + L::kTensor);
+            dy[k] = *reinterpret_cast<const Raw *>(tile + k * L::kRow + 2 * L::kTensor);
+        }
+        if (!w.tile_inside(s)) {
+#pragma unroll
+            for (int k = 0; k < kRecTile; ++k)
+                if (!w.inside(s + k)) {
+                    g[k] = closed_gates<Raw>(T());
+                    v[k] = dy[k] = 0;
+                }
+        }
+        if (++stage == STAGES) stage = 0;
+    };
+    if (SEGMENTED) {
+        F M = zero_of<F>(), D = M;
+        for (int i = n - 1; i >= 0; --i) {
+            take(first + i * kRecTile, std::false_type());
+            F m[kRecTile];
+#pragma unroll
+            for (int k = 0; k < kRecTile; ++k) m[k] = gate_less_one(widen<T>(g[k]));
+#pragma unroll
+            for (int k = kRecTile - 1; k >= 0; --k) {
+                D = less(plus(D, widen<T>(dy[k])), m[k]);
+                M = longer(M, m[k]);
+            }
+        }
+        F *runs = reinterpret_cast<F *>(smem + L::kOffRuns), *totals = reinterpret_cast<F *>(smem + L::kOffTotals);
+        runs[(warp * 32 + w.lane) * 2] = M;
+        runs[(warp * 32 + w.lane) * 2 + 1] = D;
+        __syncthreads();
+        F behind_m = zero_of<F>(), behind_d = behind_m;
+#pragma unroll 4
+        for (int r = WARPS - 1; r > warp; --r) {
+            const F qm = runs[(r * 32 + w.lane) * 2], qd = runs[(r * 32 + w.lane) * 2 + 1];
+            behind_d = through(behind_d, qm, qd);
+            behind_m = longer(behind_m, qm);
+        }
+        if (p.split > 1) {
+            cluster_wait();
+            if (warp == 0)
+                for (int r = 0; r < p.split; ++r) tell(totals + (rank * 32 + w.lane) * 2, r, longer(behind_m, M), through(behind_d, M, D));
+            cluster_sync_threads();
+            for (int r = p.split - 1; r > rank; --r) x = through(x, totals[(r * 32 + w.lane) * 2], totals[(r * 32 + w.lane) * 2 + 1]);
+        }
+        x = through(x, behind_m, behind_d);
+    }
+    const RecPut<CH> dgate(p, p.grad_gate, w), dvalue(p, p.grad_value, w);
+    // the state in front of the tile, a tile ahead
+    auto state_at = [&](int i) { return ld_state<CH>(p.states, int64_t((first + i * kRecTile) / kRecKept) * p.B * p.H + w.state); };
+    F kept = n > 0 ? state_at(n - 1) : zero_of<F>();
+    for (int i = n - 1; i >= 0; --i) {
+        const int s = first + i * kRecTile;
+        F h = kept;
+        if (i > 0) kept = state_at(i - 1);
+        take(s, std::true_type());
+        F m[kRecTile], u[kRecTile];   // -c, and -f, which becomes (h - v) (-f) with the state in front of the step
+#pragma unroll
+        for (int k = 0; k < kRecTile; ++k) m[k] = gate_less_one(widen<T>(g[k]), u[k]);
+#pragma unroll
+        for (int k = 0; k < kRecTile; ++k) {
+            const F d = minus(h, widen<T>(v[k]));
+            u[k] = times(d, u[k]);
+            h = add_times(m[k], d, h);
+        }
+#pragma unroll
+        for (int k = kRecTile - 1; k >= 0; --k) {
+            const F e = plus(x, widen<T>(dy[k])), ce = times(m[k], e);   // -c e
+            x = plus(e, ce);
+            g[k] = narrow<T>(times(ce, u[k]));
+            v[k] = narrow<T>(ce) ^ sign_bits<Raw>();
+        }
+        char *to_g = dgate.at + s * dgate.step, *to_v = dvalue.at + s * dvalue.step;
+        if (w.tile_inside(s)) {
+            if (w.in)
+#pragma unroll
+                for (int k = 0; k < kRecTile; ++k, to_g += dgate.step, to_v += dvalue.step) {
+                    *reinterpret_cast<Raw *>(to_g) = g[k];
+                    *reinterpret_cast<Raw *>(to_v) = v[k];
+                }
+        } else {
+#pragma unroll
+            for (int k = 0; k < kRecTile; ++k, to_g += dgate.step, to_v += dvalue.step)
+                if (w.in && s + k < p.T) {
+                    *reinterpret_cast<Raw *>(to_g) = w.inside(s + k) ? g[k] : Raw(0);
+                    *reinterpret_cast<Raw *>(to_v) = w.inside(s + k) ? v[k] : Raw(0);
+                }
+        }
+    }
+    if (p.grad_h0 && w.in && (!SEGMENTED || segment == 0)) st_state(p.grad_h0, w.state, x);
 }
+
+template <typename T>
+int recurrence_direct(RecDev p, bool backward, cudaStream_t stream) {
+    // no more runs than the steps fill
+    p.slabs = (p.H + 63) / 64;
+    p.runs = kRecThreads / 32;
+    while (p.runs > 1 && p.runs / 2 * kRecSteps >= p.T) p.runs /= 2;
+    const int per_cta = kRecThreads / 32 / p.runs, tile = p.runs * kRecSteps;
+    p.rounds = (p.T + tile - 1) / tile;
+    const int64_t blocks = (int64_t(p.B) * p.slabs + per_cta - 1) / per_cta;
+    if (blocks > INT32_MAX / 8) return (int)cudaErrorInvalidValue;   // slabs are counted in 32 bits
+    return launch_dependent(backward ? recurrence_direct_backward_kernel<T> : recurrence_direct_kernel<T>, int(blocks), kRecThreads, 0, stream, p);
+}
+
+// Whether copies of 16 bytes can take a tensor's rows.
+template <typename X>
+bool rec_pieces_ok(const RecDev &p, const X &x) {
+    return (reinterpret_cast<uintptr_t>(x.at) & 15u) == 0 && (p.T <= 1 || x.step % 8 == 0) && (p.B <= 1 || x.chunk % 8 == 0);
+}
+
+template <typename T, int CH, int WARPS, int STAGES, bool SEGMENTED>
+int recurrence_warps(RecDev p, int split, bool backward, cudaStream_t stream) {
+    p.slabs = (p.H + 32 * CH - 1) / (32 * CH);
+    p.split = split;
+    const int64_t all = int64_t(p.B) * p.slabs, blocks = SEGMENTED ? all * split : (all + WARPS - 1) / WARPS;
+    if (all > INT32_MAX / 16 || blocks > INT32_MAX) return (int)cudaErrorInvalidValue;   // slabs are counted in 32 bits
+    // whole tiles
+    p.segment = int(((int64_t(p.T) + split * WARPS - 1) / (split * WARPS) + kRecTile - 1) / kRecTile * kRecTile);
+    constexpr auto forward_kernel = recurrence_warp_kernel<T, CH, WARPS, STAGES, SEGMENTED>;
+    constexpr auto backward_kernel = recurrence_warp_backward_kernel<T, CH, WARPS, STAGES, SEGMENTED>;
+    constexpr int kForward = RecLayout<CH, 2, WARPS, STAGES, SEGMENTED>::kDynamic, kBackward = RecLayout<CH, 3, WARPS, STAGES, SEGMENTED>::kDynamic;
+    static_assert(kBackward <= 232448, "shared memory");
+    const int rc = backward ? configure_smem<backward_kernel>(kBackward) : configure_smem<forward_kernel>(kForward);
+    if (rc) return rc;
+    return launch_dependent_clusters(backward ? backward_kernel : forward_kernel, split, dim3(int(blocks)), WARPS * 32, backward ? kBackward : kForward, stream, p);
+}
+
 template <typename T>
 int recurrence_launch(RecDev p, bool backward, cudaStream_t stream) {
-    RecPlan plan;
-    if (!rec_plan(&p, &plan)) return (int)cudaErrorInvalidValue;
-    if (plan.split > 1) return plan.lanes == 16 ? recurrence_launch<T, 16, true>(p, plan, backward, stream) : recurrence_launch<T, 32, true>(p, plan, backward, stream);
-    return plan.lanes == 16 ? recurrence_launch<T, 16, false>(p, plan, backward, stream) : recurrence_launch<T, 32, false>(p, plan, backward, stream);
+    const bool pieces = rec_pieces_ok(p, p.gate) && rec_pieces_ok(p, p.value) && (!backward || rec_pieces_ok(p, p.grad));
+    if (!pieces || p.T <= 32) return recurrence_direct<T>(p, backward, stream);
+    const int64_t narrow_warps = int64_t(p.B) * ((p.H + 31) / 32);
+    if (narrow_warps >= 2048) return recurrence_warps<T, 2, 2, 4, false>(p, 1, backward, stream);
+    if (narrow_warps >= 400) return recurrence_warps<T, 1, 2, 8, false>(p, 1, backward, stream);
+    int split = 1;
+    while (split < kRecMostCluster && narrow_warps * split * 2 <= 160 && p.T >= split * 16 * 64) split *= 2;
+    return recurrence_warps<T, 1, 16, 4, true>(p, split, backward, stream);
 }
 
 // A tensor [T, B, H] by its strides: rows of H values that begin on 4 bytes.

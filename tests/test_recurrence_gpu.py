@@ -52,7 +52,7 @@ def near(got, want, tol):
 
 
 SIZES = [(1, 1, 2), (1, 5, 64), (7, 3, 66), (8, 2, 32), (9, 2, 30), (17, 300, 34), (63, 1, 64), (64, 2, 128), (65, 2, 130), (200, 3, 520), (1000, 2, 64),
-         (4097, 1, 34), (333, 7, 520), (1161, 1, 512), (20000, 1, 64), (520, 40, 256)]
+         (4097, 1, 34), (333, 7, 520), (1161, 1, 512), (20000, 1, 64), (520, 40, 256), (50, 130, 136), (35, 700, 96), (100, 1030, 72), (3000, 2, 40)]
 
 
 @pytest.mark.parametrize("t,b,h", SIZES)
@@ -70,14 +70,14 @@ def test_forward_and_gradients(t, b, h, dtype, layout, reverse, ragged):
             value[lengths[i]:, i] = float("inf")
     clean = (torch.nan_to_num(gate, nan=0.0), torch.nan_to_num(value, posinf=0.0))
     y, last, states = ops.linear_recurrence(gate, value, h0, lengths=lengths, reverse=reverse, save=True)
-    assert y.shape == (t, b, h) and y.dtype == dtype and last.dtype == torch.float32 and states.shape == (-(-t // 64), b, h)
+    assert y.shape == (t, b, h) and y.dtype == dtype and last.dtype == torch.float32 and states.shape == (-(-t // 16), b, h)
     num = None if lengths is None else lengths.cpu().numpy()
     want, want_last, before = ref.forward(n64(clean[0]), n64(clean[1]), n64(h0), num, reverse)
     most, unit = bounds(clean[0], clean[1], h0)
     near(last, want_last, most * unit)
     near(y, want, half(want, dtype) + most * unit * 2)
     order = before[::-1] if reverse else before
-    near(states, order[::64], most * unit)
+    near(states, order[::16], most * unit)
     plain = ops.linear_recurrence(gate, value, h0, lengths=lengths, reverse=reverse)
     assert len(plain) == 2 and torch.equal(plain[0], y) and torch.equal(plain[1], last)
 
