@@ -166,8 +166,69 @@ __device__ __forceinline__ typename RecLane<CH>::F ld_state(const float *s, int6
 template <typename F>
 __device__ __forceinline__ void st_state(float *s, int64_t at, F v) { *reinterpret_cast<F *>(s + at) = v; }
 
+// ---- a few steps ------------------------------------------------------------------------------------
+// A thread has two channels of a chunk and takes them through all of up to STEPS steps, whose loads are asked for at once: what a stream's single steps cost is a
+// launch and one trip to memory. [1, 1024, 768] through the form below, whose registers hold a tile of runs, took 15.2 us.
+template <typename T, int STEPS, bool BACKWARD>
+__global__ void __launch_bounds__(256)
+recurrence_steps_kernel(const RecDev p, const uint32_t pairs) {   // pairs of channels of all chunks
+    const uint32_t i = blockIdx.x * 256u + threadIdx.x, row = uint32_t(p.H) / 2;
+    dependency_wait();
+    if (i >= pairs) return;
+    const int b = int(i / row), channel = int(i - b * row) * 2;
+    const int64_t state = int64_t(i) * 2;
+    int from = 0, to = p.T;
+    if (p.lengths) {
+        const int length = min(max(p.lengths[b], 0), p.T);
+        from = p.reverse ? p.T - length : 0;
+        to = p.reverse ? p.T : length;
+    }
+    auto place = [&](const auto &x, int k) { return static_cast<const char *>(x.at) + (b * x.chunk + (p.reverse ? p.T - 1 - k : k) * x.step + channel) * 2; };
+    float2 h = ld_state(BACKWARD ? p.states : p.h0, state), x = BACKWARD ? ld_state(p.grad_last, state) : make_float2(0.f, 0.f);
+    uint32_t g[STEPS], v[STEPS], dy[STEPS];
+#pragma unroll
+    for (int k = 0; k < STEPS; ++k)
+        if (k < p.T) {
+            g[k] = ld_pair(place(p.gate, k));
+            v[k] = ld_pair(place(p.value, k));
+            if (BACKWARD) dy[k] = ld_pair(place(p.grad, k));
+        }
+    if (!BACKWARD && p.states) st_state(p.states, state, h);
+    float2 m[STEPS], u[STEPS];
+#pragma unroll
+    for (int k = 0; k < STEPS; ++k)
+        if (k < p.T) {
+            // behind a chunk's end nothing changes, whatever stands there
+            const bool live = k >= from && k < to;
+            if (BACKWARD) {
+                m[k] = gate_less_one(unpack2(g[k], T()), u[k]);
+                if (!live) m[k] = u[k] = make_float2(0.f, 0.f);
+                const float2 d = minus(h, live ? unpack2(v[k], T()) : h);
+                u[k] = times(d, u[k]);
+                h = add_times(m[k], d, h);
+            } else {
+                if (live) h = towards(h, gate_less_one(unpack2(g[k], T())), unpack2(v[k], T()));
+                st_pair(const_cast<char *>(place(p.out, k)), live ? pack2(h, T()) : 0);
+            }
+        }
+    if (!BACKWARD) {
+        if (p.h_last) st_state(p.h_last, state, h);
+        return;
+    }
+#pragma unroll
+    for (int k = STEPS - 1; k >= 0; --k)
+        if (k < p.T) {
+            const bool live = k >= from && k < to;
+            const float2 e = live ? add2(x, unpack2(dy[k], T())) : x, ce = mul2(m[k], e);   // -c e
+            x = add2(e, ce);
+            st_pair(const_cast<char *>(place(p.grad_gate, k)), live ? pack2(mul2(ce, u[k]), T()) : 0);
+            st_pair(const_cast<char *>(place(p.grad_value, k)), live ? pack2(ce, T()) ^ 0x80008000u : 0);
+        }
+    if (p.grad_h0) st_state(p.grad_h0, state, x);
+}
+
 // ---- through registers ----------------------------------------------------------------------------
-// For a few steps, and for strides or addresses that TMA does not take. A CTA's warps are runs of a tile (p.runs of them) of as many chunks or
+// For strides or addresses that copies of 16 bytes do not take. A CTA's warps are runs of a tile (p.runs of them) of as many chunks or
 // channels as that leaves; the next tile's loads are asked for while this one is computed.
 template <typename T>
 __global__ void __launch_bounds__(kRecThreads, 3)
@@ -435,16 +496,20 @@ recurrence_warp_kernel(const RecDev p) {
     for (int i = 0; i < STAGES - 1; ++i) ask();
     w.measure(p);
     F h = ld_state<CH>(p.h0, w.state);
-    Raw g[kRecTile], v[kRecTile];
-    auto take = [&](int s) {
+    // The next tile's gates and values: fetched a tile ahead, so that its gates are computed beside the chain of the one before. (Alone on its scheduler a
+    // warp is as fast as what it has to issue side by side.) Behind the last tile what the ring holds is fetched, and not used.
+    F m[kRecTile], next_m[kRecTile];
+    Raw v[kRecTile], next_v[kRecTile];
+    auto fetch = [&](int s) {
         copy_wait<STAGES - 2>();
         __syncwarp();                 // all lanes' copies; and all lanes have read the tile whose place the next one takes
         ask();
         const uint8_t *tile = ring + stage * L::kStage + w.lane * sizeof(Raw);
+        Raw g[kRecTile];
 #pragma unroll
         for (int k = 0; k < kRecTile; ++k) {
             g[k] = *reinterpret_cast<const Raw *>(tile + k * L::kRow);
-            v[k] = *reinterpret_cast<const Raw *>(tile + k * L::kRow + L::kTensor);
+            next_v[k] = *reinterpret_cast<const Raw *>(tile + k * L::kRow + L::kTensor);
         }
         if (!w.tile_inside(s)) {
             // behind a chunk's end nothing changes, whatever stands there
@@ -452,23 +517,32 @@ recurrence_warp_kernel(const RecDev p) {
             for (int k = 0; k < kRecTile; ++k)
                 if (!w.inside(s + k)) {
                     g[k] = closed_gates<Raw>(T());
-                    v[k] = 0;
+                    next_v[k] = 0;
                 }
         }
         if (++stage == STAGES) stage = 0;
+#pragma unroll
+        for (int k = 0; k < kRecTile; ++k) next_m[k] = gate_less_one(widen<T>(g[k]));
     };
+    auto advance = [&] {
+#pragma unroll
+        for (int k = 0; k < kRecTile; ++k) {
+            m[k] = next_m[k];
+            v[k] = next_v[k];
+        }
+    };
+    fetch(first);
+    advance();
     if (SEGMENTED) {
         F M = zero_of<F>(), V = M;
         for (int i = 0; i < n; ++i) {
-            take(first + i * kRecTile);
-            F m[kRecTile];
-#pragma unroll
-            for (int k = 0; k < kRecTile; ++k) m[k] = gate_less_one(widen<T>(g[k]));
+            fetch(i + 1 < n ? first + (i + 1) * kRecTile : first);
 #pragma unroll
             for (int k = 0; k < kRecTile; ++k) {
                 V = towards(V, m[k], widen<T>(v[k]));
                 M = longer(M, m[k]);
             }
+            advance();
         }
         F *runs = reinterpret_cast<F *>(smem + L::kOffRuns), *totals = reinterpret_cast<F *>(smem + L::kOffTotals);
         runs[(warp * 32 + w.lane) * 2] = M;
@@ -493,12 +567,8 @@ recurrence_warp_kernel(const RecDev p) {
     const RecPut<CH> out(p, p.out, w);
     for (int i = 0; i < n; ++i) {
         const int s = first + i * kRecTile;
-        take(s);
         if (p.states && w.in) st_state(p.states, int64_t(s / kRecKept) * p.B * p.H + w.state, h);
-        // Gates, then the chain, then the stores: alone on its scheduler, a warp is as fast as what it has to issue side by side.
-        F m[kRecTile];
-#pragma unroll
-        for (int k = 0; k < kRecTile; ++k) m[k] = gate_less_one(widen<T>(g[k]));
+        fetch(s + kRecTile);
 #pragma unroll
         for (int k = 0; k < kRecTile; ++k) {
             h = towards(h, m[k], widen<T>(v[k]));
@@ -514,6 +584,7 @@ recurrence_warp_kernel(const RecDev p) {
             for (int k = 0; k < kRecTile; ++k, to += out.step)
                 if (w.in && s + k < p.T) *reinterpret_cast<Raw *>(to) = w.inside(s + k) ? v[k] : Raw(0);
         }
+        advance();
     }
     // By threads that have read h0 themselves, or are behind a barrier that all who do have passed: it may lie in the same place.
     if (p.h_last && w.in && (!SEGMENTED || segment == p.split * WARPS - 1)) st_state(p.h_last, w.state, h);
@@ -611,45 +682,74 @@ recurrence_warp_backward_kernel(const RecDev p) {
         x = through(x, behind_m, behind_d);
     }
     const RecPut<CH> dgate(p, p.grad_gate, w), dvalue(p, p.grad_value, w);
-    // the state in front of the tile, a tile ahead
-    auto state_at = [&](int i) { return ld_state<CH>(p.states, int64_t((first + i * kRecTile) / kRecKept) * p.B * p.H + w.state); };
-    F kept = n > 0 ? state_at(n - 1) : zero_of<F>();
-    for (int i = n - 1; i >= 0; --i) {
-        const int s = first + i * kRecTile;
+    // the state in front of a tile, asked for a tile ahead
+    auto state_at = [&](int i) { return i >= 0 ? ld_state<CH>(p.states, int64_t((first + i * kRecTile) / kRecKept) * p.B * p.H + w.state) : zero_of<F>(); };
+    F kept = state_at(n - 1);
+    // What a tile needs from the states: -c, and (h - v) (-f) with the state h in front of the step. With one channel per lane the registers hold two
+    // tiles', and one's are computed beside the chain of the other, which goes back in time.
+    constexpr bool kAhead = CH == 1;
+    F m[kRecTile], u[kRecTile];
+    Raw e_in[kRecTile];
+    auto prepare = [&](int i, F (&tm)[kRecTile], F (&tu)[kRecTile], Raw (&te)[kRecTile]) {
         F h = kept;
-        if (i > 0) kept = state_at(i - 1);
-        take(s, std::true_type());
-        F m[kRecTile], u[kRecTile];   // -c, and -f, which becomes (h - v) (-f) with the state in front of the step
+        kept = state_at(i - 1);
+        take(first + i * kRecTile, std::true_type());
 #pragma unroll
-        for (int k = 0; k < kRecTile; ++k) m[k] = gate_less_one(widen<T>(g[k]), u[k]);
+        for (int k = 0; k < kRecTile; ++k) {
+            tm[k] = gate_less_one(widen<T>(g[k]), tu[k]);
+            te[k] = dy[k];
+        }
 #pragma unroll
         for (int k = 0; k < kRecTile; ++k) {
             const F d = minus(h, widen<T>(v[k]));
-            u[k] = times(d, u[k]);
-            h = add_times(m[k], d, h);
+            tu[k] = times(d, tu[k]);
+            h = add_times(tm[k], d, h);
         }
+    };
+    auto finish = [&](int s) {
+        Raw dg[kRecTile], dv[kRecTile];
 #pragma unroll
         for (int k = kRecTile - 1; k >= 0; --k) {
-            const F e = plus(x, widen<T>(dy[k])), ce = times(m[k], e);   // -c e
+            const F e = plus(x, widen<T>(e_in[k])), ce = times(m[k], e);   // -c e
             x = plus(e, ce);
-            g[k] = narrow<T>(times(ce, u[k]));
-            v[k] = narrow<T>(ce) ^ sign_bits<Raw>();
+            dg[k] = narrow<T>(times(ce, u[k]));
+            dv[k] = narrow<T>(ce) ^ sign_bits<Raw>();
         }
         char *to_g = dgate.at + s * dgate.step, *to_v = dvalue.at + s * dvalue.step;
         if (w.tile_inside(s)) {
             if (w.in)
 #pragma unroll
                 for (int k = 0; k < kRecTile; ++k, to_g += dgate.step, to_v += dvalue.step) {
-                    *reinterpret_cast<Raw *>(to_g) = g[k];
-                    *reinterpret_cast<Raw *>(to_v) = v[k];
+                    *reinterpret_cast<Raw *>(to_g) = dg[k];
+                    *reinterpret_cast<Raw *>(to_v) = dv[k];
                 }
         } else {
 #pragma unroll
             for (int k = 0; k < kRecTile; ++k, to_g += dgate.step, to_v += dvalue.step)
                 if (w.in && s + k < p.T) {
-                    *reinterpret_cast<Raw *>(to_g) = w.inside(s + k) ? g[k] : Raw(0);
-                    *reinterpret_cast<Raw *>(to_v) = w.inside(s + k) ? v[k] : Raw(0);
+                    *reinterpret_cast<Raw *>(to_g) = w.inside(s + k) ? dg[k] : Raw(0);
+                    *reinterpret_cast<Raw *>(to_v) = w.inside(s + k) ? dv[k] : Raw(0);
                 }
+        }
+    };
+    if constexpr (kAhead) {
+        if (n > 0) prepare(n - 1, m, u, e_in);
+        for (int i = n - 1; i >= 0; --i) {
+            F next_m[kRecTile], next_u[kRecTile];
+            Raw next_e[kRecTile];
+            prepare(i - 1, next_m, next_u, next_e);   // in front of the first tile: what the ring holds, and not used
+            finish(first + i * kRecTile);
+#pragma unroll
+            for (int k = 0; k < kRecTile; ++k) {
+                m[k] = next_m[k];
+                u[k] = next_u[k];
+                e_in[k] = next_e[k];
+            }
+        }
+    } else {
+        for (int i = n - 1; i >= 0; --i) {
+            prepare(i, m, u, e_in);
+            finish(first + i * kRecTile);
         }
     }
     if (p.grad_h0 && w.in && (!SEGMENTED || segment == 0)) st_state(p.grad_h0, w.state, x);
@@ -674,33 +774,46 @@ bool rec_pieces_ok(const RecDev &p, const X &x) {
     return (reinterpret_cast<uintptr_t>(x.at) & 15u) == 0 && (p.T <= 1 || x.step % 8 == 0) && (p.B <= 1 || x.chunk % 8 == 0);
 }
 
-template <typename T, int CH, int WARPS, int STAGES, bool SEGMENTED>
-int recurrence_warps(RecDev p, int split, bool backward, cudaStream_t stream) {
+// The two directions of a form, for its number of CTAs per cluster and its capacity.
+template <typename T, int CH, int WARPS, int STAGES, bool SEGMENTED, bool BACKWARD>
+constexpr auto rec_warp_kernel() {
+    if constexpr (BACKWARD) return recurrence_warp_backward_kernel<T, CH, WARPS, STAGES, SEGMENTED>;
+    else return recurrence_warp_kernel<T, CH, WARPS, STAGES, SEGMENTED>;
+}
+template <typename T, int CH, int WARPS, int STAGES, bool SEGMENTED, bool BACKWARD>
+int recurrence_warps(RecDev p, cudaStream_t stream) {
+    constexpr auto kernel = rec_warp_kernel<T, CH, WARPS, STAGES, SEGMENTED, BACKWARD>();
+    constexpr int kSmem = RecLayout<CH, BACKWARD ? 3 : 2, WARPS, STAGES, SEGMENTED>::kDynamic;
+    static_assert(kSmem <= 232448, "shared memory");
     p.slabs = (p.H + 32 * CH - 1) / (32 * CH);
-    p.split = split;
-    const int64_t all = int64_t(p.B) * p.slabs, blocks = SEGMENTED ? all * split : (all + WARPS - 1) / WARPS;
-    if (all > INT32_MAX / 16 || blocks > INT32_MAX) return (int)cudaErrorInvalidValue;   // slabs are counted in 32 bits
+    const int64_t all = int64_t(p.B) * p.slabs;
+    if (all > INT32_MAX / 16) return (int)cudaErrorInvalidValue;   // slabs are counted in 32 bits
+    p.split = 1;
+    if (SEGMENTED)
+        // as many CTAs per cluster as run at once, with two tiles per warp at least
+        for (int c = kRecMostCluster; c > 1 && p.split == 1; --c)
+            if (all * c <= device_sm_count() && int64_t(p.T) >= int64_t(c) * WARPS * 2 * kRecTile && all <= cluster_capacity<kernel>(c, WARPS * 32, kSmem)) p.split = c;
     // whole tiles
-    p.segment = int(((int64_t(p.T) + split * WARPS - 1) / (split * WARPS) + kRecTile - 1) / kRecTile * kRecTile);
-    constexpr auto forward_kernel = recurrence_warp_kernel<T, CH, WARPS, STAGES, SEGMENTED>;
-    constexpr auto backward_kernel = recurrence_warp_backward_kernel<T, CH, WARPS, STAGES, SEGMENTED>;
-    constexpr int kForward = RecLayout<CH, 2, WARPS, STAGES, SEGMENTED>::kDynamic, kBackward = RecLayout<CH, 3, WARPS, STAGES, SEGMENTED>::kDynamic;
-    static_assert(kBackward <= 232448, "shared memory");
-    const int rc = backward ? configure_smem<backward_kernel>(kBackward) : configure_smem<forward_kernel>(kForward);
+    p.segment = int(((int64_t(p.T) + p.split * WARPS - 1) / (p.split * WARPS) + kRecTile - 1) / kRecTile * kRecTile);
+    const int64_t blocks = SEGMENTED ? all * p.split : (all + WARPS - 1) / WARPS;
+    const int rc = configure_smem<kernel>(kSmem);
     if (rc) return rc;
-    return launch_dependent_clusters(backward ? backward_kernel : forward_kernel, split, dim3(int(blocks)), WARPS * 32, backward ? kBackward : kForward, stream, p);
+    return launch_dependent_clusters(kernel, p.split, dim3(int(blocks)), WARPS * 32, kSmem, stream, p);
 }
 
-template <typename T>
-int recurrence_launch(RecDev p, bool backward, cudaStream_t stream) {
-    const bool pieces = rec_pieces_ok(p, p.gate) && rec_pieces_ok(p, p.value) && (!backward || rec_pieces_ok(p, p.grad));
-    if (!pieces || p.T <= 32) return recurrence_direct<T>(p, backward, stream);
-    const int64_t narrow_warps = int64_t(p.B) * ((p.H + 31) / 32);
-    if (narrow_warps >= 2048) return recurrence_warps<T, 2, 2, 4, false>(p, 1, backward, stream);
-    if (narrow_warps >= 400) return recurrence_warps<T, 1, 2, 8, false>(p, 1, backward, stream);
-    int split = 1;
-    while (split < kRecMostCluster && narrow_warps * split * 2 <= 160 && p.T >= split * 16 * 64) split *= 2;
-    return recurrence_warps<T, 1, 16, 4, true>(p, split, backward, stream);
+template <typename T, bool BACKWARD>
+int recurrence_launch(RecDev p, cudaStream_t stream) {
+    const bool pieces = rec_pieces_ok(p, p.gate) && rec_pieces_ok(p, p.value) && (!BACKWARD || rec_pieces_ok(p, p.grad));
+    const int64_t pairs = int64_t(p.B) * (p.H / 2);
+    if (p.T <= 8 && pairs <= INT32_MAX - 256) {
+        auto kernel = p.T <= 1 ? recurrence_steps_kernel<T, 1, BACKWARD> : p.T <= 4 ? recurrence_steps_kernel<T, 4, BACKWARD> : recurrence_steps_kernel<T, 8, BACKWARD>;
+        return launch_dependent(kernel, int((pairs + 255) / 256), 256, 0, stream, p, uint32_t(pairs));
+    }
+    if (!pieces) return recurrence_direct<T>(p, BACKWARD, stream);
+    const int64_t narrow = int64_t(p.B) * ((p.H + 31) / 32);
+    if (narrow >= 1024 || p.T <= 64) return recurrence_warps<T, 2, 4, BACKWARD ? 3 : 4, false, BACKWARD>(p, stream);
+    if (narrow >= 200) return recurrence_warps<T, 2, 4, 4, true, BACKWARD>(p, stream);
+    return recurrence_warps<T, 1, 16, 4, true, BACKWARD>(p, stream);
 }
 
 // A tensor [T, B, H] by its strides: rows of H values that begin on 4 bytes.
@@ -785,5 +898,6 @@ extern "C" int fluke_sm100_recurrence(const fluke_sm100_recurrence_t *r, int bac
         if (p.T > 0 && out[o].H && !rec_rows_apart(out[o])) return (int)cudaErrorInvalidValue;
     }
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    return r->bf16 ? recurrence_launch<__nv_bfloat16>(p, backward != 0, s) : recurrence_launch<__half>(p, backward != 0, s);
+    if (backward) return r->bf16 ? recurrence_launch<__nv_bfloat16, true>(p, s) : recurrence_launch<__half, true>(p, s);
+    return r->bf16 ? recurrence_launch<__nv_bfloat16, false>(p, s) : recurrence_launch<__half, false>(p, s);
 }
