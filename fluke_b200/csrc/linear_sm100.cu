@@ -44,27 +44,30 @@ __host__ __device__ constexpr uint32_t make_idesc_16(int M, int N) {
 enum LinAct { kActNone = 0, kActRelu = 1, kActSilu = 2, kActGelu = 3, kActTanh = 4, kActSigmoid = 5 };
 
 template <int ACT>
-__device__ __forceinline__ float activate(float v) {
-    if constexpr (ACT == kActRelu) return v < 0.f ? 0.f : v;
+__device__ __forceinline__ float2 activate(float2 v) {
+    const auto one = [](float x) { return make_float2(x, x); };
+    const auto exp2_of = [](float2 x) { return make_float2(ex2_approx(x.x), ex2_approx(x.y)); };
+    const auto rcp_of = [](float2 x) { return make_float2(rcp_approx(x.x), rcp_approx(x.y)); };
+    if constexpr (ACT == kActRelu) return make_float2(v.x < 0.f ? 0.f : v.x, v.y < 0.f ? 0.f : v.y);
     if constexpr (ACT == kActSilu || ACT == kActSigmoid) {
-        const float s = rcp_approx(1.f + ex2_approx(-1.44269504f * v));
-        return ACT == kActSilu ? v * s : s;
+        const float2 s = rcp_of(add2(exp2_of(mul2(v, one(-1.44269504f))), one(1.f)));
+        return ACT == kActSilu ? mul2(v, s) : s;
     }
     if constexpr (ACT == kActTanh) {
-        const float t = ex2_approx(-2.88539008f * fabsf(v));
-        const float big = copysignf((1.f - t) * rcp_approx(1.f + t), v);
-        return fabsf(v) < 0.015625f ? fmaf(v * v * v, -0.333333333f, v) : big;
+        const float2 a = make_float2(fabsf(v.x), fabsf(v.y)), t = exp2_of(mul2(a, one(-2.88539008f)));
+        const float2 big = mul2(fma2(t, one(-1.f), one(1.f)), rcp_of(add2(t, one(1.f))));
+        const float2 small = fma2(mul2(mul2(v, v), v), one(-0.333333333f), v);
+        return make_float2(a.x < 0.015625f ? small.x : copysignf(big.x, v.x), a.y < 0.015625f ? small.y : copysignf(big.y, v.y));
     }
     if constexpr (ACT == kActGelu) {
-        const float a = fabsf(v), t = rcp_approx(fmaf(0.31f, a, 1.f));
-        float p = -0.0739276186f;
-        p = fmaf(p, t, 0.180445790f);
-        p = fmaf(p, t, 0.0157500077f);
-        p = fmaf(p, t, 0.133426800f);
-        p = fmaf(p, t, 0.120442092f);
-        p = fmaf(p, t, 0.123860620f);
-        const float h = p * t * ex2_approx(-0.721347520f * (a * a));
-        return v * (v < 0.f ? h : 1.f - h);
+        const float2 a = make_float2(fabsf(v.x), fabsf(v.y)), t = rcp_of(fma2(a, one(0.31f), one(1.f)));
+        float2 q = fma2(t, one(-0.0739276186f), one(0.180445790f));
+        q = fma2(q, t, one(0.0157500077f));
+        q = fma2(q, t, one(0.133426800f));
+        q = fma2(q, t, one(0.120442092f));
+        q = fma2(q, t, one(0.123860620f));
+        const float2 h = mul2(mul2(q, t), exp2_of(mul2(mul2(a, a), one(-0.721347520f)))), rest = fma2(h, one(-1.f), one(1.f));
+        return mul2(v, make_float2(v.x < 0.f ? h.x : rest.x, v.y < 0.f ? h.y : rest.y));
     }
     return v;
 }
@@ -86,7 +89,7 @@ __device__ __forceinline__ uint4 finish8(const float (&sum)[8], const uint4 *bia
     for (int i = 0; i < 4; ++i) {
         float2 v = make_float2(sum[2 * i], sum[2 * i + 1]);
         if (bias) v = add2(v, unpack2(b[i], T()));
-        v = make_float2(activate<ACT>(v.x), activate<ACT>(v.y));
+        v = activate<ACT>(v);
         if (residual) v = fma2(make_float2(alpha, alpha), unpack2(r[i], T()), v);
         w[i] = pack2(v, T());
     }
@@ -287,20 +290,20 @@ linear_split_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
 // staging that the output leaves from, ahead of the sums.
 //
 // In each CTA warp 0 loads (one thread), warp 1 owns tensor memory and (first CTA) issues MMAs, warps 2-3 are idle and the others are
-// the epilogue: 32 rows x BN / 2 columns each.
+// the epilogue, 32 rows x 64 columns each: with half as many, of 128 columns, a tile with bias and residual took its warps 9000 cycles and its MMAs at
+// K = 512 4000, most of it latency (loads of the bias and of the staging behind stores that may be to the same place; a proxy fence and a store per group).
 //
 // Pairs take tiles in turns, and the tiles are ordered in bands of kLinBand rows of tiles, column by column: what runs at the same time shares
 // rows of x and of the weight in L2.
 constexpr int kLinBand = 8;
 template <int BN>
 struct LinPairLayout {
-    static constexpr int kOperandX = 128 * 128, kOperandW = BN / 2 * 128;
-    static constexpr int kSlot = kOperandX + kOperandW;
+    static constexpr int kOperandX = 128 * 128, kOperandW = BN / 2 * 128, kSlot = kOperandX + kOperandW;
+    static constexpr int kEpilogueWarps = BN / 16, kThreads = 128 + kEpilogueWarps * 32;
     static constexpr int kStages = BN == 256 ? 5 : 7;
-    static constexpr int kGroups = BN / 128;                   // of 64 columns, per epilogue warp
-    static constexpr int kOffStaging = kStages * kSlot;
-    static constexpr int kOffBars = kOffStaging + 8 * kGroups * 32 * 128;
-    static constexpr int kBars = 2 * kStages + 4 + 8 * kGroups;
+    static constexpr int kOffStaging = kStages * kSlot;        // per epilogue warp 32 rows x 64 columns
+    static constexpr int kOffBars = kOffStaging + kEpilogueWarps * 32 * 128;
+    static constexpr int kBars = 2 * kStages + 4 + kEpilogueWarps;
     static constexpr int kDynamic = kOffBars + kBars * 8 + 16 + 1024;
     static_assert(kOffStaging % 1024 == 0 && kDynamic <= 232448, "shared memory");
 };
@@ -315,15 +318,24 @@ struct LinPairDev {
     float alpha;
 };
 
-__device__ __forceinline__ void lin_tile(const LinPairDev &p, int t, int &m, int &n) {
-    const int band = t / (kLinBand * p.n_tiles), at = t - band * kLinBand * p.n_tiles;
-    const int rows = min(kLinBand, p.m_tiles - band * kLinBand);
-    n = at / rows;
-    m = band * kLinBand + at - n * rows;
-}
+// The tiles of a pair, one after the other.
+struct LinRun {
+    int tile, m, n;
+    __device__ __forceinline__ explicit LinRun(const LinPairDev &p) : tile(int(blockIdx.x) >> 1) { place(p); }
+    __device__ __forceinline__ bool left(const LinPairDev &p) const { return tile < p.tiles; }
+    __device__ __forceinline__ void next(const LinPairDev &p) {
+        tile += int(gridDim.x) >> 1;
+        if (left(p)) place(p);
+    }
+    __device__ __forceinline__ void place(const LinPairDev &p) {
+        const int band = tile / (kLinBand * p.n_tiles), at = tile - band * kLinBand * p.n_tiles, rows = min(kLinBand, p.m_tiles - band * kLinBand);
+        n = at / rows;
+        m = band * kLinBand + at - n * rows;
+    }
+};
 
 template <typename T, int ACT, int BN>
-__global__ void __launch_bounds__(kLinThreads, 1)
+__global__ void __launch_bounds__(LinPairLayout<BN>::kThreads, 1)
 linear_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_res,
                    const __grid_constant__ CUtensorMap tm_out, const LinPairDev p) {
     using L = LinPairLayout<BN>;
@@ -336,7 +348,7 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + L::kBars);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
     const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x) >> 5, 0), lane = threadIdx.x & 31;
-    const int rank = int(blockIdx.x & 1), pair = int(blockIdx.x >> 1), pairs = int(gridDim.x >> 1);
+    const int rank = int(blockIdx.x & 1);
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; ++s) {
@@ -345,9 +357,9 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
         }
         for (int s = 0; s < 2; ++s) {
             mbar_init(&tfull_bar[s], 1);
-            mbar_init(&tempty_bar[s], 16);
+            mbar_init(&tempty_bar[s], 2 * L::kEpilogueWarps);
         }
-        for (int s = 0; s < 8 * L::kGroups; ++s) mbar_init(&res_bar[s], 1);
+        for (int s = 0; s < L::kEpilogueWarps; ++s) mbar_init(&res_bar[s], 1);
         *abort_flag = 0;
         fence_barrier_init();
         tma_prefetch_desc(&tm_x);
@@ -366,23 +378,22 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
     const uint32_t tmem = *tmem_slot;
     dependency_wait();
 
+    LinRun run(p);
     bool ok = true;
     if (warp == 0) {
         if (elect_one()) {
             int stage = 0;
             uint32_t phase = 0;
-            for (int t = pair; t < p.tiles && ok; t += pairs) {
-                int m, n;
-                lin_tile(p, t, m, n);
-                const int m0 = m * 256 + rank * 128, n0 = n * BN + rank * (BN / 2);
+            for (; run.left(p) && ok; run.next(p)) {
+                const int m0 = run.m * 256 + rank * 128, n0 = run.n * BN + rank * (BN / 2);
                 for (int ks = 0; ks < p.stages_k; ++ks) {
                     ok = mbar_wait(&empty_bar[stage], phase ^ 1u, abort_flag, 160);
                     if (!ok) break;
-                    uint8_t *sx = smem + stage * L::kSlot, *sw = sx + L::kOperandX;
+                    uint8_t *sx = smem + stage * L::kSlot;
                     const uint32_t bar = cluster_address(smem_u32(&full_bar[stage]), 0);
                     if (rank == 0) mbar_arrive_expect_tx(&full_bar[stage], 2 * L::kSlot);
                     tma_load_2d_pair(sx, &tm_x, bar, ks * kLinStageK, m0);
-                    tma_load_2d_pair(sw, &tm_w, bar, ks * kLinStageK, n0);
+                    tma_load_2d_pair(sx + L::kOperandX, &tm_w, bar, ks * kLinStageK, n0);
                     if (++stage == STAGES) { stage = 0; phase ^= 1u; }
                 }
             }
@@ -395,7 +406,7 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
             uint32_t phase = 0, buf = 0, t_phase = 0;
             bool ready = false;
             const uint32_t base_lo = desc_lo(smem_u32(smem));
-            for (int t = pair; t < p.tiles && ok; t += pairs) {
+            for (; run.left(p) && ok; run.next(p)) {
                 ok = mbar_wait_warp(&tempty_bar[buf], t_phase ^ 1u, abort_flag, 161);
                 if (!ok) break;
                 tc_fence_after_sync();
@@ -426,73 +437,73 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
         }
         __syncwarp();
     } else if (warp >= 4) {
-        const int q = warp & 3, half = (warp - 4) >> 2;
-        uint8_t *staging = smem + L::kOffStaging + (warp - 4) * (L::kGroups * 32 * 128);
-        uint64_t *loaded = res_bar + (warp - 4) * L::kGroups;
+        const int q = warp & 3, part = (warp - 4) >> 2;
+        uint8_t *staging = smem + L::kOffStaging + (warp - 4) * (32 * 128);
+        const T *bias_at = static_cast<const T *>(p.bias);
+        uint64_t *loaded = res_bar + (warp - 4);
         const uint32_t tempty = cluster_address(smem_u32(tempty_bar), 0);
-        const T *bias = static_cast<const T *>(p.bias);
-        uint32_t buf = 0, t_phase = 0, res_phase = 0;   // res_phase: a bit per group
-        for (int t = pair; t < p.tiles && ok; t += pairs) {
-            int m, n;
-            lin_tile(p, t, m, n);
-            const int m0 = m * 256 + rank * 128 + q * 32, c0 = n * BN + half * (BN / 2);
-            const bool rows = m0 < p.M;
-            // The staging of a group is free when its last store has read it; every group of every tile commits one, if an empty one.
-            if (lane == 0) {
-#pragma unroll
-                for (int g = 0; g < L::kGroups; ++g) {
-                    if (g + 1 < L::kGroups) tma_store_wait_read<L::kGroups - 1>();
-                    else tma_store_wait_read<0>();
-                    if (p.residual && rows && c0 + g * 64 < p.N) {
-                        mbar_arrive_expect_tx(&loaded[g], 32 * 128);
-                        tma_load_2d(staging + g * (32 * 128), &tm_res, &loaded[g], c0 + g * 64, m0);
+        uint32_t buf = 0, t_phase = 0, res_phase = 0;
+        for (; run.left(p) && ok; run.next(p)) {
+            const int m0 = run.m * 256 + rank * 128 + q * 32, c0 = run.n * BN + part * 64;
+            const bool live = m0 < p.M && c0 < p.N;
+            if (live) {
+                if (lane == 0) {
+                    tma_store_wait_read<0>();   // the staging is free
+                    if (p.residual) {
+                        mbar_arrive_expect_tx(loaded, 32 * 128);
+                        tma_load_2d(staging, &tm_res, loaded, c0, m0);
                     }
                 }
+                __syncwarp();
             }
-            __syncwarp();
             ok = mbar_wait_warp(&tfull_bar[buf], t_phase, abort_flag, 163);
             if (!ok) break;
             tc_fence_after_sync();
-            const uint32_t t_row = tmem + (uint32_t(q * 32) << 16) + buf * BN + half * (BN / 2);
+            const uint32_t t_row = tmem + (uint32_t(q * 32) << 16) + buf * BN + part * 64;
+            if (live && p.residual) {
+                ok = mbar_wait_warp(loaded, res_phase, abort_flag, 164);
+                if (!ok) break;
+                res_phase ^= 1u;
+            }
 #pragma unroll
-            for (int g = 0; g < L::kGroups; ++g) {
-                uint32_t a[2][32];
-                tmem_ld_32x32(t_row + g * 64, a[0]);
-                tmem_ld_32x32(t_row + g * 64 + 32, a[1]);
+            for (int h = 0; h < 2; ++h) {
+                uint32_t a[32];
+                tmem_ld_32x32(t_row + h * 32, a);
+                // everything is read before anything is written: to the compiler these may be the same places
+                uint4 bias[4], res[4];
+                if (p.bias)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int c = c0 + 32 * h + 8 * j;
+                        bias[j] = c < p.N ? *reinterpret_cast<const uint4 *>(bias_at + c) : make_uint4(0, 0, 0, 0);
+                    }
+                if (p.residual)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) res[j] = *reinterpret_cast<const uint4 *>(staging + sw128_offset(lane, 4 * h + j));
                 tmem_ld_wait();
-                if (g + 1 == L::kGroups) {
+                if (h == 1) {
                     tc_fence_before_sync();
                     __syncwarp();
                     if (lane == 0) mbar_arrive_cluster(tempty + buf * 8);
                 }
-                const int c = c0 + g * 64;
-                const bool live = rows && c < p.N;
-                uint8_t *stage_row = staging + g * (32 * 128);
-                if (live) {
-                    if (p.residual) {
-                        ok = mbar_wait_warp(&loaded[g], (res_phase >> g) & 1u, abort_flag, 164);
-                        if (!ok) break;
-                        res_phase ^= 1u << g;
-                    }
+                if (!live) continue;
+                uint4 out[4];
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        uint4 *cell = reinterpret_cast<uint4 *>(stage_row + sw128_offset(lane, j));
-                        uint4 b, r;
-                        if (bias) b = c + 8 * j < p.N ? *reinterpret_cast<const uint4 *>(bias + c + 8 * j) : make_uint4(0, 0, 0, 0);
-                        if (p.residual) r = *cell;
-                        float v[8];
+                for (int j = 0; j < 4; ++j) {
+                    float v[8];
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(a[j >> 2][(j & 3) * 8 + i]);
-                        *cell = finish8<T, ACT>(v, bias ? &b : nullptr, p.residual ? &r : nullptr, p.alpha);
-                    }
-                    fence_proxy_async_smem();
-                    __syncwarp();
+                    for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(a[8 * j + i]);
+                    out[j] = finish8<T, ACT>(v, p.bias ? &bias[j] : nullptr, p.residual ? &res[j] : nullptr, p.alpha);
                 }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) *reinterpret_cast<uint4 *>(staging + sw128_offset(lane, 4 * h + j)) = out[j];
+            }
+            if (live) {
+                fence_proxy_async_smem();
+                __syncwarp();
                 if (lane == 0) {
-                    if (live) {
-                        if (p.passes_by) tma_store_2d(&tm_out, stage_row, c, m0, l2_evict_first());
-                        else tma_store_2d(&tm_out, stage_row, c, m0);
-                    }
+                    if (p.passes_by) tma_store_2d(&tm_out, staging, c0, m0, l2_evict_first());
+                    else tma_store_2d(&tm_out, staging, c0, m0);
                     tma_store_commit();
                 }
             }
@@ -584,7 +595,7 @@ template <typename T, int ACT, int BN>
 int linear_pair_launch(const fluke_sm100_linear_t *g, cudaStream_t stream) {
     using L = LinPairLayout<BN>;
     constexpr auto kernel = linear_pair_kernel<T, ACT, BN>;
-    const int capacity = cluster_capacity<kernel>(2, kLinThreads, L::kDynamic);
+    const int capacity = cluster_capacity<kernel>(2, L::kThreads, L::kDynamic);
     if (capacity < 1) return (int)cudaErrorNotSupported;
     LinPairDev p;
     p.M = g->M; p.N = g->N;
@@ -607,12 +618,15 @@ int linear_pair_launch(const fluke_sm100_linear_t *g, cudaStream_t stream) {
     if (!rc && g->residual) rc = lin_operand(&tm_res, g->residual, g->M, g->N, g->ld_residual, 32);
     if (rc) return rc;
     const int pairs = p.tiles < capacity ? p.tiles : capacity;
-    return launch_dependent_clusters(kernel, 2, pairs * 2, kLinThreads, L::kDynamic, stream, tm_x, tm_w, tm_res, tm_out, p);
+    return launch_dependent_clusters(kernel, 2, pairs * 2, L::kThreads, L::kDynamic, stream, tm_x, tm_w, tm_res, tm_out, p);
 }
 
 template <typename T, int ACT>
 int linear_dispatch(const fluke_sm100_linear_t *g, cudaStream_t stream) {
-    if (g->M <= 64 || lin_split_tiles(g) <= device_sm_count()) return linear_split_launch<T, ACT>(g, stream);
+    const int64_t m_tiles = (int64_t(g->M) + 255) / 256, pairs = device_sm_count() / 2;
+    if (g->M <= 64 || (int64_t(g->M) + 63) / 64 * ((g->N + 127) / 128) <= device_sm_count()) return linear_split_launch<T, ACT>(g, stream);
+    const int64_t wide = (m_tiles * ((g->N + 255) / 256) + pairs - 1) / pairs, narrow = (m_tiles * ((g->N + 127) / 128) + pairs - 1) / pairs;
+    if (5 * wide > 3 * narrow) return linear_pair_launch<T, ACT, 128>(g, stream);
     return linear_pair_launch<T, ACT, 256>(g, stream);
 }
 template <typename T>
