@@ -536,16 +536,6 @@ inline int lin_operand(CUtensorMap *m, const void *base, int rows, int cols, int
     return make_tmap_2d(m, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, base, rows, cols, uint64_t(ld) * 2, box_rows, kLinStageK, true);
 }
 
-// Rows of x per tile of the split form: 64 while those tiles are all resident at once, else 128; what there is of them, if less.
-inline int lin_split_rows(const fluke_sm100_linear_t *g) {
-    if (g->M <= 32) return g->M <= 16 ? 16 : 32;
-    return int64_t((g->M + 63) / 64) * ((g->N + 127) / 128) <= device_sm_count() ? 64 : 128;
-}
-inline int64_t lin_split_tiles(const fluke_sm100_linear_t *g) {
-    const int rows = lin_split_rows(g);
-    return int64_t((g->M + rows - 1) / rows) * ((g->N + 127) / 128);
-}
-
 template <typename T, int ACT>
 int linear_split_launch(const fluke_sm100_linear_t *g, cudaStream_t stream) {
     constexpr auto kernel = linear_split_kernel<T, ACT>;
@@ -555,21 +545,30 @@ int linear_split_launch(const fluke_sm100_linear_t *g, cudaStream_t stream) {
     p.stages_k = (g->K + kLinStageK - 1) / kLinStageK;
     p.last_steps = (g->K - (p.stages_k - 1) * kLinStageK + 15) / 16;
     p.e = lin_epilogue(g);
-    const int rows = p.rows = lin_split_rows(g), sms = device_sm_count();
-    const int64_t tiles = lin_split_tiles(g);
-    if (tiles > (INT32_MAX >> 3) - 1024) return (int)cudaErrorInvalidValue;
-    // CTAs per tile, while all of them run at once and each has a stage of K at least: the number with the shortest time by what a stage takes
-    // (0.2 us) and what a hand-over of the tile's rows does (0.6 us, and 18 ns per row).
-    const int most = g->M < rows ? g->M : rows;
-    int each = p.stages_k;
+    // Rows of x per tile, and CTAs per tile while all of them run at once and each has a stage of K at least: those with the shortest time by what a stage takes
+    // (0.2 us), the epilogue (18 ns per row), and a hand-over of the tile's rows (0.6 us, and 18 ns per row). Us per call, tiles of 16 : 32 : 64 : 128 rows:
+    // [333, 512] x [1536, 512] 5.5 : 5.0 : 6.1 : 8.1, [64, 4096] x [4096, 4096] 17.6 : 11.9 : 10.9 : 11.7, [512, 2048] x [512, 2048] 9.7 : 7.5 : 7.3 : 10.2.
+    const int sms = device_sm_count();
+    int rows = 0, each = p.stages_k;
     float best = 0.f;
-    for (int c = 1; c <= 8 && c <= p.stages_k && (c == 1 || tiles * c <= sms); ++c) {
-        const int n = (p.stages_k + c - 1) / c;
-        const float us = n * 0.2f + (c > 1 ? 0.6f + 0.018f * most : 0.f);
-        if (c > 1 && (us >= best || tiles > cluster_capacity<kernel>(c, kLinThreads, kLinSplitMaxSmem + 1024))) continue;
-        best = us;
-        each = n;
+    for (int r = 16; r <= 128; r *= 2) {
+        const int64_t tiles = (int64_t(g->M) + r - 1) / r * p.n_tiles;
+        const int filled = g->M < r ? g->M : r;
+        for (int c = 1; c <= 8 && c <= p.stages_k && (c == 1 || tiles * c <= sms); ++c) {
+            const int n = (p.stages_k + c - 1) / c;
+            const float us = (n * 0.2f + 0.018f * filled) * float((tiles + sms - 1) / sms) + (c > 1 ? 0.6f + 0.018f * filled : 0.f);
+            if (rows && us >= best) continue;
+            if (c > 1 && tiles > cluster_capacity<kernel>(c, kLinThreads, kLinSplitMaxSmem + 1024)) continue;
+            best = us;
+            each = n;
+            rows = r;
+        }
+        if (r >= g->M) break;
     }
+    const int64_t tiles = (int64_t(g->M) + rows - 1) / rows * p.n_tiles;
+    if (tiles > (INT32_MAX >> 3) - 1024) return (int)cudaErrorInvalidValue;
+    const int most = g->M < rows ? g->M : rows;
+    p.rows = rows;
     const int split = p.split = (p.stages_k + each - 1) / each;
     const int stage_bytes = rows * 128 + 128 * 128;
     // a longer run of K than the ring holds streams through a deeper one, where an SM has no second CTA to run
