@@ -12,8 +12,9 @@
 // a run of steps acts on x as x_out = x_in + (D - C x_in), C as above. The states h_{t-1} are computed again, from those that the forward
 // pass keeps of every 16th step (4 bytes per 16 values): that reads 6 and writes 4 bytes per value, where states kept in full would be read as well, and rounded.
 //
-// Both are bound by memory, or else by instructions: two for every tensor and value would already be half of what an SM issues in that time. A warp takes
-// rows of 64 channels, a lane two of them; its run is some steps of a tile, and what joins the runs goes through shared memory.
+// Both are bound by memory where chunks and channels fill the device ([1000, 256, 768] f16: forward 205 us, 0.88 of the measured copy rate, gradients 360, 0.86), else by what a warp
+// issues one after the other. Four forms (recurrence_launch chooses): up to 8 steps in a thread; a warp per 64 channels of a chunk, through all steps; the same with the steps in
+// segments, for few chunks; and through registers, for rows that copies of 16 bytes do not take.
 
 namespace fluke_sm100 {
 namespace {
@@ -168,7 +169,7 @@ __device__ __forceinline__ void st_state(float *s, int64_t at, F v) { *reinterpr
 
 // ---- a few steps ------------------------------------------------------------------------------------
 // A thread has two channels of a chunk and takes them through all of up to STEPS steps, whose loads are asked for at once: what a stream's single steps cost is a
-// launch and one trip to memory. [1, 1024, 768] through the form below, whose registers hold a tile of runs, took 15.2 us.
+// launch and one trip to memory: [1, 1024, 768] 4.7 us (15.2 through the form below, whose registers hold a tile of runs).
 template <typename T, int STEPS, bool BACKWARD>
 __global__ void __launch_bounds__(256)
 recurrence_steps_kernel(const RecDev p, const uint32_t pairs) {   // pairs of channels of all chunks
@@ -372,12 +373,14 @@ recurrence_direct_backward_kernel(const RecDev p) {
 
 // ---- a warp by itself -----------------------------------------------------------------------------
 // A warp takes 64 channels of a chunk (CH = 2 per lane) or 32 (CH = 1) through all steps, in tiles of 16 that asynchronous copies of 16 bytes per lane
-// bring into a ring of its own. No warp waits for another, and a step costs its two chained operations and the gate: some 20 instructions for 64 values
-// forwards, four of them of the special-function unit, which takes 8 cycles each: 32 of a scheduler's cycles.
+// bring into a ring of its own. No warp waits for another, and a step costs its two chained operations and the gate: 26 instructions for 64 values forwards and 45
+// backwards, four of them of the special-function unit, which takes 8 cycles each. (Tiles that eight warps share and join with a barrier each took 50 and 108
+// instructions and 234 + 500 us where this form takes 205 + 360; TMA boxes of 16 rows for the copies the same time at rows of 128 bytes and more at 64.)
 //
 // SEGMENTED: where chunks and channels are fewer than that needs, the warps of a CTA (and the CTAs of a cluster) take segments of the steps. Each
 // first finds what its segment does as one run; the runs are joined once, and then the segment is walked from the state in front of it. Its tiles are read a second time,
-// from L2 as a rule.
+// from L2 as a rule. [65536, 1, 512] 81 us in 16 clusters of 6 CTAs (clusters of 8 run in two rounds: 115), [1000, 32, 512] 31.5: there the special-function unit is busy for half of the time,
+// twice per gate in either walk.
 constexpr int kRecTile = 16;
 static_assert(kRecKept == kRecTile, "a tile begins with a kept state");
 
@@ -811,6 +814,8 @@ int recurrence_launch(RecDev p, cudaStream_t stream) {
     }
     if (!pieces) return recurrence_direct<T>(p, BACKWARD, stream);
     const int64_t narrow = int64_t(p.B) * ((p.H + 31) / 32);
+    // Us per call, forward and gradients, measured with cold caches, form by form (64 channels a warp : segments of 4 warps : segments of 16 warps of 32 channels): [256, 64, 512]
+    // 18 + 25 : 26 + 29 : 36 + 44, [1000, 32, 512] 49 + 65 : 37 + 45 : 51 + 63, [333, 7, 520] 20 + 27 : 14 + 14 : 12 + 14, [16384, 4, 256] 683 + 913 : 64 + 76 : 43 + 55.
     if (narrow >= 1024 || p.T <= 64) return recurrence_warps<T, 2, 4, BACKWARD ? 3 : 4, false, BACKWARD>(p, stream);
     if (narrow >= 200) return recurrence_warps<T, 2, 4, 4, true, BACKWARD>(p, stream);
     return recurrence_warps<T, 1, 16, 4, true, BACKWARD>(p, stream);
