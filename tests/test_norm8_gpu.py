@@ -30,7 +30,7 @@ def codes_of(h, fmt):
 SHAPES = [(1, 32), (1, 4096), (3, 96), (130, 544), (33, 1024), (5, 2048), (200, 4096), (3, 16384), (700, 160), (700, 256), (1500, 512), (700, 768), (1300, 1024), (900, 1536), (700, 2048), (700, 2080)]
 
 
-@pytest.mark.parametrize("fmt", ["int8", "fp8"])
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
 @pytest.mark.parametrize("m,k", SHAPES)
 def test_pre_norm(m, k, dtype, fmt):
@@ -52,7 +52,7 @@ def test_pre_norm(m, k, dtype, fmt):
     assert np.array_equal(got[1].cpu().numpy(), codes)
 
 
-@pytest.mark.parametrize("fmt", ["int8", "fp8"])
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
 @pytest.mark.parametrize("m,k,seqlen", [(2, 512, 1), (300, 512, 100), (1300, 1024, 0), (40, 4096, 7)])
 def test_around_a_block_and_in_place(m, k, seqlen, fmt):
     g = torch.Generator().manual_seed(m)
@@ -73,7 +73,7 @@ def test_feeds_the_8_bit_products():
     g = torch.Generator(device=DEV).manual_seed(1)
     t = lambda *s: torch.randn(*s, generator=g, device=DEV)
     x, res, w = t(500, 512).half(), t(500, 512).half(), (1 + 0.1 * t(512)).half()
-    _, q, s = ops.rmsnorm_block(x, res, None, None, w, 1.0, 1e-5, quant="fp8")
+    _, q, s = ops.rmsnorm_block(x, res, None, None, w, 1.0, 1e-5, quant="e4m3")
     wq = (t(256, 512) * 8).to(torch.float8_e4m3fn)
     sb = torch.rand(256, generator=g, device=DEV) / 100
     got = ops.gemm_fp8(q, wq.view(torch.uint8), s, sb)
@@ -86,4 +86,4 @@ def test_empty_and_refusals():
     x, w = torch.zeros(0, 64, dtype=torch.float16, device=DEV), torch.ones(64, dtype=torch.float16, device=DEV)
     assert [v.shape for v in ops.rmsnorm_block(x, x, None, None, w, 1.0, 1e-5, quant="int8")] == [(0, 64), (0, 64), (0,)]
     with pytest.raises(ValueError):
-        ops.rmsnorm_block(x, x, None, None, w, 1.0, 1e-5, quant="e4m3")
+        ops.rmsnorm_block(x, x, None, None, w, 1.0, 1e-5, quant="e5m2")
