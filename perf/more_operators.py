@@ -224,7 +224,7 @@ def _own(state):
         return (y, last) + tuple(ops.linear_recurrence_backward(state["grad"], state["gate"], state["value"], saved, grad_last=state["grad_last"],
                                                                  lengths=state["lengths"], reverse=state["reverse"]))
     fmt = state["case"]["format"]
-    stream, q, scale = ops.rmsnorm_block(state["x"], state["residual"], None, None, state["weight"], 1.0, EPS, quant=fmt)
+    stream, q, scale = ops.rmsnorm_block(state["x"], state["residual"], None, None, state["weight"], 1.0, EPS, quant="int8" if fmt == "int8" else "e4m3")
     if fmt == "int8":
         # the values that the codes stand for
         return stream, torch.mul(q, scale[:, None], out=torch.empty_like(stream)), scale
