@@ -179,3 +179,18 @@ def test_run_of_a_recurrent_block():
     p = ops.gemm_i8(q, w8, s, sb)
     exact = (q.double() @ w8.double().T) * (s.double()[:, None] * sb.double())
     assert ((p.double() - exact).abs() <= exact.abs() * (2.0 ** -11 + 2.0 ** -22) + 2.0 ** -25).all()
+
+
+def test_more_than_2_pow_31_values():
+    """Offsets beyond 32 bits in the output, the residual and x."""
+    m, n, k = 270000, 8192, 64
+    g = torch.Generator(device=DEV).manual_seed(1)
+    new = lambda *s: torch.randn(*s, generator=g, device=DEV, dtype=torch.float16)
+    w, res = new(n, k), new(m, n)
+    wide = new(m, 8192)
+    x = wide[:, 5000:5000 + k]
+    assert res.numel() > 1 << 31
+    out = ops.linear(x, w, residual=res, alpha=0.5)
+    rows = slice(m - 300, m)
+    check(out[rows], x[rows], w, None, None, res[rows], 0.5)
+    check(out[:300], x[:300], w, None, None, res[:300], 0.5)

@@ -220,3 +220,78 @@ def test_refusals():
             call()
     with pytest.raises(RuntimeError):
         ops.linear_recurrence(gate.cpu(), value.cpu())
+
+
+def test_more_than_2_pow_31_values():
+    """Offsets beyond 32 bits: the last chunks of a tensor of 2^31 values and more give what they give by themselves, forwards and backwards."""
+    t, b, h = 2100, 1024, 1000
+    g = torch.Generator(device=DEV).manual_seed(1)
+    new = lambda *s: torch.randn(*s, generator=g, device=DEV, dtype=torch.float16)
+    gate, value = new(t, b, h), new(t, b, h)
+    assert gate.numel() > 1 << 31
+    y, last, states = ops.linear_recurrence(gate, value, reverse=True, save=True)
+    tail = slice(b - 64, b)   # 64 chunks of 32 runs of channels take the same form
+    want = ops.linear_recurrence(gate[:, tail], value[:, tail], reverse=True, save=True)
+    assert torch.equal(y[:, tail], want[0]) and torch.equal(last[tail], want[1]) and torch.equal(states[:, tail], want[2])
+    dg, dv, dh = ops.linear_recurrence_backward(y, gate, value, states, reverse=True)
+    part = ops.linear_recurrence_backward(y[:, tail], gate[:, tail], value[:, tail], want[2], reverse=True)
+    assert torch.equal(dg[:, tail], part[0]) and torch.equal(dv[:, tail], part[1]) and torch.equal(dh[tail], part[2])
+
+
+def test_two_threads_with_a_stream_each():
+    import threading
+    gens = [torch.Generator().manual_seed(20 + i) for i in range(2)]
+    data = [steps(g, "time", 900, 3, 96, torch.float16) for g in gens]
+    want = [ops.linear_recurrence(*d) for d in data]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        stream = torch.cuda.Stream()
+        ops.set_stream(stream)   # of this thread
+        with torch.cuda.stream(stream):
+            for _ in range(50):
+                y, last = ops.linear_recurrence(*data[i])
+                z = ops.linear(y.view(2700, 96), data[i][1].view(2700, 96)[:64])
+                stream.synchronize()
+                if not (torch.equal(y, want[i][0]) and torch.equal(last, want[i][1])):
+                    bad.append(i)
+                if z.shape != (2700, 64):
+                    bad.append(i)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    assert not bad
+
+
+def test_autograd_around_the_calls():
+    """A function as a training program writes it, against differentiated elementary operations in 64 bits."""
+    class Recurrence(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, gate, value, h0):
+            y, last, states = ops.linear_recurrence(gate, value, h0, save=True)
+            ctx.save_for_backward(gate, value, states)
+            return y, last
+
+        @staticmethod
+        def backward(ctx, dy, dlast):
+            gate, value, states = ctx.saved_tensors
+            return ops.linear_recurrence_backward(dy.contiguous(), gate, value, states, grad_last=dlast.contiguous())
+    g = torch.Generator().manual_seed(31)
+    gate, value = (t.detach().requires_grad_() for t in steps(g, "time", 21, 2, 16, torch.bfloat16))
+    h0 = torch.randn(2, 16, generator=g).to(DEV).requires_grad_()
+    wy, wl = torch.randn(21, 2, 16, generator=g).to(DEV), torch.randn(2, 16, generator=g).to(DEV)
+    y, last = Recurrence.apply(gate, value, h0)
+    ((y * wy).sum() + (last * wl).sum()).backward()
+    leaves = [t.detach().double().requires_grad_() for t in (gate, value, h0)]
+    h, total = leaves[2], 0
+    for k in range(21):
+        f = torch.sigmoid(leaves[0][k])
+        h = f * h + (1 - f) * leaves[1][k]
+        total = total + (h * wy[k].bfloat16().double()).sum()   # the gradient of y arrives in its type
+    (total + (h * wl.double()).sum()).backward()
+    for a, b in zip((gate, value, h0), leaves):
+        # half a step of the gradient's type, and f32 roundings of sums of up to 21 terms
+        assert ((a.grad.double() - b.grad).abs() <= b.grad.abs() * 2.0 ** -8 + b.grad.abs().max() * 2.0 ** -16).all()
