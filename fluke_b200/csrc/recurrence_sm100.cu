@@ -818,6 +818,9 @@ int recurrence_launch(RecDev p, cudaStream_t stream) {
     // 18 + 25 : 26 + 29 : 36 + 44, [1000, 32, 512] 49 + 65 : 37 + 45 : 51 + 63, [333, 7, 520] 20 + 27 : 14 + 14 : 12 + 14, [16384, 4, 256] 683 + 913 : 64 + 76 : 43 + 55.
     if (narrow >= 1024 || p.T <= 64) return recurrence_warps<T, 2, 4, BACKWARD ? 3 : 4, false, BACKWARD>(p, stream);
     if (narrow >= 200) return recurrence_warps<T, 2, 4, 4, true, BACKWARD>(p, stream);
+    // Long segments of 64 channels, 8 warps : of 32 channels, 16 warps: [2000, 10, 512] 39 + 45 : 43 + 55, [4096, 8, 256] 25 + 29 : 27 + 35, [8000, 3, 512] 45 + 39 : 41 + 53,
+    // [16384, 4, 256] 61 + 59 : 43 + 55.
+    if (p.T >= 1024 && narrow >= (BACKWARD ? 40 : 64)) return recurrence_warps<T, 2, 8, 3, true, BACKWARD>(p, stream);
     return recurrence_warps<T, 1, 16, 4, true, BACKWARD>(p, stream);
 }
 

@@ -52,7 +52,7 @@ def near(got, want, tol):
 
 
 SIZES = [(1, 1, 2), (1, 5, 64), (7, 3, 66), (8, 2, 32), (9, 2, 30), (17, 300, 34), (63, 1, 64), (64, 2, 128), (65, 2, 130), (200, 3, 520), (1000, 2, 64),
-         (4097, 1, 34), (333, 7, 520), (1161, 1, 512), (20000, 1, 64), (520, 40, 256), (50, 130, 136), (35, 700, 96), (100, 1030, 72), (3000, 2, 40)]
+         (4097, 1, 34), (333, 7, 520), (1161, 1, 512), (20000, 1, 64), (520, 40, 256), (50, 130, 136), (35, 700, 96), (100, 1030, 72), (3000, 2, 40), (1100, 5, 264), (1500, 8, 328)]
 
 
 @pytest.mark.parametrize("t,b,h", SIZES)
