@@ -379,7 +379,7 @@ recurrence_direct_backward_kernel(const RecDev p) {
 //
 // SEGMENTED: where chunks and channels are fewer than that needs, the warps of a CTA (and the CTAs of a cluster) take segments of the steps. Each
 // first finds what its segment does as one run; the runs are joined once, and then the segment is walked from the state in front of it. Its tiles are read a second time,
-// from L2 as a rule. [65536, 1, 512] 81 us in 16 clusters of 6 CTAs (clusters of 8 run in two rounds: 115), [1000, 32, 512] 31.5: there the special-function unit is busy for half of the time,
+// from L2 as a rule. [65536, 1, 512] 81 us in 16 clusters of 6 CTAs (with cold caches 92; clusters of 8, which run in two rounds, 130), [1000, 32, 512] 31.5: there the special-function unit is busy for half of the time,
 // twice per gate in either walk.
 constexpr int kRecTile = 16;
 static_assert(kRecKept == kRecTile, "a tile begins with a kept state");
