@@ -212,20 +212,20 @@ recurrence_steps_kernel(const RecDev p, const uint32_t pairs) {   // pairs of ch
                 st_pair(const_cast<char *>(place(p.out, k)), live ? pack2(h, T()) : 0);
             }
         }
-    if (!BACKWARD) {
+    if constexpr (!BACKWARD) {
         if (p.h_last) st_state(p.h_last, state, h);
-        return;
-    }
+    } else {
 #pragma unroll
-    for (int k = STEPS - 1; k >= 0; --k)
-        if (k < p.T) {
-            const bool live = k >= from && k < to;
-            const float2 e = live ? add2(x, unpack2(dy[k], T())) : x, ce = mul2(m[k], e);   // -c e
-            x = add2(e, ce);
-            st_pair(const_cast<char *>(place(p.grad_gate, k)), live ? pack2(mul2(ce, u[k]), T()) : 0);
-            st_pair(const_cast<char *>(place(p.grad_value, k)), live ? pack2(ce, T()) ^ 0x80008000u : 0);
-        }
-    if (p.grad_h0) st_state(p.grad_h0, state, x);
+        for (int k = STEPS - 1; k >= 0; --k)
+            if (k < p.T) {
+                const bool live = k >= from && k < to;
+                const float2 e = live ? add2(x, unpack2(dy[k], T())) : x, ce = mul2(m[k], e);   // -c e
+                x = add2(e, ce);
+                st_pair(const_cast<char *>(place(p.grad_gate, k)), live ? pack2(mul2(ce, u[k]), T()) : 0);
+                st_pair(const_cast<char *>(place(p.grad_value, k)), live ? pack2(ce, T()) ^ 0x80008000u : 0);
+            }
+        if (p.grad_h0) st_state(p.grad_h0, state, x);
+    }
 }
 
 // ---- through registers ----------------------------------------------------------------------------
