@@ -836,6 +836,7 @@ struct RecRange {
     int T, B, H;
 };
 inline RecRange rec_range(const void *at, int64_t step, int64_t chunk, const RecDev &p) {
+    if (p.T == 0) return {};
     const uint64_t last = uint64_t(p.T > 1 ? (p.T - 1) * step : 0) + uint64_t(p.B > 1 ? (p.B - 1) * chunk : 0);
     return {reinterpret_cast<uintptr_t>(at), at ? (last + p.H) * 2 : 0, step, chunk, p.T, p.B, p.H};
 }
@@ -877,7 +878,8 @@ extern "C" int fluke_sm100_recurrence(const fluke_sm100_recurrence_t *r, int bac
     p.grad = {r->grad, r->grad_step, r->grad_chunk};
     p.grad_gate = {r->grad_gate, r->grad_gate_step, r->grad_gate_chunk};
     p.grad_value = {r->grad_value, r->grad_value_step, r->grad_value_chunk};
-    p.h0 = r->h0; p.h_last = r->h_last; p.states = r->states; p.grad_last = r->grad_last; p.grad_h0 = r->grad_h0;
+    p.h0 = r->h0; p.h_last = r->h_last; p.grad_last = r->grad_last; p.grad_h0 = r->grad_h0;
+    p.states = r->T > 0 ? r->states : nullptr;   // without steps there are none, whatever the address
     auto aligned = [](const void *q, unsigned n) { return (reinterpret_cast<uintptr_t>(q) & (n - 1)) == 0; };
     if (!aligned(p.lengths, 4) || !aligned(p.h0, 8) || !aligned(p.h_last, 8) || !aligned(p.states, 8) || !aligned(p.grad_last, 8) || !aligned(p.grad_h0, 8))
         return (int)cudaErrorMisalignedAddress;
@@ -899,11 +901,11 @@ extern "C" int fluke_sm100_recurrence(const fluke_sm100_recurrence_t *r, int bac
     for (int o = 0; o < 4; ++o) {
         for (int i = 0; i < 7; ++i) {
             const bool in_place = o == 3 && i >= 5 && out[o].at == in[i].at;
-            if (p.T > 0 && !in_place && !rec_apart(out[o], in[i])) return (int)cudaErrorInvalidValue;
+            if (!in_place && !rec_apart(out[o], in[i])) return (int)cudaErrorInvalidValue;
         }
         for (int other = 0; other < o; ++other)
-            if (p.T > 0 && !rec_apart(out[o], out[other])) return (int)cudaErrorInvalidValue;
-        if (p.T > 0 && out[o].H && !rec_rows_apart(out[o])) return (int)cudaErrorInvalidValue;
+            if (!rec_apart(out[o], out[other])) return (int)cudaErrorInvalidValue;
+        if (out[o].H && !rec_rows_apart(out[o])) return (int)cudaErrorInvalidValue;
     }
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (backward) return r->bf16 ? recurrence_launch<__nv_bfloat16, true>(p, s) : recurrence_launch<__half, true>(p, s);

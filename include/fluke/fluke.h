@@ -638,7 +638,7 @@ int fluke_linear_gpu(const fluke_linear_t *linear);
  * (values between steps and between chunks: time- or batch-major, or columns of wider rows), with H values in a row. H and the
  * strides are even, the strides at least H, 16-bit tensors start on 4 bytes, f32 ones on 8. With `lengths` (int32 [B], limited to 0 .. T) the steps t >= lengths[b]
  * of chunk b are not taken: out is zero there, whatever the inputs hold. `states` receives what the gradients need: the
- * state in front of every 16th step, f32 [ceil(T / 16), B, H]. Outputs lie apart from inputs and from each other, but for h_last
+ * state in front of every 16th step, f32 [ceil(T / 16), B, H] (nothing of it is touched where T is 0). Outputs lie apart from inputs and from each other, but for h_last
  * in the place of h0. Results do not depend on how the work is spread beyond the rounding of f32, and are the same from call to call. */
 typedef struct {
     int T, B, H;
