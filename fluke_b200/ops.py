@@ -1,10 +1,12 @@
 """Tensor-level operator interface: one function per C entry point, same name without the
 `fluke_` prefix, same argument meaning and the same error behaviour (void functions exit the
 process on a bad dimension, int functions raise on a non-zero return). Inputs must be
-contiguous CUDA tensors; nothing here computes on the host. The work of a call (checks, output
+contiguous CUDA tensors; nothing here computes on the host, and no call records anything for
+autograd. The work of a call (checks, output
 allocation, the C call) is done by the extension module (csrc/native_ops.cpp); what is not called
 per step goes through ctypes.
 """
+import contextlib
 import ctypes
 
 import torch
@@ -50,8 +52,20 @@ def _check(rc, what):
 
 
 def set_stream(stream=None):
-    """Route later launches to `stream` (torch.cuda.Stream) or back to the legacy default stream."""
+    """Route later launches of this thread to `stream` (torch.cuda.Stream) or back to the legacy default stream."""
     _L().fluke_set_stream(0 if stream is None else stream.cuda_stream)
+
+
+@contextlib.contextmanager
+def on_stream(stream):
+    """Routes this thread's launches to `stream` inside a `with` block, and puts back what was set. The setting is of a thread, and torch runs
+    backward functions on threads of its own: they call under `with on_stream(torch.cuda.current_stream(device))`."""
+    before = _L().fluke_get_stream()
+    set_stream(stream)
+    try:
+        yield
+    finally:
+        _L().fluke_set_stream(before)
 
 
 # ---- memory-bound kernels -----------------------------------------------------------------
