@@ -1,15 +1,19 @@
 // recurrence_sm100.cu -- gated linear recurrence over time and its gradients on sm_100a:
-//     h_t = f_t h_{t-1} + (1 - f_t) v_t,    f_t = sigmoid(g_t),    per chunk and channel.
+//     h_t = f_t h_{t-1} + c_t v_t,    f_t = sigmoid(g_t),    c_t = 1 - f_t,    per chunk and channel.
+// A step goes from the nearer end, by the smaller of f and c, which is 1 / (1 + exp |g|):
+//     h += c (v - h) for g >= 0,    h = v + f (h - v) for g < 0.
+// A run of gates near one (a channel that remembers for thousands of steps) keeps the digits of its small c so, where f rounded to f32 would be
+// off by 2^-25 per step, and a gate that closes those of what it lets through, where 1 - c has 2^-24 / f of its value left: of a state of 100 behind a
+// gate of -12 the form h + c (v - h) alone kept 0.9 % wrong, and a small value behind a large state lost digits to it.
+//
 // Gates do not depend on the state, so any run of steps acts on the state in front of it as one step does:
-//     h_out = h_in + (V - C h_in)
-// with C = 1 - prod f and V the state that the run leaves of zero. Runs are computed side by side and joined. One minus the
-// product is carried, not the product: a step is h += c (v - h) with c = 1 - f = 1 / (1 + exp(g)), and a run of gates
-// near one (a channel that remembers for thousands of steps) keeps the digits of its small c, where f rounded to f32 would
-// be off by 2^-25 per step.
+//     h_out = P h_in + V
+// with P = prod f and V the state that the run leaves of zero. Runs are computed side by side and joined. Beside P the runs carry M = P - 1, summed up by
+// itself: where P is above 1/2, which no gate below zero has then been part of, a run is h + (V + M h), for the same reason as a step.
 //
 // Backwards, with e_t the gradient of h_t and x_t what reaches step t from the steps behind it:
-//     e_t = dy_t + x_t,    x_{t-1} = e_t - c_t e_t,    dv_t = c_t e_t,    dg_t = e_t (h_{t-1} - v_t) f_t c_t
-// a run of steps acts on x as x_out = x_in + (D - C x_in), C as above. The states h_{t-1} are computed again, from those that the forward
+//     e_t = dy_t + x_t,    x_{t-1} = f_t e_t,    dv_t = c_t e_t,    dg_t = e_t (h_{t-1} - v_t) f_t c_t
+// a run of steps acts on x as x_out = P x_in + D. The states h_{t-1} are computed again, from those that the forward
 // pass keeps of every 16th step (4 bytes per 16 values): that reads 6 and writes 4 bytes per value, where states kept in full would be read as well, and rounded.
 //
 // Both are bound by memory where chunks and channels fill the device ([1000, 256, 768] f16: forward 205 us, 0.88 of the measured copy rate, gradients 360, 0.86), else by what a warp
@@ -51,42 +55,6 @@ __device__ __forceinline__ uint32_t ld_pair(const char *p) {
     asm volatile("ld.global.L1::no_allocate.b32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
     return v;
 }
-// -1 / (1 + exp(g)): relative error below 2^-21 and, of the argument's rounding, |g| 2^-24; zero above 87, where it is below 2^-125. Its sign
-// saves the negations: packed operations have none.
-__device__ __forceinline__ float2 gate_less_one(float2 g) {
-    const float2 a = mul2(g, make_float2(1.44269504f, 1.44269504f)), one = make_float2(-1.f, -1.f);
-    const float2 d = fma2(make_float2(ex2_approx(a.x), ex2_approx(a.y)), one, one);
-    return make_float2(rcp_approx(d.x), rcp_approx(d.y));
-}
-// 1 / (1 + exp(-g)), alike.
-__device__ __forceinline__ float2 gate_of(float2 g) {
-    const float2 a = mul2(g, make_float2(-1.44269504f, -1.44269504f));
-    const float2 d = add2(make_float2(ex2_approx(a.x), ex2_approx(a.y)), make_float2(1.f, 1.f));
-    return make_float2(rcp_approx(d.x), rcp_approx(d.y));
-}
-// With m = -c: a + c (b - a), and a - c a.
-__device__ __forceinline__ float2 towards(float2 a, float2 m, float2 b) { return fma2(m, fma2(b, make_float2(-1.f, -1.f), a), a); }
-__device__ __forceinline__ float2 less(float2 a, float2 m) { return fma2(m, a, a); }
-// C of a run and one more step; a run's C is kept as its negative as well.
-__device__ __forceinline__ float2 longer(float2 M, float2 m) { return fma2(m, add2(M, make_float2(1.f, 1.f)), M); }
-// a + (b - C a): what a run makes of a
-__device__ __forceinline__ float2 through(float2 a, float2 M, float2 b) { return add2(a, fma2(M, a, b)); }
-__device__ __forceinline__ float2 low(float4 q) { return make_float2(q.x, q.y); }
-__device__ __forceinline__ float2 high(float4 q) { return make_float2(q.z, q.w); }
-__device__ __forceinline__ float4 both(float2 a, float2 b) { return make_float4(a.x, a.y, b.x, b.y); }
-// Stores into the shared memory of a CTA of the cluster.
-__device__ __forceinline__ void tell(const float2 *to, int rank, float2 a, float2 b) {
-    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(cluster_address(smem_u32(to), rank)), "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y) : "memory");
-}
-__device__ __forceinline__ void tell(const float *to, int rank, float a, float b) {
-    asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(cluster_address(smem_u32(to), rank)), "f"(a), "f"(b) : "memory");
-}
-// The same operations for one channel.
-__device__ __forceinline__ float gate_less_one(float g) { return rcp_approx(fmaf(ex2_approx(g * 1.44269504f), -1.f, -1.f)); }
-__device__ __forceinline__ float towards(float a, float m, float b) { return fmaf(m, a - b, a); }
-__device__ __forceinline__ float less(float a, float m) { return fmaf(m, a, a); }
-__device__ __forceinline__ float longer(float M, float m) { return fmaf(m, M + 1.f, M); }
-__device__ __forceinline__ float through(float a, float M, float b) { return a + fmaf(M, a, b); }
 __device__ __forceinline__ float plus(float a, float b) { return a + b; }
 __device__ __forceinline__ float minus(float a, float b) { return a - b; }
 __device__ __forceinline__ float times(float a, float b) { return a * b; }
@@ -98,26 +66,60 @@ __device__ __forceinline__ float2 add_times(float2 a, float2 b, float2 c) { retu
 template <typename F> __device__ __forceinline__ F zero_of();
 template <> __device__ __forceinline__ float zero_of<float>() { return 0.f; }
 template <> __device__ __forceinline__ float2 zero_of<float2>() { return make_float2(0.f, 0.f); }
-// -c = -1 / (1 + E), and -f = -E / (1 + E), with E = exp(g). f is not one minus c, which has no digits left where c is near one. An infinite E has c = 0, and any
-// finite f then gives the gradient of zero.
-__device__ __forceinline__ float gate_less_one(float g, float &f) {
-    const float E = ex2_approx(g * 1.44269504f), m = rcp_approx(fmaf(E, -1.f, -1.f));
-    f = fminf(E, 3.0e38f) * m;
-    return m;
+template <typename F> __device__ __forceinline__ F one_of();
+template <> __device__ __forceinline__ float one_of<float>() { return 1.f; }
+template <> __device__ __forceinline__ float2 one_of<float2>() { return make_float2(1.f, 1.f); }
+// A step as one number q: -c where the gate keeps more than half (g >= 0), else +f; -0 is a step that changes nothing, +0 one that keeps nothing. Relative
+// error below 2^-21 and, of the argument's rounding and the constant's, |g| 2^-23; zero above |g| = 87, where it is below 2^-125.
+__device__ __forceinline__ float signed_share(float share, float g) { return __uint_as_float(__float_as_uint(share) ^ (~__float_as_uint(g) & 0x80000000u)); }
+__device__ __forceinline__ float gate_step(float g) { return signed_share(rcp_approx(1.f + ex2_approx(fabsf(g * 1.44269504f))), g); }
+__device__ __forceinline__ float2 gate_step(float2 g) {
+    const float2 a = mul2(g, make_float2(1.44269504f, 1.44269504f));
+    const float2 d = add2(make_float2(ex2_approx(fabsf(a.x)), ex2_approx(fabsf(a.y))), make_float2(1.f, 1.f));
+    return make_float2(signed_share(rcp_approx(d.x), g.x), signed_share(rcp_approx(d.y), g.y));
 }
-__device__ __forceinline__ float2 gate_less_one(float2 g, float2 &f) {
-    const float2 a = mul2(g, make_float2(1.44269504f, 1.44269504f)), one = make_float2(-1.f, -1.f);
-    const float2 E = make_float2(ex2_approx(a.x), ex2_approx(a.y)), d = fma2(E, one, one), m = make_float2(rcp_approx(d.x), rcp_approx(d.y));
-    f = mul2(make_float2(fminf(E.x, 3.0e38f), fminf(E.y, 3.0e38f)), m);
-    return m;
+__device__ __forceinline__ float keeps_or(float q, float a, float b) { return __float_as_int(q) < 0 ? a : b; }
+__device__ __forceinline__ float2 keeps_or(float2 q, float2 a, float2 b) { return make_float2(keeps_or(q.x, a.x, b.x), keeps_or(q.y, a.y, b.y)); }
+// f a + c b; f a
+template <typename F> __device__ __forceinline__ F towards(F a, F q, F b) { return add_times(q, minus(a, b), keeps_or(q, a, b)); }
+template <typename F> __device__ __forceinline__ F let_through(F a, F q) { return add_times(q, a, keeps_or(q, a, zero_of<F>())); }
+// c a = a - f a
+template <typename F> __device__ __forceinline__ F let_in(F a, F q) { return minus(minus(a, keeps_or(q, a, zero_of<F>())), times(q, a)); }
+// f c = |q| (1 - |q|)
+__device__ __forceinline__ float gate_slope(float q) { return fmaf(-fabsf(q), fabsf(q), fabsf(q)); }
+__device__ __forceinline__ float2 gate_slope(float2 q) { return make_float2(gate_slope(q.x), gate_slope(q.y)); }
+// What a run does: P, and M = P - 1, which is right where P is above 1/2.
+template <typename F> struct RecRun { F P, M; };
+template <typename F> __device__ __forceinline__ RecRun<F> no_run() { return {one_of<F>(), zero_of<F>()}; }
+template <typename F> __device__ __forceinline__ void lengthen(RecRun<F> &r, F q) {
+    r.M = add_times(q, r.P, r.M);
+    r.P = let_through(r.P, q);
+}
+template <typename F> __device__ __forceinline__ RecRun<F> joined(const RecRun<F> &a, const RecRun<F> &b) { return {times(a.P, b.P), add_times(b.M, a.P, a.M)}; }
+// P a + b: what a run makes of a
+__device__ __forceinline__ float through(float a, const RecRun<float> &r, float b) {
+    const float near = a + fmaf(r.M, a, b), far = fmaf(r.P, a, b);
+    return r.P > 0.5f ? near : far;
+}
+__device__ __forceinline__ float2 through(float2 a, const RecRun<float2> &r, float2 b) {
+    return make_float2(through(a.x, RecRun<float>{r.P.x, r.M.x}, b.x), through(a.y, RecRun<float>{r.P.y, r.M.y}, b.y));
+}
+__device__ __forceinline__ float2 low(float4 q) { return make_float2(q.x, q.y); }
+__device__ __forceinline__ float2 high(float4 q) { return make_float2(q.z, q.w); }
+__device__ __forceinline__ float4 both(float2 a, float2 b) { return make_float4(a.x, a.y, b.x, b.y); }
+// Stores into the shared memory of a CTA of the cluster.
+__device__ __forceinline__ void tell(const float2 *to, int rank, float2 a) {
+    asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(cluster_address(smem_u32(to), rank)), "f"(a.x), "f"(a.y) : "memory");
+}
+__device__ __forceinline__ void tell(const float *to, int rank, float a) {
+    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(cluster_address(smem_u32(to), rank)), "f"(a) : "memory");
 }
 // 16-bit values of a lane, one or two.
 template <typename T> __device__ __forceinline__ float2 widen(uint32_t v) { return unpack2(v, T()); }
 template <typename T> __device__ __forceinline__ float widen(uint16_t v) { return unpack2(v, T()).x; }
 template <typename T> __device__ __forceinline__ uint32_t narrow(float2 v) { return pack2(v, T()); }
 template <typename T> __device__ __forceinline__ uint16_t narrow(float v) { return uint16_t(pack2(make_float2(v, 0.f), T())); }
-template <typename Raw> __device__ __forceinline__ Raw sign_bits() { return Raw(0x80008000u); }
-// Gates of plus infinity, whose 1 - f is zero.
+// Gates of plus infinity: a step that changes nothing.
 template <typename Raw> __device__ __forceinline__ Raw closed_gates(__half) { return Raw(0x7C007C00u); }
 template <typename Raw> __device__ __forceinline__ Raw closed_gates(__nv_bfloat16) { return Raw(0x7F807F80u); }
 
@@ -195,20 +197,19 @@ recurrence_steps_kernel(const RecDev p, const uint32_t pairs) {   // pairs of ch
             if (BACKWARD) dy[k] = ld_pair(place(p.grad, k));
         }
     if (!BACKWARD && p.states) st_state(p.states, state, h);
-    float2 m[STEPS], u[STEPS];
+    float2 q[STEPS], u[STEPS];
 #pragma unroll
     for (int k = 0; k < STEPS; ++k)
         if (k < p.T) {
             // behind a chunk's end nothing changes, whatever stands there
             const bool live = k >= from && k < to;
+            const float2 now = unpack2(v[k], T());
+            q[k] = gate_step(unpack2(g[k], T()));
             if (BACKWARD) {
-                m[k] = gate_less_one(unpack2(g[k], T()), u[k]);
-                if (!live) m[k] = u[k] = make_float2(0.f, 0.f);
-                const float2 d = minus(h, live ? unpack2(v[k], T()) : h);
-                u[k] = times(d, u[k]);
-                h = add_times(m[k], d, h);
+                u[k] = times(minus(h, now), gate_slope(q[k]));
+                if (live) h = towards(h, q[k], now);
             } else {
-                if (live) h = towards(h, gate_less_one(unpack2(g[k], T())), unpack2(v[k], T()));
+                if (live) h = towards(h, q[k], now);
                 st_pair(const_cast<char *>(place(p.out, k)), live ? pack2(h, T()) : 0);
             }
         }
@@ -219,10 +220,10 @@ recurrence_steps_kernel(const RecDev p, const uint32_t pairs) {   // pairs of ch
         for (int k = STEPS - 1; k >= 0; --k)
             if (k < p.T) {
                 const bool live = k >= from && k < to;
-                const float2 e = live ? add2(x, unpack2(dy[k], T())) : x, ce = mul2(m[k], e);   // -c e
-                x = add2(e, ce);
-                st_pair(const_cast<char *>(place(p.grad_gate, k)), live ? pack2(mul2(ce, u[k]), T()) : 0);
-                st_pair(const_cast<char *>(place(p.grad_value, k)), live ? pack2(ce, T()) ^ 0x80008000u : 0);
+                const float2 e = add2(x, unpack2(dy[k], T()));
+                st_pair(const_cast<char *>(place(p.grad_gate, k)), live ? pack2(mul2(e, u[k]), T()) : 0);
+                st_pair(const_cast<char *>(place(p.grad_value, k)), live ? pack2(let_in(e, q[k]), T()) : 0);
+                if (live) x = let_through(e, q[k]);
             }
         if (p.grad_h0) st_state(p.grad_h0, state, x);
     }
@@ -232,9 +233,10 @@ recurrence_steps_kernel(const RecDev p, const uint32_t pairs) {   // pairs of ch
 // For strides or addresses that copies of 16 bytes do not take. A CTA's warps are runs of a tile (p.runs of them) of as many chunks or
 // channels as that leaves; the next tile's loads are asked for while this one is computed.
 template <typename T>
-__global__ void __launch_bounds__(kRecThreads, 3)
+__global__ void __launch_bounds__(kRecThreads, 2)
 recurrence_direct_kernel(const RecDev p) {
-    __shared__ float4 run_of[2][kRecThreads / 32][32];                     // -C and V of every run
+    __shared__ float4 run_of[2][kRecThreads / 32][32];                     // P and M of every run
+    __shared__ float2 left_by[2][kRecThreads / 32][32];                    // V
     __shared__ float2 carried[2][kRecThreads / 32][32];                    // the state in front of the tile, by the last run's warp
     const int warp = threadIdx.x >> 5, run = warp & (p.runs - 1), first = warp - run, last = first + p.runs - 1;
     RecPlace w(p, int(blockIdx.x) * (kRecThreads / 32 / p.runs) + warp / p.runs);
@@ -258,29 +260,31 @@ recurrence_direct_kernel(const RecDev p) {
     if (warp == last) carried[0][warp][w.lane] = h;
     for (int round = 0; round < p.rounds; ++round, s0 += stride) {
         const int par = round & 1;
-        float2 m[kRecSteps], M = make_float2(0.f, 0.f), V = M;
+        float2 q[kRecSteps], V = make_float2(0.f, 0.f);
+        RecRun<float2> own = no_run<float2>();
         uint32_t values[kRecSteps];
 #pragma unroll
         for (int k = 0; k < kRecSteps; ++k) {
             // behind a chunk's end nothing changes, whatever stands there
             const bool live = w.inside(s0 + k);
-            m[k] = live ? gate_less_one(unpack2(g[k], T())) : make_float2(0.f, 0.f);
+            q[k] = live ? gate_step(unpack2(g[k], T())) : make_float2(-0.f, -0.f);
             values[k] = live ? v[k] : 0;
-            V = towards(V, m[k], unpack2(values[k], T()));
-            M = longer(M, m[k]);
+            V = towards(V, q[k], unpack2(values[k], T()));
+            lengthen(own, q[k]);
         }
         if (round + 1 < p.rounds) load(s0 + stride);
-        run_of[par][warp][w.lane] = both(M, V);
+        run_of[par][warp][w.lane] = both(own.P, own.M);
+        left_by[par][warp][w.lane] = V;
         __syncthreads();
         h = carried[par][last][w.lane];
         for (int r = first; r < warp; ++r) {
-            const float4 q = run_of[par][r][w.lane];
-            h = through(h, low(q), high(q));
+            const float4 run = run_of[par][r][w.lane];
+            h = through(h, {low(run), high(run)}, left_by[par][r][w.lane]);
         }
         if (p.states && s0 % kRecKept == 0 && w.in && s0 < p.T) st_state(p.states, int64_t(s0 / kRecKept) * p.B * p.H + w.state, h);
 #pragma unroll
         for (int k = 0; k < kRecSteps; ++k) {
-            h = towards(h, m[k], unpack2(values[k], T()));
+            h = towards(h, q[k], unpack2(values[k], T()));
             if (w.in && s0 + k < p.T) st_pair(out[k], w.inside(s0 + k) ? pack2(h, T()) : 0);
         }
         out.at += stride * out.step;
@@ -294,8 +298,10 @@ recurrence_direct_kernel(const RecDev p) {
 template <typename T>
 __global__ void __launch_bounds__(kRecThreads, 2)
 recurrence_direct_backward_kernel(const RecDev p) {
-    __shared__ float4 run_of[2][kRecThreads / 32][32];                     // -C and V of every run
-    __shared__ float2 run_back[2][kRecThreads / 32][32], carried[2][kRecThreads / 32][32];   // D; what reaches the tile from behind, by the first run's warp
+    __shared__ float4 run_of[2][kRecThreads / 32][32], left_by[2][kRecThreads / 32][32];     // P and M of every run; V and D
+    // a thread's own values: held in registers they took 128 registers and more, and loads that are spilled are waited for (2400 : 3070 us at [65536, 1, 514])
+    __shared__ uint32_t kept_grads[kRecSteps][kRecThreads], kept_values[kRecSteps][kRecThreads];
+    __shared__ float2 carried[2][kRecThreads / 32][32];                    // what reaches the tile from behind, by the first run's warp
     const int warp = threadIdx.x >> 5, run = warp & (p.runs - 1), first = warp - run, last = first + p.runs - 1;
     RecPlace w(p, int(blockIdx.x) * (kRecThreads / 32 / p.runs) + warp / p.runs);
     const int stride = p.runs * kRecSteps;
@@ -321,43 +327,45 @@ recurrence_direct_backward_kernel(const RecDev p) {
     if (warp == first) carried[(p.rounds - 1) & 1][warp][w.lane] = x;
     for (int round = p.rounds - 1; round >= 0; --round, s0 -= stride, tile0 -= stride) {
         const int par = round & 1;
-        float2 m[kRecSteps], M = make_float2(0.f, 0.f), V = M, D = M, h = kept;
-        uint32_t gates[kRecSteps], values[kRecSteps], grads[kRecSteps];
+        float2 q[kRecSteps], V = make_float2(0.f, 0.f), D = V, h = kept;
+        RecRun<float2> own = no_run<float2>();
 #pragma unroll
         for (int k = 0; k < kRecSteps; ++k) {
             const bool live = w.inside(s0 + k);
-            gates[k] = g[k];
-            values[k] = live ? v[k] : 0;
-            grads[k] = live ? dy[k] : 0;
-            m[k] = live ? gate_less_one(unpack2(g[k], T())) : make_float2(0.f, 0.f);
-            V = towards(V, m[k], unpack2(values[k], T()));
-            M = longer(M, m[k]);
+            const uint32_t here = live ? v[k] : 0;
+            kept_values[k][threadIdx.x] = here;
+            kept_grads[k][threadIdx.x] = live ? dy[k] : 0;
+            q[k] = live ? gate_step(unpack2(g[k], T())) : make_float2(-0.f, -0.f);
+            V = towards(V, q[k], unpack2(here, T()));
+            lengthen(own, q[k]);
         }
         if (round > 0) load(s0 - stride, tile0 - stride);
 #pragma unroll
-        for (int k = kRecSteps - 1; k >= 0; --k) D = less(add2(D, unpack2(grads[k], T())), m[k]);
-        run_of[par][warp][w.lane] = both(M, V);
-        run_back[par][warp][w.lane] = D;
+        for (int k = kRecSteps - 1; k >= 0; --k) D = let_through(add2(D, unpack2(kept_grads[k][threadIdx.x], T())), q[k]);
+        run_of[par][warp][w.lane] = both(own.P, own.M);
+        left_by[par][warp][w.lane] = both(V, D);
         __syncthreads();
         for (int r = first; r < warp; ++r) {
-            const float4 q = run_of[par][r][w.lane];
-            h = through(h, low(q), high(q));
+            const float4 run = run_of[par][r][w.lane];
+            h = through(h, {low(run), high(run)}, low(left_by[par][r][w.lane]));
         }
         x = carried[par][first][w.lane];
-        for (int r = last; r > warp; --r) x = through(x, low(run_of[par][r][w.lane]), run_back[par][r][w.lane]);
-        float2 before[kRecSteps];                               // v - h in front of each step
+        for (int r = last; r > warp; --r) {
+            const float4 run = run_of[par][r][w.lane];
+            x = through(x, {low(run), high(run)}, high(left_by[par][r][w.lane]));
+        }
+        float2 u[kRecSteps];                                    // (h - v) f c, with the state in front of each step
 #pragma unroll
         for (int k = 0; k < kRecSteps; ++k) {
-            const float2 u = unpack2(values[k], T());
-            before[k] = fma2(h, make_float2(-1.f, -1.f), u);
-            h = towards(h, m[k], u);
+            const float2 now = unpack2(kept_values[k][threadIdx.x], T());
+            u[k] = times(minus(h, now), gate_slope(q[k]));
+            h = towards(h, q[k], now);
         }
 #pragma unroll
         for (int k = kRecSteps - 1; k >= 0; --k) {
-            const float2 e = add2(x, unpack2(grads[k], T())), ce = mul2(m[k], e);   // -c e
-            x = add2(e, ce);
-            // f by itself: one minus c has no digits left where c is near one
-            const uint32_t dg = pack2(mul2(mul2(ce, before[k]), gate_of(unpack2(gates[k], T()))), T()), dv = pack2(ce, T()) ^ 0x80008000u;
+            const float2 e = add2(x, unpack2(kept_grads[k][threadIdx.x], T()));
+            const uint32_t dg = pack2(mul2(e, u[k]), T()), dv = pack2(let_in(e, q[k]), T());
+            x = let_through(e, q[k]);
             if (w.in && s0 + k < p.T) {
                 const bool live = w.inside(s0 + k);
                 st_pair(dgate[k], live ? dg : 0);
@@ -387,9 +395,9 @@ static_assert(kRecKept == kRecTile, "a tile begins with a kept state");
 template <int CH, int TENSORS, int WARPS, int STAGES, bool SEGMENTED>
 struct RecLayout {
     static constexpr int kRow = 64 * CH, kTensor = kRecTile * kRow, kStage = TENSORS * kTensor, kRing = STAGES * kStage;
-    static constexpr int kOffRuns = WARPS * kRing;                                         // (segmented) WARPS x 32 lanes of two values
-    static constexpr int kOffTotals = kOffRuns + (SEGMENTED ? WARPS * 32 * 8 * CH : 0);    // kRecMostCluster x 32
-    static constexpr int kDynamic = kOffTotals + (SEGMENTED ? kRecMostCluster * 32 * 8 * CH : 0);
+    static constexpr int kOffRuns = WARPS * kRing;                                         // (segmented) WARPS x 32 lanes: P, M and V or D
+    static constexpr int kOffTotals = kOffRuns + (SEGMENTED ? WARPS * 32 * 12 * CH : 0);   // kRecMostCluster x 32
+    static constexpr int kDynamic = kOffTotals + (SEGMENTED ? kRecMostCluster * 32 * 12 * CH : 0);
 };
 
 // Where such a warp works.
@@ -466,6 +474,26 @@ struct RecPut {
     }
 };
 
+// What the runs of a CTA's warps, or of a cluster's CTAs, do to a lane's channels: [run, P M V, lane] in shared memory.
+template <typename F>
+struct RecRuns {
+    F *at;
+    __device__ __forceinline__ RecRuns(uint8_t *smem, int lane) : at(reinterpret_cast<F *>(smem) + lane) {}
+    __device__ __forceinline__ void put(int r, const RecRun<F> &run, F left_of_zero) const {
+        at[r * 96] = run.P;
+        at[r * 96 + 32] = run.M;
+        at[r * 96 + 64] = left_of_zero;
+    }
+    __device__ __forceinline__ RecRun<F> run(int r) const { return {at[r * 96], at[r * 96 + 32]}; }
+    __device__ __forceinline__ F left(int r) const { return at[r * 96 + 64]; }
+    // into the shared memory of CTA `rank` of the cluster
+    __device__ __forceinline__ void tell_all(int r, int rank, const RecRun<F> &run, F left_of_zero) const {
+        tell(at + r * 96, rank, run.P);
+        tell(at + r * 96 + 32, rank, run.M);
+        tell(at + r * 96 + 64, rank, left_of_zero);
+    }
+};
+
 template <typename T, int CH, int WARPS, int STAGES, bool SEGMENTED>
 __global__ void __launch_bounds__(WARPS * 32)
 recurrence_warp_kernel(const RecDev p) {
@@ -501,7 +529,7 @@ recurrence_warp_kernel(const RecDev p) {
     F h = ld_state<CH>(p.h0, w.state);
     // The next tile's gates and values: fetched a tile ahead, so that its gates are computed beside the chain of the one before. (Alone on its scheduler a
     // warp is as fast as what it has to issue side by side.) Behind the last tile what the ring holds is fetched, and not used.
-    F m[kRecTile], next_m[kRecTile];
+    F q[kRecTile], next_q[kRecTile];
     Raw v[kRecTile], next_v[kRecTile];
     auto fetch = [&](int s) {
         copy_wait<STAGES - 2>();
@@ -525,47 +553,50 @@ recurrence_warp_kernel(const RecDev p) {
         }
         if (++stage == STAGES) stage = 0;
 #pragma unroll
-        for (int k = 0; k < kRecTile; ++k) next_m[k] = gate_less_one(widen<T>(g[k]));
+        for (int k = 0; k < kRecTile; ++k) next_q[k] = gate_step(widen<T>(g[k]));
     };
     auto advance = [&] {
 #pragma unroll
         for (int k = 0; k < kRecTile; ++k) {
-            m[k] = next_m[k];
+            q[k] = next_q[k];
             v[k] = next_v[k];
         }
     };
     fetch(first);
     advance();
     if (SEGMENTED) {
-        F M = zero_of<F>(), V = M;
+        RecRun<F> own = no_run<F>();
+        F V = zero_of<F>();
         for (int i = 0; i < n; ++i) {
             fetch(i + 1 < n ? first + (i + 1) * kRecTile : first);
 #pragma unroll
             for (int k = 0; k < kRecTile; ++k) {
-                V = towards(V, m[k], widen<T>(v[k]));
-                M = longer(M, m[k]);
+                V = towards(V, q[k], widen<T>(v[k]));
+                lengthen(own, q[k]);
             }
             advance();
         }
-        F *runs = reinterpret_cast<F *>(smem + L::kOffRuns), *totals = reinterpret_cast<F *>(smem + L::kOffTotals);
-        runs[(warp * 32 + w.lane) * 2] = M;
-        runs[(warp * 32 + w.lane) * 2 + 1] = V;
+        RecRuns<F> runs(smem + L::kOffRuns, w.lane), totals(smem + L::kOffTotals, w.lane);
+        runs.put(warp, own, V);
         __syncthreads();
-        F before_m = zero_of<F>(), before_v = before_m;
+        RecRun<F> before = no_run<F>();
+        F before_v = zero_of<F>();
 #pragma unroll 4
         for (int r = 0; r < warp; ++r) {
-            const F qm = runs[(r * 32 + w.lane) * 2], qv = runs[(r * 32 + w.lane) * 2 + 1];
-            before_v = through(before_v, qm, qv);
-            before_m = longer(before_m, qm);
+            before_v = through(before_v, runs.run(r), runs.left(r));
+            before = joined(before, runs.run(r));
         }
         if (p.split > 1) {
             cluster_wait();
-            if (warp == WARPS - 1)
-                for (int r = 0; r < p.split; ++r) tell(totals + (rank * 32 + w.lane) * 2, r, longer(before_m, M), through(before_v, M, V));
+            if (warp == WARPS - 1) {
+                const RecRun<F> all = joined(before, own);
+                const F all_v = through(before_v, own, V);
+                for (int r = 0; r < p.split; ++r) totals.tell_all(rank, r, all, all_v);
+            }
             cluster_sync_threads();
-            for (int r = 0; r < rank; ++r) h = through(h, totals[(r * 32 + w.lane) * 2], totals[(r * 32 + w.lane) * 2 + 1]);
+            for (int r = 0; r < rank; ++r) h = through(h, totals.run(r), totals.left(r));
         }
-        h = through(h, before_m, before_v);
+        h = through(h, before, before_v);
     }
     const RecPut<CH> out(p, p.out, w);
     for (int i = 0; i < n; ++i) {
@@ -574,7 +605,7 @@ recurrence_warp_kernel(const RecDev p) {
         fetch(s + kRecTile);
 #pragma unroll
         for (int k = 0; k < kRecTile; ++k) {
-            h = towards(h, m[k], widen<T>(v[k]));
+            h = towards(h, q[k], widen<T>(v[k]));
             v[k] = narrow<T>(h);
         }
         char *to = out.at + s * out.step;
@@ -652,71 +683,74 @@ recurrence_warp_backward_kernel(const RecDev p) {
         if (++stage == STAGES) stage = 0;
     };
     if (SEGMENTED) {
-        F M = zero_of<F>(), D = M;
+        RecRun<F> own = no_run<F>();
+        F D = zero_of<F>();
         for (int i = n - 1; i >= 0; --i) {
             take(first + i * kRecTile, std::false_type());
-            F m[kRecTile];
+            F q[kRecTile];
 #pragma unroll
-            for (int k = 0; k < kRecTile; ++k) m[k] = gate_less_one(widen<T>(g[k]));
+            for (int k = 0; k < kRecTile; ++k) q[k] = gate_step(widen<T>(g[k]));
 #pragma unroll
             for (int k = kRecTile - 1; k >= 0; --k) {
-                D = less(plus(D, widen<T>(dy[k])), m[k]);
-                M = longer(M, m[k]);
+                D = let_through(plus(D, widen<T>(dy[k])), q[k]);
+                lengthen(own, q[k]);
             }
         }
-        F *runs = reinterpret_cast<F *>(smem + L::kOffRuns), *totals = reinterpret_cast<F *>(smem + L::kOffTotals);
-        runs[(warp * 32 + w.lane) * 2] = M;
-        runs[(warp * 32 + w.lane) * 2 + 1] = D;
+        RecRuns<F> runs(smem + L::kOffRuns, w.lane), totals(smem + L::kOffTotals, w.lane);
+        runs.put(warp, own, D);
         __syncthreads();
-        F behind_m = zero_of<F>(), behind_d = behind_m;
+        RecRun<F> behind = no_run<F>();
+        F behind_d = zero_of<F>();
 #pragma unroll 4
         for (int r = WARPS - 1; r > warp; --r) {
-            const F qm = runs[(r * 32 + w.lane) * 2], qd = runs[(r * 32 + w.lane) * 2 + 1];
-            behind_d = through(behind_d, qm, qd);
-            behind_m = longer(behind_m, qm);
+            behind_d = through(behind_d, runs.run(r), runs.left(r));
+            behind = joined(behind, runs.run(r));
         }
         if (p.split > 1) {
             cluster_wait();
-            if (warp == 0)
-                for (int r = 0; r < p.split; ++r) tell(totals + (rank * 32 + w.lane) * 2, r, longer(behind_m, M), through(behind_d, M, D));
+            if (warp == 0) {
+                const RecRun<F> all = joined(behind, own);
+                const F all_d = through(behind_d, own, D);
+                for (int r = 0; r < p.split; ++r) totals.tell_all(rank, r, all, all_d);
+            }
             cluster_sync_threads();
-            for (int r = p.split - 1; r > rank; --r) x = through(x, totals[(r * 32 + w.lane) * 2], totals[(r * 32 + w.lane) * 2 + 1]);
+            for (int r = p.split - 1; r > rank; --r) x = through(x, totals.run(r), totals.left(r));
         }
-        x = through(x, behind_m, behind_d);
+        x = through(x, behind, behind_d);
     }
     const RecPut<CH> dgate(p, p.grad_gate, w), dvalue(p, p.grad_value, w);
     // the state in front of a tile, asked for a tile ahead
     auto state_at = [&](int i) { return i >= 0 ? ld_state<CH>(p.states, int64_t((first + i * kRecTile) / kRecKept) * p.B * p.H + w.state) : zero_of<F>(); };
     F kept = state_at(n - 1);
-    // What a tile needs from the states: -c, and (h - v) (-f) with the state h in front of the step. With one channel per lane the registers hold two
+    // What a tile needs of gates and states: q, and (h - v) f c with the state h in front of the step. With one channel per lane the registers hold two
     // tiles', and one's are computed beside the chain of the other, which goes back in time.
     constexpr bool kAhead = CH == 1;
-    F m[kRecTile], u[kRecTile];
+    F q[kRecTile], u[kRecTile];
     Raw e_in[kRecTile];
-    auto prepare = [&](int i, F (&tm)[kRecTile], F (&tu)[kRecTile], Raw (&te)[kRecTile]) {
+    auto prepare = [&](int i, F (&tq)[kRecTile], F (&tu)[kRecTile], Raw (&te)[kRecTile]) {
         F h = kept;
         kept = state_at(i - 1);
         take(first + i * kRecTile, std::true_type());
 #pragma unroll
         for (int k = 0; k < kRecTile; ++k) {
-            tm[k] = gate_less_one(widen<T>(g[k]), tu[k]);
+            tq[k] = gate_step(widen<T>(g[k]));
             te[k] = dy[k];
         }
 #pragma unroll
         for (int k = 0; k < kRecTile; ++k) {
-            const F d = minus(h, widen<T>(v[k]));
-            tu[k] = times(d, tu[k]);
-            h = add_times(tm[k], d, h);
+            const F now = widen<T>(v[k]);
+            tu[k] = times(minus(h, now), gate_slope(tq[k]));
+            h = towards(h, tq[k], now);
         }
     };
     auto finish = [&](int s) {
         Raw dg[kRecTile], dv[kRecTile];
 #pragma unroll
         for (int k = kRecTile - 1; k >= 0; --k) {
-            const F e = plus(x, widen<T>(e_in[k])), ce = times(m[k], e);   // -c e
-            x = plus(e, ce);
-            dg[k] = narrow<T>(times(ce, u[k]));
-            dv[k] = narrow<T>(ce) ^ sign_bits<Raw>();
+            const F e = plus(x, widen<T>(e_in[k]));
+            dg[k] = narrow<T>(times(e, u[k]));
+            dv[k] = narrow<T>(let_in(e, q[k]));
+            x = let_through(e, q[k]);
         }
         char *to_g = dgate.at + s * dgate.step, *to_v = dvalue.at + s * dvalue.step;
         if (w.tile_inside(s)) {
@@ -736,22 +770,22 @@ recurrence_warp_backward_kernel(const RecDev p) {
         }
     };
     if constexpr (kAhead) {
-        if (n > 0) prepare(n - 1, m, u, e_in);
+        if (n > 0) prepare(n - 1, q, u, e_in);
         for (int i = n - 1; i >= 0; --i) {
-            F next_m[kRecTile], next_u[kRecTile];
+            F next_q[kRecTile], next_u[kRecTile];
             Raw next_e[kRecTile];
-            prepare(i - 1, next_m, next_u, next_e);   // in front of the first tile: what the ring holds, and not used
+            prepare(i - 1, next_q, next_u, next_e);   // in front of the first tile: what the ring holds, and not used
             finish(first + i * kRecTile);
 #pragma unroll
             for (int k = 0; k < kRecTile; ++k) {
-                m[k] = next_m[k];
+                q[k] = next_q[k];
                 u[k] = next_u[k];
                 e_in[k] = next_e[k];
             }
         }
     } else {
         for (int i = n - 1; i >= 0; --i) {
-            prepare(i, m, u, e_in);
+            prepare(i, q, u, e_in);
             finish(first + i * kRecTile);
         }
     }

@@ -1,10 +1,21 @@
-"""Gated linear recurrence on the GPU at the ends of what it takes: calls without steps."""
+"""Gated linear recurrence on the GPU at the ends of what it takes, through fluke_b200.ops, against oracle/recurrence.py: calls without steps, gates
+that close.
+
+Tolerances go with the result, by a bound that is carried along with the steps. 1 / (1 + exp |g|), the smaller of f and c = 1 - f, is
+    D = 2^-21 + |g| 2^-23
+of itself off (exponential 2^-22, its argument 2^-24 of itself and the constant in it as much, the reciprocal 2^-23, a sum 2^-24), so a step from h to f h + c v
+is, beside f times what h was off, D min(f, c) (|h| + |v|) and its own roundings off. With A' = f A + c |v| from |h0|, which no
+state and no part of a joined run is above, these are four at most (the difference, the step, the product of the gates of a run and its part in the joining):
+    E' = f E + D min(f, c) (A + |v|) + 4 2^-24 A'
+and the same backwards for x' = f (x + dy). Nothing here grows with a large state that a gate has let go."""
 import ctypes
 
+import numpy as np
 import pytest
 import torch
 
 from fluke_b200 import lib as L, ops
+from oracle import recurrence as ref
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -33,3 +44,123 @@ def test_no_steps_and_a_place_for_states(b, h):
     # in place
     c_call("fluke_linear_recurrence_gpu", L.fluke_linear_recurrence_t, T=0, B=b, H=h, h0=last, h_last=last, states=around[1])
     assert torch.equal(last, first) and around.isnan().all()
+
+
+# one size at least for each form: few steps; a warp per run of channels, for short and for many chunks; segments of 4, 8 and 16 warps; clusters; through registers
+FORMS = [(1, 3, 8), (5, 130, 34), (8, 2, 64), (50, 130, 136), (100, 1030, 72), (520, 40, 256), (3000, 8, 512), (333, 7, 520), (20000, 1, 64), (4097, 1, 34), (50, 3, 6)]
+TYPES = {"f16": torch.float16, "bf16": torch.bfloat16}
+
+
+def n64(t):
+    return None if t is None else t.detach().cpu().double().numpy()
+
+
+def off(g):
+    """D of the smaller of f and c."""
+    return 2.0 ** -21 + np.minimum(np.abs(g), 128) * 2.0 ** -23
+
+
+def rounded(want, dtype):
+    """Half a step of the type, subnormal values included."""
+    return np.maximum(np.abs(want) * (torch.finfo(dtype).eps / 2), 2.0 ** -25 if dtype == torch.float16 else 2.0 ** -134)
+
+
+def state_bounds(gate, value, h0, reverse):
+    """(A, E) in front of every step, and behind the last."""
+    f, c = ref.sigmoid(gate), ref.sigmoid(-gate)
+    a, e = np.abs(h0), np.zeros_like(h0)
+    bounds_a, bounds_e = np.zeros_like(f), np.zeros_like(f)
+    for k in (range(len(f) - 1, -1, -1) if reverse else range(len(f))):
+        bounds_a[k], bounds_e[k] = a, e
+        new = f[k] * a + c[k] * np.abs(value[k])
+        e = f[k] * e + off(gate[k]) * np.minimum(f[k], c[k]) * (a + np.abs(value[k])) + 2.0 ** -22 * new
+        a = new
+    return bounds_a, bounds_e, a, e
+
+
+def grad_bounds(gate, grad, grad_last, reverse):
+    """(A, E) of the gradient of every step's state, and in front of the first."""
+    f, c = ref.sigmoid(gate), ref.sigmoid(-gate)
+    a, e = np.abs(grad_last), np.zeros_like(grad_last)
+    bounds_a, bounds_e = np.zeros_like(f), np.zeros_like(f)
+    for k in (range(len(f)) if reverse else range(len(f) - 1, -1, -1)):
+        a = a + np.abs(grad[k])
+        bounds_a[k], bounds_e[k] = a, e + 2.0 ** -24 * a
+        new = f[k] * a
+        e = f[k] * bounds_e[k] + off(gate[k]) * np.minimum(f[k], c[k]) * a + 2.0 ** -22 * new
+        a = new
+    return bounds_a, bounds_e, a, e
+
+
+def near(got, want, tol, what):
+    d = np.abs(n64(got) - want)
+    bad = ~(d <= tol)
+    assert not bad.any(), f"{what}: {int(bad.sum())} of {bad.size}, first at {tuple(np.argwhere(bad)[0])}: {n64(got)[bad][0]} for {want[bad][0]}, tolerance {np.broadcast_to(tol, d.shape)[bad][0]}"
+
+
+def check(gate, value, h0, grad, grad_last, reverse):
+    """All outputs of both directions."""
+    dtype = gate.dtype
+    y, last, states = ops.linear_recurrence(gate, value, h0, reverse=reverse, save=True)
+    g, v, s = n64(gate), n64(value), n64(h0)
+    want, want_last, before = ref.forward(g, v, s, None, reverse)
+    a, e, a_last, e_last = state_bounds(g, v, s, reverse)
+    order = slice(None, None, -1) if reverse else slice(None)
+    behind_a, behind_e = (np.concatenate((x[order][1:], last_x[None]))[order] for x, last_x in ((a, a_last), (e, e_last)))
+    tiny = 2.0 ** -126   # a gate's f or c below it counts as zero
+    near(last, want_last, e_last + tiny, "last")
+    near(y, want, rounded(want, dtype) + behind_e * (1 + torch.finfo(dtype).eps) + tiny, "out")
+    near(states, before[order][::16], e[order][::16] + tiny, "states")
+    dg, dv, dh = ops.linear_recurrence_backward(grad, gate, value, states, grad_last=grad_last, reverse=reverse)
+    wg, wv, wh, _ = ref.backward(n64(grad), g, v, before, n64(grad_last), None, reverse)
+    x, ex, x_first, e_first = grad_bounds(g, n64(grad), n64(grad_last), reverse)
+    f, c, d = ref.sigmoid(g), ref.sigmoid(-g), off(g)
+    near(dh, wh, e_first + tiny, "dh")
+    near(dv, wv, rounded(wv, dtype) + (c * ex + (d * np.minimum(f, c) + 2.0 ** -23 * c) * x) * (1 + torch.finfo(dtype).eps) + tiny, "dv")
+    size = a + np.abs(v)
+    near(dg, wg, rounded(wg, dtype) + f * c * (ex * size + 2 * x * e + (d + 8 * 2.0 ** -24) * x * size) * (1 + torch.finfo(dtype).eps) + tiny, "dg")
+
+
+def closing(seed, t, b, h, dtype):
+    """Gates that mostly keep, of which one in ten closes (0 to -16), values of a thousandth, and now and then one of a hundred that is let in."""
+    g = torch.Generator().manual_seed(seed)
+    rand = lambda *s: torch.rand(*s, generator=g)
+    gate = torch.where(rand(t, b, h) < 0.1, -16 * rand(t, b, h), 2 + 8 * rand(t, b, h))
+    value = 1e-3 * torch.randn(t, b, h, generator=g)
+    large = rand(t, b, h) < 0.02
+    gate, value = torch.where(large, torch.full_like(gate, -3.0), gate), torch.where(large, 1e5 * value, value)
+    return gate.to(dtype).to(DEV), value.to(dtype).to(DEV), (100 * torch.randn(b, h, generator=g)).to(DEV)
+
+
+@pytest.mark.parametrize("t,b,h", FORMS)
+@pytest.mark.parametrize("dtype,reverse", [("f16", False), ("bf16", True)])
+def test_gates_that_close_on_large_states(t, b, h, dtype, reverse):
+    """What is left of a large state behind a gate that closes, and what reaches a gradient through one, keeps its digits."""
+    gate, value, h0 = closing(t + b + h, t, b, h, TYPES[dtype])
+    g = torch.Generator().manual_seed(t)
+    grad_last = torch.randn(b, h, generator=g).to(DEV)
+    # a gradient of the step that is taken last, and of it alone
+    grad = torch.zeros(t, b, h, dtype=TYPES[dtype], device=DEV)
+    grad[0 if reverse else t - 1] = 1.5
+    check(gate, value, h0, grad, grad_last, reverse)
+    check(gate, value, h0, torch.randn(t, b, h, generator=g).to(TYPES[dtype]).to(DEV), 100 * grad_last, reverse)
+
+
+@pytest.mark.parametrize("gate", [-8.0, -12.0, -16.0, -1.0, 0.0, -0.0])
+def test_one_step_through_a_closed_gate(gate):
+    """f h by itself: the value is zero, and the gradient comes from behind."""
+    x = lambda v: torch.full((1, 1, 8), v, dtype=torch.bfloat16, device=DEV)
+    check(x(gate), x(0.0), torch.full((1, 8), 100.0, device=DEV), x(0.0), torch.full((1, 8), 3.0, device=DEV), False)
+    check(x(gate), x(0.125), torch.full((1, 8), 100.0, device=DEV), x(2.0), torch.full((1, 8), 3.0, device=DEV), False)
+
+
+@pytest.mark.parametrize("t,b,h", [(333, 7, 520), (3000, 8, 512), (520, 40, 256), (20000, 1, 64), (4097, 1, 34), (50, 130, 136)])
+def test_a_large_first_state_that_fades(t, b, h):
+    """Runs of steps that are joined leave nothing of a state that they have let go: behind a few steps of gates of -1 the small values stand by themselves."""
+    g = torch.Generator().manual_seed(t)
+    gate = torch.full((t, b, h), -1.0, dtype=torch.bfloat16, device=DEV)
+    value = (1e-3 * torch.randn(t, b, h, generator=g)).bfloat16().to(DEV)
+    big = torch.full((b, h), 3e4, device=DEV)
+    zero = torch.zeros(t, b, h, dtype=torch.bfloat16, device=DEV)
+    check(gate, value, big, zero, big, False)
+    check(gate, value, big, (1e-3 * torch.randn(t, b, h, generator=g)).bfloat16().to(DEV), big, True)
