@@ -11,6 +11,9 @@
 // with P = prod f and V the state that the run leaves of zero. Runs are computed side by side and joined. Beside P the runs carry M = P - 1, summed up by
 // itself: where P is above 1/2, which no gate below zero has then been part of, a run is h + (V + M h), for the same reason as a step.
 //
+// Differences are no use of infinities and of the largest bf16 values: h - v is then infinite or NaN, and the state stays one of them through any further
+// steps. Steps that a state has not come out of finite are therefore taken once more, one by one, by f h + c v itself where one is not finite.
+//
 // Backwards, with e_t the gradient of h_t and x_t what reaches step t from the steps behind it:
 //     e_t = dy_t + x_t,    x_{t-1} = f_t e_t,    dv_t = c_t e_t,    dg_t = e_t (h_{t-1} - v_t) f_t c_t
 // a run of steps acts on x as x_out = P x_in + D. The states h_{t-1} are computed again, from those that the forward
@@ -88,6 +91,23 @@ template <typename F> __device__ __forceinline__ F let_in(F a, F q) { return min
 // f c = |q| (1 - |q|)
 __device__ __forceinline__ float gate_slope(float q) { return fmaf(-fabsf(q), fabsf(q), fabsf(q)); }
 __device__ __forceinline__ float2 gate_slope(float2 q) { return make_float2(gate_slope(q.x), gate_slope(q.y)); }
+// The same where a value may be infinite, or a difference too large. A state that is not finite stays, whatever the gate.
+__device__ __forceinline__ bool finite(float a) { return fabsf(a) <= 3.402823466e38f; }
+// Whether steps from `start`, which a NaN would be right for, have left something that is not finite.
+__device__ __forceinline__ bool broke(float start, float end) { return start == start && !finite(end); }
+__device__ __forceinline__ bool broke(float2 start, float2 end) { return broke(start.x, end.x) || broke(start.y, end.y); }
+__device__ __forceinline__ float share_of_state(float q) { return keeps_or(q, 1.f - fabsf(q), fabsf(q)); }
+__device__ __forceinline__ float share_of_value(float q) { return keeps_or(q, fabsf(q), 1.f - fabsf(q)); }
+__device__ __forceinline__ float towards_any(float a, float q, float b) {
+    const float r = towards(a, q, b);
+    return finite(r) ? r : finite(a) ? fmaf(share_of_state(q), a, share_of_value(q) * b) : a + share_of_value(q) * b;
+}
+__device__ __forceinline__ float let_through_any(float a, float q) { return finite(a) ? let_through(a, q) : a; }
+__device__ __forceinline__ float let_in_any(float a, float q) { return finite(a) ? let_in(a, q) : share_of_value(q) * a; }
+__device__ __forceinline__ float slope_any(float a, float q, float b) {   // (a - b) f c
+    const float k = gate_slope(q), d = a - b;
+    return finite(d) ? d * k : fmaf(a, k, -(b * k));
+}
 // What a run does: P, and M = P - 1, which is right where P is above 1/2.
 template <typename F> struct RecRun { F P, M; };
 template <typename F> __device__ __forceinline__ RecRun<F> no_run() { return {one_of<F>(), zero_of<F>()}; }
@@ -99,7 +119,7 @@ template <typename F> __device__ __forceinline__ RecRun<F> joined(const RecRun<F
 // P a + b: what a run makes of a
 __device__ __forceinline__ float through(float a, const RecRun<float> &r, float b) {
     const float near = a + fmaf(r.M, a, b), far = fmaf(r.P, a, b);
-    return r.P > 0.5f ? near : far;
+    return !finite(a) ? a + b : r.P > 0.5f ? near : far;
 }
 __device__ __forceinline__ float2 through(float2 a, const RecRun<float2> &r, float2 b) {
     return make_float2(through(a.x, RecRun<float>{r.P.x, r.M.x}, b.x), through(a.y, RecRun<float>{r.P.y, r.M.y}, b.y));
@@ -122,6 +142,79 @@ template <typename T> __device__ __forceinline__ uint16_t narrow(float v) { retu
 // Gates of plus infinity: a step that changes nothing.
 template <typename Raw> __device__ __forceinline__ Raw closed_gates(__half) { return Raw(0x7C007C00u); }
 template <typename Raw> __device__ __forceinline__ Raw closed_gates(__nv_bfloat16) { return Raw(0x7F807F80u); }
+
+// One channel of a chunk through steps s .. end - 1 again, step by step from memory, where infinities or differences that are too large came up. What the
+// steps had written is written over, by the same thread.
+template <typename T>
+struct RecAgain {
+    const RecDev &p;
+    int b, channel, from, to;
+    template <typename X>
+    __device__ __forceinline__ uint16_t *at(const X &x, int s) const {
+        return const_cast<uint16_t *>(static_cast<const uint16_t *>(x.at)) + b * x.chunk + int64_t(p.reverse ? p.T - 1 - s : s) * x.step + channel;
+    }
+    template <typename X>
+    __device__ __forceinline__ float read(const X &x, int s) const { return widen<T>(*at(x, s)); }
+    __device__ __forceinline__ float *kept(int s) const { return p.states + (int64_t(s / kRecKept) * p.B + b) * p.H + channel; }
+    __device__ __forceinline__ bool live(int s) const { return s >= from && s < to; }
+    __device__ __forceinline__ float forward(int s, int end, float h, bool store) const {
+#pragma unroll 1
+        for (; s < end; ++s) {
+            if (store && p.states && s % kRecKept == 0) *kept(s) = h;
+            if (!live(s)) continue;
+            h = towards_any(h, gate_step(read(p.gate, s)), read(p.value, s));
+            if (store) *at(p.out, s) = narrow<T>(h);
+        }
+        return h;
+    }
+    // a run's D
+    __device__ __forceinline__ float run_back(int s, int end, float d) const {
+#pragma unroll 1
+        while (--end >= s)
+            if (live(end)) d = let_through_any(d + read(p.grad, end), gate_step(read(p.gate, end)));
+        return d;
+    }
+    // Up to kRecKept steps, h the state in front of them
+    __device__ __forceinline__ float backward_from(int s, int end, float h, float x) const {
+        float u[kRecKept];
+#pragma unroll 1
+        for (int k = 0; k < end - s; ++k)
+            if (live(s + k)) {
+                const float q = gate_step(read(p.gate, s + k)), now = read(p.value, s + k);
+                u[k] = slope_any(h, q, now);
+                h = towards_any(h, q, now);
+            }
+#pragma unroll 1
+        for (int k = end - s - 1; k >= 0; --k)
+            if (live(s + k)) {
+                const float q = gate_step(read(p.gate, s + k)), e = x + read(p.grad, s + k);
+                *at(p.grad_gate, s + k) = narrow<T>(e * u[k]);
+                *at(p.grad_value, s + k) = narrow<T>(let_in_any(e, q));
+                x = let_through_any(e, q);
+            }
+        return x;
+    }
+    // steps from a kept state on
+    __device__ __forceinline__ float backward(int s, int end, float x) const {
+        if (end <= s) return x;
+#pragma unroll 1
+        for (int tile = s + (end - s - 1) / kRecKept * kRecKept; tile >= s; tile -= kRecKept) x = backward_from(tile, min(tile + kRecKept, end), *kept(tile), x);
+        return x;
+    }
+};
+// The same for a lane's channels.
+template <typename T, typename Place>
+struct RecAgainOf {
+    RecAgain<T> a;
+    __device__ __forceinline__ RecAgainOf(const RecDev &p, const Place &w) : a{p, w.b, w.channel, w.from, w.to} {}
+    __device__ __forceinline__ RecAgain<T> second() const { return {a.p, a.b, a.channel + 1, a.from, a.to}; }
+    __device__ __forceinline__ float forward(int s, int end, float h, bool store) const { return a.forward(s, end, h, store); }
+    __device__ __forceinline__ float2 forward(int s, int end, float2 h, bool store) const { return make_float2(a.forward(s, end, h.x, store), second().forward(s, end, h.y, store)); }
+    __device__ __forceinline__ float run_back(int s, int end, float d) const { return a.run_back(s, end, d); }
+    __device__ __forceinline__ float2 run_back(int s, int end, float2 d) const { return make_float2(a.run_back(s, end, d.x), second().run_back(s, end, d.y)); }
+    __device__ __forceinline__ float backward(int s, int end, float x) const { return a.backward(s, end, x); }
+    __device__ __forceinline__ float2 backward(int s, int end, float2 x) const { return make_float2(a.backward(s, end, x.x), second().backward(s, end, x.y)); }
+};
 
 // Where a warp works: 64 channels of a chunk, and of them the steps of one run of each tile. Processing goes through steps s = 0 .. T-1, time through s
 // or T - 1 - s; a tensor is walked in processing order. What lies in [from, to) is inside the chunk.
@@ -187,7 +280,10 @@ recurrence_steps_kernel(const RecDev p, const uint32_t pairs) {   // pairs of ch
         to = p.reverse ? p.T : length;
     }
     auto place = [&](const auto &x, int k) { return static_cast<const char *>(x.at) + (b * x.chunk + (p.reverse ? p.T - 1 - k : k) * x.step + channel) * 2; };
-    float2 h = ld_state(BACKWARD ? p.states : p.h0, state), x = BACKWARD ? ld_state(p.grad_last, state) : make_float2(0.f, 0.f);
+    const float2 h0 = ld_state(BACKWARD ? p.states : p.h0, state), x0 = BACKWARD ? ld_state(p.grad_last, state) : make_float2(0.f, 0.f);
+    float2 h = h0, x = x0;
+    const struct { int b, channel, from, to; } place_of = {b, channel, from, to};
+    const RecAgainOf<T, decltype(place_of)> again(p, place_of);
     uint32_t g[STEPS], v[STEPS], dy[STEPS];
 #pragma unroll
     for (int k = 0; k < STEPS; ++k)
@@ -214,6 +310,7 @@ recurrence_steps_kernel(const RecDev p, const uint32_t pairs) {   // pairs of ch
             }
         }
     if constexpr (!BACKWARD) {
+        if (broke(h0, h)) h = again.forward(0, p.T, h0, true);
         if (p.h_last) st_state(p.h_last, state, h);
     } else {
 #pragma unroll
@@ -225,6 +322,7 @@ recurrence_steps_kernel(const RecDev p, const uint32_t pairs) {   // pairs of ch
                 st_pair(const_cast<char *>(place(p.grad_value, k)), live ? pack2(let_in(e, q[k]), T()) : 0);
                 if (live) x = let_through(e, q[k]);
             }
+        if (broke(h0, h) || broke(x0, x)) x = again.backward(0, p.T, x0);
         if (p.grad_h0) st_state(p.grad_h0, state, x);
     }
 }
@@ -290,6 +388,11 @@ recurrence_direct_kernel(const RecDev p) {
         out.at += stride * out.step;
         if (warp == last) carried[par ^ 1][warp][w.lane] = h;
     }
+    __syncthreads();                  // the other runs' outputs come first
+    if (w.in && warp == last) {
+        const float2 h0 = ld_state(p.h0, w.state);
+        if (broke(h0, h)) h = RecAgainOf<T, RecPlace>(p, w).forward(0, p.T, h0, true);
+    }
     // by the threads that have read h0, which may be the same
     if (p.h_last && w.in && warp == last) st_state(p.h_last, w.state, h);
 }
@@ -323,6 +426,7 @@ recurrence_direct_backward_kernel(const RecDev p) {
         value.at -= stride * value.step;
         grad.at -= stride * grad.step;
     };
+    bool regular = true;              // all states so far
     if (p.rounds > 0) load(s0, tile0);
     if (warp == first) carried[(p.rounds - 1) & 1][warp][w.lane] = x;
     for (int round = p.rounds - 1; round >= 0; --round, s0 -= stride, tile0 -= stride) {
@@ -344,6 +448,7 @@ recurrence_direct_backward_kernel(const RecDev p) {
         for (int k = kRecSteps - 1; k >= 0; --k) D = let_through(add2(D, unpack2(kept_grads[k][threadIdx.x], T())), q[k]);
         run_of[par][warp][w.lane] = both(own.P, own.M);
         left_by[par][warp][w.lane] = both(V, D);
+        regular = regular && !broke(zero_of<float2>(), V);
         __syncthreads();
         for (int r = first; r < warp; ++r) {
             const float4 run = run_of[par][r][w.lane];
@@ -354,6 +459,7 @@ recurrence_direct_backward_kernel(const RecDev p) {
             const float4 run = run_of[par][r][w.lane];
             x = through(x, {low(run), high(run)}, high(left_by[par][r][w.lane]));
         }
+        const float2 start = h;
         float2 u[kRecSteps];                                    // (h - v) f c, with the state in front of each step
 #pragma unroll
         for (int k = 0; k < kRecSteps; ++k) {
@@ -372,9 +478,18 @@ recurrence_direct_backward_kernel(const RecDev p) {
                 st_pair(dvalue[k], live ? dv : 0);
             }
         }
+        regular = regular && !broke(start, h);
         dgate.at -= stride * dgate.step;
         dvalue.at -= stride * dvalue.step;
         if (warp == first) carried[par ^ 1][warp][w.lane] = x;
+    }
+    __shared__ int irregular[kRecThreads / 32][32];
+    irregular[warp][w.lane] = !regular;
+    __syncthreads();                  // the other runs' outputs come first
+    if (w.in && warp == first) {
+        const float2 behind = ld_state(p.grad_last, w.state);
+        for (int r = first; r <= last; ++r) regular = regular && !irregular[r][w.lane];
+        if (!regular || broke(behind, x)) x = RecAgainOf<T, RecPlace>(p, w).backward(0, p.T, behind);
     }
     if (p.grad_h0 && w.in && warp == first) st_state(p.grad_h0, w.state, x);
 }
@@ -564,6 +679,7 @@ recurrence_warp_kernel(const RecDev p) {
     };
     fetch(first);
     advance();
+    const RecAgainOf<T, RecWarp<CH>> again(p, w);
     if (SEGMENTED) {
         RecRun<F> own = no_run<F>();
         F V = zero_of<F>();
@@ -576,6 +692,7 @@ recurrence_warp_kernel(const RecDev p) {
             }
             advance();
         }
+        if (w.in && broke(zero_of<F>(), V)) V = again.forward(first, end, zero_of<F>(), false);
         RecRuns<F> runs(smem + L::kOffRuns, w.lane), totals(smem + L::kOffTotals, w.lane);
         runs.put(warp, own, V);
         __syncthreads();
@@ -598,6 +715,7 @@ recurrence_warp_kernel(const RecDev p) {
         }
         h = through(h, before, before_v);
     }
+    const F start = h;
     const RecPut<CH> out(p, p.out, w);
     for (int i = 0; i < n; ++i) {
         const int s = first + i * kRecTile;
@@ -620,6 +738,7 @@ recurrence_warp_kernel(const RecDev p) {
         }
         advance();
     }
+    if (w.in && broke(start, h)) h = again.forward(first, end, start, true);
     // By threads that have read h0 themselves, or are behind a barrier that all who do have passed: it may lie in the same place.
     if (p.h_last && w.in && (!SEGMENTED || segment == p.split * WARPS - 1)) st_state(p.h_last, w.state, h);
 }
@@ -682,6 +801,7 @@ recurrence_warp_backward_kernel(const RecDev p) {
         }
         if (++stage == STAGES) stage = 0;
     };
+    const RecAgainOf<T, RecWarp<CH>> again(p, w);
     if (SEGMENTED) {
         RecRun<F> own = no_run<F>();
         F D = zero_of<F>();
@@ -696,6 +816,7 @@ recurrence_warp_backward_kernel(const RecDev p) {
                 lengthen(own, q[k]);
             }
         }
+        if (w.in && broke(zero_of<F>(), D)) D = again.run_back(first, end, zero_of<F>());
         RecRuns<F> runs(smem + L::kOffRuns, w.lane), totals(smem + L::kOffTotals, w.lane);
         runs.put(warp, own, D);
         __syncthreads();
@@ -727,8 +848,11 @@ recurrence_warp_backward_kernel(const RecDev p) {
     constexpr bool kAhead = CH == 1;
     F q[kRecTile], u[kRecTile];
     Raw e_in[kRecTile];
+    const F start = x;
+    bool regular = true;              // all states so far
     auto prepare = [&](int i, F (&tq)[kRecTile], F (&tu)[kRecTile], Raw (&te)[kRecTile]) {
-        F h = kept;
+        const F before = kept;
+        F h = before;
         kept = state_at(i - 1);
         take(first + i * kRecTile, std::true_type());
 #pragma unroll
@@ -742,6 +866,7 @@ recurrence_warp_backward_kernel(const RecDev p) {
             tu[k] = times(minus(h, now), gate_slope(tq[k]));
             h = towards(h, tq[k], now);
         }
+        regular = regular && !broke(before, h);
     };
     auto finish = [&](int s) {
         Raw dg[kRecTile], dv[kRecTile];
@@ -789,6 +914,7 @@ recurrence_warp_backward_kernel(const RecDev p) {
             finish(first + i * kRecTile);
         }
     }
+    if (w.in && (!regular || broke(start, x))) x = again.backward(first, end, start);
     if (p.grad_h0 && w.in && (!SEGMENTED || segment == 0)) st_state(p.grad_h0, w.state, x);
 }
 

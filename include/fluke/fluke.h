@@ -639,7 +639,8 @@ int fluke_linear_gpu(const fluke_linear_t *linear);
  * strides are even, the strides at least H, 16-bit tensors start on 4 bytes, f32 ones on 8. With `lengths` (int32 [B], limited to 0 .. T) the steps t >= lengths[b]
  * of chunk b are not taken: out is zero there, whatever the inputs hold. `states` receives what the gradients need: the
  * state in front of every 16th step, f32 [ceil(T / 16), B, H] (nothing of it is touched where T is 0). Outputs lie apart from inputs and from each other, but for h_last
- * in the place of h0. Results do not depend on how the work is spread beyond the rounding of f32, and are the same from call to call. */
+ * in the place of h0. A state that is infinite or NaN stays so, whatever gates follow (an infinity of the other sign makes NaN of it); f and 1 - f
+ * below 2^-126 (gates beyond -87 and 87) count as zero. Results do not depend on how the work is spread beyond the rounding of f32, and are the same from call to call. */
 typedef struct {
     int T, B, H;
     int dtype;                  /* of gate, value, out                                              */

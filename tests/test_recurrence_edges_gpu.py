@@ -1,5 +1,5 @@
 """Gated linear recurrence on the GPU at the ends of what it takes, through fluke_b200.ops, against oracle/recurrence.py: calls without steps, gates
-that close.
+that close or are infinite, infinite and largest values.
 
 Tolerances go with the result, by a bound that is carried along with the steps. 1 / (1 + exp |g|), the smaller of f and c = 1 - f, is
     D = 2^-21 + |g| 2^-23
@@ -164,3 +164,105 @@ def test_a_large_first_state_that_fades(t, b, h):
     zero = torch.zeros(t, b, h, dtype=torch.bfloat16, device=DEV)
     check(gate, value, big, zero, big, False)
     check(gate, value, big, (1e-3 * torch.randn(t, b, h, generator=g)).bfloat16().to(DEV), big, True)
+
+
+def same(got, want, tol, what):
+    """Infinities and NaN in the same places, and the rest within the tolerance."""
+    got = n64(got)
+    assert np.array_equal(np.isnan(got), np.isnan(want)), f"{what}: NaN at {tuple(np.argwhere(np.isnan(got) != np.isnan(want))[0])}, {(np.isnan(got) != np.isnan(want)).sum()} differ"
+    inf = np.isinf(want)
+    assert np.array_equal(got[inf], want[inf]), f"{what}: infinities"
+    ok = ~inf & ~np.isnan(want)
+    d = np.abs(got - want, where=ok, out=np.zeros_like(got))
+    with np.errstate(invalid="ignore"):
+        bad = ok & ~(d <= tol)
+    assert not bad.any(), f"{what}: {int(bad.sum())}, first at {tuple(np.argwhere(bad)[0])}: {got[bad][0]} for {want[bad][0]}"
+
+
+@pytest.mark.parametrize("t,b,h", FORMS)
+@pytest.mark.parametrize("dtype,reverse,ragged", [("f16", False, True), ("bf16", True, False)])
+def test_gates_at_their_ends_in_every_form(t, b, h, dtype, reverse, ragged):
+    """Gates of both infinities and far beyond where an exponential overflows, anywhere and at the borders of tiles and segments, on finite states."""
+    g = torch.Generator().manual_seed(t + 3 * b + h)
+    gate = 3 * torch.randn(t, b, h, generator=g)
+    some = torch.rand(t, b, h, generator=g)
+    for i, end in enumerate((float("inf"), float("-inf"), 200.0, -200.0)):
+        gate[(some > 0.02 * i) & (some < 0.02 * i + 0.02)] = end
+    gate[::16, :, ::3], gate[15::16, :, 1::3] = float("-inf"), float("inf")
+    gate = gate.to(TYPES[dtype]).to(DEV)
+    value, grad = (torch.randn(t, b, h, generator=g).to(TYPES[dtype]).to(DEV) for _ in range(2))
+    h0, grad_last = (torch.randn(b, h, generator=g).to(DEV) for _ in range(2))
+    check(gate, value, 50 * h0, grad, grad_last, reverse)
+    if ragged:   # behind a chunk's end a gate closes nothing
+        lengths = torch.randint(0, t + 1, (b,), generator=g).int().to(DEV)
+        y, last, states = ops.linear_recurrence(gate, value, h0, lengths=lengths, reverse=reverse, save=True)
+        for i in range(b):
+            n = int(lengths[i])
+            part = slice(0, n)
+            if n and i < 4:
+                one = ops.linear_recurrence(gate[part, i:i + 1], value[part, i:i + 1], h0[i:i + 1], reverse=reverse)
+                want, want_last, _ = ref.forward(n64(gate[part, i:i + 1]), n64(value[part, i:i + 1]), n64(h0[i:i + 1]), None, reverse)
+                for got, got_last in ((y[part, i:i + 1], last[i:i + 1]), one):
+                    near(got, want, rounded(want, TYPES[dtype]) + 2.0 ** -16 * 8, "out")
+                    near(got_last, want_last, 2.0 ** -16 * 8, "last")
+            elif not n:
+                assert torch.equal(last[i], h0[i])
+            assert not y[n:, i].any()
+
+
+@pytest.mark.parametrize("t,b,h", FORMS)
+@pytest.mark.parametrize("dtype,reverse", [("f16", True), ("bf16", False)])
+def test_infinities_and_the_largest_values(t, b, h, dtype, reverse):
+    """An infinite state stays one, and values of opposite sign whose difference is too large for f32 have a mean all the same."""
+    dtype = TYPES[dtype]
+    g = torch.Generator().manual_seed(5 * t + b + h)
+    gate = (4 * torch.randn(t, b, h, generator=g)).clamp(-30, 30).to(dtype)
+    value, grad = (torch.randn(t, b, h, generator=g).to(dtype) for _ in range(2))
+    h0, grad_last = (torch.randn(b, h, generator=g) for _ in range(2))
+    kind = torch.arange(b * h).view(b, h) % 8   # of a channel
+    at = lambda: torch.randint(0, t, (b, h), generator=g)
+    put = lambda x, where, when, v: x.scatter_(0, when[None], torch.where(where, torch.tensor(v, dtype=x.dtype), x.gather(0, when[None])[0])[None])
+    inf, largest = float("inf"), torch.finfo(dtype).max
+    put(value, kind == 1, at(), inf)
+    put(value, kind == 2, at(), -inf)
+    put(value, kind == 2, at(), inf)
+    h0[kind == 3] = -inf
+    put(value, kind == 4, at(), float("nan"))
+    value[:, kind == 5] = torch.where(torch.rand(t, b, h, generator=g) < 0.5, largest, -largest)[:, kind == 5].to(dtype)
+    h0[kind == 5] = -float(largest)
+    put(grad, kind == 6, at(), -inf)
+    grad_last[kind == 7] = inf
+    gate, value, grad, h0, grad_last = (x.to(DEV) for x in (gate, value, grad, h0, grad_last))
+    lengths = torch.randint(0, t + 1, (b,), generator=g).int()
+    lengths[:1] = t
+    for lens in (None, lengths.to(DEV)):
+        num = None if lens is None else lens.cpu().numpy()
+        y, last, states = ops.linear_recurrence(gate, value, h0, lengths=lens, reverse=reverse, save=True)
+        with np.errstate(all="ignore"):
+            want, want_last, before = ref.forward(n64(gate), n64(value), n64(h0), num, reverse)
+            # E of a state is below this part of the largest that its channel has seen
+            top = np.maximum(np.nanmax(np.where(np.isfinite(n64(value)), np.abs(n64(value)), 0), 0), np.where(np.isfinite(n64(h0)), np.abs(n64(h0)), 0))
+            part = top * 2.0 ** -24 * (4 * min(t, 1 / ref.sigmoid(-n64(gate)).min()) + 256)
+            same(last, want_last, part, "last")
+            same(y, want, rounded(want, dtype) + part * 1.01, "out")
+            order = slice(None, None, -1) if reverse else slice(None)
+            same(states, before[order][::16], part, "states")
+            dg, dv, dh = ops.linear_recurrence_backward(grad, gate, value, states, grad_last=grad_last, lengths=lens, reverse=reverse)
+            wg, wv, wh, e = ref.backward(n64(grad), n64(gate), n64(value), before, n64(grad_last), num, reverse)
+            back = np.nanmax(np.where(np.isfinite(e), e, 0)) * 2.0 ** -24 * (4 * min(t, 1 / ref.sigmoid(-n64(gate)).min()) + 256)
+            same(dh, wh, back, "dh")
+            same(dv, wv, rounded(wv, dtype) + 1.01 * back, "dv")
+            # A factor that is smaller than its own error may as well be zero or of the other sign, so that its product with an infinite one is any infinity or NaN:
+            # a state that f32 holds as the value itself (f of 1e-13), say, whose difference is zero there
+            x, here, dy, f = n64(grad_last), np.zeros_like(wg), n64(grad), ref.sigmoid(n64(gate))
+            for k in (range(t) if reverse else range(t - 1, -1, -1)):
+                live = (k < (np.full(b, t) if num is None else num))[:, None]
+                here[k] = np.where(live, dy[k] + x, 0)
+                x = np.where(live, f[k] * here[k], x)
+            d = before - n64(value)
+            any_of = (np.isinf(here) & (np.abs(d) <= part)) | (np.isinf(d) & (np.abs(here) <= back))
+            wg[any_of] = n64(dg)[any_of]
+            # where the product is near the end of the type its rounding decides
+            edge = np.abs(wg) > 0.99 * float(largest)
+            wg[edge & ~np.isinf(wg)] = n64(dg)[edge & ~np.isinf(wg)]
+            same(dg, wg, rounded(wg, dtype) + 1.01 * (2 * back * top + 64 * part * (1 + np.nanmax(np.where(np.isfinite(e), e, 0)))), "dg")
