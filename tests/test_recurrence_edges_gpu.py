@@ -46,6 +46,25 @@ def test_no_steps_and_a_place_for_states(b, h):
     assert torch.equal(last, first) and around.isnan().all()
 
 
+@pytest.mark.parametrize("t,b,h", [(100, 3, 8), (5, 7, 34), (300, 9, 64), (1200, 4, 512)])
+@pytest.mark.parametrize("chunks_outside", [False, True])
+def test_gradients_as_columns_of_one_tensor(t, b, h, chunks_outside):
+    """What the product in front takes back: the gradients of gates and values side by side, with columns that nobody writes around them."""
+    g = torch.Generator().manual_seed(t)
+    new = lambda *s: torch.randn(*s, generator=g).half().to(DEV)
+    gate, value, grad = new(t, b, h), new(t, b, h), new(t, b, h)
+    states = ops.linear_recurrence(gate, value, save=True)[2]
+    want = ops.linear_recurrence_backward(grad, gate, value, states)
+    wide = torch.full((b, t, 2 * h + 16) if chunks_outside else (t, b, 2 * h + 16), 7.0, dtype=torch.float16, device=DEV)
+    both = wide.transpose(0, 1) if chunks_outside else wide
+    dg, dv, dh = both[..., 8:8 + h], both[..., 8 + h:8 + 2 * h], torch.empty(b, h, device=DEV)
+    strides = {n + s: x.stride(i) for n, x in (("gate", gate), ("value", value), ("grad", grad), ("grad_gate", dg), ("grad_value", dv)) for i, s in enumerate(("_step", "_chunk"))}
+    c_call("fluke_linear_recurrence_backward_gpu", L.fluke_linear_recurrence_grad_t, T=t, B=b, H=h, gate=gate, value=value, grad=grad, grad_gate=dg, grad_value=dv,
+           states=states, grad_h0=dh, **strides)
+    assert torch.equal(dg, want[0]) and torch.equal(dv, want[1]) and torch.equal(dh, want[2])
+    assert (both[..., :8] == 7).all() and (both[..., 8 + 2 * h:] == 7).all()
+
+
 # one size at least for each form: few steps; a warp per run of channels, for short and for many chunks; segments of 4, 8 and 16 warps; clusters; through registers
 FORMS = [(1, 3, 8), (5, 130, 34), (8, 2, 64), (50, 130, 136), (100, 1030, 72), (520, 40, 256), (3000, 8, 512), (333, 7, 520), (20000, 1, 64), (4097, 1, 34), (50, 3, 6)]
 TYPES = {"f16": torch.float16, "bf16": torch.bfloat16}
