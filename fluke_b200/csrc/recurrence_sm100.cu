@@ -19,7 +19,7 @@
 // a run of steps acts on x as x_out = P x_in + D. The states h_{t-1} are computed again, from those that the forward
 // pass keeps of every 16th step (4 bytes per 16 values): that reads 6 and writes 4 bytes per value, where states kept in full would be read as well, and rounded.
 //
-// Both are bound by memory where chunks and channels fill the device ([1000, 256, 768] f16: forward 205 us, 0.88 of the measured copy rate, gradients 360, 0.86), else by what a warp
+// Both are bound by memory where chunks and channels fill the device ([1000, 256, 768] f16: forward 206 us, 0.88 of the measured copy rate, gradients 371, 0.83), else by what a warp
 // issues one after the other. Four forms (recurrence_launch chooses): up to 8 steps in a thread; a warp per 64 channels of a chunk, through all steps; the same with the steps in
 // segments, for few chunks; and through registers, for rows that copies of 16 bytes do not take.
 
@@ -108,6 +108,10 @@ __device__ __forceinline__ float slope_any(float a, float q, float b) {   // (a 
     const float k = gate_slope(q), d = a - b;
     return finite(d) ? d * k : fmaf(a, k, -(b * k));
 }
+__device__ __forceinline__ float2 towards_any(float2 a, float2 q, float2 b) { return make_float2(towards_any(a.x, q.x, b.x), towards_any(a.y, q.y, b.y)); }
+__device__ __forceinline__ float2 let_through_any(float2 a, float2 q) { return make_float2(let_through_any(a.x, q.x), let_through_any(a.y, q.y)); }
+__device__ __forceinline__ float2 let_in_any(float2 a, float2 q) { return make_float2(let_in_any(a.x, q.x), let_in_any(a.y, q.y)); }
+__device__ __forceinline__ float2 slope_any(float2 a, float2 q, float2 b) { return make_float2(slope_any(a.x, q.x, b.x), slope_any(a.y, q.y, b.y)); }
 // What a run does: P, and M = P - 1, which is right where P is above 1/2.
 template <typename F> struct RecRun { F P, M; };
 template <typename F> __device__ __forceinline__ RecRun<F> no_run() { return {one_of<F>(), zero_of<F>()}; }
@@ -143,77 +147,96 @@ template <typename T> __device__ __forceinline__ uint16_t narrow(float v) { retu
 template <typename Raw> __device__ __forceinline__ Raw closed_gates(__half) { return Raw(0x7C007C00u); }
 template <typename Raw> __device__ __forceinline__ Raw closed_gates(__nv_bfloat16) { return Raw(0x7F807F80u); }
 
-// One channel of a chunk through steps s .. end - 1 again, step by step from memory, where infinities or differences that are too large came up. What the
-// steps had written is written over, by the same thread.
-template <typename T>
+template <int CH = 2> struct RecLane;
+template <> struct RecLane<1> { typedef float F; typedef uint16_t Raw; };
+template <> struct RecLane<2> { typedef float2 F; typedef uint32_t Raw; };
+
+// A lane's channels of a chunk through steps s .. end - 1 again, from memory, where infinities or differences that are too large came up. What the steps had
+// written is written over, by the same thread. Eight steps' loads (backwards four) are asked for at once: one by one they took 2.7 us a step.
+template <typename T, int CH = 2>
 struct RecAgain {
+    using F = typename RecLane<CH>::F;
+    using Raw = typename RecLane<CH>::Raw;
     const RecDev &p;
     int b, channel, from, to;
     template <typename X>
-    __device__ __forceinline__ uint16_t *at(const X &x, int s) const {
-        return const_cast<uint16_t *>(static_cast<const uint16_t *>(x.at)) + b * x.chunk + int64_t(p.reverse ? p.T - 1 - s : s) * x.step + channel;
+    __device__ __forceinline__ Raw *at(const X &x, int s) const {
+        const uint16_t *row = static_cast<const uint16_t *>(x.at) + b * x.chunk + int64_t(p.reverse ? p.T - 1 - s : s) * x.step + channel;
+        return reinterpret_cast<Raw *>(const_cast<uint16_t *>(row));
     }
-    template <typename X>
-    __device__ __forceinline__ float read(const X &x, int s) const { return widen<T>(*at(x, s)); }
-    __device__ __forceinline__ float *kept(int s) const { return p.states + (int64_t(s / kRecKept) * p.B + b) * p.H + channel; }
+    template <int N, typename X>
+    __device__ __forceinline__ void read(Raw (&to_lane)[N], const X &x, int s, int end) const {
+#pragma unroll
+        for (int k = 0; k < N; ++k) to_lane[k] = s + k < end && live(s + k) ? *at(x, s + k) : Raw(0);
+    }
+    __device__ __forceinline__ F *kept(int s) const { return reinterpret_cast<F *>(p.states + (int64_t(s / kRecKept) * p.B + b) * p.H + channel); }
     __device__ __forceinline__ bool live(int s) const { return s >= from && s < to; }
-    __device__ __forceinline__ float forward(int s, int end, float h, bool store) const {
+    __device__ __forceinline__ F forward(int s, int end, F h, bool store) const {
 #pragma unroll 1
-        for (; s < end; ++s) {
-            if (store && p.states && s % kRecKept == 0) *kept(s) = h;
-            if (!live(s)) continue;
-            h = towards_any(h, gate_step(read(p.gate, s)), read(p.value, s));
-            if (store) *at(p.out, s) = narrow<T>(h);
+        for (; s < end; s += kRecSteps) {
+            Raw g[kRecSteps], v[kRecSteps];
+            read(g, p.gate, s, end);
+            read(v, p.value, s, end);
+#pragma unroll
+            for (int k = 0; k < kRecSteps; ++k)
+                if (s + k < end) {
+                    if (store && p.states && (s + k) % kRecKept == 0) *kept(s + k) = h;
+                    if (!live(s + k)) continue;
+                    h = towards_any(h, gate_step(widen<T>(g[k])), widen<T>(v[k]));
+                    if (store) *at(p.out, s + k) = narrow<T>(h);
+                }
         }
         return h;
     }
     // a run's D
-    __device__ __forceinline__ float run_back(int s, int end, float d) const {
+    __device__ __forceinline__ F run_back(int s, int end, F d) const {
 #pragma unroll 1
-        while (--end >= s)
-            if (live(end)) d = let_through_any(d + read(p.grad, end), gate_step(read(p.gate, end)));
+        for (int first = s + (end - s - 1) / kRecSteps * kRecSteps; end > s; end = first, first -= kRecSteps) {
+            Raw g[kRecSteps], dy[kRecSteps];
+            read(g, p.gate, first, end);
+            read(dy, p.grad, first, end);
+#pragma unroll
+            for (int k = kRecSteps - 1; k >= 0; --k)
+                if (first + k < end && live(first + k)) d = let_through_any(plus(d, widen<T>(dy[k])), gate_step(widen<T>(g[k])));
+        }
         return d;
     }
-    // Up to kRecKept steps, h the state in front of them
-    __device__ __forceinline__ float backward_from(int s, int end, float h, float x) const {
-        float u[kRecKept];
-#pragma unroll 1
-        for (int k = 0; k < end - s; ++k)
-            if (live(s + k)) {
-                const float q = gate_step(read(p.gate, s + k)), now = read(p.value, s + k);
-                u[k] = slope_any(h, q, now);
-                h = towards_any(h, q, now);
-            }
-#pragma unroll 1
-        for (int k = end - s - 1; k >= 0; --k)
-            if (live(s + k)) {
-                const float q = gate_step(read(p.gate, s + k)), e = x + read(p.grad, s + k);
-                *at(p.grad_gate, s + k) = narrow<T>(e * u[k]);
-                *at(p.grad_value, s + k) = narrow<T>(let_in_any(e, q));
-                x = let_through_any(e, q);
-            }
-        return x;
-    }
     // steps from a kept state on
-    __device__ __forceinline__ float backward(int s, int end, float x) const {
-        if (end <= s) return x;
+    static constexpr int kBack = 4;
+    __device__ __forceinline__ F backward(int s, int end, F x) const {
 #pragma unroll 1
-        for (int tile = s + (end - s - 1) / kRecKept * kRecKept; tile >= s; tile -= kRecKept) x = backward_from(tile, min(tile + kRecKept, end), *kept(tile), x);
+        for (int first = s + (end - s - 1) / kRecKept * kRecKept; end > s; end = first, first -= kRecKept) {
+            F h = *kept(first), u[kRecKept];
+#pragma unroll 1
+            for (int at0 = 0; at0 < kRecKept; at0 += kBack) {
+                Raw g[kBack], v[kBack];
+                read(g, p.gate, first + at0, end);
+                read(v, p.value, first + at0, end);
+#pragma unroll
+                for (int k = 0; k < kBack; ++k)
+                    if (first + at0 + k < end && live(first + at0 + k)) {
+                        const F q = gate_step(widen<T>(g[k])), now = widen<T>(v[k]);
+                        u[at0 + k] = slope_any(h, q, now);
+                        h = towards_any(h, q, now);
+                    }
+            }
+#pragma unroll 1
+            for (int at0 = kRecKept - kBack; at0 >= 0; at0 -= kBack) {
+                Raw g[kBack], dy[kBack];
+                read(g, p.gate, first + at0, end);
+                read(dy, p.grad, first + at0, end);
+#pragma unroll
+                for (int k = kBack - 1; k >= 0; --k)
+                    if (first + at0 + k < end && live(first + at0 + k)) {
+                        const F q = gate_step(widen<T>(g[k])), e = plus(x, widen<T>(dy[k]));
+                        *at(p.grad_gate, first + at0 + k) = narrow<T>(times(e, u[at0 + k]));
+                        *at(p.grad_value, first + at0 + k) = narrow<T>(let_in_any(e, q));
+                        x = let_through_any(e, q);
+                    }
+            }
+        }
         return x;
     }
-};
-// The same for a lane's channels.
-template <typename T, typename Place>
-struct RecAgainOf {
-    RecAgain<T> a;
-    __device__ __forceinline__ RecAgainOf(const RecDev &p, const Place &w) : a{p, w.b, w.channel, w.from, w.to} {}
-    __device__ __forceinline__ RecAgain<T> second() const { return {a.p, a.b, a.channel + 1, a.from, a.to}; }
-    __device__ __forceinline__ float forward(int s, int end, float h, bool store) const { return a.forward(s, end, h, store); }
-    __device__ __forceinline__ float2 forward(int s, int end, float2 h, bool store) const { return make_float2(a.forward(s, end, h.x, store), second().forward(s, end, h.y, store)); }
-    __device__ __forceinline__ float run_back(int s, int end, float d) const { return a.run_back(s, end, d); }
-    __device__ __forceinline__ float2 run_back(int s, int end, float2 d) const { return make_float2(a.run_back(s, end, d.x), second().run_back(s, end, d.y)); }
-    __device__ __forceinline__ float backward(int s, int end, float x) const { return a.backward(s, end, x); }
-    __device__ __forceinline__ float2 backward(int s, int end, float2 x) const { return make_float2(a.backward(s, end, x.x), second().backward(s, end, x.y)); }
 };
 
 // Where a warp works: 64 channels of a chunk, and of them the steps of one run of each tile. Processing goes through steps s = 0 .. T-1, time through s
@@ -251,9 +274,6 @@ struct RecWalk {
     __device__ __forceinline__ char *operator[](int k) const { return at + k * step; }
 };
 __device__ __forceinline__ void st_pair(char *p, uint32_t v) { *reinterpret_cast<uint32_t *>(p) = v; }
-template <int CH = 2> struct RecLane;
-template <> struct RecLane<1> { typedef float F; typedef uint16_t Raw; };
-template <> struct RecLane<2> { typedef float2 F; typedef uint32_t Raw; };
 template <int CH = 2>
 __device__ __forceinline__ typename RecLane<CH>::F ld_state(const float *s, int64_t at) {
     using F = typename RecLane<CH>::F;
@@ -264,7 +284,7 @@ __device__ __forceinline__ void st_state(float *s, int64_t at, F v) { *reinterpr
 
 // ---- a few steps ------------------------------------------------------------------------------------
 // A thread has two channels of a chunk and takes them through all of up to STEPS steps, whose loads are asked for at once: what a stream's single steps cost is a
-// launch and one trip to memory: [1, 1024, 768] 4.7 us (15.2 through the form below, whose registers hold a tile of runs).
+// launch and one trip to memory: [1, 1024, 768] 4.8 us (15.2 through the form below, whose registers hold a tile of runs).
 template <typename T, int STEPS, bool BACKWARD>
 __global__ void __launch_bounds__(256)
 recurrence_steps_kernel(const RecDev p, const uint32_t pairs) {   // pairs of channels of all chunks
@@ -281,9 +301,6 @@ recurrence_steps_kernel(const RecDev p, const uint32_t pairs) {   // pairs of ch
     }
     auto place = [&](const auto &x, int k) { return static_cast<const char *>(x.at) + (b * x.chunk + (p.reverse ? p.T - 1 - k : k) * x.step + channel) * 2; };
     const float2 h0 = ld_state(BACKWARD ? p.states : p.h0, state), x0 = BACKWARD ? ld_state(p.grad_last, state) : make_float2(0.f, 0.f);
-    float2 h = h0, x = x0;
-    const struct { int b, channel, from, to; } place_of = {b, channel, from, to};
-    const RecAgainOf<T, decltype(place_of)> again(p, place_of);
     uint32_t g[STEPS], v[STEPS], dy[STEPS];
 #pragma unroll
     for (int k = 0; k < STEPS; ++k)
@@ -292,43 +309,65 @@ recurrence_steps_kernel(const RecDev p, const uint32_t pairs) {   // pairs of ch
             v[k] = ld_pair(place(p.value, k));
             if (BACKWARD) dy[k] = ld_pair(place(p.grad, k));
         }
-    if (!BACKWARD && p.states) st_state(p.states, state, h);
-    float2 q[STEPS], u[STEPS];
+    if (!BACKWARD && p.states) st_state(p.states, state, h0);
+    float2 q[STEPS], u[STEPS], h = h0;
+    // behind a chunk's end nothing changes, whatever stands there
+    auto live = [&](int k) { return k >= from && k < to; };
 #pragma unroll
     for (int k = 0; k < STEPS; ++k)
         if (k < p.T) {
-            // behind a chunk's end nothing changes, whatever stands there
-            const bool live = k >= from && k < to;
             const float2 now = unpack2(v[k], T());
             q[k] = gate_step(unpack2(g[k], T()));
-            if (BACKWARD) {
-                u[k] = times(minus(h, now), gate_slope(q[k]));
-                if (live) h = towards(h, q[k], now);
-            } else {
-                if (live) h = towards(h, q[k], now);
-                st_pair(const_cast<char *>(place(p.out, k)), live ? pack2(h, T()) : 0);
-            }
+            if (BACKWARD) u[k] = times(minus(h, now), gate_slope(q[k]));
+            if (live(k)) h = towards(h, q[k], now);
+            if (!BACKWARD) st_pair(const_cast<char *>(place(p.out, k)), live(k) ? pack2(h, T()) : 0);
         }
+    const bool broken = broke(h0, h);
+    // Again, from the registers; eight steps' gradients from memory: 80 registers instead of 86, of which an SM has three blocks instead of two (19.8 us : 24.1 at [8, 1024, 768])
+    constexpr bool kFromMemory = BACKWARD && STEPS > 4;
+    if (!kFromMemory && broken) {
+        h = h0;
+#pragma unroll
+        for (int k = 0; k < STEPS; ++k)
+            if (k < p.T && live(k)) {
+                const float2 now = unpack2(v[k], T());
+                if (BACKWARD) u[k] = slope_any(h, q[k], now);
+                h = towards_any(h, q[k], now);
+                if (!BACKWARD) st_pair(const_cast<char *>(place(p.out, k)), pack2(h, T()));
+            }
+    }
     if constexpr (!BACKWARD) {
-        if (broke(h0, h)) h = again.forward(0, p.T, h0, true);
         if (p.h_last) st_state(p.h_last, state, h);
     } else {
+        float2 x = x0;
 #pragma unroll
         for (int k = STEPS - 1; k >= 0; --k)
             if (k < p.T) {
-                const bool live = k >= from && k < to;
                 const float2 e = add2(x, unpack2(dy[k], T()));
-                st_pair(const_cast<char *>(place(p.grad_gate, k)), live ? pack2(mul2(e, u[k]), T()) : 0);
-                st_pair(const_cast<char *>(place(p.grad_value, k)), live ? pack2(let_in(e, q[k]), T()) : 0);
-                if (live) x = let_through(e, q[k]);
+                st_pair(const_cast<char *>(place(p.grad_gate, k)), live(k) ? pack2(mul2(e, u[k]), T()) : 0);
+                st_pair(const_cast<char *>(place(p.grad_value, k)), live(k) ? pack2(let_in(e, q[k]), T()) : 0);
+                if (live(k)) x = let_through(e, q[k]);
             }
-        if (broke(h0, h) || broke(x0, x)) x = again.backward(0, p.T, x0);
+        if constexpr (kFromMemory) {
+            if (broken || broke(x0, x)) x = RecAgain<T>{p, b, channel, from, to}.backward(0, p.T, x0);
+        } else if (broke(x0, x)) {
+            x = x0;
+#pragma unroll
+            for (int k = STEPS - 1; k >= 0; --k)
+                if (k < p.T && live(k)) {
+                    const float2 e = add2(x, unpack2(dy[k], T()));
+                    st_pair(const_cast<char *>(place(p.grad_gate, k)), pack2(mul2(e, u[k]), T()));
+                    st_pair(const_cast<char *>(place(p.grad_value, k)), pack2(let_in_any(e, q[k]), T()));
+                    x = let_through_any(e, q[k]);
+                }
+        }
         if (p.grad_h0) st_state(p.grad_h0, state, x);
     }
 }
 
 // ---- through registers ----------------------------------------------------------------------------
-// For strides or addresses that copies of 16 bytes do not take. A CTA's warps are runs of a tile (p.runs of them) of as many chunks or
+// For strides or addresses that copies of 16 bytes do not take (rows of 514 values, a view that starts on an odd multiple of two). Time is not spread over CTAs here, and a tile of 64 steps
+// ends with a barrier: [1000, 32, 514] 34 us and 62 (gradients) where [1000, 32, 512] takes 34 and 43, but [65536, 1, 514] 1530 and 2530 where [65536, 1, 512] takes 94 and 127. A CTA's warps are runs of a tile (p.runs of them) of as many chunks or
 // channels as that leaves; the next tile's loads are asked for while this one is computed.
 template <typename T>
 __global__ void __launch_bounds__(kRecThreads, 2)
@@ -391,7 +430,7 @@ recurrence_direct_kernel(const RecDev p) {
     __syncthreads();                  // the other runs' outputs come first
     if (w.in && warp == last) {
         const float2 h0 = ld_state(p.h0, w.state);
-        if (broke(h0, h)) h = RecAgainOf<T, RecPlace>(p, w).forward(0, p.T, h0, true);
+        if (broke(h0, h)) h = RecAgain<T>{p, w.b, w.channel, w.from, w.to}.forward(0, p.T, h0, true);
     }
     // by the threads that have read h0, which may be the same
     if (p.h_last && w.in && warp == last) st_state(p.h_last, w.state, h);
@@ -489,21 +528,21 @@ recurrence_direct_backward_kernel(const RecDev p) {
     if (w.in && warp == first) {
         const float2 behind = ld_state(p.grad_last, w.state);
         for (int r = first; r <= last; ++r) regular = regular && !irregular[r][w.lane];
-        if (!regular || broke(behind, x)) x = RecAgainOf<T, RecPlace>(p, w).backward(0, p.T, behind);
+        if (!regular || broke(behind, x)) x = RecAgain<T>{p, w.b, w.channel, w.from, w.to}.backward(0, p.T, behind);
     }
     if (p.grad_h0 && w.in && warp == first) st_state(p.grad_h0, w.state, x);
 }
 
 // ---- a warp by itself -----------------------------------------------------------------------------
 // A warp takes 64 channels of a chunk (CH = 2 per lane) or 32 (CH = 1) through all steps, in tiles of 16 that asynchronous copies of 16 bytes per lane
-// bring into a ring of its own. No warp waits for another, and a step costs its two chained operations and the gate: 26 instructions for 64 values forwards and 45
-// backwards, four of them of the special-function unit, which takes 8 cycles each. (Tiles that eight warps share and join with a barrier each took 50 and 108
-// instructions and 234 + 500 us where this form takes 205 + 360; TMA boxes of 16 rows for the copies the same time at rows of 128 bytes and more at 64.)
+// bring into a ring of its own. No warp waits for another, and a step costs its two chained operations and the gate: 38 instructions for 64 values forwards and 55
+// backwards with copies and stores, four of them of the special-function unit. (Tiles that eight warps share and join with a barrier each took 234 + 500 us, by an earlier form of the step, where
+// this form takes 206 + 371; TMA boxes of 16 rows for the copies the same time at rows of 128 bytes and more at 64.)
 //
 // SEGMENTED: where chunks and channels are fewer than that needs, the warps of a CTA (and the CTAs of a cluster) take segments of the steps. Each
 // first finds what its segment does as one run; the runs are joined once, and then the segment is walked from the state in front of it. Its tiles are read a second time,
-// from L2 as a rule. [65536, 1, 512] 81 us in 16 clusters of 6 CTAs (with cold caches 92; clusters of 8, which run in two rounds, 130), [1000, 32, 512] 31.5: there the special-function unit is busy for half of the time,
-// twice per gate in either walk.
+// from L2 as a rule. [65536, 1, 512] 94 us in 16 clusters of 6 CTAs (with cold caches 106; clusters of 8, which run in two rounds, 156), where the 96 SMs that work issue 3.3 of 4 instructions a cycle and the 134 MB
+// of inputs do not stay in L2 between the walks; [1000, 32, 512] 34: 256 CTAs on 148 SMs, of which 108 have two, and no unit is full (special-function unit 48 %, 2.1 of 4 instructions a cycle).
 constexpr int kRecTile = 16;
 static_assert(kRecKept == kRecTile, "a tile begins with a kept state");
 
@@ -610,7 +649,7 @@ struct RecRuns {
 };
 
 template <typename T, int CH, int WARPS, int STAGES, bool SEGMENTED>
-__global__ void __launch_bounds__(WARPS * 32)
+__global__ void __launch_bounds__(WARPS * 32, 1)
 recurrence_warp_kernel(const RecDev p) {
     using L = RecLayout<CH, 2, WARPS, STAGES, SEGMENTED>;
     using F = typename RecLane<CH>::F;
@@ -679,7 +718,7 @@ recurrence_warp_kernel(const RecDev p) {
     };
     fetch(first);
     advance();
-    const RecAgainOf<T, RecWarp<CH>> again(p, w);
+    const RecAgain<T, CH> again{p, w.b, w.channel, w.from, w.to};
     if (SEGMENTED) {
         RecRun<F> own = no_run<F>();
         F V = zero_of<F>();
@@ -802,7 +841,7 @@ recurrence_warp_backward_kernel(const RecDev p) {
         }
         if (++stage == STAGES) stage = 0;
     };
-    const RecAgainOf<T, RecWarp<CH>> again(p, w);
+    const RecAgain<T, CH> again{p, w.b, w.channel, w.from, w.to};
     if (SEGMENTED) {
         RecRun<F> own = no_run<F>();
         F D = zero_of<F>();
@@ -976,12 +1015,13 @@ int recurrence_launch(RecDev p, cudaStream_t stream) {
     if (!pieces) return recurrence_direct<T>(p, BACKWARD, stream);
     const int64_t narrow = int64_t(p.B) * ((p.H + 31) / 32);
     // Us per call, forward and gradients, measured with cold caches, form by form (64 channels a warp : segments of 4 warps : segments of 16 warps of 32 channels): [256, 64, 512]
-    // 18 + 25 : 26 + 29 : 36 + 44, [1000, 32, 512] 49 + 65 : 37 + 45 : 51 + 63, [333, 7, 520] 20 + 27 : 14 + 14 : 12 + 14, [16384, 4, 256] 683 + 913 : 64 + 76 : 43 + 55.
+    // 21 + 27 : 29 + 33 : 44 + 53, [1000, 32, 512] 56 + 75 : 41 + 49 : 57 + 71, [333, 7, 520] 24 + 33 : 14 + 16 : 12 + 14, [16384, 4, 256] 769 + 1081 : 70 + 86 : 47 + 60. From 200 to 1023 runs of 32 channels the second
+    // is taken whatever the number of steps: [65536, 13, 512] 3100 + 4700 : 1407 + 1808 : 1129 + 1505.
     if (narrow >= 1024 || p.T <= 64) return recurrence_warps<T, 2, 4, BACKWARD ? 3 : 4, false, BACKWARD>(p, stream);
     if (narrow >= 200) return recurrence_warps<T, 2, 4, 4, true, BACKWARD>(p, stream);
-    // Long segments of 64 channels, 8 warps : of 32 channels, 16 warps: [2000, 10, 512] 39 + 45 : 43 + 55, [4096, 8, 256] 25 + 29 : 27 + 35, [8000, 3, 512] 45 + 39 : 41 + 53,
-    // [16384, 4, 256] 61 + 59 : 43 + 55.
-    if (p.T >= 1024 && narrow >= (BACKWARD ? 40 : 64)) return recurrence_warps<T, 2, 8, 3, true, BACKWARD>(p, stream);
+    // Long segments of 64 channels, 8 warps : of 32 channels, 16 warps: [2000, 10, 512] 41 + 51 : 47 + 59, [4096, 8, 256] 27 + 31 : 29 + 37, [8000, 3, 512] 37 + 45 : 47 + 59,
+    // [16384, 4, 256] 53 + 68 : 47 + 59.
+    if (p.T >= 1024 && narrow >= 40) return recurrence_warps<T, 2, 8, 3, true, BACKWARD>(p, stream);
     return recurrence_warps<T, 1, 16, 4, true, BACKWARD>(p, stream);
 }
 
