@@ -19,7 +19,7 @@
 // a run of steps acts on x as x_out = P x_in + D. The states h_{t-1} are computed again, from those that the forward
 // pass keeps of every 16th step (4 bytes per 16 values): that reads 6 and writes 4 bytes per value, where states kept in full would be read as well, and rounded.
 //
-// Both are bound by memory where chunks and channels fill the device ([1000, 256, 768] f16: forward 206 us, 0.88 of the measured copy rate, gradients 371, 0.83), else by what a warp
+// Both are bound by memory where chunks and channels fill the device ([1000, 256, 768] f16: forward 208 us, 0.87 of the measured copy rate, gradients 371, 0.83), else by what a warp
 // issues one after the other. Four forms (recurrence_launch chooses): up to 8 steps in a thread; a warp per 64 channels of a chunk, through all steps; the same with the steps in
 // segments, for few chunks; and through registers, for rows that copies of 16 bytes do not take.
 
@@ -284,7 +284,7 @@ __device__ __forceinline__ void st_state(float *s, int64_t at, F v) { *reinterpr
 
 // ---- a few steps ------------------------------------------------------------------------------------
 // A thread has two channels of a chunk and takes them through all of up to STEPS steps, whose loads are asked for at once: what a stream's single steps cost is a
-// launch and one trip to memory: [1, 1024, 768] 4.8 us (15.2 through the form below, whose registers hold a tile of runs).
+// launch and one trip to memory: [1, 1024, 768] 4.7 us (15.2 through the form below, whose registers hold a tile of runs).
 template <typename T, int STEPS, bool BACKWARD>
 __global__ void __launch_bounds__(256)
 recurrence_steps_kernel(const RecDev p, const uint32_t pairs) {   // pairs of channels of all chunks
@@ -367,7 +367,7 @@ recurrence_steps_kernel(const RecDev p, const uint32_t pairs) {   // pairs of ch
 
 // ---- through registers ----------------------------------------------------------------------------
 // For strides or addresses that copies of 16 bytes do not take (rows of 514 values, a view that starts on an odd multiple of two). Time is not spread over CTAs here, and a tile of 64 steps
-// ends with a barrier: [1000, 32, 514] 34 us and 62 (gradients) where [1000, 32, 512] takes 34 and 43, but [65536, 1, 514] 1530 and 2530 where [65536, 1, 512] takes 94 and 127. A CTA's warps are runs of a tile (p.runs of them) of as many chunks or
+// ends with a barrier: [1000, 32, 514] 34 us and 61 (gradients) where [1000, 32, 512] takes 33 and 42, but [65536, 1, 514] 1560 and 2520 where [65536, 1, 512] takes 90 and 130. A CTA's warps are runs of a tile (p.runs of them) of as many chunks or
 // channels as that leaves; the next tile's loads are asked for while this one is computed.
 template <typename T>
 __global__ void __launch_bounds__(kRecThreads, 2)
@@ -535,14 +535,14 @@ recurrence_direct_backward_kernel(const RecDev p) {
 
 // ---- a warp by itself -----------------------------------------------------------------------------
 // A warp takes 64 channels of a chunk (CH = 2 per lane) or 32 (CH = 1) through all steps, in tiles of 16 that asynchronous copies of 16 bytes per lane
-// bring into a ring of its own. No warp waits for another, and a step costs its two chained operations and the gate: 38 instructions for 64 values forwards and 55
+// bring into a ring of its own. No warp waits for another, and a step costs its two chained operations and the gate: 36 instructions for 64 values forwards and 55
 // backwards with copies and stores, four of them of the special-function unit. (Tiles that eight warps share and join with a barrier each took 234 + 500 us, by an earlier form of the step, where
-// this form takes 206 + 371; TMA boxes of 16 rows for the copies the same time at rows of 128 bytes and more at 64.)
+// this form takes 208 + 371; TMA boxes of 16 rows for the copies the same time at rows of 128 bytes and more at 64.)
 //
 // SEGMENTED: where chunks and channels are fewer than that needs, the warps of a CTA (and the CTAs of a cluster) take segments of the steps. Each
 // first finds what its segment does as one run; the runs are joined once, and then the segment is walked from the state in front of it. Its tiles are read a second time,
-// from L2 as a rule. [65536, 1, 512] 94 us in 16 clusters of 6 CTAs (with cold caches 106; clusters of 8, which run in two rounds, 156), where the 96 SMs that work issue 3.3 of 4 instructions a cycle and the 134 MB
-// of inputs do not stay in L2 between the walks; [1000, 32, 512] 34: 256 CTAs on 148 SMs, of which 108 have two, and no unit is full (special-function unit 48 %, 2.1 of 4 instructions a cycle).
+// from L2 as a rule. [65536, 1, 512] 90 us in 16 clusters of 6 CTAs (with cold caches 99; clusters of 8, which run in two rounds, 142), where the 96 SMs that work issue 3.3 of 4 instructions a cycle and the 134 MB
+// of inputs do not stay in L2 between the walks; [1000, 32, 512] 33: 256 CTAs on 148 SMs, of which 108 have two, and no unit is full (special-function unit 48 %, 2.1 of 4 instructions a cycle).
 constexpr int kRecTile = 16;
 static_assert(kRecKept == kRecTile, "a tile begins with a kept state");
 
@@ -648,8 +648,9 @@ struct RecRuns {
     }
 };
 
+// (Registers: three CTAs of the plain form per SM, 168 each; with 172 there were two, [1000, 128, 768] 122 us : 116. Segments run one CTA per SM or two.)
 template <typename T, int CH, int WARPS, int STAGES, bool SEGMENTED>
-__global__ void __launch_bounds__(WARPS * 32, 1)
+__global__ void __launch_bounds__(WARPS * 32, SEGMENTED ? 1 : 3)
 recurrence_warp_kernel(const RecDev p) {
     using L = RecLayout<CH, 2, WARPS, STAGES, SEGMENTED>;
     using F = typename RecLane<CH>::F;
@@ -783,7 +784,7 @@ recurrence_warp_kernel(const RecDev p) {
 }
 
 // Backwards: steps are walked from the last to the first. In a tile the states are computed again from the one that the forward pass kept.
-// (Without a bound on the blocks per SM the compiler stays at 130 registers in the plain form and issues a tile's gates one after the other: [256, 64, 512] 28.5 us : 20.1 with 212.)
+// (Without a bound on the blocks per SM the compiler stays at 130 registers in the plain form and issues a tile's gates one after the other: [256, 64, 512] 28.5 us : 20.1 with 206.)
 template <typename T, int CH, int WARPS, int STAGES, bool SEGMENTED>
 __global__ void __launch_bounds__(WARPS * 32, 1)
 recurrence_warp_backward_kernel(const RecDev p) {
@@ -1015,12 +1016,12 @@ int recurrence_launch(RecDev p, cudaStream_t stream) {
     if (!pieces) return recurrence_direct<T>(p, BACKWARD, stream);
     const int64_t narrow = int64_t(p.B) * ((p.H + 31) / 32);
     // Us per call, forward and gradients, measured with cold caches, form by form (64 channels a warp : segments of 4 warps : segments of 16 warps of 32 channels): [256, 64, 512]
-    // 21 + 27 : 29 + 33 : 44 + 53, [1000, 32, 512] 56 + 75 : 41 + 49 : 57 + 71, [333, 7, 520] 24 + 33 : 14 + 16 : 12 + 14, [16384, 4, 256] 769 + 1081 : 70 + 86 : 47 + 60. From 200 to 1023 runs of 32 channels the second
-    // is taken whatever the number of steps: [65536, 13, 512] 3100 + 4700 : 1407 + 1808 : 1129 + 1505.
+    // 21 + 27 : 29 + 33 : 43 + 53, [1000, 32, 512] 51 + 75 : 39 + 48 : 55 + 72, [333, 7, 520] 23 + 33 : 14 + 16 : 12 + 14, [16384, 4, 256] 684 + 1071 : 66 + 85 : 46 + 62. From 200 to 1023 runs of 32 channels the second
+    // is taken whatever the number of steps, also where more warps per chunk would be faster: [65536, 13, 512] 1342 + 1745 there, 1052 + 1546 in segments of 16 warps, 1008 + 1336 in those of 8 warps of 64 channels.
     if (narrow >= 1024 || p.T <= 64) return recurrence_warps<T, 2, 4, BACKWARD ? 3 : 4, false, BACKWARD>(p, stream);
     if (narrow >= 200) return recurrence_warps<T, 2, 4, 4, true, BACKWARD>(p, stream);
-    // Long segments of 64 channels, 8 warps : of 32 channels, 16 warps: [2000, 10, 512] 41 + 51 : 47 + 59, [4096, 8, 256] 27 + 31 : 29 + 37, [8000, 3, 512] 37 + 45 : 47 + 59,
-    // [16384, 4, 256] 53 + 68 : 47 + 59.
+    // Long segments of 64 channels, 8 warps : of 32 channels, 16 warps: [2000, 10, 512] 41 + 51 : 46 + 61, [4096, 8, 256] 27 + 32 : 29 + 38, [8000, 3, 512] 37 + 45 : 45 + 60,
+    // [16384, 4, 256] 53 + 70 : 46 + 62.
     if (p.T >= 1024 && narrow >= 40) return recurrence_warps<T, 2, 8, 3, true, BACKWARD>(p, stream);
     return recurrence_warps<T, 1, 16, 4, true, BACKWARD>(p, stream);
 }
