@@ -107,8 +107,9 @@ __device__ __forceinline__ uint4 finish8(const float (&sum)[8], const uint4 *bia
 // up a share of the tile from all of them, in the order of the ranks. What bounds it is latency, and for one or a few rows
 // reading the weights.
 //
-// A CTA takes less than half of an SM's shared memory, so that the next kernel's CTAs are set up beside it, and 128 of its 512
-// tensor-memory columns.
+// A CTA takes 128 of an SM's 512 tensor-memory columns, and less than half of its shared memory (a ring of up to 104 KB; the sums and the shares of tiles
+// of up to 64 rows are less), so that the next kernel's CTAs are set up beside it. Two kinds of launches take more and leave no room for them: the deep ring, 152 KB, for a run of
+// K that a smaller one does not hold, and split tiles of 128 rows, up to 135 KB of sums and shares.
 constexpr int kLinSplitSmem = 104 * 1024, kLinSplitMinSmem = 78 * 1024, kLinSplitDeep = 152 * 1024, kLinSplitMaxSmem = 160 * 1024;
 constexpr int kLinSplitStages = 8, kLinSplitCols = 128;
 constexpr int kLinSumPitch = 132;              // floats between rows of the sums
@@ -585,7 +586,7 @@ int linear_split_launch(const fluke_sm100_linear_t *g, cudaStream_t stream) {
     int smem = p.stages * stage_bytes;
     if (smem < p.sums_at + sums) smem = p.sums_at + sums;
     if (smem < kLinSplitMinSmem) smem = kLinSplitMinSmem;
-    if (smem > kLinSplitMaxSmem) return (int)cudaErrorInvalidValue;   // 128 rows, split: 133 KB
+    if (smem > kLinSplitMaxSmem) return (int)cudaErrorInvalidValue;   // 128 rows, split: 135 KB at most (6 or 7 CTAs per tile)
     CUtensorMap tm_x, tm_w;
     int rc = lin_operand(&tm_x, g->x, g->M, g->K, g->ld_x, rows);
     if (!rc) rc = lin_operand(&tm_w, g->w, g->N, g->K, g->K, 128);
