@@ -220,7 +220,7 @@ def gated_mlp_nvfp4(a, a_scale, a_row, gate, gate_scale, gate_row, up, up_scale,
 def rmsnorm_block(x, residual, post_weight, gate, pre_weight, alpha, eps, seqlen=0, quant=None, residual_out=None):
     """Norms around a block: stream = alpha * residual + gate * norm(x, post_weight), then norm(stream, pre_weight)
     for the next block, as 16-bit values (quant None) or quantised: "mxfp4", "nvfp4", or "int8" (int8 codes) and "e4m3"
-    (fp8 bytes) under an f32 scale per row, as the 8-bit products take them. gate [cols], or
+    (fp8 bytes) under an f32 scale per row, as the 8-bit products take them (up to 1024 columns; wider rows have no product here). gate [cols], or
     [ceil(rows / seqlen), cols] with seqlen > 0. post_weight, gate and pre_weight may be None. Returns the
     stream (written to `residual_out`, which may be `residual` or `x`, or to a new tensor) followed by the
     next block's input: (stream, out), (stream, codes, scale[, row_scale]) with the row scales alone for 8 bits, or (stream,) without

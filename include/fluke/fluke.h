@@ -548,7 +548,7 @@ int fluke_factored_lstm_layer_i8_noalloc_gpu(const fluke_flstm_layer_t *layer);
  * ---------------------------------------------------------------------------------- */
 enum { FLUKE_F16 = 0, FLUKE_BF16 = 1 };
 enum { FLUKE_FP4_MX = 1, FLUKE_FP4_NV = 2 };
-/* 8-bit output of the norms around a block, for the 8-bit products: scale[row] = max(amax, 1e-12) / 127 (int8) or / 448 (e4m3),
+/* 8-bit output of the norms around a block, for the 8-bit products (which take up to 1024 columns; wider rows have none here): scale[row] = max(amax, 1e-12) / 127 (int8) or / 448 (e4m3),
  * code = v * (127 or 448 / max(amax, 1e-12)) to the nearest, ties to even. A row with an infinity or a NaN has the scale NaN and zeros. */
 enum { FLUKE_ROW_INT8 = 4, FLUKE_ROW_FP8 = 5 };
 
